@@ -317,6 +317,97 @@ int specq_kv_append_int8(const void* k_new, const void* v_new, int64_t s_nb, int
                          int H_KV, int D, int PAGE, const int32_t* plan, void* stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Paged attention over a cache with block scales (no reference counterpart): as specq_paged_attn,
+ * with int8 (code_fp8 = 0) or e4m3 (1) codes and one fp32 scale for each block of `block` tokens and
+ * KV head:  s_t = (q . k_t) ks[blk(t)] sm_scale,  o = sum_t softmax_t(s) vs[blk(t)] v_t.
+ *   kc, vc   codes [pages, PAGE, H_KV, D], as specq_paged_attn
+ *   ks, vs   fp32 [pages, PAGE / block, H_KV], strides s_sp (page), s_sb (block), s_sh, shared
+ *   block    a multiple of 16 that divides PAGE
+ *   Probabilities are rounded to fp16 once, after their V scale, under a power of two that keeps them
+ *   normal whatever the scales' size.  Scales, and e4m3 NaN codes, of tokens that a row does not see do
+ *   not reach it.  Everything else, the workspace (specq_paged_attn_workspace_size) too, as
+ *   specq_paged_attn; QPP = 1, fused, eager and plan-mode calls agree bit for bit unless a probability
+ *   is an fp16 subnormal.
+ * ------------------------------------------------------------------------------------- */
+int specq_paged_attn_block(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh,
+                           const void* kc, const void* vc, int code_fp8, int64_t s_kp, int64_t s_ko, int64_t s_kh,
+                           const float* ks, const float* vs, int64_t s_sp, int64_t s_sb, int64_t s_sh, int block,
+                           const int32_t* block_tbl, int64_t s_bt, int max_pages, int n_pages,
+                           const int32_t* ctx_len, void* out, int64_t s_ob, int64_t s_ot, int64_t s_oh,
+                           int B_grid, int n_seqs, int q_len, int ql_grid, int H, int H_KV, int D, int PAGE, int QPP,
+                           float sm_scale, const int32_t* plan, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Append to a paged cache with block scales (no reference counterpart): the new tokens' K/V quantised
+ * into the pages that specq_paged_attn_block reads.  Tokens, tables and plan as specq_kv_append_int8.
+ * A block that new tokens reach gets s' = max(amax, 1e-8) / Q over them (Q = 127 for int8, 448 for
+ * e4m3), or its present scale where that is larger and the block holds earlier tokens of the sequence;
+ * codes are rne(x / s'), earlier codes rne(c s / s') where s' > s.  fp32, IEEE division.  Infinities
+ * count as +-65504, NaN as 0.  Slots that hold no token of the sequence are not written.  A page may be
+ * written for one sequence only.
+ *   D must be 64, 128 or 256; cache rows 8-byte, new rows 16-byte aligned.
+ * ------------------------------------------------------------------------------------- */
+int specq_kv_append_block(const void* k_new, const void* v_new, int64_t s_nb, int64_t s_nt, int64_t s_nh,
+                          void* kc, void* vc, int code_fp8, int64_t s_kp, int64_t s_ko, int64_t s_kh,
+                          float* ks, float* vs, int64_t s_sp, int64_t s_sb, int64_t s_sh, int block,
+                          const int32_t* block_tbl, int64_t s_bt, int max_pages, int n_pages,
+                          const int32_t* ctx_len, int B_grid, int n_seqs, int q_len, int ql_grid,
+                          int H_KV, int D, int PAGE, const int32_t* plan, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Rotary positions (no reference counterpart): pair j of the first R of D dimensions -- (j, j + R/2),
+ * or (2j, 2j + 1) with interleaved -- is turned by pos * inv_freq[j] and scaled by mscale; the other
+ * dimensions are copied.  Angles are formed in fp64, everything else in fp32 with one rounding.
+ *   q, q_out  fp16 [B_grid, ql_grid, H, D], strides of their own (d contiguous); outputs may be the inputs
+ *   k, k_out  fp16 [B_grid, ql_grid, H_KV, D], or NULL with H_KV = 0
+ *   inv_freq  fp32 or (freq_fp64) fp64 [R / 2];  R even, R <= D <= 512
+ *   ctx_len   int32 [B_grid]: token i of sequence b is at ctx_len[b] - q_len + i; or, where not NULL,
+ *   positions int32 [B_grid, ql_grid], row stride s_pb
+ *   plan      NULL, or device int32*: plan[0] = n_seqs, plan[1] = q_len.  Inactive tokens are not written.
+ * ------------------------------------------------------------------------------------- */
+int specq_rotary(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh,
+                 const void* k, int64_t s_kb, int64_t s_kt, int64_t s_kh,
+                 void* q_out, int64_t s_qob, int64_t s_qot, int64_t s_qoh,
+                 void* k_out, int64_t s_kob, int64_t s_kot, int64_t s_koh,
+                 const void* inv_freq, int freq_fp64, float mscale,
+                 const int32_t* ctx_len, const int32_t* positions, int64_t s_pb,
+                 int B_grid, int n_seqs, int q_len, int ql_grid, int H, int H_KV, int D, int R,
+                 int interleaved, const int32_t* plan, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Page tables of a paged cache (no reference counterpart), changed in place on the device:
+ *   block_tbl int32 [B, max_pages], row stride s_bt; an id outside [0, n_pages) is no page
+ *   ref       int32 [n_pages]: how often the tables name each page; <= 0 is free
+ * Pages are handed out lowest id first, in the table's order; what cannot be had is -1, and
+ * shortage[0] counts it.
+ *   reserve   entries of row b's first ceil(lens[b] / PAGE) columns that name no page get one (ref 1)
+ *   free      entries past row b's first ceil(keep[b] / PAGE) columns become -1, their pages' ref falls
+ *   fork      row b becomes a copy of row parent[b] (outside [0, B): empty), lens[b] that row's length.
+ *             Full pages are shared; of the rows with one parent the lowest keeps its partly filled
+ *             last page and the others get a copy of it in every page tensor
+ *   compact   with n pages in use, the i-th of them at or past n moves to the i-th free page below n,
+ *             in every page tensor, in ref and in block_tbl; page_map[n_pages] gives each page's id
+ *   copy      pages src[i] -> dst[i]; destinations distinct and none a source; ids outside the pool skip
+ *             the pair
+ * Page tensors: n_tensors base pointers, page strides and page sizes in bytes (host arrays, read during
+ * the call).  Workspace: specq_kv_pages_workspace_size() bytes, as the workspaces above. */
+size_t specq_kv_pages_workspace_size(int B, int max_pages, int n_pages);
+int specq_kv_pages_reserve(int32_t* block_tbl, int64_t s_bt, int B, int max_pages, int32_t* ref, int n_pages,
+                           const int32_t* lens, int PAGE, int32_t* shortage,
+                           void* workspace, size_t workspace_bytes, void* stream);
+int specq_kv_pages_free(int32_t* block_tbl, int64_t s_bt, int B, int max_pages, int32_t* ref, int n_pages,
+                        const int32_t* keep, int PAGE, void* stream);
+int specq_kv_pages_fork(int32_t* block_tbl, int64_t s_bt, int B, int max_pages, int32_t* ref, int n_pages,
+                        int32_t* lens, const int32_t* parent, int PAGE, int n_tensors, void* const* base,
+                        const int64_t* page_stride, const int64_t* page_bytes, int32_t* shortage,
+                        void* workspace, size_t workspace_bytes, void* stream);
+int specq_kv_pages_compact(int32_t* block_tbl, int64_t s_bt, int B, int max_pages, int32_t* ref, int n_pages,
+                           int32_t* page_map, int n_tensors, void* const* base, const int64_t* page_stride,
+                           const int64_t* page_bytes, void* workspace, size_t workspace_bytes, void* stream);
+int specq_kv_pages_copy(const int32_t* src, const int32_t* dst, int n, int n_pages, int n_tensors, void* const* base,
+                        const int64_t* page_stride, const int64_t* page_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Elementwise steps around the GEMMs of a verification layer.
  * specq_silu_mul: h[m, n] = fp16( silu(float(gate[m,n])) * float(up[m,n]) ), m < M.
  *   No reference counterpart (the reference's graph stack has no MLP activation,
@@ -341,7 +432,8 @@ int specq_silu_mul_quant_int8(const void* gate, int64_t ld_gate, const void* up,
  * compiled-kernel metadata ck.n_regs / ck.n_spills / ck.metadata.shared, regs.py:29-32).
  * kind: 0 = W8A8 (weight layout in `variant`: 0 row-major, 1 packed, 2 the packed INT4 weight
  * of W4A8), 1 = W4A16 (layout in
- * `variant`), 2 = paged attention (D in `variant`, | 1 << 16 for fp32 K/V scales).  For the GEMMs, `variant` | 16 describes a
+ * `variant`), 2 = paged attention (D in `variant`, | 1 << 16 for fp32 K/V scales, | 1 << 17 / 1 << 18 for
+ * int8 / e4m3 caches with block scales).  For the GEMMs, `variant` | 16 describes a
  * call made with a plan (m_grid is then grid_m_max); a plan-mode GEMM call with automatic
  * tiles reports the tiling it runs when the active M is m_grid.  `variant` | 32 (GEMMs): the best
  * tile that explicit block_m, block_n and split_k can name.  An eager call of many rows with

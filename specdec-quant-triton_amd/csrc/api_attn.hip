@@ -1,4 +1,5 @@
-// C ABI for the INT8 paged verification attention: validation, grid, workspace and launch.
+// C ABI for the paged verification attention over INT8 caches with per-token scales and over int8 /
+// e4m3 caches with block scales: validation, grid, workspace and launch.
 #include <algorithm>
 #include <atomic>
 
@@ -14,6 +15,8 @@ std::atomic<int> g_attn_target{0};
 
 const void* attn_plan_fn_d64(int rb_max, int fp32);   // attn_plan_d64.hip
 const void* attn_plan_fn_d128(int rb_max, int fp32);  // attn_plan_d128.hip
+const void* attn_block_fn_d64(int rb, int f8, int plan);   // attn_block_d64.hip
+const void* attn_block_fn_d128(int rb, int f8, int plan);  // attn_block_d128.hip
 
 namespace {
 
@@ -32,10 +35,15 @@ const void* attn_fn_d(int rb, int fp32) {
   return nullptr;
 }
 
-const void* attn_fn(int D, int rb, int fp32) {
-  if (D == 128) return attn_fn_d<128>(rb, fp32);
-  if (D == 64) return attn_fn_d<64>(rb, fp32);
-  return nullptr;
+// Cache kinds: per-token fp16 / fp32 scales on int8, block scales on int8 / e4m3.
+enum { kTokF16 = 0, kTokF32 = 1, kBlkI8 = 2, kBlkF8 = 3 };
+
+// The eager kernel of rb row blocks, or (plan) the one that takes its row blocks from the active q_len.
+const void* attn_fn(int D, int rb, int kind, bool plan) {
+  if (D != 64 && D != 128) return nullptr;
+  if (kind >= kBlkI8) return D == 128 ? attn_block_fn_d128(rb, kind - kBlkI8, plan) : attn_block_fn_d64(rb, kind - kBlkI8, plan);
+  if (plan) return D == 128 ? attn_plan_fn_d128(rb, kind) : attn_plan_fn_d64(rb, kind);
+  return D == 128 ? attn_fn_d<128>(rb, kind) : attn_fn_d<64>(rb, kind);
 }
 
 // grid.x: the splits of a block table of max_pages * PAGE tokens when at least `pairs_min`
@@ -48,18 +56,21 @@ int n_splits_for(int max_pages, int PAGE, int pairs_min, int target) {
 
 }  // namespace
 
-// `variant` is the head dim, | kAttrsScaleFp32 for fp32 K/V scales.
+// `variant` is the head dim, | kAttrsScaleFp32 for fp32 K/V scales, | kAttrsBlockI8 / kAttrsBlockF8 for
+// block-scaled caches.
 int attn_attrs(int variant, int rows, specq_kernel_attrs* out) {
-  const bool fp32 = (variant & kAttrsScaleFp32) != 0;
-  const int D = variant & ~kAttrsScaleFp32;
+  const int kind = (variant & kAttrsBlockI8) ? kBlkI8 : (variant & kAttrsBlockF8) ? kBlkF8
+                   : (variant & kAttrsScaleFp32) ? kTokF32 : kTokF16;
+  const int D = variant & ~(kAttrsScaleFp32 | kAttrsBlockI8 | kAttrsBlockF8);
   SPECQ_REQUIRE(rows >= 1 && rows <= 64, SPECQ_ENOTSUP, "paged_attn: %d packed rows (1..64 supported)", rows);
   const int rb = ceil_div(rows, 16);
-  const void* fn = attn_fn(D, rb, fp32 ? 1 : 0);
+  const void* fn = attn_fn(D, rb, kind, false);
   SPECQ_REQUIRE(fn != nullptr, SPECQ_ENOTSUP, "paged_attn: head_dim %d not supported", D);
   hipFuncAttributes fa;
   if (hipFuncGetAttributes(&fa, fn) != hipSuccess) return fail(SPECQ_EIO, "paged_attn: hipFuncGetAttributes failed");
+  static const char* const kNames[] = {"_Float16", "float", "specq::BlockI8", "specq::BlockF8"};
   // The name carries the template arguments exactly as profilers print the kernel symbol.
-  snprintf(out->name, sizeof(out->name), "specq::paged_attn_kernel<%d, %d, %s>", D, rb, fp32 ? "float" : "_Float16");
+  snprintf(out->name, sizeof(out->name), "specq::paged_attn_kernel<%d, %d, %s>", D, rb, kNames[kind]);
   out->num_regs = fa.numRegs;
   out->lds_bytes = (int)fa.sharedSizeBytes;
   out->scratch_bytes = (int)fa.localSizeBytes;
@@ -89,14 +100,13 @@ extern "C" size_t specq_paged_attn_workspace_size(int B_grid, int H, int H_KV, i
   return kCounterBytes + align_up(part, 256);
 }
 
-extern "C" int specq_paged_attn(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh, const int8_t* kc,
-                                const int8_t* vc, int64_t s_kp, int64_t s_ko, int64_t s_kh, const void* ks,
-                                const void* vs, int64_t s_sp, int64_t s_so, int64_t s_sh, int scale_fp32,
-                                const int32_t* block_tbl, int64_t s_bt, int max_pages, int n_pages,
-                                const int32_t* ctx_len,
-                                void* out, int64_t s_ob, int64_t s_ot, int64_t s_oh, int B_grid, int n_seqs,
-                                int q_len, int ql_grid, int H, int H_KV, int D, int PAGE, int QPP, float sm_scale,
-                                const int32_t* plan, void* workspace, size_t workspace_bytes, void* stream) {
+// Both entry points: `kind` is the cache's, `sb` its tokens per scale block (block scales only).
+static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh, const void* kc, const void* vc,
+                     int64_t s_kp, int64_t s_ko, int64_t s_kh, const void* ks, const void* vs, int64_t s_sp,
+                     int64_t s_so, int64_t s_sh, int sb, const int32_t* block_tbl, int64_t s_bt, int max_pages,
+                     int n_pages, const int32_t* ctx_len, void* out, int64_t s_ob, int64_t s_ot, int64_t s_oh,
+                     int B_grid, int n_seqs, int q_len, int ql_grid, int H, int H_KV, int D, int PAGE, int QPP,
+                     float sm_scale, const int32_t* plan, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   SPECQ_REQUIRE(q && kc && vc && ks && vs && block_tbl && ctx_len && out, SPECQ_EINVAL,
                 "paged_attn: null tensor pointer");
@@ -129,9 +139,7 @@ extern "C" int specq_paged_attn(const void* q, int64_t s_qb, int64_t s_qt, int64
   const int rb = ceil_div(QPP * G, 16);
   // Plan mode with more than one row block runs the launch that sizes its programs to the
   // active q_len on the device (the rows of a program whose queries are inactive do nothing).
-  const void* fn = plan != nullptr && rb > 1
-                       ? (D == 128 ? attn_plan_fn_d128(rb, scale_fp32 ? 1 : 0) : attn_plan_fn_d64(rb, scale_fp32 ? 1 : 0))
-                       : attn_fn(D, rb, scale_fp32 ? 1 : 0);
+  const void* fn = attn_fn(D, rb, kind, plan != nullptr && rb > 1);
   SPECQ_REQUIRE(fn != nullptr, SPECQ_ENOTSUP, "paged_attn: no kernel for D=%d rows=%d", D, QPP * G);
   const int n_qc = ceil_div(plan ? ql_grid : q_len, QPP);
   if (n_qc == 0) return SPECQ_OK;
@@ -162,7 +170,7 @@ extern "C" int specq_paged_attn(const void* q, int64_t s_qb, int64_t s_qt, int64
   SPECQ_REQUIRE(wgs <= INT32_MAX, SPECQ_ENOTSUP, "paged_attn: grid too large");
   AttnParams p;
   p.q = (const _Float16*)q; p.s_qb = s_qb; p.s_qt = s_qt; p.s_qh = s_qh;
-  p.kc = kc; p.vc = vc; p.s_kp = s_kp; p.s_ko = s_ko; p.s_kh = s_kh;
+  p.kc = (const int8_t*)kc; p.vc = (const int8_t*)vc; p.s_kp = s_kp; p.s_ko = s_ko; p.s_kh = s_kh;
   p.ks = ks; p.vs = vs; p.s_sp = s_sp; p.s_so = s_so; p.s_sh = s_sh;
   p.bt = block_tbl; p.s_bt = s_bt; p.max_pages = max_pages; p.n_pages = n_pages; p.ctx_len = ctx_len;
   p.out = (_Float16*)out; p.s_ob = s_ob; p.s_ot = s_ot; p.s_oh = s_oh;
@@ -172,6 +180,7 @@ extern "C" int specq_paged_attn(const void* q, int64_t s_qb, int64_t s_qt, int64
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.counters = need ? (int32_t*)workspace : nullptr;
   p.part = need ? (float*)((char*)workspace + kCounterBytes) : nullptr;
+  p.sb = sb;
   diag_timeline(&p.tl, &p.tl_cap);
   void* args[] = {&p};
   hipError_t e = hipLaunchKernel(fn, dim3((unsigned)wgs), dim3(kAttnThreads), args, 0, (hipStream_t)stream);
@@ -180,4 +189,35 @@ extern "C" int specq_paged_attn(const void* q, int64_t s_qb, int64_t s_qt, int64
     return SPECQ_EIO;
   }
   return SPECQ_OK;
+}
+
+extern "C" int specq_paged_attn(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh, const int8_t* kc,
+                                const int8_t* vc, int64_t s_kp, int64_t s_ko, int64_t s_kh, const void* ks,
+                                const void* vs, int64_t s_sp, int64_t s_so, int64_t s_sh, int scale_fp32,
+                                const int32_t* block_tbl, int64_t s_bt, int max_pages, int n_pages,
+                                const int32_t* ctx_len,
+                                void* out, int64_t s_ob, int64_t s_ot, int64_t s_oh, int B_grid, int n_seqs,
+                                int q_len, int ql_grid, int H, int H_KV, int D, int PAGE, int QPP, float sm_scale,
+                                const int32_t* plan, void* workspace, size_t workspace_bytes, void* stream) {
+  return attn_call(scale_fp32 ? kTokF32 : kTokF16, q, s_qb, s_qt, s_qh, kc, vc, s_kp, s_ko, s_kh, ks, vs, s_sp, s_so,
+                   s_sh, 0, block_tbl, s_bt, max_pages, n_pages, ctx_len, out, s_ob, s_ot, s_oh, B_grid, n_seqs, q_len,
+                   ql_grid, H, H_KV, D, PAGE, QPP, sm_scale, plan, workspace, workspace_bytes, stream);
+}
+
+extern "C" int specq_paged_attn_block(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh, const void* kc,
+                                      const void* vc, int code_fp8, int64_t s_kp, int64_t s_ko, int64_t s_kh,
+                                      const float* ks, const float* vs, int64_t s_sp, int64_t s_sb, int64_t s_sh,
+                                      int block, const int32_t* block_tbl, int64_t s_bt, int max_pages, int n_pages,
+                                      const int32_t* ctx_len, void* out, int64_t s_ob, int64_t s_ot, int64_t s_oh,
+                                      int B_grid, int n_seqs, int q_len, int ql_grid, int H, int H_KV, int D, int PAGE,
+                                      int QPP, float sm_scale, const int32_t* plan, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  clear_error();
+  SPECQ_REQUIRE(block > 0 && block % 16 == 0 && PAGE > 0 && PAGE % block == 0, SPECQ_ENOTSUP,
+                "paged_attn_block: block=%d must be a multiple of 16 that divides PAGE=%d", block, PAGE);
+  SPECQ_REQUIRE((uintptr_t)ks % 4 == 0 && (uintptr_t)vs % 4 == 0 && s_sp >= 0 && s_sb >= 0 && s_sh >= 0, SPECQ_EINVAL,
+                "paged_attn_block: bad scale pointer or strides");
+  return attn_call(code_fp8 ? kBlkF8 : kBlkI8, q, s_qb, s_qt, s_qh, kc, vc, s_kp, s_ko, s_kh, ks, vs, s_sp, s_sb, s_sh,
+                   block, block_tbl, s_bt, max_pages, n_pages, ctx_len, out, s_ob, s_ot, s_oh, B_grid, n_seqs, q_len,
+                   ql_grid, H, H_KV, D, PAGE, QPP, sm_scale, plan, workspace, workspace_bytes, stream);
 }

@@ -37,6 +37,8 @@ constexpr int kAttrsPlan = 16;
 constexpr int kAttrsStreaming = 32;
 // Flag in the `variant` of an attention resource query: fp32 K/V scales (else fp16).
 constexpr int kAttrsScaleFp32 = 1 << 16;
+// ... or a cache with block scales, of int8 or e4m3 codes.
+constexpr int kAttrsBlockI8 = 1 << 17, kAttrsBlockF8 = 1 << 18;
 
 // Every workspace starts with a fixed counter region (zero between calls), then scratch.
 constexpr size_t kCounterBytes = 256 * 1024;

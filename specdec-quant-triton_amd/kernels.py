@@ -17,7 +17,10 @@ and the steps either side of them on the device: paged_kv_append (the new tokens
 quantised into the cache pages, the q8 of kernels.py:280-284), silu_mul /
 silu_mul_quant_int8 / quantize_act_int8_gpu (kernels.py:58-62 on the device), and
 w4a8_matmul (INT4 weights on the INT8 MFMA path, the reference's REPORT.md:156
-recommendation; no reference kernel).
+recommendation; no reference kernel).  Without a reference counterpart: rotary_embed (positions
+of q and k), paged_kv_append_block_scaled and paged_attention_block_scaled (an int8 or e4m3
+cache with one scale for each block of tokens and head), and the cache's page tables,
+paged_kv_reserve / _free / _fork / _compact / _copy.
 
 Every launcher takes `plan` (an int32 device tensor read by the kernel at run time) and a
 fixed grid size, so a single captured graph replays every (B, k) (reference kernels.py:14-17).
@@ -71,6 +74,8 @@ __all__ = [
     "pack_int4_i32", "KernelInfo", "PackedWeightInt8", "pack_weight_int8", "PackedWeightInt4", "pack_weight_int4",
     "w4a8_matmul", "quantize_weight_int4_channel", "PackedWeightW4A8", "pack_weight_w4a8",
     "w8a8_matmul_grouped", "w4a16_matmul_grouped", "set_weight_pack_cache", "clear_weight_pack_cache",
+    "rotary_embed", "rotary_inv_freq", "paged_kv_append_block_scaled", "paged_attention_block_scaled",
+    "paged_kv_reserve", "paged_kv_free", "paged_kv_fork", "paged_kv_compact", "paged_kv_copy",
 ]
 
 
@@ -996,3 +1001,404 @@ def w4a8_matmul(a_q, sa, wq, sw, out=None, BLOCK_M=16, BLOCK_N=None, BLOCK_K=128
               wptr, wbytes, _stream_ptr(a_q))
     _w8a8_kernel._note(a_q.device.index or 0, (bm, bn, nw, "w4a8"))
     return out, KernelInfo(0, 2 | (16 if plan is not None else 0), m_grid, N, K, bm, bn, nw, split_k)
+
+
+# ----------------------------------------------------------------------------------------
+# Rotary positions, and the paged cache with block scales (no reference counterpart)
+# ----------------------------------------------------------------------------------------
+class _Here:
+    """Context of a call whose tensors live on the current device: nothing to switch."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE_CTX = _Here()
+
+
+def _on_one_device(who: str, *ts):
+    """All tensors (None left out) on one GPU; the context that makes it the current one, so that the
+    launch and the CU count are that GPU's."""
+    dev = ts[0].device
+    if dev.type != "cuda":
+        raise RuntimeError(f"specq kernels run on the GPU only; got a {dev} tensor")
+    for t in ts[1:]:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{who}: tensors on {dev} and {t.device}")
+    return _HERE_CTX if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _raw_stream(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def _plan_of(plan, need: int, who: str) -> int:
+    if plan is None:
+        return 0
+    if plan.dtype != torch.int32 or plan.numel() < need or plan.stride(-1) != 1:
+        raise RuntimeError(f"{who}: plan must be an int32 device tensor of at least {need} entries")
+    return plan.data_ptr()
+
+
+def _token_grid(who: str, B: int, QL: int, q_len, n_seqs, plan):
+    """(sequences and tokens of the grid, n_seqs, q_len) of a call on [B, QL, ...] tensors."""
+    q_len = QL if q_len is None else int(q_len)
+    n_seqs = B if n_seqs is None else int(n_seqs)
+    if not (0 <= n_seqs <= B and 0 <= q_len <= QL):
+        raise RuntimeError(f"{who}: need 0 <= n_seqs <= {B} and 0 <= q_len <= {QL}")
+    return (B, QL, n_seqs, q_len) if plan is not None else (n_seqs, q_len, n_seqs, q_len)
+
+
+def _int32_vec(who: str, name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < n or (t.stride(0) != 1 and t.shape[0] > 1):
+        raise RuntimeError(f"{who}: {name} must be a contiguous int32 vector of at least {n} entries")
+
+
+def rotary_inv_freq(dim: int, base: float = 10000.0, scaling=None, factor: float = 1.0, original_len: int = 8192,
+                    low_freq_factor: float = 1.0, high_freq_factor: float = 4.0, beta_fast: float = 32.0,
+                    beta_slow: float = 1.0, device="cuda"):
+    """(inv_freq fp64 [dim / 2], mscale) for rotary_embed: f_j = base^(-2j / dim), stretched for long contexts.
+
+    scaling: None; "linear" (f / factor); "ntk" (base * factor^(dim / (dim - 2))); "wavelength" (waves longer
+    than original_len / low_freq_factor divided by factor, those shorter than original_len / high_freq_factor
+    kept, a blend between); "yarn" (f / factor for pairs that turn less than beta_slow times in original_len
+    tokens, f for those above beta_fast, a ramp over the pair's index between; mscale 0.1 ln(factor) + 1).
+    """
+    dim = int(dim)
+    if dim < 2 or dim % 2:
+        raise RuntimeError(f"rotary_inv_freq: dim={dim} must be even and at least 2")
+    if not (base > 1 and factor > 0 and original_len > 0):
+        raise RuntimeError("rotary_inv_freq: need base > 1, factor > 0 and original_len > 0")
+    if scaling == "ntk":
+        if dim == 2:
+            raise RuntimeError("rotary_inv_freq: \"ntk\" needs dim > 2")
+        base = base * factor ** (dim / (dim - 2))
+    f = torch.tensor([base ** (-2.0 * j / dim) for j in range(dim // 2)], dtype=torch.float64)
+    mscale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "wavelength":
+        if not high_freq_factor > low_freq_factor:
+            raise RuntimeError("rotary_inv_freq: high_freq_factor must exceed low_freq_factor")
+        turns = original_len * f / (2 * math.pi)
+        keep = ((turns - low_freq_factor) / (high_freq_factor - low_freq_factor)).clamp(0, 1)
+        f = f * keep + f / factor * (1 - keep)
+    elif scaling == "yarn":
+        index = lambda turns: dim * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+        lo, hi = max(math.floor(index(beta_fast)), 0), min(math.ceil(index(beta_slow)), dim // 2 - 1)
+        ramp = ((torch.arange(dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        f = f / factor * ramp + f * (1 - ramp)
+        mscale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif scaling not in (None, "ntk"):
+        raise RuntimeError(f"rotary_inv_freq: unknown scaling {scaling!r}")
+    return f.to(device), mscale
+
+
+def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, interleaved=False, mscale=1.0, plan=None,
+                 n_seqs=None, q_out=None, k_out=None):
+    """Rotary positions of the new tokens' q and k; returns (q_out, k_out).
+
+    q fp16 [B, QL, H, D], k fp16 [B, QL, H_KV, D] or None; inv_freq fp32 or fp64 [R / 2], R <= D <= 512
+    (rotary_inv_freq).  Pair j of the first R dimensions -- (j, j + R/2), or (2j, 2j + 1) with
+    interleaved -- is turned by pos * inv_freq[j] and scaled by mscale; the other dimensions are copied.
+    Token i of sequence b is at ctx_len[b] - q_len + i (ctx_len counts the new tokens, as the K/V append
+    and the attention have it), or at positions[b, i] (int32 [B, QL]).  Angles are formed in fp64.
+    Outputs may be the inputs (in place); they must not overlap them otherwise.  With `plan`,
+    (n_seqs, q_len) = plan[0:2] on the device and the grid covers (B, QL).  Tokens that are not active
+    are not written (an omitted output holds anything there).
+    """
+    who = "rotary_embed"
+    ctx = _on_one_device(who, q, k, inv_freq, ctx_len, positions, plan, q_out, k_out)
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+        raise RuntimeError(f"{who}: q [B, QL, H, D] and k [B, QL, H_KV, D] expected")
+    B, QL, H, D = q.shape
+    q_out = torch.empty_like(q) if q_out is None else q_out
+    if k is None:
+        H_KV = 0
+        if k_out is not None:
+            raise RuntimeError(f"{who}: k_out without k")
+    else:
+        H_KV = k.shape[2]
+        k_out = torch.empty_like(k) if k_out is None else k_out
+    for x, y in ((q, q_out), (k, k_out)):
+        if x is None:
+            continue
+        if x.dtype != torch.float16 or y.dtype != torch.float16 or x.shape != y.shape:
+            raise RuntimeError(f"{who}: inputs and outputs must be fp16 of one shape")
+        if D > 1 and (x.stride(3) != 1 or y.stride(3) != 1):
+            raise RuntimeError(f"{who}: head_dim must be contiguous")
+    if inv_freq.dtype not in (torch.float32, torch.float64) or inv_freq.dim() != 1 or \
+            (inv_freq.stride(0) != 1 and inv_freq.shape[0] > 1):
+        raise RuntimeError(f"{who}: inv_freq must be a contiguous fp32 or fp64 vector")
+    R = 2 * inv_freq.shape[0]
+    Bg, Qg, n_seqs, q_len = _token_grid(who, B, QL, q_len, n_seqs, plan)
+    s_pb = 0
+    if positions is not None:
+        if positions.dtype != torch.int32 or positions.dim() != 2 or positions.shape[0] < Bg or \
+                positions.shape[1] < Qg or (positions.stride(1) != 1 and positions.shape[1] > 1):
+            raise RuntimeError(f"{who}: positions must be int32 [B, QL] with unit inner stride")
+        s_pb = positions.stride(0)
+    elif ctx_len is not None:
+        _int32_vec(who, "ctx_len", ctx_len, Bg)
+    else:
+        raise RuntimeError(f"{who}: ctx_len or positions must be given")
+    if Bg == 0 or Qg == 0:
+        return q_out, k_out
+    qs, qo = q.stride(), q_out.stride()
+    ks, ko = (k.stride(), k_out.stride()) if k is not None else ((0, 0, 0), (0, 0, 0))
+    with ctx:
+        _lib.call("specq_rotary", q.data_ptr(), qs[0], qs[1], qs[2], _ptr(k), ks[0], ks[1], ks[2],
+                  q_out.data_ptr(), qo[0], qo[1], qo[2], _ptr(k_out), ko[0], ko[1], ko[2],
+                  inv_freq.data_ptr(), 1 if inv_freq.dtype == torch.float64 else 0, float(mscale),
+                  _ptr(ctx_len), _ptr(positions), s_pb, Bg, n_seqs, q_len, Qg, H, H_KV, D, R,
+                  1 if interleaved else 0, _plan_of(plan, 2, who), _raw_stream(q))
+    return q_out, k_out
+
+
+def _block_cache(who: str, kc, vc, ks, vs, block_tbl, ctx_len, seqs: int, H_KV: int, D: int):
+    """Checks a block-scaled cache for `seqs` sequences; returns (e4m3 codes, tokens per block)."""
+    if kc.dtype != vc.dtype or kc.dtype not in (torch.int8, torch.float8_e4m3fn):
+        raise RuntimeError(f"{who} expects int8 or float8_e4m3fn K/V caches of one type")
+    if kc.dim() != 4 or kc.shape != vc.shape or kc.stride() != vc.stride() or kc.stride(3) != 1:
+        raise RuntimeError(f"{who}: K/V caches must share a layout [pages, PAGE, H_KV, D] with contiguous head_dim")
+    if kc.shape[2] != H_KV or kc.shape[3] != D:
+        raise RuntimeError(f"{who}: cache {tuple(kc.shape)} does not fit {H_KV} K/V heads of {D}")
+    P, PAGE = kc.shape[0], kc.shape[1]
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.dim() != 3 or ks.shape != vs.shape or \
+            ks.stride() != vs.stride():
+        raise RuntimeError(f"{who}: scales must be fp32 [pages, blocks, H_KV] of one layout")
+    NB = ks.shape[1]
+    if ks.shape[0] != P or ks.shape[2] != H_KV or NB < 1 or PAGE % NB or (PAGE // NB) % 16:
+        raise RuntimeError(f"{who}: scales {tuple(ks.shape)} must be [{P}, blocks, {H_KV}] with blocks of a multiple "
+                           f"of 16 of the page's {PAGE} tokens")
+    if block_tbl.dtype != torch.int32 or block_tbl.dim() != 2 or block_tbl.shape[0] < seqs or \
+            (block_tbl.stride(1) != 1 and block_tbl.shape[1] > 1):
+        raise RuntimeError(f"{who}: block_tbl must be int32 [B, max_pages] with unit inner stride for {seqs} sequences")
+    _int32_vec(who, "ctx_len", ctx_len, seqs)
+    return kc.dtype == torch.float8_e4m3fn, PAGE // NB
+
+
+def paged_kv_append_block_scaled(k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_len, q_len=None, plan=None, n_seqs=None):
+    """Quantise the new tokens' K/V into a paged cache with block scales, in place.
+
+    k_new, v_new fp16 [B, QLMAX, H_KV, D], D 64, 128 or 256; kc/vc int8 or float8_e4m3fn [pages, PAGE,
+    H_KV, D]; ks/vs fp32 [pages, PAGE / SB, H_KV], one scale for each block of SB tokens (a multiple of
+    16) and head; block_tbl int32 [B, max_pages]; ctx_len int32 [B], counting the new tokens.  A block
+    that new tokens reach gets s' = max(amax, 1e-8) / Q (Q = 127 or 448) over them, or its present
+    scale where that is larger and the block holds earlier tokens of the sequence; the new codes are
+    rne(x / s'), and where the scale grows the earlier codes become rne(c * s / s').  Infinities count
+    as +-65504, NaN as 0.  Tokens at positions below zero, past the table or on a page outside the pool
+    are skipped, every other slot keeps what it holds.  A page that the call writes must belong to one
+    sequence only (paged_kv_fork sees to that).  With `plan`, (n_seqs, q_len) = plan[0:2] on the device
+    and the grid covers (B, QLMAX).
+    """
+    who = "paged_kv_append_block_scaled"
+    ctx = _on_one_device(who, k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_len, plan)
+    if k_new.dim() != 4 or v_new.shape != k_new.shape:
+        raise RuntimeError(f"{who}: k_new and v_new must have one shape [B, QLMAX, H_KV, D]")
+    if k_new.dtype != torch.float16 or v_new.dtype != torch.float16:
+        raise RuntimeError(f"{who} expects fp16 k_new and v_new")
+    B, QL, H_KV, D = k_new.shape
+    Bg, Qg, n_seqs, q_len = _token_grid(who, B, QL, q_len, n_seqs, plan)
+    f8, sb = _block_cache(who, kc, vc, ks, vs, block_tbl, ctx_len, Bg, H_KV, D)
+    if k_new.stride() != v_new.stride() or k_new.stride(3) != 1:
+        k_new, v_new = k_new.contiguous(), v_new.contiguous()
+    if Bg == 0 or Qg == 0:
+        return
+    kn, cs, ss = k_new.stride(), kc.stride(), ks.stride()
+    with ctx:
+        _lib.call("specq_kv_append_block", k_new.data_ptr(), v_new.data_ptr(), kn[0], kn[1], kn[2],
+                  kc.data_ptr(), vc.data_ptr(), 1 if f8 else 0, cs[0], cs[1], cs[2],
+                  ks.data_ptr(), vs.data_ptr(), ss[0], ss[1], ss[2], sb,
+                  block_tbl.data_ptr(), block_tbl.stride(0), block_tbl.shape[1], min(kc.shape[0], 2**31 - 1),
+                  ctx_len.data_ptr(), Bg, n_seqs, q_len, Qg, H_KV, D, kc.shape[1], _plan_of(plan, 2, who),
+                  _raw_stream(k_new))
+
+
+def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=None, QPP=None, plan=None, n_seqs=None,
+                                 out=None, sm_scale=None, workspace=None):
+    """Verification attention over a paged cache with block scales.  Returns (out, ck).
+
+    q fp16 [B, QLMAX, H, D], D 64 or 128; kc/vc int8 or float8_e4m3fn [pages, PAGE, H_KV, D]; ks/vs fp32
+    [pages, PAGE / SB, H_KV] (paged_kv_append_block_scaled); block_tbl int32 [B, max_pages]; ctx_len
+    int32 [B], counting the q_len new tokens, which are each sequence's last ones and see one another
+    causally.  Block-table ids outside [0, pages) mask their page's tokens; a row that sees no token
+    gives 0.  QPP query tokens run in one program, at most 64 rows of H / H_KV heads each (default: as
+    many as fit).  sm_scale defaults to D^-1/2.  With `plan`, (n_seqs, q_len) = plan[0:2] on the device
+    and the grid covers (B, QLMAX); rows that are not active are not written (an omitted `out` is zero
+    there).  Calls that may run at the same time on several streams need a workspace each.
+    """
+    who = "paged_attention_block_scaled"
+    ctx = _on_one_device(who, q, kc, vc, ks, vs, block_tbl, ctx_len, plan, out)
+    if q.dim() != 4 or q.dtype != torch.float16 or q.stride(3) != 1:
+        raise RuntimeError(f"{who} expects fp16 q [B, QLMAX, H, D] with contiguous head_dim")
+    B, QL, H, D = q.shape
+    if kc.dim() != 4 or kc.shape[2] < 1 or H % kc.shape[2]:
+        raise RuntimeError(f"{who}: cache {tuple(kc.shape)} does not fit q {tuple(q.shape)}")
+    H_KV = kc.shape[2]
+    G = H // H_KV
+    Bg, Qg, n_seqs, q_len = _token_grid(who, B, QL, q_len, n_seqs, plan)
+    f8, sb = _block_cache(who, kc, vc, ks, vs, block_tbl, ctx_len, Bg, H_KV, D)
+    if QPP is None:
+        QPP = max(1, min(Qg, 64 // G))
+    elif int(QPP) < 1:
+        raise RuntimeError(f"{who}: QPP={QPP} must be at least 1")
+    if out is None:
+        out = torch.empty_like(q) if plan is None and n_seqs == B and q_len == QL else torch.zeros_like(q)
+    elif out.dtype != torch.float16 or out.shape != q.shape or out.stride(3) != 1:
+        raise RuntimeError(f"{who}: out must be fp16 of q's shape {tuple(q.shape)} with contiguous head_dim")
+    PAGE, max_pages = kc.shape[1], block_tbl.shape[1]
+    qs, cs, ss, os_ = q.stride(), kc.stride(), ks.stride(), out.stride()
+    QPP = int(QPP)
+    with ctx:
+        ck = KernelInfo(2, D | (1 << 18 if f8 else 1 << 17), 0, 0, 0, QPP * G, 0, 4, 0)
+        if Bg == 0 or Qg == 0:
+            return out, ck
+        need = _lib.lib().specq_paged_attn_workspace_size(Bg, H, H_KV, Qg, QPP, max_pages, PAGE)
+        wptr, wbytes = (workspace or _ws.shared(q.device)).ensure(need)
+        _lib.call("specq_paged_attn_block", q.data_ptr(), qs[0], qs[1], qs[2],
+                  kc.data_ptr(), vc.data_ptr(), 1 if f8 else 0, cs[0], cs[1], cs[2],
+                  ks.data_ptr(), vs.data_ptr(), ss[0], ss[1], ss[2], sb,
+                  block_tbl.data_ptr(), block_tbl.stride(0), max_pages, min(kc.shape[0], 2**31 - 1),
+                  ctx_len.data_ptr(), out.data_ptr(), os_[0], os_[1], os_[2],
+                  Bg, n_seqs, q_len, Qg, H, H_KV, D, PAGE, QPP,
+                  1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _plan_of(plan, 2, who),
+                  wptr, wbytes, _raw_stream(q))
+    _paged_attn_kernel._note(q.device.index, (D, (QPP * G + 15) // 16, str(kc.dtype)))
+    return out, ck
+
+
+# ----------------------------------------------------------------------------------------
+# Page tables of the paged caches
+# ----------------------------------------------------------------------------------------
+def _page_state(who: str, block_tbl, ref, *vecs):
+    """Checks the table, the counts and per-row vectors (name, tensor); returns (context, B, C, P)."""
+    ctx = _on_one_device(who, block_tbl, ref, *(t for _, t in vecs))
+    if block_tbl.dtype != torch.int32 or block_tbl.dim() != 2 or block_tbl.shape[0] < 1 or block_tbl.shape[1] < 1 or \
+            (block_tbl.stride(1) != 1 and block_tbl.shape[1] > 1):
+        raise RuntimeError(f"{who}: block_tbl must be int32 [B, max_pages] with unit inner stride")
+    if block_tbl.shape[0] > 1 and block_tbl.stride(0) < block_tbl.shape[1]:
+        raise RuntimeError(f"{who}: block_tbl rows overlap")
+    _int32_vec(who, "ref", ref, 1)
+    B, C = block_tbl.shape
+    for name, t in vecs:
+        _int32_vec(who, name, t, B)
+    return ctx, B, C, ref.shape[0]
+
+
+def _page_tensors(who: str, caches, pages: int, dev):
+    """ctypes arrays (count, base, page stride, page bytes) of the page tensors of a pool."""
+    base, stride, nbytes = [], [], []
+    for t in caches:
+        if t.device != dev:
+            raise RuntimeError(f"{who}: cache on {t.device}, table on {dev}")
+        if t.dim() < 1 or t.shape[0] != pages or t.numel() == 0 or not t[0].is_contiguous():
+            raise RuntimeError(f"{who}: a cache {tuple(t.shape)} must have {pages} pages, each contiguous")
+        size = t.element_size()
+        nbytes.append(t.numel() // pages * size)
+        stride.append(t.stride(0) * size if pages > 1 else nbytes[-1])
+        base.append(t.data_ptr())
+    n = len(base)
+    return n, (ctypes.c_void_p * n)(*base), (ctypes.c_int64 * n)(*stride), (ctypes.c_int64 * n)(*nbytes)
+
+
+def _pages_workspace(workspace, dev, B: int, C: int, P: int):
+    return (workspace or _ws.shared(dev)).ensure(_lib.lib().specq_kv_pages_workspace_size(B, C, P))
+
+
+def paged_kv_reserve(block_tbl, ref, lens, PAGE, shortage=None, workspace=None):
+    """Give the rows of a block table the pages that lens[b] tokens need, in place.
+
+    block_tbl int32 [B, max_pages]; ref int32 [pages], how often the tables name each page (<= 0: free);
+    lens int32 [B].  Entries of a row's first ceil(lens / PAGE) columns that name no page (an id outside
+    [0, pages)) get the lowest free page, in the table's order; ref of a page given becomes 1.  Where the
+    free pages run out, entries get -1.  Returns shortage, int32 [1]: how many pages are missing.
+    """
+    who = "paged_kv_reserve"
+    ctx, B, C, P = _page_state(who, block_tbl, ref, ("lens", lens))
+    shortage = torch.empty(1, dtype=torch.int32, device=ref.device) if shortage is None else shortage
+    _int32_vec(who, "shortage", shortage, 1)
+    with ctx:
+        wptr, wbytes = _pages_workspace(workspace, ref.device, B, C, P)
+        _lib.call("specq_kv_pages_reserve", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C,
+                  ref.data_ptr(), P, lens.data_ptr(), int(PAGE), shortage.data_ptr(), wptr, wbytes, _raw_stream(ref))
+    return shortage
+
+
+def paged_kv_free(block_tbl, ref, keep, PAGE):
+    """Let go of the pages past each row's first keep[b] tokens (0: the whole row), in place.
+
+    Entries past a row's first ceil(keep / PAGE) columns become -1, and ref of each page they named
+    falls by one; a page that no table names any more (ref 0) is free.
+    """
+    who = "paged_kv_free"
+    ctx, B, C, P = _page_state(who, block_tbl, ref, ("keep", keep))
+    with ctx:
+        _lib.call("specq_kv_pages_free", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C,
+                  ref.data_ptr(), P, keep.data_ptr(), int(PAGE), _raw_stream(ref))
+
+
+def paged_kv_fork(block_tbl, ref, lens, parent, caches, PAGE, shortage=None, workspace=None):
+    """Make row b a copy of row parent[b], in place: several samples of a prompt, a beam's survivors.
+
+    lens int32 [B], tokens each row holds, becomes lens[parent]; parent int32 [B], an id outside [0, B)
+    empties the row.  Rows share their parent's full pages.  Of the rows with one parent the lowest
+    keeps its partly filled last page, the others get a free page each (lowest first, in the order of the
+    rows) with a copy of it, in every tensor of `caches` ([pages, ...], each page contiguous; K, V and
+    scales of any number of layers).  ref follows; pages that no row names any more are free, and may be
+    given out by this very call.  Where the free pages run out a row's last entry is -1.  A row's pages
+    past its tokens are let go of.  Returns shortage, int32 [1]: how many pages are missing.
+    """
+    who = "paged_kv_fork"
+    ctx, B, C, P = _page_state(who, block_tbl, ref, ("lens", lens), ("parent", parent))
+    tensors = _page_tensors(who, caches, P, ref.device)
+    shortage = torch.empty(1, dtype=torch.int32, device=ref.device) if shortage is None else shortage
+    _int32_vec(who, "shortage", shortage, 1)
+    with ctx:
+        wptr, wbytes = _pages_workspace(workspace, ref.device, B, C, P)
+        _lib.call("specq_kv_pages_fork", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C,
+                  ref.data_ptr(), P, lens.data_ptr(), parent.data_ptr(), int(PAGE), *tensors, shortage.data_ptr(),
+                  wptr, wbytes, _raw_stream(ref))
+    return shortage
+
+
+def paged_kv_compact(block_tbl, ref, caches, page_map=None, workspace=None):
+    """Move the pages in use below their own number, in place; returns page_map.
+
+    With n pages in use (ref > 0), the i-th of them at or past n moves to the i-th free page below n:
+    its contents in every tensor of `caches`, its count, and its entries of block_tbl.  page_map int32
+    [pages] holds every page's id afterwards, for other holders of ids.
+    """
+    who = "paged_kv_compact"
+    ctx, B, C, P = _page_state(who, block_tbl, ref)
+    tensors = _page_tensors(who, caches, P, ref.device)
+    page_map = torch.empty(P, dtype=torch.int32, device=ref.device) if page_map is None else page_map
+    _int32_vec(who, "page_map", page_map, P)
+    with ctx:
+        wptr, wbytes = _pages_workspace(workspace, ref.device, B, C, P)
+        _lib.call("specq_kv_pages_compact", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C,
+                  ref.data_ptr(), P, page_map.data_ptr(), *tensors, wptr, wbytes, _raw_stream(ref))
+    return page_map
+
+
+def paged_kv_copy(src, dst, caches):
+    """Copy pages src[i] to dst[i] (int32 vectors) in every tensor of `caches` ([pages, ...]), in place.
+
+    The destinations must be distinct, and none of them a source.  Pairs with an id outside [0, pages)
+    are left out.
+    """
+    who = "paged_kv_copy"
+    if len(caches) == 0:
+        raise RuntimeError(f"{who}: no caches")
+    ctx = _on_one_device(who, src, dst)
+    n, P = src.numel(), caches[0].shape[0]
+    _int32_vec(who, "src", src, n)
+    _int32_vec(who, "dst", dst, n)
+    if dst.numel() != n:
+        raise RuntimeError(f"{who}: {n} sources and {dst.numel()} destinations")
+    tensors = _page_tensors(who, caches, P, src.device)
+    with ctx:
+        _lib.call("specq_kv_pages_copy", src.data_ptr(), dst.data_ptr(), n, P, *tensors, _raw_stream(src))

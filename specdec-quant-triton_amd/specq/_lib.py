@@ -89,6 +89,31 @@ SIGNATURES = {
     "specq_quantize_act_int8": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp]),
     "specq_silu_mul_quant_int8": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp,
                                            _c_int, _c_int, _c_int, _c_vp, _c_vp]),
+    "specq_paged_attn_block": (_c_int, [_c_vp, _c_i64, _c_i64, _c_i64,
+                                        _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_i64,
+                                        _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_int,
+                                        _c_vp, _c_i64, _c_int, _c_int, _c_vp,
+                                        _c_vp, _c_i64, _c_i64, _c_i64,
+                                        _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                        _c_int, _c_int, _c_float, _c_vp, _c_vp, _c_size, _c_vp]),
+    "specq_kv_append_block": (_c_int, [_c_vp, _c_vp, _c_i64, _c_i64, _c_i64,
+                                       _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_i64,
+                                       _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_int,
+                                       _c_vp, _c_i64, _c_int, _c_int, _c_vp,
+                                       _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp]),
+    "specq_rotary": (_c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64,
+                              _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64,
+                              _c_vp, _c_int, _c_float, _c_vp, _c_vp, _c_i64,
+                              _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp]),
+    "specq_kv_pages_workspace_size": (_c_size, [_c_int, _c_int, _c_int]),
+    "specq_kv_pages_reserve": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_int, _c_vp,
+                                        _c_vp, _c_size, _c_vp]),
+    "specq_kv_pages_free": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_int, _c_vp]),
+    "specq_kv_pages_fork": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_vp, _c_int,
+                                     _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_size, _c_vp]),
+    "specq_kv_pages_compact": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_vp, _c_int, _c_vp,
+                                        _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_size, _c_vp]),
+    "specq_kv_pages_copy": (_c_int, [_c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp]),
     "specq_kernel_attrs_query": (_c_int, [_c_int] * 9 + [ctypes.POINTER(KernelAttrs)]),
 }
 
