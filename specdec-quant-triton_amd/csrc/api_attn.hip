@@ -17,6 +17,8 @@ const void* attn_plan_fn_d64(int rb_max, int fp32);   // attn_plan_d64.hip
 const void* attn_plan_fn_d128(int rb_max, int fp32);  // attn_plan_d128.hip
 const void* attn_block_fn_d64(int rb, int f8, int plan);   // attn_block_d64.hip
 const void* attn_block_fn_d128(int rb, int f8, int plan);  // attn_block_d128.hip
+const void* attn_merge_fn_d64();
+const void* attn_merge_fn_d128();
 
 namespace {
 
@@ -48,9 +50,9 @@ const void* attn_fn(int D, int rb, int kind, bool plan) {
 
 // grid.x: the splits of a block table of max_pages * PAGE tokens when at least `pairs_min`
 // (sequence, KV head) pairs are active (fewer pairs never means fewer splits).
-int n_splits_for(int max_pages, int PAGE, int pairs_min, int target) {
+int n_splits_for(int max_pages, int PAGE, int pairs_min, int target, int most) {
   const int cap = max_pages * PAGE;
-  const int per = kAttnUnit * attn_split_units(cap, pairs_min, target);
+  const int per = kAttnUnit * attn_split_units(cap, pairs_min, target, most);
   return std::max(1, ceil_div(cap, per));
 }
 
@@ -83,8 +85,7 @@ int attn_attrs(int variant, int rows, specq_kernel_attrs* out) {
 
 using namespace specq;
 
-extern "C" size_t specq_paged_attn_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP, int max_pages,
-                                                  int PAGE) {
+static size_t attn_workspace(int most, int B_grid, int H, int H_KV, int ql_grid, int QPP, int max_pages, int PAGE) {
   if (B_grid <= 0 || H_KV <= 0 || H % H_KV != 0 || QPP <= 0 || ql_grid <= 0 || max_pages <= 0 || PAGE <= 0) return 0;
   const int G = H / H_KV;
   const int rows = ceil_div(QPP * G, 16) * 16;
@@ -93,11 +94,21 @@ extern "C" size_t specq_paged_attn_workspace_size(int B_grid, int H, int H_KV, i
   if ((int64_t)max_pages * PAGE > kAttnMaxTokens) return 0;
   // Plan-mode bound: at least one active sequence.
   const int tgt = g_attn_target.load();
-  const int ns = n_splits_for(max_pages, PAGE, H_KV, tgt > 0 ? tgt : device_cus());
+  const int ns = n_splits_for(max_pages, PAGE, H_KV, tgt > 0 ? tgt : device_cus(), most);
   if (ns <= 1) return 0;
   // Sized for D = 128 (the largest supported head dimension).
   const size_t part = (size_t)progs * ns * rows * (128 + 2) * 4;
   return kCounterBytes + align_up(part, 256);
+}
+
+extern "C" size_t specq_paged_attn_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP, int max_pages,
+                                                  int PAGE) {
+  return attn_workspace(kAttnMergeMax, B_grid, H, H_KV, ql_grid, QPP, max_pages, PAGE);
+}
+
+extern "C" size_t specq_paged_attn_block_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP,
+                                                        int max_pages, int PAGE) {
+  return attn_workspace(kBlkMergeMax, B_grid, H, H_KV, ql_grid, QPP, max_pages, PAGE);
 }
 
 // Both entry points: `kind` is the cache's, `sb` its tokens per scale block (block scales only).
@@ -145,13 +156,15 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
   if (n_qc == 0) return SPECQ_OK;
   const int target = g_attn_target.load() > 0 ? g_attn_target.load() : device_cus();
   // Eager calls know the active sequences; a plan may activate as few as one.
+  const int most = kind >= kBlkI8 ? kBlkMergeMax : kAttnMergeMax;
   const int ns = n_splits_for(max_pages, PAGE, plan ? H_KV : std::max(n_seqs, 1) * H_KV * attn_row_programs(q_len, G),
-                              target);
+                              target, most);
+  const bool defer = kind >= kBlkI8 && ns > kBlkMergeIn;
   const int64_t progs = (int64_t)B_grid * H_KV * n_qc;
   const int rows = rb * 16;
   size_t need = 0;
   if (ns > 1) {
-    SPECQ_REQUIRE(progs <= kMaxCounters, SPECQ_ENOTSUP, "paged_attn: %lld programs exceed the counter region",
+    SPECQ_REQUIRE(defer || progs <= kMaxCounters, SPECQ_ENOTSUP, "paged_attn: %lld programs exceed the counter region",
                   (long long)progs);
     need = kCounterBytes + align_up((size_t)progs * ns * rows * (D + 2) * 4, 256);
   }
@@ -164,7 +177,7 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
     // Active query tokens that fill one program cut a sequence finest; past that the cut gets coarser.
     wgs = 0;
     for (int s = 1; s <= B_grid; ++s)
-      wgs = std::max(wgs, (int64_t)s * H_KV * n_qc * n_splits_for(max_pages, PAGE, s * H_KV, target));
+      wgs = std::max(wgs, (int64_t)s * H_KV * n_qc * n_splits_for(max_pages, PAGE, s * H_KV, target, most));
   }
   if (wgs == 0) return SPECQ_OK;
   SPECQ_REQUIRE(wgs <= INT32_MAX, SPECQ_ENOTSUP, "paged_attn: grid too large");
@@ -181,6 +194,7 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
   p.counters = need ? (int32_t*)workspace : nullptr;
   p.part = need ? (float*)((char*)workspace + kCounterBytes) : nullptr;
   p.sb = sb;
+  p.defer = defer;
   diag_timeline(&p.tl, &p.tl_cap);
   void* args[] = {&p};
   hipError_t e = hipLaunchKernel(fn, dim3((unsigned)wgs), dim3(kAttnThreads), args, 0, (hipStream_t)stream);
@@ -188,7 +202,10 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
     set_error("paged_attn: hipLaunchKernel failed: %s", hipGetErrorString(e));
     return SPECQ_EIO;
   }
-  return SPECQ_OK;
+  if (!defer) return SPECQ_OK;
+  const int64_t merge = (int64_t)(plan ? B_grid : n_seqs) * H_KV * n_qc * QPP * G;
+  SPECQ_REQUIRE(merge <= INT32_MAX, SPECQ_ENOTSUP, "paged_attn: grid too large");
+  return launch(D == 128 ? attn_merge_fn_d128() : attn_merge_fn_d64(), (int)merge, 256, 0, (hipStream_t)stream, &p);
 }
 
 extern "C" int specq_paged_attn(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh, const int8_t* kc,

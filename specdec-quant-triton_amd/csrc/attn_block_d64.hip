@@ -1,5 +1,5 @@
 // Instantiations of paged attention over block-scaled int8 / e4m3 caches, head dim 64: the eager
-// launches (1 to 4 row blocks) and the plan-mode launches (runtime row blocks, 2 to 4).
+// launches (1 to 4 row blocks) and the plan-mode launches (runtime row blocks, 2 to 4), and the merge of many splits.
 #include "paged_attn.hpp"
 
 namespace specq {
@@ -23,5 +23,7 @@ const void* attn_block_fn_d64(int rb, int f8, int plan) {
   }
   return nullptr;
 }
+
+const void* attn_merge_fn_d64() { return reinterpret_cast<const void*>(&attn_merge_kernel<64>); }
 
 }  // namespace specq

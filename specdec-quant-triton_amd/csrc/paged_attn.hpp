@@ -94,7 +94,9 @@ struct AttnParams {
   int32_t* counters;   // [progs]
   uint64_t* tl;        // diagnostics build only: per-workgroup timestamps (null otherwise)
   int tl_cap;          // workgroups tl has room for
-  int sb;              // tokens per scale block (block-scaled caches only)
+  // Block-scaled caches only:
+  int sb;              // tokens per scale block
+  int defer;           // splits are merged by attn_merge_kernel behind this launch
 };
 
 // Scale types of the kernels below: _Float16 or float per token, or one of these per block.
@@ -117,6 +119,18 @@ constexpr int kAttnRing = 4;                        // LDS chunk slots per wave
 // p * vs stays at most 64 * 65504 / 127 < 65504, inside fp16, for the V scale of any fp16 row
 // quantised to int8 (vs <= 65504 / 127).
 constexpr float kAttnLazyP = 64.f;
+// Block-scaled caches: up to kBlkMergeIn splits are merged by the program's last workgroup, more by a
+// launch of their own, a workgroup to each row (at most kBlkMergeMax, one per thread there).  One
+// workgroup reads its program's partial rows at some 60 GB/s: B = 1, 2 K/V heads, 5 tokens, context
+// 131072, D = 64: 64 splits merged in place 37.6 us in a graph, 128 splits and the
+// launch 21.9; 8 K/V heads, context 65536, D = 128: 32 splits 42.5 and 38.7; context 4096, 11 splits 17.6 and
+// 16.9.  Four splits of 64 programs are 28.9 in place and 33.1 with the launch.
+constexpr int kBlkMergeIn = 8;
+constexpr int kBlkMergeMax = 256;
+template <typename ST>
+constexpr int attn_merge_most() {
+  return std::is_same_v<ST, BlockI8> || std::is_same_v<ST, BlockF8> ? kBlkMergeMax : kAttnMergeMax;
+}
 constexpr int64_t kAttnMaxTokens = (int64_t)kAttnUnit * kAttnMaxUnits * kAttnMergeMax;  // 524288
 
 // Programs of 64 packed rows a (sequence, KV head) pair of q_len query tokens fills: what its work
@@ -129,12 +143,13 @@ __host__ __device__ inline int attn_row_programs(int q_len, int G) { return q_le
 
 // 128-token units per split for a sequence of L tokens when `pairs` (sequence, KV head) pairs
 // (times their row programs) are active and the device has `target` CUs.
-__host__ __device__ inline int attn_split_units(int L, int pairs, int target) {
+// `most`: the splits a sequence may have at most.
+__host__ __device__ inline int attn_split_units(int L, int pairs, int target, int most = kAttnMergeMax) {
   const int n = L > 0 ? (L + kAttnUnit - 1) / kAttnUnit : 1;
   const int pr = pairs > 0 ? pairs : 1;
   const int want = pr >= target ? 1 : (target + pr - 1) / pr;
   int u = (n + want - 1) / want;
-  const int u_min = (n + kAttnMergeMax - 1) / kAttnMergeMax;
+  const int u_min = (n + most - 1) / most;
   if (u < u_min) u = u_min;
   // Splits of one or two chunks per wave leave the merge and hand-off to dominate; from 4096
   // tokens (32 units) up the shortest split is three units (B = 1, ctx 4096: 25.0 -> 22.9 us in
@@ -318,7 +333,8 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
   // page ids of the split can be fetched together with the context length and Q: one memory
   // round trip before the first K/V DMA.
   const int cap = p.max_pages * p.PAGE;
-  const int split_tokens = kAttnUnit * attn_split_units(cap, n_seqs * p.H_KV * attn_row_programs(q_len, p.G), p.target_wgs);
+  const int split_tokens = kAttnUnit * attn_split_units(cap, n_seqs * p.H_KV * attn_row_programs(q_len, p.G), p.target_wgs,
+                                                         attn_merge_most<ST>());
   // The grid is one-dimensional: workgroup id = program * splits + split (the exception for
   // eager calls with several query chunks and long splits is below), with the split count
   // of the active sequences, so the workgroups that have work are the first ones dispatched and
@@ -613,7 +629,7 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
       st.cs[rb] = c;
     }
   };
-  auto stage_b = [&](int it, const Staged& st) __attribute__((always_inline)) {
+  auto stage_b = [&](int it, Staged& st) __attribute__((always_inline)) {
     const int t0 = chunk_t0(it);
     // A chunk on a page outside the pool: every token masked (wave-uniform).
     const bool bad = ((bad_chunks >> (it & 63)) & 1) != 0;
@@ -698,34 +714,28 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
         }
       }
     }
-    // NaN codes of V in a chunk with masked tokens (see the notes at the top).
-    bool vnan = false;
+    // NaN codes of V in a chunk with masked tokens (see the notes at the top): out of line, so that
+    // the product below stays one block.
     if constexpr (F8) {
+      uint32_t any = 0;
       if (!full) {
-        uint32_t any = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
           for (int c = 0; c < ND / 4; ++c) any |= f8_nan_bits(st.vx[e][c]);
-        vnan = __builtin_amdgcn_ballot_w64(any != 0) != 0;
       }
-    }
-    // V bytes to d-major: vt[db] = the 4 token bytes (operand slots 4g..4g+3) of d = ND*r + db.
+      if (__builtin_amdgcn_ballot_w64(any != 0) != 0) {
 #pragma unroll
-    for (int c = 0; c < ND / 4; ++c) {
-      const uint32_t x[4] = {st.vx[0][c], st.vx[1][c], st.vx[2][c], st.vx[3][c]};
-      uint32_t y[4];
-      transpose4x4(x, y);
+        for (int c = 0; c < ND / 4; ++c) {
+          const uint32_t x[4] = {st.vx[0][c], st.vx[1][c], st.vx[2][c], st.vx[3][c]};
+          uint32_t y[4];
+          transpose4x4(x, y);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v2h lo, hi;
-        if constexpr (F8) {
-          if (vnan) {
+          for (int e = 0; e < 4; ++e) {
             const uint32_t nb = f8_nan_bits(y[e]);
             v4h isnan;
 #pragma unroll
             for (int j = 0; j < 4; ++j) isnan[j] = (_Float16)((nb >> (8 * j + 7)) & 1 ? 1.f : 0.f);
-            y[e] &= ~((nb >> 7) * 0xffu);
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
               v4h seen;
@@ -737,7 +747,20 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
                 if (hits[j] > 0.f) acc[rb][4 * c + e][j] = __builtin_nanf("");
             }
           }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) st.vx[e][c] &= ~((f8_nan_bits(st.vx[e][c]) >> 7) * 0xffu);
         }
+      }
+    }
+    // V bytes to d-major: vt[db] = the 4 token bytes (operand slots 4g..4g+3) of d = ND*r + db.
+#pragma unroll
+    for (int c = 0; c < ND / 4; ++c) {
+      const uint32_t x[4] = {st.vx[0][c], st.vx[1][c], st.vx[2][c], st.vx[3][c]};
+      uint32_t y[4];
+      transpose4x4(x, y);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v2h lo, hi;
         code4_to_h2x2<F8>(y[e], lo, hi);
         const v4h vf = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
@@ -964,6 +987,9 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
     publish(mlp + 1, l);
   }
   tl_mark(p.tl, p.tl_cap, 5);  // diagnostics build: partials issued
+  if constexpr (BLK) {
+    if (p.defer) return;
+  }
   if (!arrive_last(p.counters + prog, n_active, &s_last, p.tl, p.tl_cap)) {
     tl_mark(p.tl, p.tl_cap, 6);  // diagnostics build: hand-off done (not the last split)
     return;
@@ -1091,5 +1117,79 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_plan_kernel(AttnParam
   }
 }
 #undef SPECQ_ATTN_LDS
+
+// Merge of block-scaled launches with many splits: workgroup (program, packed row).  Thread t holds
+// split t's (m, l); the row's weights exp2(m - max) / l go to LDS, and the 256 / (D / 4) thread groups
+// sum every such-th split's row, the groups then in order.  The sum's order depends on nothing but
+// the number of splits, and splits in which the row sees nothing add zeros.  Bound by latency: three
+// dependent round trips (length, statistics, rows), the rows' loads eight in flight.
+template <int D>
+__global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams p) {
+  constexpr int LN = D / 4, NG = 256 / LN, IN_FLIGHT = 8;
+  int n_seqs = p.n_seqs, q_len = p.q_len;
+  if (p.plan != nullptr) {
+    n_seqs = min(max(p.plan[0], 0), p.B_grid);
+    q_len = min(max(p.plan[1], 0), p.ql_grid);
+  }
+  n_seqs = uniform(n_seqs);
+  q_len = uniform(q_len);
+  const int per = p.QPP * p.G, rows = (per + 15) / 16 * 16;
+  const int prog = (int)blockIdx.x / per, row = (int)blockIdx.x - prog * per;
+  const int qc = prog % p.n_qc, kvh = (prog / p.n_qc) % p.H_KV, b = prog / (p.n_qc * p.H_KV);
+  const int qi = qc * p.QPP + row / p.G;
+  if (b >= n_seqs || qi >= q_len) return;
+  const int cap = p.max_pages * p.PAGE;
+  const int split_tokens = kAttnUnit * attn_split_units(cap, n_seqs * p.H_KV * attn_row_programs(q_len, p.G), p.target_wgs,
+                                                         kBlkMergeMax);
+  const int L = uniform(min(p.ctx_len[b], cap));
+  const int kv_end = L - q_len + min(qc * p.QPP + p.QPP, q_len);
+  const int n = kv_end > split_tokens ? (kv_end + split_tokens - 1) / split_tokens : 1;
+  if (n == 1) return;  // the row's only split has stored it
+  const int64_t base = (int64_t)prog * p.n_splits * rows + row;  // the row in split 0, in rows
+  const float* ml = p.part + (int64_t)p.B_grid * p.H_KV * p.n_qc * p.n_splits * rows * D;
+  const int t = threadIdx.x;
+  __shared__ float wt[kBlkMergeMax], red[2][4];
+  __shared__ v4f sum[NG][LN];
+  float m = -INFINITY, l = 0.f;
+  if (t < n) {
+    m = ml[(base + (int64_t)t * rows) * 2];
+    l = ml[(base + (int64_t)t * rows) * 2 + 1];
+  }
+  float mx = m;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+  if (lane_id() == 0) red[0][wave_id()] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  const float w = fast_exp2(m - (mx == -INFINITY ? 0.f : mx));
+  float ls = t < n ? w * l : 0.f;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) ls += __shfl_xor(ls, o);
+  if (lane_id() == 0) red[1][wave_id()] = ls;
+  wt[t] = t < n ? w : 0.f;
+  __syncthreads();
+  ls = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  const float inv = ls == 0.f ? 0.f : 1.f / ls;
+  const int g = t / LN, c = t % LN;
+  const v4f* o_part = reinterpret_cast<const v4f*>(p.part) + base * LN + c;
+  v4f o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = g; s0 < n; s0 += NG * IN_FLIGHT) {
+    v4f x[IN_FLIGHT];
+#pragma unroll
+    for (int u = 0; u < IN_FLIGHT; ++u) x[u] = o_part[(int64_t)min(s0 + u * NG, n - 1) * rows * LN];
+#pragma unroll
+    for (int u = 0; u < IN_FLIGHT; ++u)
+      if (s0 + u * NG < n) o += wt[s0 + u * NG] * x[u];
+  }
+  sum[g][c] = o;
+  __syncthreads();
+  if (g == 0) {
+    for (int i = 1; i < NG; ++i) o += sum[i][c];
+    o *= inv;
+    const int head = kvh * p.G + row % p.G;
+    *reinterpret_cast<v4h*>(p.out + (int64_t)b * p.s_ob + (int64_t)qi * p.s_ot + (int64_t)head * p.s_oh + 4 * c) =
+        v4h{(_Float16)f32_opaque(o.x), (_Float16)f32_opaque(o.y), (_Float16)f32_opaque(o.z), (_Float16)f32_opaque(o.w)};
+  }
+}
 
 }  // namespace specq

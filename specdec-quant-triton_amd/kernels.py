@@ -1257,7 +1257,7 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
         ck = KernelInfo(2, D | (1 << 18 if f8 else 1 << 17), 0, 0, 0, QPP * G, 0, 4, 0)
         if Bg == 0 or Qg == 0:
             return out, ck
-        need = _lib.lib().specq_paged_attn_workspace_size(Bg, H, H_KV, Qg, QPP, max_pages, PAGE)
+        need = _lib.lib().specq_paged_attn_block_workspace_size(Bg, H, H_KV, Qg, QPP, max_pages, PAGE)
         wptr, wbytes = (workspace or _ws.shared(q.device)).ensure(need)
         _lib.call("specq_paged_attn_block", q.data_ptr(), qs[0], qs[1], qs[2],
                   kc.data_ptr(), vc.data_ptr(), 1 if f8 else 0, cs[0], cs[1], cs[2],
