@@ -323,11 +323,10 @@ int specq_kv_append_int8(const void* k_new, const void* v_new, int64_t s_nb, int
  *   kc, vc   codes [pages, PAGE, H_KV, D], as specq_paged_attn
  *   ks, vs   fp32 [pages, PAGE / block, H_KV], strides s_sp (page), s_sb (block), s_sh, shared
  *   block    a multiple of 16 that divides PAGE
- *   Probabilities are rounded to fp16 once, after their V scale, under a power of two that keeps them
- *   normal whatever the scales' size.  Scales, and e4m3 NaN codes, of tokens that a row does not see do
+ *   Probabilities are rounded to fp16 once, after their V scale, against a running max of what the tokens
+ *   contribute.  Scales, and e4m3 NaN codes, of tokens that a row does not see do
  *   not reach it.  Everything else as specq_paged_attn (the workspace:
- *   specq_paged_attn_block_workspace_size; a sequence may be cut into up to 256 splits); QPP = 1, fused, eager and plan-mode calls agree bit for bit unless a probability
- *   is an fp16 subnormal.
+ *   specq_paged_attn_block_workspace_size; a sequence may be cut into up to 256 splits); QPP = 1, fused, eager and plan-mode calls agree bit for bit.
  * ------------------------------------------------------------------------------------- */
 size_t specq_paged_attn_block_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP, int max_pages, int PAGE);
 int specq_paged_attn_block(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh,

@@ -4,7 +4,7 @@
 #include <atomic>
 
 #include "api_common.hpp"
-#include "paged_attn.hpp"
+#include "paged_attn_block.hpp"
 
 namespace specq {
 
@@ -50,9 +50,9 @@ const void* attn_fn(int D, int rb, int kind, bool plan) {
 
 // grid.x: the splits of a block table of max_pages * PAGE tokens when at least `pairs_min`
 // (sequence, KV head) pairs are active (fewer pairs never means fewer splits).
-int n_splits_for(int max_pages, int PAGE, int pairs_min, int target, int most) {
+int n_splits_for(bool blk, int max_pages, int PAGE, int pairs_min, int target) {
   const int cap = max_pages * PAGE;
-  const int per = kAttnUnit * attn_split_units(cap, pairs_min, target, most);
+  const int per = blk ? kBlkUnit * blk_split_units(cap, pairs_min, target) : kAttnUnit * attn_split_units(cap, pairs_min, target);
   return std::max(1, ceil_div(cap, per));
 }
 
@@ -70,9 +70,12 @@ int attn_attrs(int variant, int rows, specq_kernel_attrs* out) {
   SPECQ_REQUIRE(fn != nullptr, SPECQ_ENOTSUP, "paged_attn: head_dim %d not supported", D);
   hipFuncAttributes fa;
   if (hipFuncGetAttributes(&fa, fn) != hipSuccess) return fail(SPECQ_EIO, "paged_attn: hipFuncGetAttributes failed");
-  static const char* const kNames[] = {"_Float16", "float", "specq::BlockI8", "specq::BlockF8"};
+  static const char* const kNames[] = {"paged_attn_kernel<%d, %d, _Float16>", "paged_attn_kernel<%d, %d, float>",
+                                       "attn_block_kernel<%d, %d, false>", "attn_block_kernel<%d, %d, true>"};
   // The name carries the template arguments exactly as profilers print the kernel symbol.
-  snprintf(out->name, sizeof(out->name), "specq::paged_attn_kernel<%d, %d, %s>", D, rb, kNames[kind]);
+  char name[64];
+  snprintf(name, sizeof(name), kNames[kind], D, rb);
+  snprintf(out->name, sizeof(out->name), "specq::%s", name);
   out->num_regs = fa.numRegs;
   out->lds_bytes = (int)fa.sharedSizeBytes;
   out->scratch_bytes = (int)fa.localSizeBytes;
@@ -85,16 +88,16 @@ int attn_attrs(int variant, int rows, specq_kernel_attrs* out) {
 
 using namespace specq;
 
-static size_t attn_workspace(int most, int B_grid, int H, int H_KV, int ql_grid, int QPP, int max_pages, int PAGE) {
+static size_t attn_workspace(bool blk, int B_grid, int H, int H_KV, int ql_grid, int QPP, int max_pages, int PAGE) {
   if (B_grid <= 0 || H_KV <= 0 || H % H_KV != 0 || QPP <= 0 || ql_grid <= 0 || max_pages <= 0 || PAGE <= 0) return 0;
   const int G = H / H_KV;
   const int rows = ceil_div(QPP * G, 16) * 16;
   const int n_qc = ceil_div(ql_grid, QPP);
   const int64_t progs = (int64_t)B_grid * H_KV * n_qc;
-  if ((int64_t)max_pages * PAGE > kAttnMaxTokens) return 0;
+  if ((int64_t)max_pages * PAGE > (blk ? kBlkMaxTokens : kAttnMaxTokens)) return 0;
   // Plan-mode bound: at least one active sequence.
   const int tgt = g_attn_target.load();
-  const int ns = n_splits_for(max_pages, PAGE, H_KV, tgt > 0 ? tgt : device_cus(), most);
+  const int ns = n_splits_for(blk, max_pages, PAGE, H_KV, tgt > 0 ? tgt : device_cus());
   if (ns <= 1) return 0;
   // Sized for D = 128 (the largest supported head dimension).
   const size_t part = (size_t)progs * ns * rows * (128 + 2) * 4;
@@ -103,12 +106,12 @@ static size_t attn_workspace(int most, int B_grid, int H, int H_KV, int ql_grid,
 
 extern "C" size_t specq_paged_attn_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP, int max_pages,
                                                   int PAGE) {
-  return attn_workspace(kAttnMergeMax, B_grid, H, H_KV, ql_grid, QPP, max_pages, PAGE);
+  return attn_workspace(false, B_grid, H, H_KV, ql_grid, QPP, max_pages, PAGE);
 }
 
 extern "C" size_t specq_paged_attn_block_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP,
                                                         int max_pages, int PAGE) {
-  return attn_workspace(kBlkMergeMax, B_grid, H, H_KV, ql_grid, QPP, max_pages, PAGE);
+  return attn_workspace(true, B_grid, H, H_KV, ql_grid, QPP, max_pages, PAGE);
 }
 
 // Both entry points: `kind` is the cache's, `sb` its tokens per scale block (block scales only).
@@ -127,9 +130,10 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
   SPECQ_REQUIRE(PAGE > 0 && PAGE % 16 == 0, SPECQ_ENOTSUP, "paged_attn: PAGE=%d must be a multiple of 16", PAGE);
   SPECQ_REQUIRE(max_pages > 0, SPECQ_EINVAL, "paged_attn: empty block table");
   SPECQ_REQUIRE(n_pages > 0, SPECQ_EINVAL, "paged_attn: empty K/V pool (n_pages=%d)", n_pages);
-  SPECQ_REQUIRE((int64_t)max_pages * PAGE <= kAttnMaxTokens, SPECQ_ENOTSUP,
-                "paged_attn: block table of %lld tokens exceeds %lld", (long long)max_pages * PAGE,
-                (long long)kAttnMaxTokens);
+  const bool blk = kind >= kBlkI8;
+  const int64_t most = blk ? kBlkMaxTokens : kAttnMaxTokens;
+  SPECQ_REQUIRE((int64_t)max_pages * PAGE <= most, SPECQ_ENOTSUP, "paged_attn: block table of %lld tokens exceeds %lld",
+                (long long)max_pages * PAGE, (long long)most);
   SPECQ_REQUIRE(QPP > 0, SPECQ_EINVAL, "paged_attn: QPP=%d", QPP);
   const int G = H / H_KV;
   SPECQ_REQUIRE(QPP * G <= 64, SPECQ_ENOTSUP, "paged_attn: QPP*G=%d packed rows exceed 64", QPP * G);
@@ -156,10 +160,9 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
   if (n_qc == 0) return SPECQ_OK;
   const int target = g_attn_target.load() > 0 ? g_attn_target.load() : device_cus();
   // Eager calls know the active sequences; a plan may activate as few as one.
-  const int most = kind >= kBlkI8 ? kBlkMergeMax : kAttnMergeMax;
-  const int ns = n_splits_for(max_pages, PAGE, plan ? H_KV : std::max(n_seqs, 1) * H_KV * attn_row_programs(q_len, G),
-                              target, most);
-  const bool defer = kind >= kBlkI8 && ns > kBlkMergeIn;
+  const int ns = n_splits_for(blk, max_pages, PAGE,
+                              plan ? H_KV : std::max(n_seqs, 1) * H_KV * attn_row_programs(q_len, G), target);
+  const bool defer = blk && ns > kBlkMergeIn;
   const int64_t progs = (int64_t)B_grid * H_KV * n_qc;
   const int rows = rb * 16;
   size_t need = 0;
@@ -177,11 +180,11 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
     // Active query tokens that fill one program cut a sequence finest; past that the cut gets coarser.
     wgs = 0;
     for (int s = 1; s <= B_grid; ++s)
-      wgs = std::max(wgs, (int64_t)s * H_KV * n_qc * n_splits_for(max_pages, PAGE, s * H_KV, target, most));
+      wgs = std::max(wgs, (int64_t)s * H_KV * n_qc * n_splits_for(blk, max_pages, PAGE, s * H_KV, target));
   }
   if (wgs == 0) return SPECQ_OK;
   SPECQ_REQUIRE(wgs <= INT32_MAX, SPECQ_ENOTSUP, "paged_attn: grid too large");
-  AttnParams p;
+  AttnBlockParams p;  // the per-token kernels take its AttnParams
   p.q = (const _Float16*)q; p.s_qb = s_qb; p.s_qt = s_qt; p.s_qh = s_qh;
   p.kc = (const int8_t*)kc; p.vc = (const int8_t*)vc; p.s_kp = s_kp; p.s_ko = s_ko; p.s_kh = s_kh;
   p.ks = ks; p.vs = vs; p.s_sp = s_sp; p.s_so = s_so; p.s_sh = s_sh;

@@ -53,24 +53,6 @@
 //    eagerly or from a plan-mode graph.
 //  * Plan mode reads (n_seqs, q_len) from plan[0..1]; programs for inactive sequences or
 //    query slots return before any load or store.
-//
-// Block-scaled caches (ST = BlockI8 or BlockF8): int8 or e4m3 codes with one fp32 scale for each
-// (block of SB tokens, KV head), scales [pages, PAGE / SB, H_KV], SB a multiple of 16 dividing PAGE:
-//   s_t = (q . k_t) * ks_blk(t) * sm_scale,   o = (sum_t p_t * vs_blk(t) * v_t) / sum_t p_t.
-// The schedule is the one above.  What the block scales change:
-//  * A 16-token chunk lies in one block, so its two scales are wave-uniform.  They are fetched once,
-//    with the split's page ids (lane c holds those of the wave's chunk c), by two LDS DMAs ahead of
-//    the ring's, and picked with v_readlane: no scale DMA per chunk, and the staged state of a chunk
-//    is 8 registers smaller.
-//  * P is rounded to fp16 once, as p * vs * 2^j with 2^j one power of two for the wave, chosen so
-//    that its largest finite V scale lies in [256, 512): p * vs * 2^j < 2^15, whatever the scales'
-//    size, and what is 2^-22 of the largest is still a normal fp16.  2^-j goes into the merge
-//    weight.  A power of two leaves every rounding where it was, so results do not depend on the
-//    wave's other chunks (but for fp16 subnormals).
-//  * e4m3 codes become fp16 exactly (v_cvt_scalef32_pk_f16_fp8), NaN codes NaN.  A NaN in V must not
-//    reach the rows that do not see its token (0 * NaN): chunks that need the causal mask multiply V
-//    with its NaNs cleared, and where there are any, a second product of the two indicators
-//    (token seen, code NaN) says which outputs are NaN.
 #pragma once
 #include "common.hpp"
 
@@ -94,14 +76,7 @@ struct AttnParams {
   int32_t* counters;   // [progs]
   uint64_t* tl;        // diagnostics build only: per-workgroup timestamps (null otherwise)
   int tl_cap;          // workgroups tl has room for
-  // Block-scaled caches only:
-  int sb;              // tokens per scale block
-  int defer;           // splits are merged by attn_merge_kernel behind this launch
 };
-
-// Scale types of the kernels below: _Float16 or float per token, or one of these per block.
-struct BlockI8 {};  // int8 codes
-struct BlockF8 {};  // e4m3 codes
 
 
 constexpr int kAttnChunk = 16;                      // tokens per wave iteration (one page sub-tile)
@@ -119,18 +94,6 @@ constexpr int kAttnRing = 4;                        // LDS chunk slots per wave
 // p * vs stays at most 64 * 65504 / 127 < 65504, inside fp16, for the V scale of any fp16 row
 // quantised to int8 (vs <= 65504 / 127).
 constexpr float kAttnLazyP = 64.f;
-// Block-scaled caches: up to kBlkMergeIn splits are merged by the program's last workgroup, more by a
-// launch of their own, a workgroup to each row (at most kBlkMergeMax, one per thread there).  One
-// workgroup reads its program's partial rows at some 60 GB/s: B = 1, 2 K/V heads, 5 tokens, context
-// 131072, D = 64: 64 splits merged in place 37.6 us in a graph, 128 splits and the
-// launch 21.9; 8 K/V heads, context 65536, D = 128: 32 splits 42.5 and 38.7; context 4096, 11 splits 17.6 and
-// 16.9.  Four splits of 64 programs are 28.9 in place and 33.1 with the launch.
-constexpr int kBlkMergeIn = 8;
-constexpr int kBlkMergeMax = 256;
-template <typename ST>
-constexpr int attn_merge_most() {
-  return std::is_same_v<ST, BlockI8> || std::is_same_v<ST, BlockF8> ? kBlkMergeMax : kAttnMergeMax;
-}
 constexpr int64_t kAttnMaxTokens = (int64_t)kAttnUnit * kAttnMaxUnits * kAttnMergeMax;  // 524288
 
 // Programs of 64 packed rows a (sequence, KV head) pair of q_len query tokens fills: what its work
@@ -143,13 +106,12 @@ __host__ __device__ inline int attn_row_programs(int q_len, int G) { return q_le
 
 // 128-token units per split for a sequence of L tokens when `pairs` (sequence, KV head) pairs
 // (times their row programs) are active and the device has `target` CUs.
-// `most`: the splits a sequence may have at most.
-__host__ __device__ inline int attn_split_units(int L, int pairs, int target, int most = kAttnMergeMax) {
+__host__ __device__ inline int attn_split_units(int L, int pairs, int target) {
   const int n = L > 0 ? (L + kAttnUnit - 1) / kAttnUnit : 1;
   const int pr = pairs > 0 ? pairs : 1;
   const int want = pr >= target ? 1 : (target + pr - 1) / pr;
   int u = (n + want - 1) / want;
-  const int u_min = (n + most - 1) / most;
+  const int u_min = (n + kAttnMergeMax - 1) / kAttnMergeMax;
   if (u < u_min) u = u_min;
   // Splits of one or two chunks per wave leave the merge and hand-off to dominate; from 4096
   // tokens (32 units) up the shortest split is three units (B = 1, ctx 4096: 25.0 -> 22.9 us in
@@ -192,41 +154,6 @@ __device__ __forceinline__ float group_max4(float x) {
   const uint32_t v = __builtin_bit_cast(uint32_t, m1);
   const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
-}
-
-// Four cache codes in a dword -> two packed half2, eight -> v8h (int8 or e4m3; both exact).
-template <bool F8>
-__device__ __forceinline__ void code4_to_h2x2(uint32_t x, v2h& lo, v2h& hi) {
-  if constexpr (F8) {
-    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x, 1.0f, false);
-    const auto b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x, 1.0f, true);
-    lo = v2h{(_Float16)a[0], (_Float16)a[1]};
-    hi = v2h{(_Float16)b[0], (_Float16)b[1]};
-  } else {
-    i8x4_to_h2x2(x, lo, hi);
-  }
-}
-template <bool F8>
-__device__ __forceinline__ v8h code8_to_h8(uint32_t x0, uint32_t x1) {
-  if constexpr (!F8) return i8x8_to_h8(x0, x1);
-  v2h a, b, c, d;
-  code4_to_h2x2<F8>(x0, a, b);
-  code4_to_h2x2<F8>(x1, c, d);
-  return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-// Bit 7 of every byte of x that is an e4m3 NaN (0x7f, 0xff).
-__device__ __forceinline__ uint32_t f8_nan_bits(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-
-// Max over the wave of values >= 0.
-__device__ __forceinline__ uint32_t wave_umax(uint32_t u) {
-  u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x128, 0xf, 0xf, false));  // row_ror:8, 4, 2, 1
-  u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x124, 0xf, 0xf, false));
-  u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x122, 0xf, 0xf, false));
-  u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x121, 0xf, 0xf, false));
-  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const uint32_t m1 = max((uint32_t)a[0], (uint32_t)a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(m1, m1, false, false);
-  return max((uint32_t)b[0], (uint32_t)b[1]);
 }
 
 // Unsigned max over the four 16-lane rows of a lane's column (lanes l, l^16, l^32, l^48).
@@ -280,10 +207,6 @@ __device__ __forceinline__ int64_t readlane64(int64_t v, int l) {
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
-__device__ __forceinline__ float readlane_f(float v, int l) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
-}
-
 // LDS bytes of one ring slot: K, V, then ks / vs (one dword per lane).
 template <int D>
 struct AttnSlot { static constexpr int value = 2 * kAttnChunk * D + 256; };
@@ -312,9 +235,7 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
   constexpr int SLOT = AttnSlot<D>::value;
   static_assert(SLOT == 2 * KB + 256, "slot layout");
   constexpr int NDMA = KB / 1024;         // 1 KB DMA instructions for K, and again for V
-  constexpr bool F8 = std::is_same_v<ST, BlockF8>;
-  constexpr bool BLK = F8 || std::is_same_v<ST, BlockI8>;
-  constexpr int NVM = 2 * NDMA + (BLK ? 0 : 1);  // DMA instructions per chunk (K, V, per-token scales)
+  constexpr int NVM = 2 * NDMA + 1;       // DMA instructions per chunk (K, V, scales)
   constexpr int HALF = 8 * D * 4;         // bytes of 8 fp32 O rows: one half of a merge block
   static_assert(D == 64 || D == 128, "head dim");
   static_assert(RB >= 1 && RB <= NS && HALF <= SLOT, "merge block halves fit a ring slot");
@@ -333,8 +254,7 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
   // page ids of the split can be fetched together with the context length and Q: one memory
   // round trip before the first K/V DMA.
   const int cap = p.max_pages * p.PAGE;
-  const int split_tokens = kAttnUnit * attn_split_units(cap, n_seqs * p.H_KV * attn_row_programs(q_len, p.G), p.target_wgs,
-                                                         attn_merge_most<ST>());
+  const int split_tokens = kAttnUnit * attn_split_units(cap, n_seqs * p.H_KV * attn_row_programs(q_len, p.G), p.target_wgs);
   // The grid is one-dimensional: workgroup id = program * splits + split (the exception for
   // eager calls with several query chunks and long splits is below), with the split count
   // of the active sequences, so the workgroups that have work are the first ones dispatched and
@@ -467,7 +387,7 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
   }
   const int sc_T = attn_perm(lane & 15);
   const uint8_t* sc_src = reinterpret_cast<const uint8_t*>((lane & 16) ? p.vs : p.ks);
-  const uint8_t* sc_lane = sc_src + (BLK ? 0 : (int64_t)sc_T * p.s_so * (int64_t)sizeof(ST));
+  const uint8_t* sc_lane = sc_src + (int64_t)sc_T * p.s_so * (int64_t)sizeof(ST);
   // Per-chunk bases, lane c holding the wave's chunk c: the byte offset of the chunk's page
   // sub-tile of this KV head in the K/V cache, and that of its first token's scales.  Chunks
   // at or past the wave's last use page 0 (their DMAs read nothing or a fixed valid address).
@@ -480,13 +400,7 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
     const int pg = lane < n_it && page_ok ? page_v : 0;
     const int tk = chunk_t0(lane) % p.PAGE;
     kv_base_v = (int64_t)pg * p.s_kp + (int64_t)tk * p.s_ko + (int64_t)kvh * p.s_kh;
-    if constexpr (BLK) {
-      sc_base_v = ((int64_t)pg * p.s_sp + (int64_t)(tk / p.sb) * p.s_so + (int64_t)kvh * p.s_sh) * 4;
-      dma4_global(reinterpret_cast<const uint8_t*>(p.ks) + sc_base_v, ring1[w] + SC);
-      dma4_global(reinterpret_cast<const uint8_t*>(p.vs) + sc_base_v, ring2[w] + SC);
-    } else {
-      sc_base_v = ((int64_t)pg * p.s_sp + (int64_t)tk * p.s_so + (int64_t)kvh * p.s_sh) * (int64_t)sizeof(ST);
-    }
+    sc_base_v = ((int64_t)pg * p.s_sp + (int64_t)tk * p.s_so + (int64_t)kvh * p.s_sh) * (int64_t)sizeof(ST);
   }
   // One query chunk and D = 128: no other program reads these K/V lines, and keeping them out of L2
   // leaves the lines of scales there, which the sequence's KV heads share.  Measured in a graph, us, kept ->
@@ -520,11 +434,9 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
 #pragma unroll
         for (int i = 0; i < NDMA; ++i) dma16_rs<false>(rv, kvoff[i], dst + KB + 1024 * i);
       }
-      if constexpr (!BLK) {
-        const uint8_t* src = sc_lane + sb;
-        if constexpr (sizeof(ST) == 4) dma4_global(src, dst + SC);
-        else dma2_global(src, dst + SC);
-      }
+      const uint8_t* src = sc_lane + sb;
+      if constexpr (sizeof(ST) == 4) dma4_global(src, dst + SC);
+      else dma2_global(src, dst + SC);
     } else {
 #pragma unroll
       for (int i = 0; i < NDMA; ++i) {
@@ -536,12 +448,10 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
         const bool ok = real && t0 + (64 * i + lane) / GR < kv_end;
         dma16_rs<false>(rv, oob_unless(ok, kvoff[i]), dst + KB + 1024 * i);
       }
-      if constexpr (!BLK) {
-        const bool ok = real && t0 + sc_T < kv_end;
-        const uint8_t* src = ok ? sc_lane + sb : sc_src;
-        if constexpr (sizeof(ST) == 4) dma4_global(src, dst + SC);
-        else dma2_global(src, dst + SC);
-      }
+      const bool ok = real && t0 + sc_T < kv_end;
+      const uint8_t* src = ok ? sc_lane + sb : sc_src;
+      if constexpr (sizeof(ST) == 4) dma4_global(src, dst + SC);
+      else dma2_global(src, dst + SC);
     }
   };
 
@@ -559,15 +469,12 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
   // chunk it + 1 before stage B of chunk it, so the S^T MFMAs of one chunk are in flight
   // while the other's softmax runs.  Each chunk's arithmetic is unchanged, so the results do
   // not depend on the pipelining.
-  // Block-scaled caches: lane c holds the K scale * sm_scale * log2(e) and the V scale * 2^j of the
-  // wave's chunk c; blk_out = 2^-j.
-  float blk_k = 0.f, blk_v = 0.f, blk_out = 1.f;
   struct Staged {
     v4f cs[RB];                // S^T of the chunk before the scales
-    float ksc[BLK ? 1 : 4], vsc[BLK ? 1 : 4];  // K scale * sm_scale * log2(e), V scale, in operand order
+    float ksc[4], vsc[4];      // K scale * sm_scale * log2(e), V scale, in operand order
     uint32_t vx[4][ND / 4];    // V bytes of operand slots 4g..4g+3
   };
-  auto stage_a = [&](auto slc, int it, Staged& st) __attribute__((always_inline)) {
+  auto stage_a = [&](auto slc, Staged& st) __attribute__((always_inline)) {
     const uint8_t* kb = ring_of(slc, w);
     const uint8_t* vb = kb + KB;
     // K operands: lane (r, g) holds head-dim bytes [DS*g, DS*g + DS) of token perm(r).
@@ -577,8 +484,8 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
 #pragma unroll
       for (int h = 0; h < KV4; ++h) {
         const v4i x = *reinterpret_cast<const v4i*>(kb + T * D + 16 * ((g * KV4 + h) ^ key));
-        kf[2 * h] = code8_to_h8<F8>((uint32_t)x.x, (uint32_t)x.y);
-        kf[2 * h + 1] = code8_to_h8<F8>((uint32_t)x.z, (uint32_t)x.w);
+        kf[2 * h] = i8x8_to_h8((uint32_t)x.x, (uint32_t)x.y);
+        kf[2 * h + 1] = i8x8_to_h8((uint32_t)x.z, (uint32_t)x.w);
       }
     }
     // V^T operands: lane (r, g) reads bytes [ND*r, ND*r + ND) of tokens perm(4g + e), operand
@@ -597,10 +504,7 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
     }
     // Scales in operand order: dword 4g + e holds ks of token perm(4g + e), dword 16 + 4g + e
     // its vs (an fp16 scale in the low half).
-    if constexpr (BLK) {
-      st.ksc[0] = readlane_f(blk_k, it & 63);
-      st.vsc[0] = readlane_f(blk_v, it & 63);
-    } else {
+    {
       const v4i kr = *reinterpret_cast<const v4i*>(kb + SC + 16 * g);
       const v4i vr = *reinterpret_cast<const v4i*>(kb + SC + 64 + 16 * g);
 #pragma unroll
@@ -629,14 +533,14 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
       st.cs[rb] = c;
     }
   };
-  auto stage_b = [&](int it, Staged& st) __attribute__((always_inline)) {
+  auto stage_b = [&](int it, const Staged& st) __attribute__((always_inline)) {
     const int t0 = chunk_t0(it);
     // A chunk on a page outside the pool: every token masked (wave-uniform).
     const bool bad = ((bad_chunks >> (it & 63)) & 1) != 0;
     // Zero V scale for tokens at or past kv_end and of masked chunks (their scale slots hold
     // the dummy address's).
-    float vsc[4] = {st.vsc[0], st.vsc[BLK ? 0 : 1], st.vsc[BLK ? 0 : 2], st.vsc[BLK ? 0 : 3]};
-    if (!BLK && (bad || t0 + kAttnChunk > kv_end)) {
+    float vsc[4] = {st.vsc[0], st.vsc[1], st.vsc[2], st.vsc[3]};
+    if (bad || t0 + kAttnChunk > kv_end) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (bad || t0 + attn_perm(4 * g + e) >= kv_end) vsc[e] = 0.f;
@@ -651,7 +555,7 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pr[rb][e] = fast_exp2(fmaf(st.cs[rb][e], st.ksc[BLK ? 0 : e], -m_run[rb]));
+      for (int e = 0; e < 4; ++e) pr[rb][e] = fast_exp2(fmaf(st.cs[rb][e], st.ksc[e], -m_run[rb]));
       if (!full) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -679,7 +583,7 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
         float s[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[e] = st.cs[rb][e] * st.ksc[BLK ? 0 : e];
+          s[e] = st.cs[rb][e] * st.ksc[e];
           if (!full && (bad || t0 + attn_perm(4 * g + e) > qpos[rb])) s[e] = -INFINITY;
         }
         const float rmax = group_max4(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
@@ -689,7 +593,7 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
           grew = true;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            pr[rb][e] = s[e] == -INFINITY ? 0.f : fast_exp2(fmaf(st.cs[rb][e], st.ksc[BLK ? 0 : e], -rmax));
+            pr[rb][e] = s[e] == -INFINITY ? 0.f : fast_exp2(fmaf(st.cs[rb][e], st.ksc[e], -rmax));
         }
       }
       // alpha is exactly 1 for every row whose m did not move.
@@ -706,51 +610,6 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
       l_run[rb] = l_run[rb] * alpha[rb] + ((pr[rb][0] + pr[rb][1]) + (pr[rb][2] + pr[rb][3]));
 #pragma unroll
       for (int e = 0; e < 4; ++e) pf[rb][e] = (_Float16)f32_opaque(pr[rb][e] * vsc[e]);  // fp32 product, then fp16 (kernels.py:232)
-      if constexpr (BLK) {  // a masked token's block may hold an infinite or NaN scale
-        if (!full) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (bad || t0 + attn_perm(4 * g + e) > qpos[rb]) pf[rb][e] = (_Float16)0.f;
-        }
-      }
-    }
-    // NaN codes of V in a chunk with masked tokens (see the notes at the top): out of line, so that
-    // the product below stays one block.
-    if constexpr (F8) {
-      uint32_t any = 0;
-      if (!full) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int c = 0; c < ND / 4; ++c) any |= f8_nan_bits(st.vx[e][c]);
-      }
-      if (__builtin_amdgcn_ballot_w64(any != 0) != 0) {
-#pragma unroll
-        for (int c = 0; c < ND / 4; ++c) {
-          const uint32_t x[4] = {st.vx[0][c], st.vx[1][c], st.vx[2][c], st.vx[3][c]};
-          uint32_t y[4];
-          transpose4x4(x, y);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t nb = f8_nan_bits(y[e]);
-            v4h isnan;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) isnan[j] = (_Float16)((nb >> (8 * j + 7)) & 1 ? 1.f : 0.f);
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-              v4h seen;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) seen[j] = (_Float16)(!bad && t0 + attn_perm(4 * g + j) <= qpos[rb] ? 1.f : 0.f);
-              const v4f hits = __builtin_amdgcn_mfma_f32_16x16x16f16(isnan, seen, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (hits[j] > 0.f) acc[rb][4 * c + e][j] = __builtin_nanf("");
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) st.vx[e][c] &= ~((f8_nan_bits(st.vx[e][c]) >> 7) * 0xffu);
-        }
-      }
     }
     // V bytes to d-major: vt[db] = the 4 token bytes (operand slots 4g..4g+3) of d = ND*r + db.
 #pragma unroll
@@ -761,7 +620,7 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         v2h lo, hi;
-        code4_to_h2x2<F8>(y[e], lo, hi);
+        i8x4_to_h2x2(y[e], lo, hi);
         const v4h vf = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
@@ -784,17 +643,6 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
 #pragma unroll
       for (int u = 0; u < NU; ++u) qreg[rb][u] = q_lds[rb][u][lane];
   }
-  if constexpr (BLK) {
-    wait_vmcnt<(NS - 1) * NVM>();  // the chunks' scales have landed (the ring's DMAs stay in flight)
-    const float kv = *reinterpret_cast<const float*>(ring1[w] + SC + 4 * lane);
-    const float vv = *reinterpret_cast<const float*>(ring2[w] + SC + 4 * lane);
-    const uint32_t mag = __builtin_bit_cast(uint32_t, vv) & 0x7fffffffu;
-    // Biased exponent of the wave's largest finite V scale, kept where 2^(135 - ex) is a normal float.
-    const uint32_t ex = max(wave_umax(lane < n_it && page_ok && mag < 0x7f800000u ? mag : 0u) >> 23, 9u);
-    blk_k = kv * p.scale_log2;
-    blk_v = vv * __builtin_bit_cast(float, (262u - ex) << 23);
-    blk_out = __builtin_bit_cast(float, (ex - 8u) << 23);
-  }
   // Steady state, step it: issue chunk it + NS - 1 into the slot chunk it - 1 left (both its
   // stages have run), wait for chunk it + 1 (NS - 2 chunks may stay in flight), run stage A of
   // chunk it + 1, then stage B of chunk it.  Chunk it's staged state lives in st[it % 2]; NS is
@@ -807,14 +655,14 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
     Staged st[2];
     wait_vmcnt<(NS - 2) * NVM>();  // chunk 0 has landed
     tl_mark(p.tl, p.tl_cap, 2);    // diagnostics build: first chunk landed
-    if (n_it > 0) stage_a(std::integral_constant<int, 1 % NS>{}, 0, st[0]);
+    if (n_it > 0) stage_a(std::integral_constant<int, 1 % NS>{}, st[0]);
     for (int base = 0; base < n_it; base += NS) {
       static_for<0, NS>([&](auto ic) __attribute__((always_inline)) {
         constexpr int i = decltype(ic)::value;
         const int it = base + i;
         issue(ic, it + NS - 1);
         wait_vmcnt<(NS - 2) * NVM>();
-        if (it + 1 < n_it) stage_a(std::integral_constant<int, (i + 2) % NS>{}, it + 1, st[(i + 1) & 1]);
+        if (it + 1 < n_it) stage_a(std::integral_constant<int, (i + 2) % NS>{}, st[(i + 1) & 1]);
         if (it < n_it) stage_b(it, st[i & 1]);
       });
     }
@@ -827,7 +675,7 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
         wait_vmcnt<(NS - 1) * NVM>();
         if (it < n_it) {
           Staged st;
-          stage_a(std::integral_constant<int, (i + 1) % NS>{}, it, st);
+          stage_a(std::integral_constant<int, (i + 1) % NS>{}, st);
           stage_b(it, st);
         }
       });
@@ -871,7 +719,6 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
     for (int ww = 1; ww < kAttnWaves; ++ww) mx = fmaxf(mx, mv[ww]);
     const float ms = (mx == -INFINITY) ? 0.f : mx;
     wsc[rb] = fast_exp2(m_run[rb] - ms);
-    if constexpr (BLK) wsc[rb] *= blk_out;
     if (w == 0 && g == 0) {
       float l = 0.f;
 #pragma unroll
@@ -987,9 +834,6 @@ __device__ __forceinline__ void paged_attn_body(const AttnParams& p, uint8_t (&r
     publish(mlp + 1, l);
   }
   tl_mark(p.tl, p.tl_cap, 5);  // diagnostics build: partials issued
-  if constexpr (BLK) {
-    if (p.defer) return;
-  }
   if (!arrive_last(p.counters + prog, n_active, &s_last, p.tl, p.tl_cap)) {
     tl_mark(p.tl, p.tl_cap, 6);  // diagnostics build: hand-off done (not the last split)
     return;
@@ -1117,79 +961,5 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_plan_kernel(AttnParam
   }
 }
 #undef SPECQ_ATTN_LDS
-
-// Merge of block-scaled launches with many splits: workgroup (program, packed row).  Thread t holds
-// split t's (m, l); the row's weights exp2(m - max) / l go to LDS, and the 256 / (D / 4) thread groups
-// sum every such-th split's row, the groups then in order.  The sum's order depends on nothing but
-// the number of splits, and splits in which the row sees nothing add zeros.  Bound by latency: three
-// dependent round trips (length, statistics, rows), the rows' loads eight in flight.
-template <int D>
-__global__ __launch_bounds__(256) void attn_merge_kernel(AttnParams p) {
-  constexpr int LN = D / 4, NG = 256 / LN, IN_FLIGHT = 8;
-  int n_seqs = p.n_seqs, q_len = p.q_len;
-  if (p.plan != nullptr) {
-    n_seqs = min(max(p.plan[0], 0), p.B_grid);
-    q_len = min(max(p.plan[1], 0), p.ql_grid);
-  }
-  n_seqs = uniform(n_seqs);
-  q_len = uniform(q_len);
-  const int per = p.QPP * p.G, rows = (per + 15) / 16 * 16;
-  const int prog = (int)blockIdx.x / per, row = (int)blockIdx.x - prog * per;
-  const int qc = prog % p.n_qc, kvh = (prog / p.n_qc) % p.H_KV, b = prog / (p.n_qc * p.H_KV);
-  const int qi = qc * p.QPP + row / p.G;
-  if (b >= n_seqs || qi >= q_len) return;
-  const int cap = p.max_pages * p.PAGE;
-  const int split_tokens = kAttnUnit * attn_split_units(cap, n_seqs * p.H_KV * attn_row_programs(q_len, p.G), p.target_wgs,
-                                                         kBlkMergeMax);
-  const int L = uniform(min(p.ctx_len[b], cap));
-  const int kv_end = L - q_len + min(qc * p.QPP + p.QPP, q_len);
-  const int n = kv_end > split_tokens ? (kv_end + split_tokens - 1) / split_tokens : 1;
-  if (n == 1) return;  // the row's only split has stored it
-  const int64_t base = (int64_t)prog * p.n_splits * rows + row;  // the row in split 0, in rows
-  const float* ml = p.part + (int64_t)p.B_grid * p.H_KV * p.n_qc * p.n_splits * rows * D;
-  const int t = threadIdx.x;
-  __shared__ float wt[kBlkMergeMax], red[2][4];
-  __shared__ v4f sum[NG][LN];
-  float m = -INFINITY, l = 0.f;
-  if (t < n) {
-    m = ml[(base + (int64_t)t * rows) * 2];
-    l = ml[(base + (int64_t)t * rows) * 2 + 1];
-  }
-  float mx = m;
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-  if (lane_id() == 0) red[0][wave_id()] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  const float w = fast_exp2(m - (mx == -INFINITY ? 0.f : mx));
-  float ls = t < n ? w * l : 0.f;
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) ls += __shfl_xor(ls, o);
-  if (lane_id() == 0) red[1][wave_id()] = ls;
-  wt[t] = t < n ? w : 0.f;
-  __syncthreads();
-  ls = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-  const float inv = ls == 0.f ? 0.f : 1.f / ls;
-  const int g = t / LN, c = t % LN;
-  const v4f* o_part = reinterpret_cast<const v4f*>(p.part) + base * LN + c;
-  v4f o = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = g; s0 < n; s0 += NG * IN_FLIGHT) {
-    v4f x[IN_FLIGHT];
-#pragma unroll
-    for (int u = 0; u < IN_FLIGHT; ++u) x[u] = o_part[(int64_t)min(s0 + u * NG, n - 1) * rows * LN];
-#pragma unroll
-    for (int u = 0; u < IN_FLIGHT; ++u)
-      if (s0 + u * NG < n) o += wt[s0 + u * NG] * x[u];
-  }
-  sum[g][c] = o;
-  __syncthreads();
-  if (g == 0) {
-    for (int i = 1; i < NG; ++i) o += sum[i][c];
-    o *= inv;
-    const int head = kvh * p.G + row % p.G;
-    *reinterpret_cast<v4h*>(p.out + (int64_t)b * p.s_ob + (int64_t)qi * p.s_ot + (int64_t)head * p.s_oh + 4 * c) =
-        v4h{(_Float16)f32_opaque(o.x), (_Float16)f32_opaque(o.y), (_Float16)f32_opaque(o.z), (_Float16)f32_opaque(o.w)};
-  }
-}
 
 }  // namespace specq

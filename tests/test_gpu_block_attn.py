@@ -53,7 +53,7 @@ def test_matches_float64(ctx, q_len, H, H_KV, D, PAGE, SB, fmt):
     out, ck = K.paged_attention_block_scaled(*gpu(q, *cache), q_len)
     torch.cuda.synchronize()
     check(out, ref, q_len, len(ctx), D, "default")
-    assert ck.n_regs > 0 and ("BlockF8" if fmt == "fp8" else "BlockI8") in ck.name
+    assert ck.n_regs > 0 and ("true>" if fmt == "fp8" else "false>") in ck.name
     for b, n in enumerate(ctx):  # rows that see nothing
         assert bool((out[b, :max(0, q_len - n)] == 0).all())
 
