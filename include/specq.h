@@ -407,6 +407,11 @@ int specq_kv_pages_compact(int32_t* block_tbl, int64_t s_bt, int B, int max_page
 int specq_kv_pages_copy(const int32_t* src, const int32_t* dst, int n, int n_pages, int n_tensors, void* const* base,
                         const int64_t* page_stride, const int64_t* page_bytes, void* stream);
 
+/* Calls specq_<name> (specq_rotary, specq_kv_append_block, specq_paged_attn_block or a specq_kv_pages_
+ * function that returns int) with its n arguments as 64-bit words in their order: pointers and integers as they
+ * are, floats as the bits of a double.  For bindings that pay for every argument they convert. */
+int specq_call_packed(const char* name, const int64_t* words, int n);
+
 /* ---------------------------------------------------------------------------------------
  * Elementwise steps around the GEMMs of a verification layer.
  * specq_silu_mul: h[m, n] = fp16( silu(float(gate[m,n])) * float(up[m,n]) ), m < M.

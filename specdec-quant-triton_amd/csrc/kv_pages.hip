@@ -14,8 +14,10 @@
 //            the i-th free page below it.
 //
 // Handing out is a scan of ref by one workgroup of 1024 threads, 16 counts a thread and step, that ends
-// when enough free pages are found.  Bound by latency: a few dependent round trips of about a
-// microsecond each; the page copies behind fork and compact are bound by HBM.
+// when enough free pages are found.  Bound by latency, a few dependent round trips of about a
+// microsecond each, so the first step's counts are loaded ahead of everything else and what one part
+// hands the next stays in LDS where it fits (the table's bits up to kPagesBits words, ids up to kPagesList;
+// the workspace otherwise).  The page copies behind fork and compact are bound by HBM.
 #include "api_common.hpp"
 #include "common.hpp"
 
@@ -25,6 +27,9 @@ constexpr int kPagesThreads = 1024, kPagesWaves = kPagesThreads / kWave;
 constexpr int kPagesPer = 16;  // counts a thread scans per step
 constexpr int kPagesTensors = 64;
 constexpr int kPagesChunk = 16384;  // bytes of a page one workgroup copies at a time
+constexpr int kPagesStep = kPagesThreads * kPagesPer;
+constexpr int kPagesList = 8192;  // page ids kept in LDS
+constexpr int kPagesBits = 4096;  // words of 64 table entries kept in LDS
 
 struct PagesParams {
   int32_t* tbl; int64_t s_bt; int B, C;
@@ -32,9 +37,11 @@ struct PagesParams {
   int32_t* lens; const int32_t* parent; int PAGE;
   int32_t* shortage;  // [1]: pages that could not be given
   int32_t* map;       // compact: [P] the page's id afterwards
-  // Workspace: rows [B] counts then offsets, list [P] free page ids; fork: the new rows [B * C], the
-  // copies' sources and destinations [B] each; compact: moves [P] each, and their number.
-  int32_t* rows; int32_t* list; int32_t* table; int32_t* src; int32_t* dst; int32_t* n_moves;
+  // Workspace: list [P] free page ids; reserve: a bit for each entry [B][ceil(C / 64)] and
+  // (in table) each word's place; fork: the new rows
+  // [B * C] and their lengths [B], the copies' sources and destinations [B] each; compact: moves [P] each, and
+  // their number.
+  uint64_t* bits; int32_t* rows; int32_t* list; int32_t* table; int32_t* src; int32_t* dst; int32_t* n_moves;
 };
 
 struct PagesCopyParams {
@@ -43,6 +50,9 @@ struct PagesCopyParams {
   int32_t first[kPagesTensors + 1];                     // chunks of the tensors before this one
   const int32_t* src; const int32_t* dst; const int32_t* n_dev;
   int n, P, tensors, vec;  // vec: bytes of one access, 16, 4 or 1
+  int large;               // tensors whose pages are cut into chunks; the others go with a page's first chunk
+  // compact: the workgroups ahead of the copies' put the table under the new ids.
+  int remap; int32_t* tbl; int64_t s_bt; int B, C; const int32_t* map;
 };
 
 // Columns of a row that n tokens fill.
@@ -53,12 +63,14 @@ __device__ __forceinline__ bool is_page(int id, int P) { return (uint32_t)id < (
 
 // Exclusive prefix of x over the workgroup; `total` is the sum.
 __device__ __forceinline__ int block_prefix(int x, int& total, int (&part)[kPagesWaves]) {
+  // Inclusive sums over the wave: within rows of 16 lanes, then the row before, then the two before.
   int v = x;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int y = __shfl_up(v, o);
-    if (lane_id() >= o) v += y;
-  }
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
   __syncthreads();  // the last call's readers of part are done
   if (lane_id() == kWave - 1) part[wave_id()] = v;
   __syncthreads();
@@ -73,18 +85,51 @@ __device__ __forceinline__ int block_prefix(int x, int& total, int (&part)[kPage
   return before + v - x;
 }
 
-// The lowest `need` ids with ref <= 0, in order, to list; returns how many there are (at most need).
-__device__ __forceinline__ int find_free(const int32_t* ref, int P, int need, int32_t* list, int (&part)[kPagesWaves]) {
-  int found = 0;
-  for (int base = 0; base < P && found < need; base += kPagesThreads * kPagesPer) {
-    const int at = base + (int)threadIdx.x * kPagesPer;
-    uint32_t free_bits = 0;
+// The thread's 16 counts from page `base` on (its own 64 bytes of ref); pages past the pool count as `past`.
+struct PageCounts {
+  v4i x[kPagesPer / 4];
+  __device__ __forceinline__ uint32_t used() const {
+    uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < kPagesPer; ++i)
-      if (at + i < P && ref[at + i] <= 0) free_bits |= 1u << i;
+    for (int i = 0; i < kPagesPer; ++i) bits |= (uint32_t)(x[i / 4][i % 4] > 0) << i;
+    return bits;
+  }
+};
+__device__ __forceinline__ PageCounts load_counts(const int32_t* ref, int P, int base, int past) {
+  const int at = base + (int)threadIdx.x * kPagesPer;
+  PageCounts c;
+  if (at + kPagesPer <= P && ((uintptr_t)ref & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < kPagesPer / 4; ++i) c.x[i] = reinterpret_cast<const v4i*>(ref + at)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPagesPer; ++i) c.x[i / 4][i % 4] = at + i < P ? ref[at + i] : past;
+  }
+  return c;
+}
+
+// Page ids in order: the first kPagesList in LDS, the rest in the workspace.
+struct PageList {
+  int* near;
+  int32_t* far;
+  __device__ __forceinline__ void put(int i, int id) const {
+    if (i < kPagesList) near[i] = id;
+    else far[i] = id;
+  }
+  __device__ __forceinline__ int get(int i) const { return i < kPagesList ? near[i] : far[i]; }
+};
+
+// The lowest `need` free ids, in order, to list; returns how many there are (at most need).  `first`: the
+// first step's used().
+__device__ __forceinline__ int find_free(const int32_t* ref, int P, int need, uint32_t first, const PageList& list,
+                                         int (&part)[kPagesWaves]) {
+  int found = 0;
+  for (int base = 0; base < P && found < need; base += kPagesStep) {
+    uint32_t free_bits = ~(base == 0 ? first : load_counts(ref, P, base, 1).used()) & ((1u << kPagesPer) - 1);
     int total;
     int rank = found + block_prefix(__popc(free_bits), total, part);
-    for (; free_bits != 0 && rank < need; free_bits &= free_bits - 1) list[rank++] = at + __ffs(free_bits) - 1;
+    for (; free_bits != 0 && rank < need; free_bits &= free_bits - 1)
+      list.put(rank++, base + (int)threadIdx.x * kPagesPer + __ffs(free_bits) - 1);
     found += total;
   }
   __syncthreads();
@@ -92,48 +137,68 @@ __device__ __forceinline__ int find_free(const int32_t* ref, int P, int need, in
 }
 
 __global__ __launch_bounds__(kPagesThreads) void pages_reserve_kernel(PagesParams p) {
-  __shared__ int part[kPagesWaves];
+  __shared__ int part[kPagesWaves], near_list[kPagesList];
+  __shared__ uint64_t near_bits[kPagesBits];
+  __shared__ int near_at[kPagesBits];
   const int lane = lane_id(), w = uniform(wave_id());
-  // A wave counts the entries that want a page, row by row; then the rows' offsets.
-  for (int b = w; b < p.B; b += kPagesWaves) {
-    const int np = pages_of(p.lens[b], p.PAGE, p.C);
-    int n = 0;
-    for (int c0 = 0; c0 < np; c0 += kWave) {
-      const int c = c0 + lane;
-      const bool want = c < np && !is_page(p.tbl[b * p.s_bt + c], p.P);
-      n += __popcll(__builtin_amdgcn_ballot_w64(want));
+  const PageCounts first = load_counts(p.ref, p.P, 0, 1);
+  // A word for each 64 entries of a row, with the bits of those that want a page: eight to a wave in flight.
+  const int words = (p.C + kWave - 1) / kWave, units = p.B * words;
+  uint64_t* bits = units <= kPagesBits ? near_bits : p.bits;
+  int* at = units <= kPagesBits ? near_at : p.table;
+  constexpr int U = 8;
+  for (int u0 = w * U; u0 < units; u0 += kPagesWaves * U) {
+    int id[U], np[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = min(u0 + i, units - 1), b = u / words, c = (u - b * words) * kWave + lane;
+      np[i] = pages_of(p.lens[b], p.PAGE, p.C) - (u - b * words) * kWave;  // columns of the word that count
+      id[i] = p.tbl[b * p.s_bt + min(c, p.C - 1)];
     }
-    if (lane == 0) p.rows[b] = n;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const uint64_t m = __builtin_amdgcn_ballot_w64(lane < np[i] && !is_page(id[i], p.P));
+      if (lane == 0 && u0 + i < units) bits[u0 + i] = m;
+    }
   }
   __syncthreads();
+  // Each word's place among the wants, four words to a thread.
+  constexpr int WPT = 4;
   int need = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kPagesThreads) {
-    const int b = b0 + (int)threadIdx.x;
-    const int n = b < p.B ? p.rows[b] : 0;
-    int total;
-    const int off = need + block_prefix(n, total, part);
-    if (b < p.B) p.rows[b] = n > 0 ? off : -1;
+  for (int base = 0; base < units; base += kPagesThreads * WPT) {
+    int n[WPT], all = 0, total;
+#pragma unroll
+    for (int i = 0; i < WPT; ++i) {
+      const int u = base + (int)threadIdx.x * WPT + i;
+      n[i] = u < units ? __popcll(bits[u]) : 0;
+      all += n[i];
+    }
+    int rank = need + block_prefix(all, total, part);
+#pragma unroll
+    for (int i = 0; i < WPT; ++i) {
+      const int u = base + (int)threadIdx.x * WPT + i;
+      if (u < units) at[u] = rank;
+      rank += n[i];
+    }
     need += total;
   }
-  __syncthreads();
-  const int found = find_free(p.ref, p.P, need, p.list, part);
+  const PageList list = {near_list, p.list};
+  const int found = find_free(p.ref, p.P, need, first.used(), list, part);
   if (threadIdx.x == 0) *p.shortage = need - found;
   if (need == 0) return;
-  for (int b = w; b < p.B; b += kPagesWaves) {
-    int rank = p.rows[b];
-    if (rank < 0) continue;
-    const int np = pages_of(p.lens[b], p.PAGE, p.C);
-    for (int c0 = 0; c0 < np; c0 += kWave) {
-      const int c = c0 + lane;
-      const bool want = c < np && !is_page(p.tbl[b * p.s_bt + c], p.P);
-      const uint64_t m = __builtin_amdgcn_ballot_w64(want);
-      if (want) {
-        const int r = rank + __popcll(m & ((1ull << lane) - 1));
-        const int id = r < found ? p.list[r] : -1;
-        p.tbl[b * p.s_bt + c] = id;
-        if (id >= 0) p.ref[id] = 1;
-      }
-      rank += __popcll(m);
+  // Words are dealt to the waves in turn; a wave looks at 64 of its at once and hands out those that want any, a
+  // lane to an entry.
+  for (int u0 = w; u0 < units; u0 += kPagesThreads) {
+    const int mine = u0 + kPagesWaves * lane;
+    uint64_t todo = __builtin_amdgcn_ballot_w64(mine < units && bits[min(mine, units - 1)] != 0);
+    for (; todo != 0; todo &= todo - 1) {
+      const int u = uniform(u0 + kPagesWaves * (__ffsll((unsigned long long)todo) - 1)), b = u / words;
+      const uint64_t m = bits[u];
+      if (((m >> lane) & 1) == 0) continue;
+      const int rank = at[u] + __popcll(m & ((1ull << lane) - 1));
+      const int id = rank < found ? list.get(rank) : -1;
+      p.tbl[b * p.s_bt + (u - b * words) * kWave + lane] = id;
+      if (id >= 0) p.ref[id] = 1;
     }
   }
 }
@@ -202,7 +267,8 @@ __global__ __launch_bounds__(kPagesThreads) void pages_fork_assign_kernel(PagesP
     }
     return;
   }
-  __shared__ int part[kPagesWaves];
+  __shared__ int part[kPagesWaves], near_list[kPagesList];
+  const PageCounts first = load_counts(p.ref, p.P, 0, 1);
   int need = 0;
   for (int b0 = 0; b0 < p.B; b0 += kPagesThreads) {
     const int b = b0 + (int)threadIdx.x;
@@ -212,13 +278,13 @@ __global__ __launch_bounds__(kPagesThreads) void pages_fork_assign_kernel(PagesP
     if (b < p.B) p.dst[b] = want ? r : -1;
     need += total;
   }
-  __syncthreads();
-  const int found = find_free(p.ref, p.P, need, p.list, part);
+  const PageList list = {near_list, p.list};
+  const int found = find_free(p.ref, p.P, need, first.used(), list, part);
   if (threadIdx.x == 0) *p.shortage = need - found;
-  for (int b = threadIdx.x; b < p.B; b += kPagesThreads) {
+  for (int b = threadIdx.x; b < p.B; b += kPagesThreads) {  // the rows this thread ranked
     const int r = p.dst[b];
     if (r < 0) continue;
-    const int id = r < found ? p.list[r] : -1;
+    const int id = r < found ? list.get(r) : -1;
     p.tbl[b * p.s_bt + p.rows[b] / p.PAGE] = id;
     p.dst[b] = id;
     if (id >= 0) p.ref[id] = 1;
@@ -227,24 +293,32 @@ __global__ __launch_bounds__(kPagesThreads) void pages_fork_assign_kernel(PagesP
 
 // Compact, the plan: the moves in order, every page's id afterwards, and the counts as they will be.
 __global__ __launch_bounds__(kPagesThreads) void pages_compact_kernel(PagesParams p) {
-  __shared__ int part[kPagesWaves];
+  __shared__ int part[kPagesWaves], near_list[kPagesList];
+  const PageCounts first = load_counts(p.ref, p.P, 0, 0);
+  auto counts = [&](int base) { return base == 0 ? first : load_counts(p.ref, p.P, base, 0); };
   int used = 0;
-  for (int base = 0; base < p.P; base += kPagesThreads * kPagesPer) {
-    const int at = base + (int)threadIdx.x * kPagesPer;
-    int n = 0, total;
-#pragma unroll
-    for (int i = 0; i < kPagesPer; ++i) n += at + i < p.P && p.ref[at + i] > 0;
-    block_prefix(n, total, part);
+  for (int base = 0; base < p.P; base += kPagesStep) {
+    int total;
+    block_prefix(__popc(counts(base).used()), total, part);
     used += total;
   }
-  const int moves = find_free(p.ref, used, used, p.dst, part);  // the free pages below `used`
+  // The free pages below `used`, as many as there are used ones past it.
+  const PageList holes = {near_list, p.list};
+  int found = 0;
+  for (int base = 0; base < used; base += kPagesStep) {
+    const int at = base + (int)threadIdx.x * kPagesPer, below = min(max(used - at, 0), kPagesPer);
+    uint32_t bits = ~counts(base).used() & ((1u << below) - 1);
+    int total;
+    int rank = found + block_prefix(__popc(bits), total, part);
+    for (; bits != 0; bits &= bits - 1) holes.put(rank++, at + __ffs(bits) - 1);
+    found += total;
+  }
+  __syncthreads();
   int done = 0;
-  for (int base = 0; base < p.P; base += kPagesThreads * kPagesPer) {
-    const int at = base + (int)threadIdx.x * kPagesPer;
-    uint32_t bits = 0;
-#pragma unroll
-    for (int i = 0; i < kPagesPer; ++i)
-      if (at + i < p.P && at + i >= used && p.ref[at + i] > 0) bits |= 1u << i;
+  for (int base = 0; base < p.P; base += kPagesStep) {
+    const int at = base + (int)threadIdx.x * kPagesPer, below = min(max(used - at, 0), kPagesPer);
+    const PageCounts c = counts(base);
+    const uint32_t bits = c.used() & ~((1u << below) - 1);
     int total;
     int rank = done + block_prefix(__popc(bits), total, part);
 #pragma unroll
@@ -252,29 +326,17 @@ __global__ __launch_bounds__(kPagesThreads) void pages_compact_kernel(PagesParam
       if (at + i >= p.P) continue;
       int to = at + i;
       if ((bits >> i) & 1) {
-        to = p.dst[rank];
-        p.src[rank++] = at + i;
-        p.ref[to] = p.ref[at + i];
+        to = holes.get(rank);
+        p.src[rank] = at + i;
+        p.dst[rank++] = to;
+        p.ref[to] = c.x[i / 4][i % 4];
         p.ref[at + i] = 0;
       }
       p.map[at + i] = to;
     }
     done += total;
   }
-  if (threadIdx.x == 0) *p.n_moves = moves;
-}
-
-// The table under the new ids.
-__global__ __launch_bounds__(256) void pages_remap_kernel(PagesParams p) {
-  const int64_t n = (int64_t)p.B * p.C;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
-    const int b = (int)(e / p.C);
-    int32_t* at = p.tbl + b * p.s_bt + (e - (int64_t)b * p.C);
-    const int id = *at;
-    if (!is_page(id, p.P)) continue;
-    const int to = p.map[id];
-    if (to != id) *at = to;
-  }
+  if (threadIdx.x == 0) *p.n_moves = found;
 }
 
 template <typename T>
@@ -294,28 +356,49 @@ __device__ __forceinline__ void copy_chunk(const uint8_t* src, uint8_t* dst, int
   for (; i < n; i += 256) d[i] = s[i];
 }
 
-// Pages src[i] -> dst[i] of every tensor; a pair with an id outside the pool is left out.
+// Pages src[i] -> dst[i] of every tensor; a pair with an id outside the pool is left out.  A unit is a chunk of
+// kPagesChunk bytes of a large tensor's page, four 16-byte loads a thread in flight; pages of at most a
+// quarter of that (scales) would leave most of a unit idle, and are copied with their pair's first one.
 __global__ __launch_bounds__(256) void pages_copy_kernel(PagesCopyParams p) {
+  if ((int)blockIdx.x < p.remap) {
+    const int64_t n = (int64_t)p.B * p.C;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)p.remap * 256) {
+      const int b = (int)(e / p.C);
+      int32_t* at = p.tbl + b * p.s_bt + (e - (int64_t)b * p.C);
+      const int id = *at;
+      if (!is_page(id, p.P)) continue;
+      const int to = p.map[id];
+      if (to != id) *at = to;
+    }
+    return;
+  }
   const int pairs = p.n_dev != nullptr ? min(uniform(*p.n_dev), p.n) : p.n;
-  const int per = p.first[p.tensors];
-  for (int64_t u = blockIdx.x; u < (int64_t)pairs * per; u += gridDim.x) {
+  const int per = max(p.first[p.large], 1);
+  for (int64_t u = (int)blockIdx.x - p.remap; u < (int64_t)pairs * per; u += (int)gridDim.x - p.remap) {
     const int pair = (int)(u / per), k = (int)(u - (int64_t)pair * per);
     const int from = uniform(p.src[pair]), to = uniform(p.dst[pair]);
     if (!is_page(from, p.P) || !is_page(to, p.P) || from == to) continue;
-    int i = 0;
-    while (k >= p.first[i + 1]) ++i;
-    const int64_t off = (int64_t)(k - p.first[i]) * kPagesChunk;
-    const uint8_t* s = p.base[i] + from * p.stride[i] + off;
-    uint8_t* d = p.base[i] + to * p.stride[i] + off;
-    const int64_t left = p.bytes[i] - off;
-    const int bytes = left < kPagesChunk ? (int)left : kPagesChunk;
-    if (p.vec == 16) copy_chunk<v4i>(s, d, bytes);
-    else if (p.vec == 4) copy_chunk<int>(s, d, bytes);
-    else copy_chunk<uint8_t>(s, d, bytes);
+    auto copy = [&](int i, int64_t off, int bytes) {
+      const uint8_t* s = p.base[i] + from * p.stride[i] + off;
+      uint8_t* d = p.base[i] + to * p.stride[i] + off;
+      if (p.vec == 16) copy_chunk<v4i>(s, d, bytes);
+      else if (p.vec == 4) copy_chunk<int>(s, d, bytes);
+      else copy_chunk<uint8_t>(s, d, bytes);
+    };
+    if (k < p.first[p.large]) {
+      int i = 0;
+      while (k >= p.first[i + 1]) ++i;
+      const int64_t off = (int64_t)(k - p.first[i]) * kPagesChunk, left = p.bytes[i] - off;
+      copy(i, off, left < kPagesChunk ? (int)left : kPagesChunk);
+    }
+    if (k == 0)
+      for (int i = p.large; i < p.tensors; ++i) copy(i, 0, (int)p.bytes[i]);
   }
 }
 
-static size_t pages_ints(int B, int C, int P) { return (size_t)B * C + 3 * (size_t)B + 3 * (size_t)P + 16; }
+static size_t pages_ints(int B, int C, int P) {
+  return 2 * (size_t)B * ceil_div(C, 64) + (size_t)B * C + 3 * (size_t)B + 3 * (size_t)P + 16;
+}
 
 static int pages_setup(PagesParams& p, const char* who, int32_t* tbl, int64_t s_bt, int B, int C, int32_t* ref, int P,
                        int PAGE) {
@@ -324,7 +407,7 @@ static int pages_setup(PagesParams& p, const char* who, int32_t* tbl, int64_t s_
                 "%s: bad sizes B=%d columns=%d pages=%d PAGE=%d", who, B, C, P, PAGE);
   SPECQ_REQUIRE((int64_t)C * PAGE <= INT32_MAX && P <= INT32_MAX - kPagesThreads * kPagesPer, SPECQ_ENOTSUP,
                 "%s: a row of %lld tokens or a pool of %d pages is too large", who, (long long)C * PAGE, P);
-  SPECQ_REQUIRE((int64_t)B * ceil_div(C, 1024) <= INT32_MAX, SPECQ_ENOTSUP, "%s: block table too large", who);
+  SPECQ_REQUIRE((int64_t)B * ceil_div(C, 64) <= INT32_MAX / 2, SPECQ_ENOTSUP, "%s: block table too large", who);
   p = {};
   p.tbl = tbl; p.s_bt = s_bt; p.B = B; p.C = C; p.ref = ref; p.P = P; p.PAGE = PAGE;
   return SPECQ_OK;
@@ -336,7 +419,8 @@ static int pages_scratch(PagesParams& p, const char* who, void* workspace, size_
                 workspace ? bytes : (size_t)0);
   int32_t* at = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + kCounterBytes);
   p.n_moves = at;
-  p.rows = at + 16;
+  p.bits = reinterpret_cast<uint64_t*>(at + 16);
+  p.rows = at + 16 + 2 * (int64_t)p.B * ceil_div(p.C, 64);
   p.list = p.rows + p.B;
   p.src = p.list + p.P;
   p.dst = p.src + (p.B > p.P ? p.B : p.P);
@@ -354,24 +438,36 @@ static int pages_tensors(const char* who, int n, void* const* base, const int64_
 }
 
 static int pages_copy(int n_tensors, void* const* base, const int64_t* stride, const int64_t* bytes, const int32_t* src,
-                      const int32_t* dst, int n, const int32_t* n_dev, int P, hipStream_t stream) {
-  for (int t0 = 0; t0 < n_tensors; t0 += kPagesTensors) {
+                      const int32_t* dst, int n, const int32_t* n_dev, int P, const PagesParams* remap,
+                      hipStream_t stream) {
+  for (int t0 = 0; t0 < n_tensors || (t0 == 0 && remap != nullptr); t0 += kPagesTensors) {
     PagesCopyParams c = {};
-    c.tensors = n_tensors - t0 < kPagesTensors ? n_tensors - t0 : kPagesTensors;
+    const int t1 = n_tensors - t0 < kPagesTensors ? n_tensors : t0 + kPagesTensors;
     uint64_t bits = 0;
-    for (int i = 0; i < c.tensors; ++i) {
-      c.base[i] = static_cast<uint8_t*>(base[t0 + i]);
-      c.stride[i] = stride[t0 + i];
-      c.bytes[i] = bytes[t0 + i];
-      c.first[i + 1] = c.first[i] + (int)ceil_div64(bytes[t0 + i], kPagesChunk);
-      bits |= (uintptr_t)base[t0 + i] | (uint64_t)stride[t0 + i] | (uint64_t)bytes[t0 + i];
+    for (int small = 0; small < 2; ++small) {  // the large tensors first
+      for (int t = t0; t < t1; ++t) {
+        if ((bytes[t] <= kPagesChunk / 4) != (small == 1)) continue;
+        const int i = c.tensors++;
+        c.base[i] = static_cast<uint8_t*>(base[t]);
+        c.stride[i] = stride[t];
+        c.bytes[i] = bytes[t];
+        c.first[i + 1] = c.first[i] + (small ? 0 : (int)ceil_div64(bytes[t], kPagesChunk));
+        bits |= (uintptr_t)base[t] | (uint64_t)stride[t] | (uint64_t)bytes[t];
+      }
+      if (small == 0) c.large = c.tensors;
     }
     c.vec = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
     c.src = src; c.dst = dst; c.n_dev = n_dev; c.n = n; c.P = P;
-    // Eight workgroups of 256 threads to a CU, each walking its chunks.
-    const int64_t units = (int64_t)n * c.first[c.tensors], most = 8ll * device_cus();
-    const int rc = launch(reinterpret_cast<const void*>(&pages_copy_kernel), (int)(units < most ? units : most), 256, 0,
-                          stream, &c);
+    if (remap != nullptr && t0 == 0) {
+      const int64_t wgs = ceil_div64((int64_t)remap->B * remap->C, 1024);
+      c.remap = (int)(wgs < 256 ? wgs : 256);
+      c.tbl = remap->tbl; c.s_bt = remap->s_bt; c.B = remap->B; c.C = remap->C; c.map = remap->map;
+    }
+    // Eight workgroups of 256 threads to a CU, each walking its units.
+    const int per = c.first[c.large] > 1 ? c.first[c.large] : 1;
+    const int64_t units = c.tensors == 0 ? 0 : (int64_t)n * per, most = 8ll * device_cus();
+    const int rc = launch(reinterpret_cast<const void*>(&pages_copy_kernel), c.remap + (int)(units < most ? units : most),
+                          256, 0, stream, &c);
     if (rc != SPECQ_OK) return rc;
   }
   return SPECQ_OK;
@@ -428,7 +524,7 @@ extern "C" int specq_kv_pages_fork(int32_t* block_tbl, int64_t s_bt, int B, int 
   if (int rc = launch(reinterpret_cast<const void*>(&pages_fork_assign_kernel), 1 + (int)(back < 512 ? back : 512),
                       kPagesThreads, 0, st, &p))
     return rc;
-  return pages_copy(n_tensors, base, page_stride, page_bytes, p.src, p.dst, B, nullptr, n_pages, st);
+  return pages_copy(n_tensors, base, page_stride, page_bytes, p.src, p.dst, B, nullptr, n_pages, nullptr, st);
 }
 
 extern "C" int specq_kv_pages_compact(int32_t* block_tbl, int64_t s_bt, int B, int max_pages, int32_t* ref, int n_pages,
@@ -444,10 +540,7 @@ extern "C" int specq_kv_pages_compact(int32_t* block_tbl, int64_t s_bt, int B, i
   p.map = page_map;
   hipStream_t st = (hipStream_t)stream;
   if (int rc = launch(reinterpret_cast<const void*>(&pages_compact_kernel), 1, kPagesThreads, 0, st, &p)) return rc;
-  const int64_t wgs = ceil_div64((int64_t)B * max_pages, 1024);
-  if (int rc = launch(reinterpret_cast<const void*>(&pages_remap_kernel), (int)(wgs < 2048 ? wgs : 2048), 256, 0, st, &p))
-    return rc;
-  return pages_copy(n_tensors, base, page_stride, page_bytes, p.src, p.dst, n_pages, p.n_moves, n_pages, st);
+  return pages_copy(n_tensors, base, page_stride, page_bytes, p.src, p.dst, n_pages, p.n_moves, n_pages, &p, st);
 }
 
 extern "C" int specq_kv_pages_copy(const int32_t* src, const int32_t* dst, int n, int n_pages, int n_tensors,
@@ -457,5 +550,5 @@ extern "C" int specq_kv_pages_copy(const int32_t* src, const int32_t* dst, int n
   SPECQ_REQUIRE(n >= 0 && n_pages > 0 && (n == 0 || (src && dst)), SPECQ_EINVAL, "kv_pages_copy: bad sizes or pointers");
   if (int rc = pages_tensors("kv_pages_copy", n_tensors, base, page_stride, page_bytes)) return rc;
   if (n == 0) return SPECQ_OK;
-  return pages_copy(n_tensors, base, page_stride, page_bytes, src, dst, n, nullptr, n_pages, (hipStream_t)stream);
+  return pages_copy(n_tensors, base, page_stride, page_bytes, src, dst, n, nullptr, n_pages, nullptr, (hipStream_t)stream);
 }

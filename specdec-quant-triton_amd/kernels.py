@@ -52,7 +52,9 @@ Differences a caller may notice:
 """
 from __future__ import annotations
 
+import array
 import ctypes
+import functools
 import math
 import os
 import sys
@@ -1006,33 +1008,25 @@ def w4a8_matmul(a_q, sa, wq, sw, out=None, BLOCK_M=16, BLOCK_N=None, BLOCK_K=128
 # ----------------------------------------------------------------------------------------
 # Rotary positions, and the paged cache with block scales (no reference counterpart)
 # ----------------------------------------------------------------------------------------
-class _Here:
-    """Context of a call whose tensors live on the current device: nothing to switch."""
-
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE_CTX = _Here()
+def _gpu_of(who: str, *ts) -> int:
+    """The index of the GPU that holds all tensors (None left out)."""
+    dev = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise RuntimeError(f"{who}: tensors on {ts[0].device} and {t.device}")
+    if dev < 0 or ts[0].device.type != "cuda":
+        raise RuntimeError(f"specq kernels run on the GPU only; got a {ts[0].device} tensor")
+    return dev
 
 
-def _on_one_device(who: str, *ts):
-    """All tensors (None left out) on one GPU; the context that makes it the current one, so that the
-    launch and the CU count are that GPU's."""
-    dev = ts[0].device
-    if dev.type != "cuda":
-        raise RuntimeError(f"specq kernels run on the GPU only; got a {dev} tensor")
-    for t in ts[1:]:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"{who}: tensors on {dev} and {t.device}")
-    return _HERE_CTX if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
-def _raw_stream(t: torch.Tensor) -> int:
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+def _call_on(dev: int, name: str, *args) -> None:
+    """Call an entry point on GPU `dev`'s current stream (its last argument), with that GPU the current one, so
+    that the launch and the CU count are its own."""
+    if dev == torch._C._cuda_getDevice():
+        _lib.packed(name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.packed(name)(*args, torch._C._cuda_getCurrentRawStream(dev))
 
 
 def _plan_of(plan, need: int, who: str) -> int:
@@ -1111,7 +1105,7 @@ def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, inter
     are not written (an omitted output holds anything there).
     """
     who = "rotary_embed"
-    ctx = _on_one_device(who, q, k, inv_freq, ctx_len, positions, plan, q_out, k_out)
+    dev = _gpu_of(who, q, k, inv_freq, ctx_len, positions, plan, q_out, k_out)
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
         raise RuntimeError(f"{who}: q [B, QL, H, D] and k [B, QL, H_KV, D] expected")
     B, QL, H, D = q.shape
@@ -1149,12 +1143,11 @@ def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, inter
         return q_out, k_out
     qs, qo = q.stride(), q_out.stride()
     ks, ko = (k.stride(), k_out.stride()) if k is not None else ((0, 0, 0), (0, 0, 0))
-    with ctx:
-        _lib.call("specq_rotary", q.data_ptr(), qs[0], qs[1], qs[2], _ptr(k), ks[0], ks[1], ks[2],
-                  q_out.data_ptr(), qo[0], qo[1], qo[2], _ptr(k_out), ko[0], ko[1], ko[2],
-                  inv_freq.data_ptr(), 1 if inv_freq.dtype == torch.float64 else 0, float(mscale),
-                  _ptr(ctx_len), _ptr(positions), s_pb, Bg, n_seqs, q_len, Qg, H, H_KV, D, R,
-                  1 if interleaved else 0, _plan_of(plan, 2, who), _raw_stream(q))
+    _call_on(dev, "specq_rotary", q.data_ptr(), qs[0], qs[1], qs[2], _ptr(k), ks[0], ks[1], ks[2],
+             q_out.data_ptr(), qo[0], qo[1], qo[2], _ptr(k_out), ko[0], ko[1], ko[2],
+             inv_freq.data_ptr(), inv_freq.dtype == torch.float64, mscale,
+             _ptr(ctx_len), _ptr(positions), s_pb, Bg, n_seqs, q_len, Qg, H, H_KV, D, R,
+             bool(interleaved), _plan_of(plan, 2, who))
     return q_out, k_out
 
 
@@ -1196,7 +1189,7 @@ def paged_kv_append_block_scaled(k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_le
     and the grid covers (B, QLMAX).
     """
     who = "paged_kv_append_block_scaled"
-    ctx = _on_one_device(who, k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_len, plan)
+    dev = _gpu_of(who, k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_len, plan)
     if k_new.dim() != 4 or v_new.shape != k_new.shape:
         raise RuntimeError(f"{who}: k_new and v_new must have one shape [B, QLMAX, H_KV, D]")
     if k_new.dtype != torch.float16 or v_new.dtype != torch.float16:
@@ -1209,13 +1202,24 @@ def paged_kv_append_block_scaled(k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_le
     if Bg == 0 or Qg == 0:
         return
     kn, cs, ss = k_new.stride(), kc.stride(), ks.stride()
-    with ctx:
-        _lib.call("specq_kv_append_block", k_new.data_ptr(), v_new.data_ptr(), kn[0], kn[1], kn[2],
-                  kc.data_ptr(), vc.data_ptr(), 1 if f8 else 0, cs[0], cs[1], cs[2],
-                  ks.data_ptr(), vs.data_ptr(), ss[0], ss[1], ss[2], sb,
-                  block_tbl.data_ptr(), block_tbl.stride(0), block_tbl.shape[1], min(kc.shape[0], 2**31 - 1),
-                  ctx_len.data_ptr(), Bg, n_seqs, q_len, Qg, H_KV, D, kc.shape[1], _plan_of(plan, 2, who),
-                  _raw_stream(k_new))
+    _call_on(dev, "specq_kv_append_block", k_new.data_ptr(), v_new.data_ptr(), kn[0], kn[1], kn[2],
+             kc.data_ptr(), vc.data_ptr(), f8, cs[0], cs[1], cs[2],
+             ks.data_ptr(), vs.data_ptr(), ss[0], ss[1], ss[2], sb,
+             block_tbl.data_ptr(), block_tbl.stride(0), block_tbl.shape[1], min(kc.shape[0], 2**31 - 1),
+             ctx_len.data_ptr(), Bg, n_seqs, q_len, Qg, H_KV, D, kc.shape[1], _plan_of(plan, 2, who))
+
+
+@functools.lru_cache(maxsize=None)
+def _block_attn_workspace(Bg, H, H_KV, Qg, QPP, max_pages, PAGE, dev, options) -> int:
+    """Bytes a call needs: a function of its sizes, the GPU's CU count and the library options."""
+    with torch.cuda.device(dev):
+        return _lib.lib().specq_paged_attn_block_workspace_size(Bg, H, H_KV, Qg, QPP, max_pages, PAGE)
+
+
+@functools.lru_cache(maxsize=None)
+def _block_attn_info(D, f8, rows, dev) -> KernelInfo:
+    with torch.cuda.device(dev):
+        return KernelInfo(2, D | (1 << 18 if f8 else 1 << 17), 0, 0, 0, rows, 0, 4, 0)
 
 
 def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=None, QPP=None, plan=None, n_seqs=None,
@@ -1232,7 +1236,7 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
     there).  Calls that may run at the same time on several streams need a workspace each.
     """
     who = "paged_attention_block_scaled"
-    ctx = _on_one_device(who, q, kc, vc, ks, vs, block_tbl, ctx_len, plan, out)
+    dev = _gpu_of(who, q, kc, vc, ks, vs, block_tbl, ctx_len, plan, out)
     if q.dim() != 4 or q.dtype != torch.float16 or q.stride(3) != 1:
         raise RuntimeError(f"{who} expects fp16 q [B, QLMAX, H, D] with contiguous head_dim")
     B, QL, H, D = q.shape
@@ -1253,21 +1257,19 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
     PAGE, max_pages = kc.shape[1], block_tbl.shape[1]
     qs, cs, ss, os_ = q.stride(), kc.stride(), ks.stride(), out.stride()
     QPP = int(QPP)
-    with ctx:
-        ck = KernelInfo(2, D | (1 << 18 if f8 else 1 << 17), 0, 0, 0, QPP * G, 0, 4, 0)
-        if Bg == 0 or Qg == 0:
-            return out, ck
-        need = _lib.lib().specq_paged_attn_block_workspace_size(Bg, H, H_KV, Qg, QPP, max_pages, PAGE)
-        wptr, wbytes = (workspace or _ws.shared(q.device)).ensure(need)
-        _lib.call("specq_paged_attn_block", q.data_ptr(), qs[0], qs[1], qs[2],
-                  kc.data_ptr(), vc.data_ptr(), 1 if f8 else 0, cs[0], cs[1], cs[2],
-                  ks.data_ptr(), vs.data_ptr(), ss[0], ss[1], ss[2], sb,
-                  block_tbl.data_ptr(), block_tbl.stride(0), max_pages, min(kc.shape[0], 2**31 - 1),
-                  ctx_len.data_ptr(), out.data_ptr(), os_[0], os_[1], os_[2],
-                  Bg, n_seqs, q_len, Qg, H, H_KV, D, PAGE, QPP,
-                  1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), _plan_of(plan, 2, who),
-                  wptr, wbytes, _raw_stream(q))
-    _paged_attn_kernel._note(q.device.index, (D, (QPP * G + 15) // 16, str(kc.dtype)))
+    ck = _block_attn_info(D, f8, QPP * G, dev)
+    if Bg == 0 or Qg == 0:
+        return out, ck
+    need = _block_attn_workspace(Bg, H, H_KV, Qg, QPP, max_pages, PAGE, dev, _lib.options_key())
+    wptr, wbytes = (workspace or _ws.shared_cuda(dev)).ensure(need)
+    _call_on(dev, "specq_paged_attn_block", q.data_ptr(), qs[0], qs[1], qs[2],
+             kc.data_ptr(), vc.data_ptr(), f8, cs[0], cs[1], cs[2],
+             ks.data_ptr(), vs.data_ptr(), ss[0], ss[1], ss[2], sb,
+             block_tbl.data_ptr(), block_tbl.stride(0), max_pages, min(kc.shape[0], 2**31 - 1),
+             ctx_len.data_ptr(), out.data_ptr(), os_[0], os_[1], os_[2],
+             Bg, n_seqs, q_len, Qg, H, H_KV, D, PAGE, QPP,
+             D ** -0.5 if sm_scale is None else sm_scale, _plan_of(plan, 2, who), wptr, wbytes)
+    _paged_attn_kernel._note(dev, (D, (QPP * G + 15) // 16, kc.dtype))
     return out, ck
 
 
@@ -1275,8 +1277,8 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
 # Page tables of the paged caches
 # ----------------------------------------------------------------------------------------
 def _page_state(who: str, block_tbl, ref, *vecs):
-    """Checks the table, the counts and per-row vectors (name, tensor); returns (context, B, C, P)."""
-    ctx = _on_one_device(who, block_tbl, ref, *(t for _, t in vecs))
+    """Checks the table, the counts and per-row vectors (name, tensor); returns (GPU, B, C, P)."""
+    dev = _gpu_of(who, block_tbl, ref, *(t for _, t in vecs))
     if block_tbl.dtype != torch.int32 or block_tbl.dim() != 2 or block_tbl.shape[0] < 1 or block_tbl.shape[1] < 1 or \
             (block_tbl.stride(1) != 1 and block_tbl.shape[1] > 1):
         raise RuntimeError(f"{who}: block_tbl must be int32 [B, max_pages] with unit inner stride")
@@ -1286,27 +1288,35 @@ def _page_state(who: str, block_tbl, ref, *vecs):
     B, C = block_tbl.shape
     for name, t in vecs:
         _int32_vec(who, name, t, B)
-    return ctx, B, C, ref.shape[0]
+    return dev, B, C, ref.shape[0]
 
 
-def _page_tensors(who: str, caches, pages: int, dev):
-    """ctypes arrays (count, base, page stride, page bytes) of the page tensors of a pool."""
+def _page_tensors(who: str, caches, pages: int, dev: int):
+    """The page tensors of a pool: (their number, [bases, page strides, page bytes] as one array)."""
     base, stride, nbytes = [], [], []
     for t in caches:
-        if t.device != dev:
-            raise RuntimeError(f"{who}: cache on {t.device}, table on {dev}")
-        if t.dim() < 1 or t.shape[0] != pages or t.numel() == 0 or not t[0].is_contiguous():
-            raise RuntimeError(f"{who}: a cache {tuple(t.shape)} must have {pages} pages, each contiguous")
+        if t.get_device() != dev:
+            raise RuntimeError(f"{who}: a cache on {t.device}, the table on GPU {dev}")
+        if t.dim() < 1 or t.shape[0] != pages or t.numel() == 0:
+            raise RuntimeError(f"{who}: a cache {tuple(t.shape)} must have {pages} pages")
+        if not t.is_contiguous() and not t[0].is_contiguous():
+            raise RuntimeError(f"{who}: the pages of a cache must be contiguous")
         size = t.element_size()
-        nbytes.append(t.numel() // pages * size)
-        stride.append(t.stride(0) * size if pages > 1 else nbytes[-1])
+        n = t.numel() // pages * size
+        nbytes.append(n)
+        stride.append(t.stride(0) * size if pages > 1 else n)
         base.append(t.data_ptr())
-    n = len(base)
-    return n, (ctypes.c_void_p * n)(*base), (ctypes.c_int64 * n)(*stride), (ctypes.c_int64 * n)(*nbytes)
+    return len(base), array.array("q", base + stride + nbytes)
 
 
-def _pages_workspace(workspace, dev, B: int, C: int, P: int):
-    return (workspace or _ws.shared(dev)).ensure(_lib.lib().specq_kv_pages_workspace_size(B, C, P))
+def _page_tensor_args(n: int, words) -> tuple:
+    at = words.buffer_info()[0]
+    return n, at, at + 8 * n, at + 16 * n
+
+
+def _pages_workspace(workspace, dev: int, B: int, C: int, P: int):
+    need = _lib.lib().specq_kv_pages_workspace_size(B, C, P)
+    return (workspace or _ws.shared_cuda(dev)).ensure(need)
 
 
 def paged_kv_reserve(block_tbl, ref, lens, PAGE, shortage=None, workspace=None):
@@ -1318,13 +1328,12 @@ def paged_kv_reserve(block_tbl, ref, lens, PAGE, shortage=None, workspace=None):
     free pages run out, entries get -1.  Returns shortage, int32 [1]: how many pages are missing.
     """
     who = "paged_kv_reserve"
-    ctx, B, C, P = _page_state(who, block_tbl, ref, ("lens", lens))
+    dev, B, C, P = _page_state(who, block_tbl, ref, ("lens", lens))
     shortage = torch.empty(1, dtype=torch.int32, device=ref.device) if shortage is None else shortage
     _int32_vec(who, "shortage", shortage, 1)
-    with ctx:
-        wptr, wbytes = _pages_workspace(workspace, ref.device, B, C, P)
-        _lib.call("specq_kv_pages_reserve", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C,
-                  ref.data_ptr(), P, lens.data_ptr(), int(PAGE), shortage.data_ptr(), wptr, wbytes, _raw_stream(ref))
+    wptr, wbytes = _pages_workspace(workspace, dev, B, C, P)
+    _call_on(dev, "specq_kv_pages_reserve", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C,
+             ref.data_ptr(), P, lens.data_ptr(), int(PAGE), shortage.data_ptr(), wptr, wbytes)
     return shortage
 
 
@@ -1335,10 +1344,9 @@ def paged_kv_free(block_tbl, ref, keep, PAGE):
     falls by one; a page that no table names any more (ref 0) is free.
     """
     who = "paged_kv_free"
-    ctx, B, C, P = _page_state(who, block_tbl, ref, ("keep", keep))
-    with ctx:
-        _lib.call("specq_kv_pages_free", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C,
-                  ref.data_ptr(), P, keep.data_ptr(), int(PAGE), _raw_stream(ref))
+    dev, B, C, P = _page_state(who, block_tbl, ref, ("keep", keep))
+    _call_on(dev, "specq_kv_pages_free", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C,
+             ref.data_ptr(), P, keep.data_ptr(), int(PAGE))
 
 
 def paged_kv_fork(block_tbl, ref, lens, parent, caches, PAGE, shortage=None, workspace=None):
@@ -1353,15 +1361,14 @@ def paged_kv_fork(block_tbl, ref, lens, parent, caches, PAGE, shortage=None, wor
     past its tokens are let go of.  Returns shortage, int32 [1]: how many pages are missing.
     """
     who = "paged_kv_fork"
-    ctx, B, C, P = _page_state(who, block_tbl, ref, ("lens", lens), ("parent", parent))
-    tensors = _page_tensors(who, caches, P, ref.device)
+    dev, B, C, P = _page_state(who, block_tbl, ref, ("lens", lens), ("parent", parent))
+    n, words = _page_tensors(who, caches, P, dev)
     shortage = torch.empty(1, dtype=torch.int32, device=ref.device) if shortage is None else shortage
     _int32_vec(who, "shortage", shortage, 1)
-    with ctx:
-        wptr, wbytes = _pages_workspace(workspace, ref.device, B, C, P)
-        _lib.call("specq_kv_pages_fork", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C,
-                  ref.data_ptr(), P, lens.data_ptr(), parent.data_ptr(), int(PAGE), *tensors, shortage.data_ptr(),
-                  wptr, wbytes, _raw_stream(ref))
+    wptr, wbytes = _pages_workspace(workspace, dev, B, C, P)
+    _call_on(dev, "specq_kv_pages_fork", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C,
+             ref.data_ptr(), P, lens.data_ptr(), parent.data_ptr(), int(PAGE), *_page_tensor_args(n, words),
+             shortage.data_ptr(), wptr, wbytes)
     return shortage
 
 
@@ -1373,14 +1380,13 @@ def paged_kv_compact(block_tbl, ref, caches, page_map=None, workspace=None):
     [pages] holds every page's id afterwards, for other holders of ids.
     """
     who = "paged_kv_compact"
-    ctx, B, C, P = _page_state(who, block_tbl, ref)
-    tensors = _page_tensors(who, caches, P, ref.device)
+    dev, B, C, P = _page_state(who, block_tbl, ref)
+    n, words = _page_tensors(who, caches, P, dev)
     page_map = torch.empty(P, dtype=torch.int32, device=ref.device) if page_map is None else page_map
     _int32_vec(who, "page_map", page_map, P)
-    with ctx:
-        wptr, wbytes = _pages_workspace(workspace, ref.device, B, C, P)
-        _lib.call("specq_kv_pages_compact", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C,
-                  ref.data_ptr(), P, page_map.data_ptr(), *tensors, wptr, wbytes, _raw_stream(ref))
+    wptr, wbytes = _pages_workspace(workspace, dev, B, C, P)
+    _call_on(dev, "specq_kv_pages_compact", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C,
+             ref.data_ptr(), P, page_map.data_ptr(), *_page_tensor_args(n, words), wptr, wbytes)
     return page_map
 
 
@@ -1393,12 +1399,11 @@ def paged_kv_copy(src, dst, caches):
     who = "paged_kv_copy"
     if len(caches) == 0:
         raise RuntimeError(f"{who}: no caches")
-    ctx = _on_one_device(who, src, dst)
+    dev = _gpu_of(who, src, dst)
     n, P = src.numel(), caches[0].shape[0]
     _int32_vec(who, "src", src, n)
     _int32_vec(who, "dst", dst, n)
     if dst.numel() != n:
         raise RuntimeError(f"{who}: {n} sources and {dst.numel()} destinations")
-    tensors = _page_tensors(who, caches, P, src.device)
-    with ctx:
-        _lib.call("specq_kv_pages_copy", src.data_ptr(), dst.data_ptr(), n, P, *tensors, _raw_stream(src))
+    m, words = _page_tensors(who, caches, P, dev)
+    _call_on(dev, "specq_kv_pages_copy", src.data_ptr(), dst.data_ptr(), n, P, *_page_tensor_args(m, words))

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -115,6 +116,7 @@ SIGNATURES = {
     "specq_kv_pages_compact": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_vp, _c_int, _c_vp,
                                         _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_size, _c_vp]),
     "specq_kv_pages_copy": (_c_int, [_c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "specq_call_packed": (_c_int, [ctypes.c_char_p, ctypes.c_char_p, _c_int]),
     "specq_kernel_attrs_query": (_c_int, [_c_int] * 9 + [ctypes.POINTER(KernelAttrs)]),
 }
 
@@ -174,6 +176,27 @@ def call(name: str, *args) -> int:
     rc = getattr(lib(), name)(*args)
     check(rc, name)
     return rc
+
+
+_packed: dict = {}
+
+
+def packed(name: str):
+    """A function that calls entry point `name` with its arguments (numbers; pointers as integers) packed into one
+    buffer: ctypes converts three arguments instead of some thirty.  Raises like call()."""
+    f = _packed.get(name)
+    if f is None:
+        argtypes = SIGNATURES[name][1]
+        pack = struct.Struct("".join("d" if t is _c_float else "q" for t in argtypes)).pack
+        fn, key, n = lib().specq_call_packed, name.encode(), len(argtypes)
+
+        def f(*args):
+            rc = fn(key, pack(*args), n)
+            if rc != 0:
+                check(rc, name)
+
+        _packed[name] = f
+    return f
 
 
 _OPTIONS: dict = {}

@@ -50,7 +50,16 @@ class Workspace:
 
 
 _shared: dict = {}
+_shared_cuda: dict = {}  # the same workspaces by GPU index
 _shared_lock = threading.Lock()
+
+
+def shared_cuda(index: int) -> Workspace:
+    """shared() of GPU `index`, without forming a device."""
+    ws = _shared_cuda.get(index)
+    if ws is None:
+        ws = _shared_cuda[index] = shared(torch.device("cuda", index))
+    return ws
 
 
 def shared(device) -> Workspace:
