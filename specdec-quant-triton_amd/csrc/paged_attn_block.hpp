@@ -54,7 +54,7 @@ constexpr int kBlkSub = 16;                                  // tokens of a sub-
 constexpr int kBlkChunk = 2 * kBlkSub;                       // tokens per wave iteration
 constexpr int kBlkUnit = kBlkChunk * kAttnWaves;             // 256 tokens: one chunk of every wave
 constexpr int kBlkMaxUnits = 64 / 2;                         // longest split: the 64 sub-tiles a wave's lanes hold
-constexpr int kBlkMinUnits = 1;                              // shortest split: 256 tokens
+constexpr int kBlkOneSplit = 2;                              // tables of up to 512 tokens are one split
 constexpr int kBlkRegion = 16384;                            // LDS ring bytes of a wave
 // Up to kBlkMergeIn splits are merged by the program's last workgroup, more by a launch of their own, a
 // workgroup to each row (at most kBlkMergeMax, one per thread there).  One workgroup reads its
@@ -68,6 +68,8 @@ constexpr int64_t kBlkMaxTokens = (int64_t)kBlkUnit * kBlkMaxUnits * kBlkMergeMa
 
 // 256-token units per split for a table of L tokens when `pairs` (sequence, KV head) pairs (times their
 // row programs) are active: as many splits as bring the workgroups to `target`, evened out.
+// A second unit of a split costs 1.3 us, the merge of two splits 2.9 (B = 1, 8 heads, D = 64, table of
+// 304 tokens: 8.5 us as one split, 10.1 as two; B = 8, context 1024: 11.4 as four, 12.7 as two).
 __host__ __device__ inline int blk_split_units(int L, int pairs, int target) {
   const int n = L > 0 ? (L + kBlkUnit - 1) / kBlkUnit : 1;
   const int pr = pairs > 0 ? pairs : 1;
@@ -75,7 +77,7 @@ __host__ __device__ inline int blk_split_units(int L, int pairs, int target) {
   int u = (n + want - 1) / want;
   const int u_min = (n + kBlkMergeMax - 1) / kBlkMergeMax;
   if (u < u_min) u = u_min;
-  if (u < kBlkMinUnits) u = kBlkMinUnits;
+  if (n <= kBlkOneSplit) u = n;
   if (u > kBlkMaxUnits) u = kBlkMaxUnits;
   const int ns = (n + u - 1) / u;
   return (n + ns - 1) / ns;
