@@ -6,16 +6,18 @@
 // with Q = 127 (int8) or 448 (e4m3) and x the new tokens' values in the block:
 //   s' = max(amax |x|, 1e-8) / Q;  where the block holds earlier tokens of the sequence (its positions
 //        below the first new one), s' = max(s', s) with s its scale so far;
-//   new codes      rne(x / s'), clamped to +-Q;
-//   earlier codes  rne(c * s / s') where s' > s, untouched otherwise.
-// fp32, the division IEEE.  Infinities count as +-65504 and NaN as 0, so that one bad value does not
+//   new codes      rne(x / s');
+//   earlier codes  rne(c * s / s'), clamped to +-Q, where s' > s, untouched otherwise.
+// fp32, the quotients rounded as IEEE division rounds them.  Infinities count as +-65504 and NaN as 0, so that one bad value does not
 // take the block's other tokens with it.  Slots past the last new token are not touched.
 //
 // One workgroup per (sequence, block, K or V, head): SB * D values, eight to a thread and pass, held in
 // registers between the amax and the codes (up to 16384 values; larger blocks are read twice).  The
 // block's earlier codes and its scale are fetched together with the new values' amax pass, so that
 // the requantisation adds no round trip.  Bound by the latency of its three dependent loads (context
-// length, page id, codes) for a verification step and by HBM for a prompt.
+// length, page id, codes) for a verification step (B = 8, 9 tokens, 8 heads of 128, int8, blocks of 16:
+// 4.0 us) and for a prompt by that and the instructions of the conversion (2 x 2048 tokens, e4m3, blocks
+// of 32, 25 MB: 10.2 us = 2.5 TB/s, and 12.9 with a division and a clamp for each value).
 #include "api_common.hpp"
 #include "common.hpp"
 
@@ -32,12 +34,30 @@ struct KvAppendBlockParams {
   int log_dv;                                                  // log2(D / 8)
 };
 
-// New values as they are quantised: NaN as 0, infinities as the largest finite fp16.
-__device__ __forceinline__ float finite16(_Float16 h) {
-  const float x = (float)h;
-  return x != x ? 0.f : fminf(fmaxf(x, -65504.f), 65504.f);
+typedef uint16_t v2u16 __attribute__((ext_vector_type(2)));
+typedef uint16_t v8u16 __attribute__((ext_vector_type(8)));
+
+// Largest magnitude of eight fp16 values as fp16 bits, which order as the magnitudes do (not finite: 0x7c00
+// and above).
+__device__ __forceinline__ uint32_t top16(v8h x) {
+  const v8u16 a = __builtin_bit_cast(v8u16, x) & (uint16_t)0x7fff;
+  const v2u16 m = __builtin_elementwise_max(__builtin_elementwise_max(v2u16{a[0], a[1]}, v2u16{a[2], a[3]}),
+                                            __builtin_elementwise_max(v2u16{a[4], a[5]}, v2u16{a[6], a[7]}));
+  return max((uint32_t)m[0], (uint32_t)m[1]);
+}
+// New values as they are quantised: NaN as 0, infinities as the largest finite fp16.  Returns top16 of that.
+__device__ __forceinline__ uint32_t clean16(v8h& x) {
+  const uint32_t m = top16(x);
+  if (m < 0x7c00) return m;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float f = (float)x[e];
+    x[e] = (_Float16)(f != f ? 0.f : fminf(fmaxf(f, -65504.f), 65504.f));
+  }
+  return top16(x);
 }
 
+// Codes of eight values over the scale s.
 template <bool F8>
 __device__ __forceinline__ v2i encode8(const float (&x)[8], float s) {
   int w[2] = {0, 0};
@@ -55,6 +75,36 @@ __device__ __forceinline__ v2i encode8(const float (&x)[8], float s) {
     for (int j = 0; j < 8; ++j) {
       const float q = fminf(fmaxf(rintf(x[j] / s), -127.f), 127.f);
       w[j >> 2] |= ((int)q & 0xff) << (8 * (j & 3));
+    }
+  }
+  return v2i{w[0], w[1]};
+}
+// The same for |x| <= Q s with s in [2^-60, 2^60] and y = 1 / s rounded to nearest.  x / s comes out as the
+// division rounds it: q0 = x y is within an ulp or two, its remainder x - q0 s is exact in one FMA, and
+// q0 plus remainder times a correctly rounded reciprocal is the rounded quotient (Markstein; equal to the
+// division for every finite fp16 x and every scale max(amax, 1e-8) / Q above it).  It is at most
+// Q (1 + 2^-23), whose code is Q's, so nothing is clamped; adding 1.5 * 2^23 rounds to an integer, ties to
+// even, in the low bits.
+template <bool F8>
+__device__ __forceinline__ v2i encode8_by(v8h x, float s, float y) {
+  float q[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float f = (float)x[j], q0 = f * y;
+    q[j] = fmaf(fmaf(-q0, s, f), y, q0);
+  }
+  int w[2] = {0, 0};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (F8) {
+      w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * h], q[4 * h + 1], w[h], false);
+      w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * h + 2], q[4 * h + 3], w[h], true);
+    } else {
+      uint32_t u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] = __builtin_bit_cast(uint32_t, q[4 * h + e] + 12582912.f);
+      const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), b = __builtin_amdgcn_perm(u[3], u[2], 0x0c0c0400u);
+      w[h] = (int)__builtin_amdgcn_perm(b, a, 0x05040100u);
     }
   }
   return v2i{w[0], w[1]};
@@ -134,52 +184,71 @@ __global__ __launch_bounds__(256) void kv_append_block_kernel(KvAppendBlockParam
       if (is_old(t + 256 * i)) c[i] = *code_at(t + 256 * i);
   }
 
-  float amax = 0.f;
-  auto take = [&](v8h v) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(finite16(v[e])));
-  };
+  uint32_t top = 0;
   if constexpr (VPT > 0) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
-      if (is_new(t + 256 * i)) take(x[i]);
+      if (is_new(t + 256 * i)) top = max(top, clean16(x[i]));
   } else {
     for (int i = t; i < n_vec; i += 256)
-      if (is_new(i)) take(load_new(i));
+      if (is_new(i)) {
+        v8h v = load_new(i);
+        top = max(top, clean16(v));
+      }
   }
-  __shared__ float red[4];
+  __shared__ uint32_t red[4];
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-  if (lane_id() == 0) red[wave_id()] = amax;
+  for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+  if (lane_id() == 0) red[wave_id()] = top;
   __syncthreads();
-  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  top = max(max(red[0], red[1]), max(red[2], red[3]));
+  const float amax = (float)__builtin_bit_cast(_Float16, (uint16_t)top);
   constexpr float Q = F8 ? 448.f : 127.f;
   const float s_new = fmaxf(amax, 1e-8f) / Q;
   const float s = n_old > 0 ? fmaxf(s_old, s_new) : s_new;
   const bool grew = n_old > 0 && !(s <= s_old);
 
-  auto put = [&](int i, v8h xv, v2i cv) {
-    float f[8];
-    if (is_new(i)) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = finite16(xv[e]);
+  const bool plain = s >= 0x1p-60f && s <= 0x1p60f;  // always, but for a scale of the cache's that was not written here
+  const float y = 1.f / s;
+  auto put_new = [&](int i, v8h v) {
+    if (plain) {
+      *code_at(i) = encode8_by<F8>(v, s, y);
     } else {
-      decode8<F8>(cv, f);
+      float f[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= s_old;
+      for (int e = 0; e < 8; ++e) f[e] = (float)v[e];
+      *code_at(i) = encode8<F8>(f, s);
     }
+  };
+  auto put_old = [&](int i, v2i v) {
+    float f[8];
+    decode8<F8>(v, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= s_old;
     *code_at(i) = encode8<F8>(f, s);
   };
   if constexpr (VPT > 0) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int v = t + 256 * i;
-      if (is_new(v) || (grew && is_old(v))) put(v, x[i], c[i]);
+      if (is_new(v)) put_new(v, x[i]);
+    }
+    if (grew) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int v = t + 256 * i;
+        if (is_old(v)) put_old(v, c[i]);
+      }
     }
   } else {
     for (int v = t; v < n_vec; v += 256) {
-      if (is_new(v)) put(v, load_new(v), v2i{0, 0});
-      else if (grew) put(v, v8h{}, *code_at(v));
+      if (is_new(v)) {
+        v8h xv = load_new(v);
+        clean16(xv);
+        put_new(v, xv);
+      } else if (grew) {
+        put_old(v, *code_at(v));
+      }
     }
   }
   if (t == 0) *scale = s;
