@@ -124,6 +124,7 @@ __device__ __forceinline__ float readlane_f(float v, int l) {
 }
 typedef __attribute__((address_space(3))) v2i* lds_v2i;
 typedef const __attribute__((address_space(3))) v4i* lds_v4i;
+typedef const __attribute__((address_space(3))) v8h* lds_v8h;
 
 template <int RBL, int D>
 struct AttnBlockLds {
@@ -327,9 +328,10 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
 #pragma unroll
       for (int u = 0; u < NU; ++u) qreg[rb][u] = lds.q[rb][u][lane];
   }
+  uint32_t q_at = lds_addr(&lds.q[0][0][lane]);
   auto qfrag = [&](int rb, int u) -> v8h {
     if constexpr (QREG) return qreg[rb][u];
-    else return lds.q[rb][u][lane];
+    else return *(lds_v8h)(q_at + (rb * NU + u) * 1024);
   };
   wait_vmcnt<NS * NVM>();  // the scales have landed
   // Lane j: the K scale * sm_scale * log2(e) of sub-tile j; its V scale, that scale's log2 and reciprocal;
@@ -353,29 +355,24 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
   // S^T of a slot's chunk, both sub-tiles, before the scales, for the row blocks [RB0, RB1).
   auto scores = [&](auto rb0c, auto rb1c, uint32_t slot, v4f (&cs)[RB][2]) __attribute__((always_inline)) {
     constexpr int RB0 = decltype(rb0c)::value, RB1 = decltype(rb1c)::value;
-    v8h kf[2][NU];
-    {
-      v4i kx[2][KV4];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+    for (int rb = RB0; rb < RB1; ++rb) cs[rb][0] = cs[rb][1] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int h = 0; h < KV4; ++h) kx[s][h] = *(lds_v4i)((k_at ^ (16 * h + 8 * GR * s)) + slot + s * SB_);
+    for (int h = 0; h < KV4; ++h) {
+      v4i kx[2];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s) kx[s] = *(lds_v4i)((k_at ^ (16 * h + 8 * GR * s)) + slot + s * SB_);
 #pragma unroll
-        for (int h = 0; h < KV4; ++h) {
-          kf[s][2 * h] = code8_to_h8<F8>((uint32_t)kx[s][h].x, (uint32_t)kx[s][h].y);
-          kf[s][2 * h + 1] = code8_to_h8<F8>((uint32_t)kx[s][h].z, (uint32_t)kx[s][h].w);
+      for (int i = 0; i < 2; ++i) {
+        v8h kf[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) kf[s] = code8_to_h8<F8>((uint32_t)kx[s][2 * i], (uint32_t)kx[s][2 * i + 1]);
+#pragma unroll
+        for (int rb = RB0; rb < RB1; ++rb) {
+          const v8h q = qfrag(rb, 2 * h + i);
+#pragma unroll
+          for (int s = 0; s < 2; ++s) cs[rb][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[s], q, cs[rb][s], 0, 0, 0);
         }
-    }
-#pragma unroll
-    for (int rb = RB0; rb < RB1; ++rb) {
-      cs[rb][0] = cs[rb][1] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        const v8h q = qfrag(rb, u);
-#pragma unroll
-        for (int s = 0; s < 2; ++s) cs[rb][s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[s][u], q, cs[rb][s], 0, 0, 0);
       }
     }
   };
@@ -389,7 +386,7 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
       issue(ring + slot, it + NS);
       return;
     }
-    if constexpr (LATE) asm volatile("" : "+v"(k_at), "+v"(v_at));  // addresses are formed here, not kept
+    if constexpr (LATE) asm volatile("" : "+v"(k_at), "+v"(v_at), "+v"(q_at));  // addresses are formed here, not kept
     v2i vx[ND];
     v4f cs[RB][2];
     auto read_v = [&]() __attribute__((always_inline)) {
@@ -508,11 +505,13 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
           for (int db = 0; db < ND; ++db) {
             const v2i nb = {(int)f8_nan_bits((uint32_t)vx[db].x), (int)f8_nan_bits((uint32_t)vx[db].y)};
             const v8h isnan = bits_to_h8(nb);
+            int at = t0 + 4 * g;  // the indicators are formed for each db, not kept in registers
+            asm volatile("" : "+v"(at));
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
               v8h seen;
 #pragma unroll
-              for (int j = 0; j < 8; ++j) seen[j] = (_Float16)(hidden(rb, j >> 2, j & 3) ? 0.f : 1.f);
+              for (int j = 0; j < 8; ++j) seen[j] = (_Float16)(((bad >> (j >> 2)) & 1) != 0 || at + kBlkSub * (j >> 2) + (j & 3) > qpos[rb] ? 0.f : 1.f);
               const v4f hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(isnan, seen, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
               for (int j = 0; j < 4; ++j)

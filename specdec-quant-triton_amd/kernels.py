@@ -1222,17 +1222,6 @@ def _block_attn_info(D, f8, rows, dev) -> KernelInfo:
         return KernelInfo(2, D | (1 << 18 if f8 else 1 << 17), 0, 0, 0, rows, 0, 4, 0)
 
 
-def _block_attn_qpp(Q: int, G: int, D: int) -> int:
-    """Query tokens of a program, of Q with G heads a K/V head.  D = 64: as many as 64 rows hold (B = 2,
-    256 tokens, context 4096, 32 / 8 heads, int8: 16, 32, 64 rows a program 80.6, 51.2, 40.2 us).
-    D = 128: 32 rows (106.6, 68.6, 71.3 us), or 48 where those save a third of the programs (9 tokens: one
-    program of 48 rows 28.0 us, two of 32 43.1; 17: two 34.5, three 48.0; but 16: two 82.1, two of 32 63.0)."""
-    if D == 64:
-        return max(1, min(Q, 64 // G))
-    rows32, rows48 = max(1, min(Q, 32 // G)), max(1, min(Q, 48 // G))
-    return rows48 if 3 * -(-Q // rows48) <= 2 * -(-Q // rows32) else rows32
-
-
 def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=None, QPP=None, plan=None, n_seqs=None,
                                  out=None, sm_scale=None, workspace=None):
     """Verification attention over a paged cache with block scales.  Returns (out, ck).
@@ -1241,10 +1230,11 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
     [pages, PAGE / SB, H_KV] (paged_kv_append_block_scaled); block_tbl int32 [B, max_pages]; ctx_len
     int32 [B], counting the q_len new tokens, which are each sequence's last ones and see one another
     causally.  Block-table ids outside [0, pages) mask their page's tokens; a row that sees no token
-    gives 0.  QPP query tokens run in one program, at most 64 rows of H / H_KV heads each (default: chosen
-    by _block_attn_qpp).  sm_scale defaults to D^-1/2.  With `plan`, (n_seqs, q_len) = plan[0:2] on the device
-    and the grid covers (B, QLMAX); rows that are not active are not written (an omitted `out` is zero
-    there).  Calls that may run at the same time on several streams need a workspace each.
+    gives 0.  QPP query tokens run in one program, at most 64 rows of H / H_KV heads each (default: as few
+    programs as that takes, of even size).  sm_scale defaults to D^-1/2.  With `plan`, (n_seqs, q_len) =
+    plan[0:2] on the device and the grid covers (B, QLMAX); rows that are not active are not written (an
+    omitted `out` is zero there).  Calls that may run at the same time on several streams need a workspace
+    each.
     """
     who = "paged_attention_block_scaled"
     dev = _gpu_of(who, q, kc, vc, ks, vs, block_tbl, ctx_len, plan, out)
@@ -1258,7 +1248,8 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
     Bg, Qg, n_seqs, q_len = _token_grid(who, B, QL, q_len, n_seqs, plan)
     f8, sb = _block_cache(who, kc, vc, ks, vs, block_tbl, ctx_len, Bg, H_KV, D)
     if QPP is None:
-        QPP = _block_attn_qpp(Qg, G, D)
+        n = -(-Qg // max(1, 64 // G))  # programs
+        QPP = max(1, -(-Qg // max(1, n)))
     elif int(QPP) < 1:
         raise RuntimeError(f"{who}: QPP={QPP} must be at least 1")
     if out is None:
