@@ -282,43 +282,34 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
     }
   // One query chunk and D = 128: no other program reads these lines, and they are not kept in L2.
   const bool read_once = D == 128 && p.n_qc == 1;
-  // The DMAs of chunk `it` into ring slot `dst`.  Granules of sub-tiles off the pool, of chunks past the
-  // wave's last and of tokens at or past kv_end are out of range (zeros).
-  auto issue = [&](uint8_t* dst, int it) __attribute__((always_inline)) {
+  // The DMAs of chunk `it` into the ring slot at `slot`.  Sub-tiles off the pool, chunks past the wave's
+  // last and tokens at or past kv_end are behind the end of their buffers (zeros).
+  auto issue = [&](uint32_t slot, int it) __attribute__((always_inline)) {
+    uint8_t* dst = ring + slot;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const int j = min(2 * it + s, 63), t0 = sub_t0(2 * it + s);
+      const int j = min(2 * it + s, 63), n = kv_end - sub_t0(2 * it + s);
       const bool real = it < n_it && ((bad_subs >> j) & 1) == 0;
       const int64_t kb = readlane64(kv_base_v, j);
-      const v4i rk = attn_rsrc(p.kc + kb), rv = attn_rsrc(p.vc + kb);
+      v4i rk = attn_rsrc(p.kc + kb), rv = attn_rsrc(p.vc + kb);
+      rk.z = rv.z = !real || n <= 0 ? 0 : n >= kBlkSub ? (int)kOOB : (int)(n * p.s_ko);
       uint8_t* dk = dst + s * SB_;
       uint8_t* dv = dst + 2 * SB_ + s * SB_;
-      if (real && t0 + kBlkSub <= kv_end) {
-        if (read_once) {
+      if (read_once) {
 #pragma unroll
-          for (int i = 0; i < NDMA; ++i) dma16_rs<true>(rk, kvoff[s][i], dk + 1024 * i);
+        for (int i = 0; i < NDMA; ++i) dma16_rs<true>(rk, kvoff[s][i], dk + 1024 * i);
 #pragma unroll
-          for (int i = 0; i < NDMA; ++i) dma16_rs<true>(rv, kvoff[s][i], dv + 1024 * i);
-        } else {
-#pragma unroll
-          for (int i = 0; i < NDMA; ++i) dma16_rs<false>(rk, kvoff[s][i], dk + 1024 * i);
-#pragma unroll
-          for (int i = 0; i < NDMA; ++i) dma16_rs<false>(rv, kvoff[s][i], dv + 1024 * i);
-        }
+        for (int i = 0; i < NDMA; ++i) dma16_rs<true>(rv, kvoff[s][i], dv + 1024 * i);
       } else {
 #pragma unroll
-        for (int i = 0; i < NDMA; ++i) {
-          const uint32_t off = oob_unless(real && t0 + (64 * i + lane) / GR < kv_end, kvoff[s][i]);
-          dma16_rs<false>(rk, off, dk + 1024 * i);
-          dma16_rs<false>(rv, off, dv + 1024 * i);
-        }
+        for (int i = 0; i < NDMA; ++i) dma16_rs<false>(rk, kvoff[s][i], dk + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < NDMA; ++i) dma16_rs<false>(rv, kvoff[s][i], dv + 1024 * i);
       }
     }
   };
-  static_for<0, NS>([&](auto ic) __attribute__((always_inline)) {
-    constexpr int i = decltype(ic)::value;
-    issue(ring + i * SLOT, i);
-  });
+#pragma unroll 1
+  for (int i = 0; i < NS; ++i) issue(i * SLOT, i);
   wg_barrier_lds();
   constexpr bool QREG = RB <= 2;  // Q fragments in registers; deeper packings read them from LDS per chunk
   v8h qreg[QREG ? RB : 1][NU];
@@ -353,7 +344,7 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
   }
 
   // S^T of a slot's chunk, both sub-tiles, before the scales, for the row blocks [RB0, RB1).
-  auto scores = [&](auto rb0c, auto rb1c, uint32_t slot, v4f (&cs)[RB][2]) __attribute__((always_inline)) {
+  auto scores = [&](auto rb0c, auto rb1c, uint32_t k_s, v4f (&cs)[RB][2]) __attribute__((always_inline)) {
     constexpr int RB0 = decltype(rb0c)::value, RB1 = decltype(rb1c)::value;
 #pragma unroll
     for (int rb = RB0; rb < RB1; ++rb) cs[rb][0] = cs[rb][1] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -361,7 +352,7 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
     for (int h = 0; h < KV4; ++h) {
       v4i kx[2];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) kx[s] = *(lds_v4i)((k_at ^ (16 * h + 8 * GR * s)) + slot + s * SB_);
+      for (int s = 0; s < 2; ++s) kx[s] = *(lds_v4i)((k_s ^ (16 * h + 8 * GR * s)) + s * SB_);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         v8h kf[2];
@@ -380,24 +371,20 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
   // accumulator: they read V behind the softmax, refill the slot then, and form the scores again in the
   // rare case that a row's max moves.
   constexpr bool LATE = RB >= 3 && D == 128;
-  auto chunk = [&](auto slc, int it) __attribute__((always_inline)) {
-    constexpr uint32_t slot = decltype(slc)::value * SLOT;
-    if (it >= n_it) {
-      issue(ring + slot, it + NS);
-      return;
-    }
-    if constexpr (LATE) asm volatile("" : "+v"(k_at), "+v"(v_at), "+v"(q_at));  // addresses are formed here, not kept
+  auto chunk = [&](uint32_t slot, int it) __attribute__((always_inline)) {
+    const uint32_t k_s = k_at + slot, v_s = v_at + slot;
+    if constexpr (LATE) asm volatile("" : "+v"(q_at));  // Q's addresses are formed here, not kept
     v2i vx[ND];
     v4f cs[RB][2];
     auto read_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int db = 0; db < ND; ++db) vx[db] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)((v_at ^ (16 * db)) + slot));
+      for (int db = 0; db < ND; ++db) vx[db] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(v_s ^ (16 * db)));
     };
     if constexpr (!LATE) read_v();
-    scores(std::integral_constant<int, 0>{}, std::integral_constant<int, RB>{}, slot, cs);
+    scores(std::integral_constant<int, 0>{}, std::integral_constant<int, RB>{}, k_s, cs);
     if constexpr (!LATE) {  // the slot has been read: its next chunk may come
       wait_lgkm0();
-      issue(ring + slot, it + NS);
+      issue(slot, it + NS);
     }
 
     // ---- Softmax.  P' = exp2(s_raw ks + log2 vs - m), masked tokens 0.
@@ -405,10 +392,33 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
     const uint32_t bad = (uint32_t)(bad_subs >> j0) & 3u;  // sub-tiles off the pool
     // Every row of the program sees every token of the chunk: no mask needed.
     const bool full = bad == 0 && t0 + kBlkChunk - 1 <= L - q_len + qc * p.QPP;
-    auto hidden = [&](int rb, int s, int e) { return ((bad >> s) & 1) != 0 || t0 + kBlkSub * s + 4 * g + e > qpos[rb]; };
+    // Row block rb sees tokens e <= limit of the lane's four in sub-tile s.
+    auto limit = [&](int rb, int s) { return ((bad >> s) & 1) != 0 ? -1 : qpos[rb] - (t0 + kBlkSub * s + 4 * g); };
     const float kb[2] = {readlane_f(sub_k, j0), readlane_f(sub_k, j0 + 1)};
     const float lv[2] = {readlane_f(sub_lv, j0), readlane_f(sub_lv, j0 + 1)};
     const float iv[2] = {readlane_f(sub_iv, j0), readlane_f(sub_iv, j0 + 1)};
+    // Row block rb's largest score of the chunk, less kBlkRoom; sc: its scores, -inf where hidden.
+    auto top_score = [&](int rb, float (&sc)[2][4]) __attribute__((always_inline)) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int lim = full ? 4 : limit(rb, s);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sc[s][e] = fmaf(cs[rb][s][e], kb[s], lv[s]);
+          sc[s][e] = e > lim ? -INFINITY : sc[s][e];
+          mx = fmaxf(mx, sc[s][e]);
+        }
+      }
+      return group_max4(mx) - kBlkRoom;
+    };
+    if (it == 0) {  // the max moves there for certain
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        float sc[2][4];
+        m_run[rb] = top_score(rb, sc);
+      }
+    }
     float pr[RB][2][4], big = 0.f;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
@@ -418,9 +428,9 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
 #pragma unroll
         for (int e = 0; e < 4; ++e) pr[rb][s][e] = fast_exp2(fmaf(cs[rb][s][e], kb[s], a));
         if (!full) {
+          const int lim = limit(rb, s);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (hidden(rb, s, e)) pr[rb][s][e] = 0.f;
+          for (int e = 0; e < 4; ++e) pr[rb][s][e] = e > lim ? 0.f : pr[rb][s][e];
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) big = fmaxf(big, pr[rb][s][e]);
@@ -438,18 +448,10 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
         rows |= rows >> 16;
         if constexpr (LATE) {
           asm volatile("" ::: "memory");  // formed again, not kept
-          scores(rbc, std::integral_constant<int, rb + 1>{}, slot, cs);
+          scores(rbc, std::integral_constant<int, rb + 1>{}, k_s, cs);
         }
-        float sc[2][4], mx = -INFINITY;
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            sc[s][e] = fmaf(cs[rb][s][e], kb[s], lv[s]);
-            if (!full && hidden(rb, s, e)) sc[s][e] = -INFINITY;
-            mx = fmaxf(mx, sc[s][e]);
-          }
-        mx = group_max4(mx) - kBlkRoom;
+        float sc[2][4];
+        const float mx = top_score(rb, sc);
         if ((rows >> r) & 1) {
           const float alpha = fast_exp2(m_run[rb] - mx);  // 0 from m = -inf
           m_run[rb] = mx;
@@ -486,7 +488,7 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
     if constexpr (LATE) {
       read_v();
       wait_lgkm0();
-      issue(ring + slot, it + NS);
+      issue(slot, it + NS);
     }
     v8h pf[RB];
 #pragma unroll
@@ -530,11 +532,13 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
       for (int rb = 0; rb < RB; ++rb) acc[rb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rb], acc[rb][db], 0, 0, 0);
     }
   };
-  for (int base = 0; base < n_it; base += NS) {
-    static_for<0, NS>([&](auto ic) __attribute__((always_inline)) {
-      wait_vmcnt<(NS - 1) * NVM>();  // chunk base + i has landed
-      chunk(ic, base + decltype(ic)::value);
-    });
+  // One copy of the loop's code serves all slots: a launch finds the instruction cache cold, and most calls
+  // go around a few times only.
+#pragma unroll 1
+  for (int it = 0, slot = 0; it < n_it; ++it) {
+    wait_vmcnt<(NS - 1) * NVM>();  // chunk `it` has landed
+    chunk(slot, it);
+    slot = slot == (NS - 1) * SLOT ? 0 : slot + SLOT;
   }
   // Every DMA has landed before the ring is reused for the merge.
   wait_vmcnt<0>();
