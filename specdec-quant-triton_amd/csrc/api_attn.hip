@@ -136,7 +136,8 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
                 (long long)max_pages * PAGE, (long long)most);
   SPECQ_REQUIRE(QPP > 0, SPECQ_EINVAL, "paged_attn: QPP=%d", QPP);
   const int G = H / H_KV;
-  SPECQ_REQUIRE(QPP * G <= 64, SPECQ_ENOTSUP, "paged_attn: QPP*G=%d packed rows exceed 64", QPP * G);
+  SPECQ_REQUIRE((int64_t)QPP * G <= 64, SPECQ_ENOTSUP, "paged_attn: QPP*G=%lld packed rows exceed 64",
+                (long long)QPP * G);
   if (plan == nullptr) {
     SPECQ_REQUIRE(n_seqs >= 0 && n_seqs <= B_grid && q_len >= 0 && q_len <= ql_grid, SPECQ_EINVAL,
                   "paged_attn: n_seqs=%d q_len=%d outside the grid (%d, %d)", n_seqs, q_len, B_grid, ql_grid);
@@ -148,6 +149,8 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
   SPECQ_REQUIRE((uintptr_t)kc % 16 == 0 && (uintptr_t)vc % 16 == 0 && s_kp % 16 == 0 && s_ko % 16 == 0 &&
                     s_kh % 16 == 0,
                 SPECQ_ENOTSUP, "paged_attn: K/V cache rows must be 16-byte aligned");
+  SPECQ_REQUIRE(!blk || s_ko >= D, SPECQ_ENOTSUP, "paged_attn: rows of the K/V cache overlap (token stride %lld)",
+                (long long)s_ko);
   SPECQ_REQUIRE(s_ko > 0 && 16 * s_ko + D < ((int64_t)1 << 31), SPECQ_ENOTSUP,
                 "paged_attn: token stride %lld of the K/V cache outside (0, 2^27)", (long long)s_ko);
   if (B_grid == 0) return SPECQ_OK;

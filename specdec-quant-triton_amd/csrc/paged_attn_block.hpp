@@ -10,12 +10,13 @@
 // Programs, splits, the grid and the plan are those of the attention over per-token scales
 // (paged_attn.hpp): a workgroup is a (KV split, KV head, query chunk, sequence), its QPP * G rows packed
 // into RB blocks of 16, with the page ids of a split fetched ahead of the sequence's length.  The
-// loop is built for what bounds it: a wave issues at most one instruction in 8 cycles here (one VALU
-// instruction in 4 takes two waves a SIMD, measured with loops of one instruction), so a chunk
-// costs its instruction count, and everything below is there to have fewer of them for each token.
+// loop is built for what bounds it: HBM for few rows, instructions for many.  A wave issues at most one
+// VALU instruction in 8 cycles here and two waves of a SIMD one in 4 (measured with loops of one
+// instruction), so a chunk costs its instruction count, and everything below is there to have fewer of
+// them for each token; 64 rows share what it takes to read and convert K and V.
 //  * Eight waves take interleaved chunks of 32 tokens, two page sub-tiles of 16, through a
 //    wave-private LDS ring filled by LDS DMA.  A slot is refilled as soon as its chunk has been read
-//    into registers, ahead of the softmax, so NS chunks a wave are in flight or in use.
+//    into registers, so NS chunks a wave are in flight or in use.
 //  * A sub-tile lies in one block: its scales are wave-uniform, fetched once with the split's page
 //    ids (lane j holds those of the wave's sub-tile j) and picked with v_readlane.
 //  * S^T = K . Q^T on v_mfma_f32_16x16x32_f16, one product per sub-tile, so lane (r, g) gets query row r,
@@ -30,10 +31,16 @@
 //    The row sum is that of P' / vs, one FMA a sub-tile.  Sub-tiles whose V scale is not in
 //    (2^-100, 2^100) (zero, negative, not finite) count as 1 there and multiply theirs onto P'.
 //  * The running max is lazy: m lies 8 below the row's largest s + log2 vs when it moves, which it does
-//    where P' passes 2^14; so P' fits fp16, and most chunks leave the accumulator alone.
+//    where P' passes 2^14; so P' fits fp16, and most chunks leave the accumulator alone.  A wave's first
+//    chunk takes its max before its exponentials.
 //  * The waves merge through the ring, every wave writing its rows once and all threads summing eight,
 //    two row blocks at a time.  Up to kBlkMergeIn splits are merged by the program's last workgroup to
 //    arrive, more by attn_merge_kernel behind the launch.
+// Measured in a graph, 32 / 8 heads, D = 128, codes read per second: 32 sequences of one token, contexts up to
+// 8192, int8 85.5 us = 3.8 TB/s; 8 and 32 sequences of 9 tokens, context 4096, e4m3 25.9 us = 2.6 TB/s and
+// 62.9 us = 4.3 TB/s (of the 25.9, 14 are the loop, the rest start, first loads and merges); 2 x 256
+// tokens, contexts up to 4096, int8 50.0 us, e4m3 46.2, bound by instructions; one sequence of 5 tokens,
+// context 131072, 16 / 2 heads, D = 64, e4m3 21.8 us, 4.4 of them the merge launch.
 // A row's result does not depend on the rows packed with it: split boundaries, chunks and merge orders are
 // fixed, so QPP = 1, fused, eager and plan calls agree bit for bit.
 //
@@ -57,10 +64,9 @@ constexpr int kBlkMaxUnits = 64 / 2;                         // longest split: t
 constexpr int kBlkOneSplit = 2;                              // tables of up to 512 tokens are one split
 constexpr int kBlkRegion = 16384;                            // LDS ring bytes of a wave
 // Up to kBlkMergeIn splits are merged by the program's last workgroup, more by a launch of their own, a
-// workgroup to each row (at most kBlkMergeMax, one per thread there).  One workgroup reads its
-// program's partial rows at some 60 GB/s: with 16-token chunks, B = 1, 2 K/V heads, 5 tokens, context
-// 131072, D = 64, 64 splits merged in place took 37.6 us in a graph, 128 splits and the launch 21.9; 8 K/V
-// heads, context 65536, D = 128: 32 splits 42.5 and 38.7; four splits of 64 programs 28.9 and 33.1.
+// workgroup to each row (at most kBlkMergeMax, one per thread there).  In a graph, 5 tokens, 32 / 8 heads,
+// D = 128, e4m3: 8 splits in place and by a launch 23.8 and 26.1 us (B = 4, context 8192), 14.5 and 16.2
+// (context 2048); 16 splits 25.1 and 25.5 (B = 2, context 16384), 17.2 and 15.8 (context 4096).
 constexpr int kBlkMergeIn = 8;
 constexpr int kBlkMergeMax = 256;
 constexpr float kBlkRoom = 8.f, kBlkLazyP = 16384.f;         // m below the max when it moves; the P' that moves it
@@ -369,7 +375,7 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
   };
   // Programs of 48 and 64 rows at D = 128 have no registers for the chunk's V and its scores next to the
   // accumulator: they read V behind the softmax, refill the slot then, and form the scores again in the
-  // rare case that a row's max moves.
+  // rare case that a row's max moves behind the first chunk.
   constexpr bool LATE = RB >= 3 && D == 128;
   auto chunk = [&](uint32_t slot, int it) __attribute__((always_inline)) {
     const uint32_t k_s = k_at + slot, v_s = v_at + slot;
