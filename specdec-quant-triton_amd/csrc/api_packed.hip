@@ -9,6 +9,13 @@
 namespace specq {
 namespace {
 
+// Whether a word holds an argument of type T.
+template <typename T>
+bool fits(int64_t w) {
+  if constexpr (std::is_integral_v<T>) return static_cast<int64_t>(static_cast<T>(w)) == w;
+  else return true;
+}
+
 template <typename T>
 T from_word(int64_t w) {
   if constexpr (std::is_pointer_v<T>) {
@@ -24,6 +31,7 @@ T from_word(int64_t w) {
 
 template <typename... A, size_t... I>
 int apply(int (*fn)(A...), const int64_t* w, std::index_sequence<I...>) {
+  SPECQ_REQUIRE((fits<A>(w[I]) && ...), SPECQ_EINVAL, "call_packed: an integer argument is out of its type's range");
   return fn(from_word<A>(w[I])...);
 }
 

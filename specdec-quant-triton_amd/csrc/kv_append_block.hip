@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256) void kv_append_block_kernel(KvAppendBlockParam
   }
   nb = uniform(nb);
   ql = uniform(ql);
-  if (b >= nb || ql == 0) return;
+  if (b >= nb || ql == 0 || L <= 0) return;
   const int pos0 = uniform(L) - ql;  // position of the first new token (negative ones are skipped)
   const int64_t first = ((int64_t)(max(pos0, 0) / p.SB) + j) * p.SB;
   if (first / p.PAGE >= p.max_pages) return;

@@ -405,7 +405,7 @@ static int pages_setup(PagesParams& p, const char* who, int32_t* tbl, int64_t s_
   SPECQ_REQUIRE(tbl && ref, SPECQ_EINVAL, "%s: null tensor pointer", who);
   SPECQ_REQUIRE(B > 0 && C > 0 && P > 0 && PAGE > 0 && s_bt >= C, SPECQ_EINVAL,
                 "%s: bad sizes B=%d columns=%d pages=%d PAGE=%d", who, B, C, P, PAGE);
-  SPECQ_REQUIRE((int64_t)C * PAGE <= INT32_MAX && P <= INT32_MAX - kPagesThreads * kPagesPer, SPECQ_ENOTSUP,
+  SPECQ_REQUIRE((int64_t)C * PAGE <= INT32_MAX && C <= (1 << 30) && P <= INT32_MAX - kPagesThreads * kPagesPer, SPECQ_ENOTSUP,
                 "%s: a row of %lld tokens or a pool of %d pages is too large", who, (long long)C * PAGE, P);
   SPECQ_REQUIRE((int64_t)B * ceil_div(C, 64) <= INT32_MAX / 2, SPECQ_ENOTSUP, "%s: block table too large", who);
   p = {};

@@ -237,7 +237,7 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
     qtmp[i] = ok ? x : v8h{0, 0, 0, 0, 0, 0, 0, 0};
   }
 
-  const int L = uniform(min(L_raw, cap));
+  const int L = uniform(max(min(L_raw, cap), 0));
   const int kv_end = L - q_len + min(qc * p.QPP + p.QPP, q_len);
   // Split 0 always runs, so rows with no visible key still get their zero output.
   if (split > 0 && s0 >= kv_end) return;
@@ -746,7 +746,7 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnBlockParams p) {
   if (b >= n_seqs || qi >= q_len) return;
   const int cap = p.max_pages * p.PAGE;
   const int split_tokens = kBlkUnit * blk_split_units(cap, n_seqs * p.H_KV * attn_row_programs(q_len, p.G), p.target_wgs);
-  const int L = uniform(min(p.ctx_len[b], cap));
+  const int L = uniform(max(min(p.ctx_len[b], cap), 0));
   const int kv_end = L - q_len + min(qc * p.QPP + p.QPP, q_len);
   const int n = kv_end > split_tokens ? (kv_end + split_tokens - 1) / split_tokens : 1;
   if (n == 1) return;  // the row's only split has stored it

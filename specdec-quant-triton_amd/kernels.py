@@ -1184,8 +1184,8 @@ def paged_kv_append_block_scaled(k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_le
     scale where that is larger and the block holds earlier tokens of the sequence; the new codes are
     rne(x / s'), and where the scale grows the earlier codes become rne(c * s / s').  Infinities count
     as +-65504, NaN as 0.  Tokens at positions below zero, past the table or on a page outside the pool
-    are skipped, every other slot keeps what it holds.  A page that the call writes must belong to one
-    sequence only (paged_kv_fork sees to that).  With `plan`, (n_seqs, q_len) = plan[0:2] on the device
+    are skipped, every other slot keeps what it holds.  A page that the call writes must be named by one
+    entry of the table only (paged_kv_fork sees to that).  With `plan`, (n_seqs, q_len) = plan[0:2] on the device
     and the grid covers (B, QLMAX).
     """
     who = "paged_kv_append_block_scaled"
@@ -1209,7 +1209,7 @@ def paged_kv_append_block_scaled(k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_le
              ctx_len.data_ptr(), Bg, n_seqs, q_len, Qg, H_KV, D, kc.shape[1], _plan_of(plan, 2, who))
 
 
-@functools.lru_cache(maxsize=None)
+@functools.lru_cache(maxsize=4096)
 def _block_attn_workspace(Bg, H, H_KV, Qg, QPP, max_pages, PAGE, dev, options) -> int:
     """Bytes a call needs: a function of its sizes, the GPU's CU count and the library options."""
     with torch.cuda.device(dev):
@@ -1229,8 +1229,8 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
     q fp16 [B, QLMAX, H, D], D 64 or 128; kc/vc int8 or float8_e4m3fn [pages, PAGE, H_KV, D]; ks/vs fp32
     [pages, PAGE / SB, H_KV] (paged_kv_append_block_scaled); block_tbl int32 [B, max_pages]; ctx_len
     int32 [B], counting the q_len new tokens, which are each sequence's last ones and see one another
-    causally.  Block-table ids outside [0, pages) mask their page's tokens; a row that sees no token
-    gives 0.  QPP query tokens run in one program, at most 64 rows of H / H_KV heads each (default: as few
+    causally; a context longer than the table counts as the table's length.  Block-table ids outside
+    [0, pages) mask their page's tokens; a row that sees no token gives 0.  QPP query tokens run in one program, at most 64 rows of H / H_KV heads each (default: as few
     programs as that takes, of even size).  sm_scale defaults to D^-1/2.  With `plan`, (n_seqs, q_len) =
     plan[0:2] on the device and the grid covers (B, QLMAX); rows that are not active are not written (an
     omitted `out` is zero there).  Calls that may run at the same time on several streams need a workspace
@@ -1399,8 +1399,8 @@ def paged_kv_copy(src, dst, caches):
     are left out.
     """
     who = "paged_kv_copy"
-    if len(caches) == 0:
-        raise RuntimeError(f"{who}: no caches")
+    if len(caches) == 0 or caches[0].dim() < 1:
+        raise RuntimeError(f"{who}: no caches of [pages, ...]")
     dev = _gpu_of(who, src, dst)
     n, P = src.numel(), caches[0].shape[0]
     _int32_vec(who, "src", src, n)
@@ -1408,4 +1408,5 @@ def paged_kv_copy(src, dst, caches):
     if dst.numel() != n:
         raise RuntimeError(f"{who}: {n} sources and {dst.numel()} destinations")
     m, words = _page_tensors(who, caches, P, dev)
-    _call_on(dev, "specq_kv_pages_copy", src.data_ptr(), dst.data_ptr(), n, P, *_page_tensor_args(m, words))
+    _call_on(dev, "specq_kv_pages_copy", src.data_ptr(), dst.data_ptr(), n, min(P, 2**31 - 1),
+             *_page_tensor_args(m, words))

@@ -159,6 +159,18 @@ def test_views_and_plan_graph():
     assert all(bool((p[:, 1] == 3).all()) for p in pools)
 
 
+def test_negative_lengths_write_nothing():
+    rng = np.random.default_rng(21)
+    kc, vc, ks, vs, bt, _ = make_cache(rng, [64, 64, 64], 2, 64, 16, 16, "int8")
+    new = rng.standard_normal((2, 3, 4, 2, 64)).astype(np.float16)
+    t = gpu(kc, vc, ks, vs, bt)
+    note("block append negative lengths")
+    K.paged_kv_append_block_scaled(*gpu(new[0], new[1]), *t, *gpu(np.asarray([-2 ** 31, -1, 0], np.int32)), 4)
+    torch.cuda.synchronize()
+    for got, was in zip(t, (kc, vc, ks, vs)):
+        assert np.array_equal(raw(got), was)
+
+
 def test_refusals():
     rng = np.random.default_rng(1)
     k, v, kc, vc, ks, vs, bt, cl = gpu(*new_kv(rng, 2, 4, 2, 128), *make_cache(rng, [40, 20], 2, 128, 32, 16, "int8"))

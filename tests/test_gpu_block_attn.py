@@ -274,6 +274,38 @@ def test_streams_with_their_own_workspaces():
             check(o, ref, 3, 2, 128, f"stream {i}")
 
 
+def test_lengths_out_of_range():
+    """Negative contexts see nothing, ones past the table end with it; the splits' counters are back at zero."""
+    rng = np.random.default_rng(15)
+    H, HK, D, ql = 8, 2, 128, 5
+    kc, vc, ks, vs, bt, _ = make_cache(rng, [2048, 2048, 700, 2048, 1], HK, D, 16, 16, "int8")
+    bt = bt[:, :128]  # 2048 tokens
+    q = queries(rng, 5, ql, H, D)
+    note("block attn lengths out of range")
+    for given, counted in (([-2 ** 31, 2048, -3, 2 ** 31 - 1, 4], [0, 2048, 0, 2048, 4]),
+                           ([2048, -2 ** 31 + 7, 700, 2050, -1], [2048, 0, 700, 2048, 0])):
+        cache = (kc, vc, ks, vs, bt)
+        ref = C.attention_block(q, *cache, np.asarray(counted, np.int32), ql, "int8")
+        out = K.paged_attention_block_scaled(*gpu(q, *cache, np.asarray(given, np.int32)), ql)[0]
+        torch.cuda.synchronize()
+        check(out, ref, ql, 5, D, given)
+
+
+@pytest.mark.parametrize("D,fmt", [(64, "int8"), (64, "fp8"), (128, "int8"), (128, "fp8")])
+def test_even_programs_of_many_tokens(D, fmt):
+    """More tokens than a program holds, with every number of row blocks, masked chunks first and last."""
+    rng = np.random.default_rng(D)
+    for q_len, ctx in ((17, [900, 17, 3]), (33, [515, 40, 33]), (49, [300, 1024, 60])):
+        cache = make_cache(rng, ctx, 2, D, 16, 16, fmt)
+        q = queries(rng, len(ctx), q_len, 8, D)
+        note(f"block attn even programs {fmt} D={D} q_len={q_len}")
+        t = gpu(q, *cache)
+        out = K.paged_attention_block_scaled(*t, q_len)[0]
+        check(out, C.attention_block(q, *cache, q_len, fmt), q_len, len(ctx), D, q_len)
+        for QPP in (1, 8, 12, 16):
+            assert torch.equal(out, K.paged_attention_block_scaled(*t, q_len, QPP=QPP)[0]), (q_len, QPP)
+
+
 def test_refusals():
     rng = np.random.default_rng(1)
     q, kc, vc, ks, vs, bt, cl = gpu(queries(rng, 2, 4, 8, 128), *make_cache(rng, [40, 20], 2, 128, 32, 16, "int8"))

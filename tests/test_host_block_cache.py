@@ -93,6 +93,20 @@ def test_pages_refusals(built_lib):
     assert size(0, 1, 1) == 0 and size(4, 8, 100) >= 256 * 1024 + 4 * (4 * 8 + 3 * 4 + 3 * 100)
 
 
+def test_sizes_past_their_types(built_lib):
+    _fail("specq_paged_attn_block", ATTN, -95, s_ko=112), _fail("specq_paged_attn_block", ATTN, -95, QPP=1 << 30)
+    free = dict(bt=16, s_bt=1 << 31, B=4, C=(1 << 30) + 1, ref=16, P=100, keep=16, PAGE=1, stream=0)
+    _fail("specq_kv_pages_free", free, -95)
+    from specq import _lib
+    words = list(ATTN.values())
+    with pytest.raises(RuntimeError, match="range"):
+        _lib.packed("specq_paged_attn_block")(*[w if k != "n_pages" else 2 ** 32 + 100 for k, w in zip(ATTN, words)])
+    with pytest.raises(RuntimeError, match="arguments"):
+        _lib.check(_lib.lib().specq_call_packed(b"specq_rotary", b"\0" * 64, 8), "specq_rotary")
+    with pytest.raises(RuntimeError, match="no entry point"):
+        _lib.check(_lib.lib().specq_call_packed(b"specq_version", b"\0" * 8, 1), "specq_version")
+
+
 def test_python_entry_points_want_gpu_tensors():
     import kernels as K
     z = torch.zeros((1, 1, 2, 64), dtype=torch.float16)
