@@ -13,23 +13,28 @@
 //   compact  the pages in use move below their own number: the i-th used page at or past it goes to
 //            the i-th free page below it.
 //
-// Handing out is a scan of ref by one workgroup of 1024 threads, 16 counts a thread and step, that ends
+// Handing out is a scan of ref by one workgroup of 1024 threads, eight counts a thread and step, that ends
 // when enough free pages are found.  Bound by latency, a few dependent round trips of about a
 // microsecond each, so the first step's counts are loaded ahead of everything else and what one part
 // hands the next stays in LDS where it fits (the table's bits up to kPagesBits words, ids up to kPagesList;
-// the workspace otherwise).  The page copies behind fork and compact are bound by HBM.
+// the workspace otherwise).  The page copies behind fork and compact are bound by HBM.  Kernel times:
+// reserve 6.8 us (32 rows of 258 columns, one page each), free 2.6, fork 3.7 + 3.8 and 4.1 for the copies of 24
+// pages of 128 KB, compact 6.2 (4104 pages) and 13.2 for the copies of a thousand pages of 32 KB (4.9 TB/s).
 #include "api_common.hpp"
 #include "common.hpp"
 
 namespace specq {
 
 constexpr int kPagesThreads = 1024, kPagesWaves = kPagesThreads / kWave;
-constexpr int kPagesPer = 16;  // counts a thread scans per step
+// Counts a thread scans per step.  Compacting 512, 4104, 65536, 262144 pages, 70 % used, took (with the launch and
+// no copies) 15.5, 18.1, 66, 237 us with 16, 13.9, 15.7, 57, 195 with 8 and 15.0, 17.1, 63, 217 with 4.
+constexpr int kPagesPer = 8;
 constexpr int kPagesTensors = 64;
 constexpr int kPagesChunk = 16384;  // bytes of a page one workgroup copies at a time
 constexpr int kPagesStep = kPagesThreads * kPagesPer;
 constexpr int kPagesList = 8192;  // page ids kept in LDS
 constexpr int kPagesBits = 4096;  // words of 64 table entries kept in LDS
+constexpr int kPagesRows = 4096;  // rows whose lengths are kept in LDS
 
 struct PagesParams {
   int32_t* tbl; int64_t s_bt; int B, C;
@@ -85,7 +90,7 @@ __device__ __forceinline__ int block_prefix(int x, int& total, int (&part)[kPage
   return before + v - x;
 }
 
-// The thread's 16 counts from page `base` on (its own 64 bytes of ref); pages past the pool count as `past`.
+// The thread's kPagesPer counts from page `base` on; pages past the pool count as `past`.
 struct PageCounts {
   v4i x[kPagesPer / 4];
   __device__ __forceinline__ uint32_t used() const {
@@ -140,25 +145,45 @@ __global__ __launch_bounds__(kPagesThreads) void pages_reserve_kernel(PagesParam
   __shared__ int part[kPagesWaves], near_list[kPagesList];
   __shared__ uint64_t near_bits[kPagesBits];
   __shared__ int near_at[kPagesBits];
+  __shared__ int cols[kPagesRows];
   const int lane = lane_id(), w = uniform(wave_id());
   const PageCounts first = load_counts(p.ref, p.P, 0, 1);
-  // A word for each 64 entries of a row, with the bits of those that want a page: eight to a wave in flight.
+  for (int b = threadIdx.x; b < min(p.B, kPagesRows); b += kPagesThreads) cols[b] = pages_of(p.lens[b], p.PAGE, p.C);
+  __syncthreads();
+  // A word for each 64 entries of a row, with the bits of those that want a page.  Of each 1024 words a wave has
+  // one of every 16; which of them turns with their number, so that words a fixed step apart -- rows that
+  // grow by a page each -- fall to different waves.  A wave looks at its 64 words at once, a lane to a word,
+  // and then reads the entries of those that count, eight words in flight: tables are as wide as the longest
+  // row may become (32 rows of 4096 columns, a page each, with the launch: 84 us when every entry was read).
   const int words = (p.C + kWave - 1) / kWave, units = p.B * words;
   uint64_t* bits = units <= kPagesBits ? near_bits : p.bits;
   int* at = units <= kPagesBits ? near_at : p.table;
+  auto word = [&](int u0, int l) { return u0 + kPagesWaves * l + ((w + l + l / 4 + l / 16) & (kPagesWaves - 1)); };
   constexpr int U = 8;
-  for (int u0 = w * U; u0 < units; u0 += kPagesWaves * U) {
-    int id[U], np[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int u = min(u0 + i, units - 1), b = u / words, c = (u - b * words) * kWave + lane;
-      np[i] = pages_of(p.lens[b], p.PAGE, p.C) - (u - b * words) * kWave;  // columns of the word that count
-      id[i] = p.tbl[b * p.s_bt + min(c, p.C - 1)];
+  for (int u0 = 0; u0 < units; u0 += kPagesThreads) {
+    const int mine = word(u0, lane), row = min(mine, units - 1) / words, k = mine - row * words;
+    int count = 0;  // columns of the word that count
+    if (mine < units) {
+      count = (row < kPagesRows ? cols[row] : pages_of(p.lens[row], p.PAGE, p.C)) - k * kWave;
+      if (count <= 0) bits[mine] = 0;
     }
+    uint64_t todo = __builtin_amdgcn_ballot_w64(count > 0);
+    while (todo != 0) {
+      int id[U], l[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const uint64_t m = __builtin_amdgcn_ballot_w64(lane < np[i] && !is_page(id[i], p.P));
-      if (lane == 0 && u0 + i < units) bits[u0 + i] = m;
+      for (int i = 0; i < U; ++i) {
+        l[i] = todo != 0 ? __ffsll((unsigned long long)todo) - 1 : -1;
+        todo &= todo - 1;  // stays 0
+        if (l[i] < 0) continue;
+        const int c = __builtin_amdgcn_readlane(k, l[i]) * kWave + lane;
+        id[i] = p.tbl[__builtin_amdgcn_readlane(row, l[i]) * p.s_bt + min(c, p.C - 1)];
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (l[i] < 0) continue;
+        const uint64_t m = __builtin_amdgcn_ballot_w64(lane < __builtin_amdgcn_readlane(count, l[i]) && !is_page(id[i], p.P));
+        if (lane == 0) bits[word(u0, l[i])] = m;
+      }
     }
   }
   __syncthreads();
@@ -186,13 +211,12 @@ __global__ __launch_bounds__(kPagesThreads) void pages_reserve_kernel(PagesParam
   const int found = find_free(p.ref, p.P, need, first.used(), list, part);
   if (threadIdx.x == 0) *p.shortage = need - found;
   if (need == 0) return;
-  // Words are dealt to the waves in turn; a wave looks at 64 of its at once and hands out those that want any, a
-  // lane to an entry.
-  for (int u0 = w; u0 < units; u0 += kPagesThreads) {
-    const int mine = u0 + kPagesWaves * lane;
+  // A wave hands out its words' wants, a lane to an entry.
+  for (int u0 = 0; u0 < units; u0 += kPagesThreads) {
+    const int mine = word(u0, lane);
     uint64_t todo = __builtin_amdgcn_ballot_w64(mine < units && bits[min(mine, units - 1)] != 0);
     for (; todo != 0; todo &= todo - 1) {
-      const int u = uniform(u0 + kPagesWaves * (__ffsll((unsigned long long)todo) - 1)), b = u / words;
+      const int u = uniform(word(u0, __ffsll((unsigned long long)todo) - 1)), b = u / words;
       const uint64_t m = bits[u];
       if (((m >> lane) & 1) == 0) continue;
       const int rank = at[u] + __popcll(m & ((1ull << lane) - 1));
@@ -321,18 +345,24 @@ __global__ __launch_bounds__(kPagesThreads) void pages_compact_kernel(PagesParam
     const uint32_t bits = c.used() & ~((1u << below) - 1);
     int total;
     int rank = done + block_prefix(__popc(bits), total, part);
+    v4i to[kPagesPer / 4];
 #pragma unroll
     for (int i = 0; i < kPagesPer; ++i) {
-      if (at + i >= p.P) continue;
-      int to = at + i;
-      if ((bits >> i) & 1) {
-        to = holes.get(rank);
-        p.src[rank] = at + i;
-        p.dst[rank++] = to;
-        p.ref[to] = c.x[i / 4][i % 4];
-        p.ref[at + i] = 0;
-      }
-      p.map[at + i] = to;
+      to[i / 4][i % 4] = at + i;
+      if (((bits >> i) & 1) == 0) continue;
+      const int hole = to[i / 4][i % 4] = holes.get(rank);
+      p.src[rank] = at + i;
+      p.dst[rank++] = hole;
+      p.ref[hole] = c.x[i / 4][i % 4];
+      p.ref[at + i] = 0;
+    }
+    if (at + kPagesPer <= p.P && ((uintptr_t)p.map & 15) == 0) {
+#pragma unroll
+      for (int i = 0; i < kPagesPer / 4; ++i) reinterpret_cast<v4i*>(p.map + at)[i] = to[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPagesPer; ++i)
+        if (at + i < p.P) p.map[at + i] = to[i / 4][i % 4];
     }
     done += total;
   }

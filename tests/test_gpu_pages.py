@@ -73,6 +73,41 @@ def test_reserve_and_free(B, cols, P, page, room):
     equal("table", tt, t3), equal("ref", tr, r3)
 
 
+def test_more_rows_wants_and_moves_than_stay_on_the_chip():
+    """5000 rows, 15000 wants at once and as many moves; then rows that grow by a page each in a wide table."""
+    rng = np.random.default_rng(5)
+    B, cols, P, page = 5000, 3, 60000, 16
+    tbl, ref = np.full((B, cols), -1, np.int32), np.zeros(P, np.int32)
+    ref[rng.permutation(P)[:P // 2]] = 1  # held elsewhere
+    lens = np.full(B, cols * page, np.int32)
+    lens[::7] = rng.integers(-5, cols * page, lens[::7].shape)
+    note("pages many rows and moves")
+    tt, tr = gpu(tbl, ref)
+    short = K.paged_kv_reserve(tt, tr, gpu(lens)[0], page)
+    t2, r2, s2 = C.reserve(tbl, ref, lens, page)
+    torch.cuda.synchronize()
+    equal("table", tt, t2), equal("ref", tr, r2), equal("shortage", short, np.asarray([s2], np.int32))
+    perm = rng.permutation(P).astype(np.int32)  # the same pages, spread over the pool
+    t3, r3 = perm[t2] * (t2 >= 0) - (t2 < 0), np.zeros(P, np.int32)
+    t3 = t3.astype(np.int32)
+    r3[t3[t3 >= 0]] = 1
+    tt, tr = gpu(t3, r3)
+    got = K.paged_kv_compact(tt, tr, [])
+    t4, r4, m4, _ = C.compact(t3, r3)
+    torch.cuda.synchronize()
+    assert (m4 != np.arange(P)).sum() > 8192
+    equal("table", tt, t4), equal("ref", tr, r4), equal("map", got, m4)
+    wide, ref = np.full((70, 1024), -1, np.int32), np.zeros(900, np.int32)
+    tt, tr = gpu(wide, ref)
+    for n in (1, 17, 100, 161):
+        lens = np.full(70, n, np.int32)
+        lens[3], lens[69] = 0, n + 16
+        short = K.paged_kv_reserve(tt, tr, gpu(lens)[0], page)
+        wide, ref, s2 = C.reserve(wide, ref, lens, page)
+        torch.cuda.synchronize()
+        equal("table", tt, wide), equal("ref", tr, ref), equal("shortage", short, np.asarray([s2], np.int32))
+
+
 @pytest.mark.parametrize("B,cols,P,page,extra", [(1, 1, 4, 16, 4), (4, 6, 60, 16, 40), (32, 40, 1500, 16, 64),
                                                  (9, 1030, 5000, 16, 9), (300, 4, 1500, 48, 20), (6, 5, 33, 16, 2)])
 def test_fork(B, cols, P, page, extra):
