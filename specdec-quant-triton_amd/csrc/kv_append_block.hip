@@ -8,8 +8,9 @@
 //        below the first new one), s' = max(s', s) with s its scale so far;
 //   new codes      rne(x / s');
 //   earlier codes  rne(c * s / s'), clamped to +-Q, where s' > s, untouched otherwise.
-// fp32, the quotients rounded as IEEE division rounds them.  Infinities count as +-65504 and NaN as 0, so that one bad value does not
-// take the block's other tokens with it.  Slots past the last new token are not touched.
+// fp32, the quotients rounded as IEEE division rounds them.  Infinities count as +-65504 and NaN as 0, so
+// that one bad value does not take the block's other tokens with it.  Slots past the last new token are
+// not touched.
 //
 // One workgroup per (sequence, block, K or V, head): SB * D values, eight to a thread and pass, held in
 // registers between the amax and the codes (up to 16384 values; larger blocks are read twice).  The

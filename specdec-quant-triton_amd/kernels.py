@@ -1091,6 +1091,20 @@ def rotary_inv_freq(dim: int, base: float = 10000.0, scaling=None, factor: float
     return f.to(device), mscale
 
 
+def _rotary_out(who: str, x, shape, strides, D: int, out):
+    """Checks an input of rotary_embed and its output, made where omitted; returns the output and its strides."""
+    if x.dtype != torch.float16 or (D > 1 and strides[3] != 1):
+        raise RuntimeError(f"{who}: inputs must be fp16 with contiguous head_dim")
+    if out is None:
+        out = torch.empty_like(x)
+    elif out.dtype != torch.float16 or out.shape != shape:
+        raise RuntimeError(f"{who}: inputs and outputs must be fp16 of one shape")
+    so = out.stride()
+    if D > 1 and so[3] != 1:
+        raise RuntimeError(f"{who}: head_dim must be contiguous")
+    return out, so
+
+
 def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, interleaved=False, mscale=1.0, plan=None,
                  n_seqs=None, q_out=None, k_out=None):
     """Rotary positions of the new tokens' q and k; returns (q_out, k_out).
@@ -1106,24 +1120,21 @@ def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, inter
     """
     who = "rotary_embed"
     dev = _gpu_of(who, q, k, inv_freq, ctx_len, positions, plan, q_out, k_out)
-    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
-        raise RuntimeError(f"{who}: q [B, QL, H, D] and k [B, QL, H_KV, D] expected")
-    B, QL, H, D = q.shape
-    q_out = torch.empty_like(q) if q_out is None else q_out
-    if k is None:
-        H_KV = 0
-        if k_out is not None:
-            raise RuntimeError(f"{who}: k_out without k")
+    shape, qs = q.shape, q.stride()
+    if len(shape) != 4:
+        raise RuntimeError(f"{who}: q [B, QL, H, D] expected")
+    B, QL, H, D = shape
+    q_out, qo = _rotary_out(who, q, shape, qs, D, q_out)
+    if k is not None:
+        shape, ks = k.shape, k.stride()
+        if len(shape) != 4 or shape[0] != B or shape[1] != QL or shape[3] != D:
+            raise RuntimeError(f"{who}: k [B, QL, H_KV, D] expected")
+        H_KV = shape[2]
+        k_out, ko = _rotary_out(who, k, shape, ks, D, k_out)
+    elif k_out is not None:
+        raise RuntimeError(f"{who}: k_out without k")
     else:
-        H_KV = k.shape[2]
-        k_out = torch.empty_like(k) if k_out is None else k_out
-    for x, y in ((q, q_out), (k, k_out)):
-        if x is None:
-            continue
-        if x.dtype != torch.float16 or y.dtype != torch.float16 or x.shape != y.shape:
-            raise RuntimeError(f"{who}: inputs and outputs must be fp16 of one shape")
-        if D > 1 and (x.stride(3) != 1 or y.stride(3) != 1):
-            raise RuntimeError(f"{who}: head_dim must be contiguous")
+        H_KV, ks, ko = 0, (0, 0, 0), (0, 0, 0)
     if inv_freq.dtype not in (torch.float32, torch.float64) or inv_freq.dim() != 1 or \
             (inv_freq.stride(0) != 1 and inv_freq.shape[0] > 1):
         raise RuntimeError(f"{who}: inv_freq must be a contiguous fp32 or fp64 vector")
@@ -1141,8 +1152,6 @@ def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, inter
         raise RuntimeError(f"{who}: ctx_len or positions must be given")
     if Bg == 0 or Qg == 0:
         return q_out, k_out
-    qs, qo = q.stride(), q_out.stride()
-    ks, ko = (k.stride(), k_out.stride()) if k is not None else ((0, 0, 0), (0, 0, 0))
     _call_on(dev, "specq_rotary", q.data_ptr(), qs[0], qs[1], qs[2], _ptr(k), ks[0], ks[1], ks[2],
              q_out.data_ptr(), qo[0], qo[1], qo[2], _ptr(k_out), ko[0], ko[1], ko[2],
              inv_freq.data_ptr(), inv_freq.dtype == torch.float64, mscale,
@@ -1152,26 +1161,29 @@ def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, inter
 
 
 def _block_cache(who: str, kc, vc, ks, vs, block_tbl, ctx_len, seqs: int, H_KV: int, D: int):
-    """Checks a block-scaled cache for `seqs` sequences; returns (e4m3 codes, tokens per block)."""
-    if kc.dtype != vc.dtype or kc.dtype not in (torch.int8, torch.float8_e4m3fn):
+    """Checks a block-scaled cache for `seqs` sequences; returns (e4m3 codes, tokens per block, strides of the codes
+    and of the scales)."""
+    kind = kc.dtype
+    if kind != vc.dtype or kind not in (torch.int8, torch.float8_e4m3fn):
         raise RuntimeError(f"{who} expects int8 or float8_e4m3fn K/V caches of one type")
-    if kc.dim() != 4 or kc.shape != vc.shape or kc.stride() != vc.stride() or kc.stride(3) != 1:
+    shape, cs = kc.shape, kc.stride()
+    if len(shape) != 4 or shape != vc.shape or cs != vc.stride() or cs[3] != 1:
         raise RuntimeError(f"{who}: K/V caches must share a layout [pages, PAGE, H_KV, D] with contiguous head_dim")
-    if kc.shape[2] != H_KV or kc.shape[3] != D:
-        raise RuntimeError(f"{who}: cache {tuple(kc.shape)} does not fit {H_KV} K/V heads of {D}")
-    P, PAGE = kc.shape[0], kc.shape[1]
-    if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.dim() != 3 or ks.shape != vs.shape or \
-            ks.stride() != vs.stride():
+    P, PAGE, heads, dim = shape
+    if heads != H_KV or dim != D:
+        raise RuntimeError(f"{who}: cache {tuple(shape)} does not fit {H_KV} K/V heads of {D}")
+    shape, ss = ks.shape, ks.stride()
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32 or len(shape) != 3 or shape != vs.shape or ss != vs.stride():
         raise RuntimeError(f"{who}: scales must be fp32 [pages, blocks, H_KV] of one layout")
-    NB = ks.shape[1]
-    if ks.shape[0] != P or ks.shape[2] != H_KV or NB < 1 or PAGE % NB or (PAGE // NB) % 16:
-        raise RuntimeError(f"{who}: scales {tuple(ks.shape)} must be [{P}, blocks, {H_KV}] with blocks of a multiple "
+    NB = shape[1]
+    if shape[0] != P or shape[2] != H_KV or NB < 1 or PAGE % NB or (PAGE // NB) % 16:
+        raise RuntimeError(f"{who}: scales {tuple(shape)} must be [{P}, blocks, {H_KV}] with blocks of a multiple "
                            f"of 16 of the page's {PAGE} tokens")
     if block_tbl.dtype != torch.int32 or block_tbl.dim() != 2 or block_tbl.shape[0] < seqs or \
             (block_tbl.stride(1) != 1 and block_tbl.shape[1] > 1):
         raise RuntimeError(f"{who}: block_tbl must be int32 [B, max_pages] with unit inner stride for {seqs} sequences")
     _int32_vec(who, "ctx_len", ctx_len, seqs)
-    return kc.dtype == torch.float8_e4m3fn, PAGE // NB
+    return kind == torch.float8_e4m3fn, PAGE // NB, cs, ss
 
 
 def paged_kv_append_block_scaled(k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_len, q_len=None, plan=None, n_seqs=None):
@@ -1196,12 +1208,12 @@ def paged_kv_append_block_scaled(k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_le
         raise RuntimeError(f"{who} expects fp16 k_new and v_new")
     B, QL, H_KV, D = k_new.shape
     Bg, Qg, n_seqs, q_len = _token_grid(who, B, QL, q_len, n_seqs, plan)
-    f8, sb = _block_cache(who, kc, vc, ks, vs, block_tbl, ctx_len, Bg, H_KV, D)
+    f8, sb, cs, ss = _block_cache(who, kc, vc, ks, vs, block_tbl, ctx_len, Bg, H_KV, D)
     if k_new.stride() != v_new.stride() or k_new.stride(3) != 1:
         k_new, v_new = k_new.contiguous(), v_new.contiguous()
     if Bg == 0 or Qg == 0:
         return
-    kn, cs, ss = k_new.stride(), kc.stride(), ks.stride()
+    kn = k_new.stride()
     _call_on(dev, "specq_kv_append_block", k_new.data_ptr(), v_new.data_ptr(), kn[0], kn[1], kn[2],
              kc.data_ptr(), vc.data_ptr(), f8, cs[0], cs[1], cs[2],
              ks.data_ptr(), vs.data_ptr(), ss[0], ss[1], ss[2], sb,
@@ -1246,7 +1258,7 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
     H_KV = kc.shape[2]
     G = H // H_KV
     Bg, Qg, n_seqs, q_len = _token_grid(who, B, QL, q_len, n_seqs, plan)
-    f8, sb = _block_cache(who, kc, vc, ks, vs, block_tbl, ctx_len, Bg, H_KV, D)
+    f8, sb, cs, ss = _block_cache(who, kc, vc, ks, vs, block_tbl, ctx_len, Bg, H_KV, D)
     if QPP is None:
         n = -(-Qg // max(1, 64 // G))  # programs
         QPP = max(1, -(-Qg // max(1, n)))
@@ -1257,7 +1269,7 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
     elif out.dtype != torch.float16 or out.shape != q.shape or out.stride(3) != 1:
         raise RuntimeError(f"{who}: out must be fp16 of q's shape {tuple(q.shape)} with contiguous head_dim")
     PAGE, max_pages = kc.shape[1], block_tbl.shape[1]
-    qs, cs, ss, os_ = q.stride(), kc.stride(), ks.stride(), out.stride()
+    qs, os_ = q.stride(), out.stride()
     QPP = int(QPP)
     ck = _block_attn_info(D, f8, QPP * G, dev)
     if Bg == 0 or Qg == 0:
