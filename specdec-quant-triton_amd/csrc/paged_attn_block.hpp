@@ -39,7 +39,7 @@
 // Measured in a graph, 32 / 8 heads, D = 128, codes read per second: 32 sequences of one token, contexts up to
 // 8192, int8 85.5 us = 3.8 TB/s; 8 and 32 sequences of 9 tokens, context 4096, e4m3 25.9 us = 2.6 TB/s and
 // 62.9 us = 4.3 TB/s (of the 25.9, 14 are the loop, the rest start, first loads and merges); 2 x 256
-// tokens, contexts up to 4096, int8 50.0 us, e4m3 46.2, bound by instructions; one sequence of 5 tokens,
+// tokens, contexts up to 4096, int8 48.3 us, e4m3 45.3, bound by instructions; one sequence of 5 tokens,
 // context 131072, 16 / 2 heads, D = 64, e4m3 21.8 us, 4.4 of them the merge launch.
 // A row's result does not depend on the rows packed with it: split boundaries, chunks and merge orders are
 // fixed, so QPP = 1, fused, eager and plan calls agree bit for bit.
@@ -377,6 +377,9 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
   // accumulator: they read V behind the softmax, refill the slot then, and form the scores again in the
   // rare case that a row's max moves behind the first chunk.
   constexpr bool LATE = RB >= 3 && D == 128;
+  // A wave between its matrix instructions goes before the SIMD's other wave in its softmax, which fills the gaps
+  // (2 x 256 tokens, context 4096, D = 128: int8 51.9 -> 50.3 us, e4m3 46.2 -> 45.4; nothing at 16 or 32 rows).
+  constexpr bool PRIO = RB >= 3;
   auto chunk = [&](uint32_t slot, int it) __attribute__((always_inline)) {
     const uint32_t k_s = k_at + slot, v_s = v_at + slot;
     if constexpr (LATE) asm volatile("" : "+v"(q_at));  // Q's addresses are formed here, not kept
@@ -387,7 +390,9 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
       for (int db = 0; db < ND; ++db) vx[db] = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i)(v_s ^ (16 * db)));
     };
     if constexpr (!LATE) read_v();
+    if constexpr (PRIO) __builtin_amdgcn_s_setprio(1);
     scores(std::integral_constant<int, 0>{}, std::integral_constant<int, RB>{}, k_s, cs);
+    if constexpr (PRIO) __builtin_amdgcn_s_setprio(0);
     if constexpr (!LATE) {  // the slot has been read: its next chunk may come
       wait_lgkm0();
       issue(slot, it + NS);
@@ -531,12 +536,14 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
         }
       }
     }
+    if constexpr (PRIO) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int db = 0; db < ND; ++db) {
       const v8h vf = code8_to_h8<F8>((uint32_t)vx[db].x, (uint32_t)vx[db].y);
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) acc[rb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rb], acc[rb][db], 0, 0, 0);
     }
+    if constexpr (PRIO) __builtin_amdgcn_s_setprio(0);
   };
   // One copy of the loop's code serves all slots: a launch finds the instruction cache cold, and most calls
   // go around a few times only.
