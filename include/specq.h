@@ -323,10 +323,12 @@ int specq_kv_append_int8(const void* k_new, const void* v_new, int64_t s_nb, int
  *   kc, vc   codes [pages, PAGE, H_KV, D], as specq_paged_attn
  *   ks, vs   fp32 [pages, PAGE / block, H_KV], strides s_sp (page), s_sb (block), s_sh, shared
  *   block    a multiple of 16 that divides PAGE
+ *   s_ko     at least D: the rows of a page must not overlap
  *   Probabilities are rounded to fp16 once, after their V scale, against a running max of what the tokens
- *   contribute.  Scales, and e4m3 NaN codes, of tokens that a row does not see do
- *   not reach it.  Everything else as specq_paged_attn (the workspace:
- *   specq_paged_attn_block_workspace_size; a sequence may be cut into up to 256 splits); QPP = 1, fused, eager and plan-mode calls agree bit for bit.
+ *   contribute.  Scales, and e4m3 NaN codes, of tokens that a row does not see do not reach it.  A context
+ *   longer than the table counts as the table's length, a negative one as 0.  Everything else as
+ *   specq_paged_attn (the workspace: specq_paged_attn_block_workspace_size; a sequence may be cut into up
+ *   to 256 splits); QPP = 1, fused, eager and plan-mode calls agree bit for bit.
  * ------------------------------------------------------------------------------------- */
 size_t specq_paged_attn_block_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP, int max_pages, int PAGE);
 int specq_paged_attn_block(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh,
@@ -343,8 +345,8 @@ int specq_paged_attn_block(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_
  * A block that new tokens reach gets s' = max(amax, 1e-8) / Q over them (Q = 127 for int8, 448 for
  * e4m3), or its present scale where that is larger and the block holds earlier tokens of the sequence;
  * codes are rne(x / s'), earlier codes rne(c s / s') where s' > s.  fp32, IEEE division.  Infinities
- * count as +-65504, NaN as 0.  Slots that hold no token of the sequence are not written.  A page may be
- * written for one sequence only.
+ * count as +-65504, NaN as 0.  Slots that hold no token of the sequence are not written.  A page that is
+ * written must be named by one entry of the table only.
  *   D must be 64, 128 or 256; cache rows 8-byte, new rows 16-byte aligned.
  * ------------------------------------------------------------------------------------- */
 int specq_kv_append_block(const void* k_new, const void* v_new, int64_t s_nb, int64_t s_nt, int64_t s_nh,
@@ -409,7 +411,8 @@ int specq_kv_pages_copy(const int32_t* src, const int32_t* dst, int n, int n_pag
 
 /* Calls specq_<name> (specq_rotary, specq_kv_append_block, specq_paged_attn_block or a specq_kv_pages_
  * function that returns int) with its n arguments as 64-bit words in their order: pointers and integers as they
- * are, floats as the bits of a double.  For bindings that pay for every argument they convert. */
+ * are, floats as the bits of a double.  An integer that does not fit its argument's type is -22.  For bindings
+ * that pay for every argument they convert. */
 int specq_call_packed(const char* name, const int64_t* words, int n);
 
 /* ---------------------------------------------------------------------------------------

@@ -1242,8 +1242,9 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
     [pages, PAGE / SB, H_KV] (paged_kv_append_block_scaled); block_tbl int32 [B, max_pages]; ctx_len
     int32 [B], counting the q_len new tokens, which are each sequence's last ones and see one another
     causally; a context longer than the table counts as the table's length.  Block-table ids outside
-    [0, pages) mask their page's tokens; a row that sees no token gives 0.  QPP query tokens run in one program, at most 64 rows of H / H_KV heads each (default: as few
-    programs as that takes, of even size).  sm_scale defaults to D^-1/2.  With `plan`, (n_seqs, q_len) =
+    [0, pages) mask their page's tokens; a row that sees no token gives 0.  QPP query tokens run in one
+    program, at most 64 rows of H / H_KV heads each (default: as few programs as that takes, of even
+    size); every QPP gives the same bits.  sm_scale defaults to D^-1/2.  With `plan`, (n_seqs, q_len) =
     plan[0:2] on the device and the grid covers (B, QLMAX); rows that are not active are not written (an
     omitted `out` is zero there).  Calls that may run at the same time on several streams need a workspace
     each.
