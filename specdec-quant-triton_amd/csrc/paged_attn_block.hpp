@@ -658,11 +658,14 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
   tl_mark(p.tl, p.tl_cap, 5);  // diagnostics build: partials issued
   if (p.defer) return;
   if (!arrive_last(p.counters + prog, n_active, &lds.last, p.tl, p.tl_cap)) return;
-  // The last split to arrive sums the program's, in split order: weights exp2(m_s - max) / l first (one
-  // thread a row and all pairs in flight together), then the rows.
+  // The last split to arrive sums the program's, in split order: weights exp2(m_s - max) and 1 / l first (one
+  // thread a row and all pairs in flight together), then the rows.  A plan-mode call may merge the same
+  // splits by attn_merge_kernel, and both take the same steps: products rounded on their own, l summed as
+  // a butterfly over lanes sums it, the rows in split order, then 1 / l.
   float* wts = reinterpret_cast<float*>(lds.ring[0]);  // [ROWS][kBlkMergeIn]
   if (threadIdx.x < ROWS) {
-    float mv[kBlkMergeIn], lv[kBlkMergeIn], mx = -INFINITY, l = 0.f;
+#pragma clang fp contract(off)
+    float mv[kBlkMergeIn], lv[kBlkMergeIn], mx = -INFINITY;
 #pragma unroll
     for (int sp = 0; sp < kBlkMergeIn; ++sp) {
       const float* src = mlpart + ((prog_base + min(sp, n_active - 1)) * ROWS + threadIdx.x) * 2;
@@ -674,14 +677,16 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
       if (sp < n_active) mx = fmaxf(mx, mv[sp]);
     const float mxs = (mx == -INFINITY) ? 0.f : mx;
 #pragma unroll
-    for (int sp = 0; sp < kBlkMergeIn; ++sp)
-      if (sp < n_active) {
-        mv[sp] = fast_exp2(mv[sp] - mxs);
-        l += mv[sp] * lv[sp];
-      }
-    const float inv = (l == 0.f) ? 0.f : 1.f / l;
+    for (int sp = 0; sp < kBlkMergeIn; ++sp) {
+      const float wt = sp < n_active ? fast_exp2(mv[sp] - mxs) : 0.f;
+      wts[threadIdx.x * kBlkMergeIn + sp] = wt;
+      lv[sp] = sp < n_active ? wt * lv[sp] : 0.f;
+    }
 #pragma unroll
-    for (int sp = 0; sp < kBlkMergeIn; ++sp) wts[threadIdx.x * kBlkMergeIn + sp] = mv[sp] * inv;
+    for (int h = kBlkMergeIn / 2; h >= 1; h /= 2)
+#pragma unroll
+      for (int sp = 0; sp < h; ++sp) lv[sp] += lv[sp + h];
+    lds.row[1][threadIdx.x] = lv[0] == 0.f ? 0.f : 1.f / lv[0];
   }
   v4i part[ITEMS <= 2 ? kBlkMergeIn : kBlkMergeIn / 2][ITEMS];
   constexpr int SBT = ITEMS <= 2 ? kBlkMergeIn : kBlkMergeIn / 2;  // splits whose rows are in flight together
@@ -699,12 +704,14 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
     for (int u = 0; u < SBT; ++u)
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it)
-        if (ivalid[it] && sp0 + u < n_active)
+        if (ivalid[it] && sp0 + u < n_active) {
+#pragma clang fp contract(off)
           o[it] += wts[((int)threadIdx.x / QPR + RPI * it) * kBlkMergeIn + sp0 + u] * __builtin_bit_cast(v4f, part[u][it]);
+        }
   }
 #pragma unroll
   for (int it = 0; it < ITEMS; ++it)
-    if (ivalid[it]) store_row4(it, o[it]);
+    if (ivalid[it]) store_row4(it, o[it] * lds.row[1][(int)threadIdx.x / QPR + RPI * it]);
   tl_mark_drained(p.tl, p.tl_cap, 6);  // diagnostics build: splits merged and stored
 }
 
@@ -746,7 +753,8 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnBlockParams p) {
   }
   n_seqs = uniform(n_seqs);
   q_len = uniform(q_len);
-  const int per = p.QPP * p.G, rows = (per + 15) / 16 * 16;
+  // Rows of a program's partials: those of the row blocks it ran with, in plan mode the active q_len's.
+  const int per = p.QPP * p.G, rows = ((p.plan != nullptr ? min(q_len, p.QPP) * p.G : per) + 15) / 16 * 16;
   const int prog = (int)blockIdx.x / per, row = (int)blockIdx.x - prog * per;
   const int qc = prog % p.n_qc, kvh = (prog / p.n_qc) % p.H_KV, b = prog / (p.n_qc * p.H_KV);
   const int qi = qc * p.QPP + row / p.G;
@@ -774,9 +782,13 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnBlockParams p) {
   __syncthreads();
   mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   const float w = fast_exp2(m - (mx == -INFINITY ? 0.f : mx));
-  float ls = t < n ? w * l : 0.f;
+  float ls;
+  {
+#pragma clang fp contract(off)
+    ls = t < n ? w * l : 0.f;
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) ls += __shfl_xor(ls, o);
+    for (int o = 32; o >= 1; o >>= 1) ls += __shfl_xor(ls, o);
+  }
   if (lane_id() == 0) red[1][wave_id()] = ls;
   wt[t] = t < n ? w : 0.f;
   __syncthreads();

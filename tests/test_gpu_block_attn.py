@@ -252,6 +252,37 @@ def test_plan_mode_equals_eager_and_leaves_the_rest():
         assert torch.equal(out, eager), (n, ql)
 
 
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("ctx,q_len,QM,H,H_KV,D", [
+    ([5000, 63], 1, 4, 40, 8, 128),      # merged by a launch: one row block, captured for two
+    ([5000, 5000], 1, 8, 8, 2, 128),     # ... for two
+    ([3000, 2000], 3, 16, 32, 8, 64),    # ... for four
+    ([4096, 300], 9, 20, 32, 8, 128),    # three of four, two programs
+    ([5000, 2100], 1, 1, 16, 16, 128),   # eight splits an eager call merges in place and the graph does not
+    ([4100, 1000], 2, 5, 16, 16, 64),
+])
+def test_plan_mode_of_many_splits(ctx, q_len, QM, H, H_KV, D, fmt):
+    rng = np.random.default_rng(sum(ctx) + QM)
+    cache = make_cache(rng, ctx, H_KV, D, 64, 64, fmt)
+    q = queries(rng, len(ctx), q_len, H, D)
+    ref = C.attention_block(q, *cache, q_len, fmt)
+    q, *cache = gpu(q, *cache)
+    eager = K.paged_attention_block_scaled(q, *cache, q_len)[0]
+    note(f"block attn plan of many splits {fmt} ctx={ctx} q_len={q_len} QM={QM}")
+    grid = torch.full((len(ctx), QM, H, D), 3, dtype=torch.float16, device=DEV)
+    grid[:, :q_len] = q
+    out = torch.full_like(grid, 7)
+    plan = torch.tensor([len(ctx), q_len], dtype=torch.int32, device=DEV)
+    K.paged_attention_block_scaled(grid, *cache, plan=plan, out=out)
+    torch.cuda.synchronize()
+    check(out, ref, q_len, len(ctx), D, "plan")
+    assert torch.equal(out[:, :q_len], eager) and bool((out[:, q_len:] == 7).all())
+    plan[0] = 1
+    K.paged_attention_block_scaled(grid, *cache, plan=plan, out=out)
+    one = K.paged_attention_block_scaled(q[:1], *cache[:4], cache[4][:1], cache[5][:1], q_len)[0]
+    assert torch.equal(out[:1, :q_len], one) and torch.equal(out[1:, :q_len], eager[1:])
+
+
 def test_streams_with_their_own_workspaces():
     from specq.workspace import Workspace
     rng = np.random.default_rng(14)
