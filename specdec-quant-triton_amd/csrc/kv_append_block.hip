@@ -93,6 +93,7 @@ __device__ __forceinline__ v2i encode8_by(v8h x, float s, float y) {
   for (int j = 0; j < 8; ++j) {
     const float f = (float)x[j], q0 = f * y;
     q[j] = fmaf(fmaf(-q0, s, f), y, q0);
+    if constexpr (F8) q[j] = __builtin_copysignf(q[j], f);  // -0 stays -0
   }
   int w[2] = {0, 0};
 #pragma unroll

@@ -159,6 +159,30 @@ def test_views_and_plan_graph():
     assert all(bool((p[:, 1] == 3).all()) for p in pools)
 
 
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_every_small_and_negative_zero(fmt):
+    """Zeros of both signs, subnormals, and every value next to them, below amax from one subnormal to the largest."""
+    bits = np.concatenate([np.arange(0, 1024), np.arange(1024, 0x7C00, 37)]).astype(np.uint16)
+    bits = np.concatenate([bits, bits | 0x8000])
+    rows = -(-len(bits) // 64)
+    x = np.zeros(rows * 64, np.uint16)
+    x[:len(bits)] = bits
+    x = np.random.default_rng(3).permutation(x).view(np.float16).reshape(rows, 64)
+    for top in (0.0, 6e-8, 6e-5, 0.37, 65504.0):
+        new = np.where(np.abs(x) <= np.float16(top), x, np.copysign(np.float16(0), x))
+        new = np.stack([new, -new])[:, None, :, None, :]
+        pages = -(-rows // 16)
+        kc, vc, ks, vs, bt, ctx = make_cache(np.random.default_rng(1), [rows], 1, 64, 16, 16, fmt)
+        note(f"block append zeros {fmt} {top}")
+        t = gpu(new[0], new[1], kc, vc, ks, vs, bt, ctx)
+        K.paged_kv_append_block_scaled(*t, rows)
+        torch.cuda.synchronize()
+        want = C.append_block(new[0], new[1], kc, vc, ks, vs, bt, ctx, rows, fmt)
+        assert (bt[0] >= 0).sum() == pages
+        for got, w in zip(t[2:6], want):
+            assert np.array_equal(raw(got), w), top
+
+
 def test_negative_lengths_write_nothing():
     rng = np.random.default_rng(21)
     kc, vc, ks, vs, bt, _ = make_cache(rng, [64, 64, 64], 2, 64, 16, 16, "int8")
