@@ -658,10 +658,10 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
   tl_mark(p.tl, p.tl_cap, 5);  // diagnostics build: partials issued
   if (p.defer) return;
   if (!arrive_last(p.counters + prog, n_active, &lds.last, p.tl, p.tl_cap)) return;
-  // The last split to arrive sums the program's, in split order: weights exp2(m_s - max) and 1 / l first (one
+  // The last split to arrive sums the program's, in split order: weights exp2(m_s - max) / l first (one
   // thread a row and all pairs in flight together), then the rows.  A plan-mode call may merge the same
   // splits by attn_merge_kernel, and both take the same steps: products rounded on their own, l summed as
-  // a butterfly over lanes sums it, the rows in split order, then 1 / l.
+  // a butterfly over lanes sums it, the weighted rows in split order.
   float* wts = reinterpret_cast<float*>(lds.ring[0]);  // [ROWS][kBlkMergeIn]
   if (threadIdx.x < ROWS) {
 #pragma clang fp contract(off)
@@ -678,15 +678,20 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
     const float mxs = (mx == -INFINITY) ? 0.f : mx;
 #pragma unroll
     for (int sp = 0; sp < kBlkMergeIn; ++sp) {
-      const float wt = sp < n_active ? fast_exp2(mv[sp] - mxs) : 0.f;
-      wts[threadIdx.x * kBlkMergeIn + sp] = wt;
-      lv[sp] = sp < n_active ? wt * lv[sp] : 0.f;
+      if (sp < n_active) {
+        mv[sp] = fast_exp2(mv[sp] - mxs);
+        lv[sp] = mv[sp] * lv[sp];
+      } else {
+        mv[sp] = lv[sp] = 0.f;
+      }
     }
 #pragma unroll
     for (int h = kBlkMergeIn / 2; h >= 1; h /= 2)
 #pragma unroll
       for (int sp = 0; sp < h; ++sp) lv[sp] += lv[sp + h];
-    lds.row[1][threadIdx.x] = lv[0] == 0.f ? 0.f : 1.f / lv[0];
+    const float inv = lv[0] == 0.f ? 0.f : 1.f / lv[0];
+#pragma unroll
+    for (int sp = 0; sp < kBlkMergeIn; ++sp) wts[threadIdx.x * kBlkMergeIn + sp] = mv[sp] * inv;
   }
   v4i part[ITEMS <= 2 ? kBlkMergeIn : kBlkMergeIn / 2][ITEMS];
   constexpr int SBT = ITEMS <= 2 ? kBlkMergeIn : kBlkMergeIn / 2;  // splits whose rows are in flight together
@@ -711,7 +716,7 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
   }
 #pragma unroll
   for (int it = 0; it < ITEMS; ++it)
-    if (ivalid[it]) store_row4(it, o[it] * lds.row[1][(int)threadIdx.x / QPR + RPI * it]);
+    if (ivalid[it]) store_row4(it, o[it]);
   tl_mark_drained(p.tl, p.tl_cap, 6);  // diagnostics build: splits merged and stored
 }
 
@@ -803,13 +808,15 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnBlockParams p) {
     for (int u = 0; u < IN_FLIGHT; ++u) x[u] = o_part[(int64_t)min(s0 + u * NG, n - 1) * rows * LN];
 #pragma unroll
     for (int u = 0; u < IN_FLIGHT; ++u)
-      if (s0 + u * NG < n) o += wt[s0 + u * NG] * x[u];
+      if (s0 + u * NG < n) {
+#pragma clang fp contract(off)
+        o += wt[s0 + u * NG] * inv * x[u];
+      }
   }
   sum[g][c] = o;
   __syncthreads();
   if (g == 0) {
     for (int i = 1; i < NG; ++i) o += sum[i][c];
-    o *= inv;
     const int head = kvh * p.G + row % p.G;
     *reinterpret_cast<v2i*>(p.out + (int64_t)b * p.s_ob + (int64_t)qi * p.s_ot + (int64_t)head * p.s_oh + 4 * c) =
         v2i{(int)pack_h2(o.x, o.y), (int)pack_h2(o.z, o.w)};
