@@ -165,8 +165,8 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
   // Eager calls know the active sequences; a plan may activate as few as one.
   const int ns = n_splits_for(blk, max_pages, PAGE,
                               plan ? H_KV : std::max(n_seqs, 1) * H_KV * attn_row_programs(q_len, G), target);
-  const bool defer = blk && ns > kBlkMergeIn;
   const int64_t progs = (int64_t)B_grid * H_KV * n_qc;
+  const bool defer = blk && (ns > kBlkMergeIn || (ns > 1 && progs > kMaxCounters));
   const int rows = rb * 16;
   size_t need = 0;
   if (ns > 1) {

@@ -283,6 +283,24 @@ def test_plan_mode_of_many_splits(ctx, q_len, QM, H, H_KV, D, fmt):
     assert torch.equal(out[:1, :q_len], one) and torch.equal(out[1:, :q_len], eager[1:])
 
 
+def test_more_programs_than_counters():
+    """1100 sequences of 64 heads: 70400 programs, two splits each; a few of them long, on the same pages."""
+    rng = np.random.default_rng(8)
+    B, H, D, PAGE = 1100, 64, 64, 16
+    kc, vc, ks, vs, row, _ = make_cache(rng, [9000], H, D, PAGE, 16, "int8", spare=0)
+    ctx = np.full(B, 20, np.int32)
+    ctx[[0, 700, 1099]] = 9000, 8193, 8500
+    bt = np.full((B, 1024), -1, np.int32)  # 16384 tokens
+    bt[:, :row.shape[1]] = row
+    q = queries(rng, B, 1, H, D)
+    note("block attn more programs than counters")
+    out = K.paged_attention_block_scaled(*gpu(q, kc, vc, ks, vs, bt, ctx), 1)[0]
+    torch.cuda.synchronize()
+    some = [0, 1, 350, 700, 1098, 1099]
+    ref = C.attention_block(q[some], kc, vc, ks, vs, bt[some], ctx[some], 1, "int8")
+    check(out[some], ref, 1, len(some), D, "many programs")
+
+
 def test_streams_with_their_own_workspaces():
     from specq.workspace import Workspace
     rng = np.random.default_rng(14)
