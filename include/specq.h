@@ -330,7 +330,10 @@ int specq_kv_append_int8(const void* k_new, const void* v_new, int64_t s_nb, int
  *   specq_paged_attn (the workspace: specq_paged_attn_block_workspace_size; a sequence may be cut into up
  *   to 256 splits); QPP = 1, fused, eager and plan-mode calls agree bit for bit.
  * ------------------------------------------------------------------------------------- */
-size_t specq_paged_attn_block_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP, int max_pages, int PAGE);
+/* Bytes for an eager call (plan = 0) of n_seqs = B_grid sequences and q_len = ql_grid tokens, or for a plan-mode call on
+ * that grid; the latter suffice for eager calls of no more sequences and tokens, too. */
+size_t specq_paged_attn_block_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP, int D, int max_pages,
+                                             int PAGE, int plan);
 int specq_paged_attn_block(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh,
                            const void* kc, const void* vc, int code_fp8, int64_t s_kp, int64_t s_ko, int64_t s_kh,
                            const float* ks, const float* vs, int64_t s_sp, int64_t s_sb, int64_t s_sh, int block,

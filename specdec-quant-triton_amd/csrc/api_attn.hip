@@ -56,6 +56,27 @@ int n_splits_for(bool blk, int max_pages, int PAGE, int pairs_min, int target) {
   return std::max(1, ceil_div(cap, per));
 }
 
+// Splits, and the one-dimensional grid of program x split (the kernel derives both from the active count): the
+// exact count for an eager call, the most any active count needs in plan mode.
+struct AttnGrid {
+  int ns;
+  int64_t wgs;
+};
+AttnGrid attn_grid(bool blk, bool plan, int B_grid, int n_seqs, int q_len, int n_qc, int H_KV, int G, int max_pages,
+                   int PAGE, int target) {
+  // Eager calls know the active sequences; a plan may activate as few as one.
+  const int ns = n_splits_for(blk, max_pages, PAGE,
+                              plan ? H_KV : std::max(n_seqs, 1) * H_KV * attn_row_programs(q_len, G), target);
+  int64_t wgs = (int64_t)n_seqs * H_KV * n_qc * ns;
+  if (plan) {
+    // Active query tokens that fill one program cut a sequence finest; past that the cut gets coarser.
+    wgs = 0;
+    for (int s = 1; s <= B_grid; ++s)
+      wgs = std::max(wgs, (int64_t)s * H_KV * n_qc * n_splits_for(blk, max_pages, PAGE, s * H_KV, target));
+  }
+  return {ns, wgs};
+}
+
 }  // namespace
 
 // `variant` is the head dim, | kAttrsScaleFp32 for fp32 K/V scales, | kAttrsBlockI8 / kAttrsBlockF8 for
@@ -88,30 +109,35 @@ int attn_attrs(int variant, int rows, specq_kernel_attrs* out) {
 
 using namespace specq;
 
-static size_t attn_workspace(bool blk, int B_grid, int H, int H_KV, int ql_grid, int QPP, int max_pages, int PAGE) {
+extern "C" size_t specq_paged_attn_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP, int max_pages,
+                                                  int PAGE) {
   if (B_grid <= 0 || H_KV <= 0 || H % H_KV != 0 || QPP <= 0 || ql_grid <= 0 || max_pages <= 0 || PAGE <= 0) return 0;
   const int G = H / H_KV;
   const int rows = ceil_div(QPP * G, 16) * 16;
   const int n_qc = ceil_div(ql_grid, QPP);
   const int64_t progs = (int64_t)B_grid * H_KV * n_qc;
-  if ((int64_t)max_pages * PAGE > (blk ? kBlkMaxTokens : kAttnMaxTokens)) return 0;
+  if ((int64_t)max_pages * PAGE > kAttnMaxTokens) return 0;
   // Plan-mode bound: at least one active sequence.
   const int tgt = g_attn_target.load();
-  const int ns = n_splits_for(blk, max_pages, PAGE, H_KV, tgt > 0 ? tgt : device_cus());
+  const int ns = n_splits_for(false, max_pages, PAGE, H_KV, tgt > 0 ? tgt : device_cus());
   if (ns <= 1) return 0;
   // Sized for D = 128 (the largest supported head dimension).
   const size_t part = (size_t)progs * ns * rows * (128 + 2) * 4;
   return kCounterBytes + align_up(part, 256);
 }
 
-extern "C" size_t specq_paged_attn_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP, int max_pages,
-                                                  int PAGE) {
-  return attn_workspace(false, B_grid, H, H_KV, ql_grid, QPP, max_pages, PAGE);
+static size_t attn_block_bytes(const AttnGrid& g, int rows, int D) {
+  return g.ns <= 1 || g.wgs == 0 ? 0 : kCounterBytes + align_up((size_t)g.wgs * rows * (D + 2) * 4, 256);
 }
 
-extern "C" size_t specq_paged_attn_block_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP,
-                                                        int max_pages, int PAGE) {
-  return attn_workspace(true, B_grid, H, H_KV, ql_grid, QPP, max_pages, PAGE);
+extern "C" size_t specq_paged_attn_block_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int QPP, int D,
+                                                        int max_pages, int PAGE, int plan) {
+  if (B_grid <= 0 || H_KV <= 0 || H % H_KV != 0 || QPP <= 0 || ql_grid <= 0 || max_pages <= 0 || PAGE <= 0) return 0;
+  const int G = H / H_KV, tgt = g_attn_target.load();
+  if ((int64_t)max_pages * PAGE > kBlkMaxTokens || (int64_t)QPP * G > 64) return 0;
+  return attn_block_bytes(attn_grid(true, plan != 0, B_grid, B_grid, ql_grid, ceil_div(ql_grid, QPP), H_KV, G, max_pages,
+                                    PAGE, tgt > 0 ? tgt : device_cus()),
+                          ceil_div(QPP * G, 16) * 16, D);
 }
 
 // Both entry points: `kind` is the cache's, `sb` its tokens per scale block (block scales only).
@@ -162,9 +188,8 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
   const int n_qc = ceil_div(plan ? ql_grid : q_len, QPP);
   if (n_qc == 0) return SPECQ_OK;
   const int target = g_attn_target.load() > 0 ? g_attn_target.load() : device_cus();
-  // Eager calls know the active sequences; a plan may activate as few as one.
-  const int ns = n_splits_for(blk, max_pages, PAGE,
-                              plan ? H_KV : std::max(n_seqs, 1) * H_KV * attn_row_programs(q_len, G), target);
+  const AttnGrid grid = attn_grid(blk, plan != nullptr, B_grid, n_seqs, q_len, n_qc, H_KV, G, max_pages, PAGE, target);
+  const int ns = grid.ns;
   const int64_t progs = (int64_t)B_grid * H_KV * n_qc;
   const bool defer = blk && (ns > kBlkMergeIn || (ns > 1 && progs > kMaxCounters));
   const int rows = rb * 16;
@@ -172,19 +197,12 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
   if (ns > 1) {
     SPECQ_REQUIRE(defer || progs <= kMaxCounters, SPECQ_ENOTSUP, "paged_attn: %lld programs exceed the counter region",
                   (long long)progs);
-    need = kCounterBytes + align_up((size_t)progs * ns * rows * (D + 2) * 4, 256);
+    need = blk ? attn_block_bytes(grid, rows, D)
+               : kCounterBytes + align_up((size_t)progs * ns * rows * (D + 2) * 4, 256);
   }
   SPECQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), SPECQ_ENOSPC,
                 "paged_attn: workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : 0);
-  // One-dimensional grid of program x split (the kernel derives both from the active count):
-  // the exact count for an eager call, the most any active count needs in plan mode.
-  int64_t wgs = (int64_t)(plan ? B_grid : n_seqs) * H_KV * n_qc * ns;
-  if (plan) {
-    // Active query tokens that fill one program cut a sequence finest; past that the cut gets coarser.
-    wgs = 0;
-    for (int s = 1; s <= B_grid; ++s)
-      wgs = std::max(wgs, (int64_t)s * H_KV * n_qc * n_splits_for(blk, max_pages, PAGE, s * H_KV, target));
-  }
+  const int64_t wgs = grid.wgs;
   if (wgs == 0) return SPECQ_OK;
   SPECQ_REQUIRE(wgs <= INT32_MAX, SPECQ_ENOTSUP, "paged_attn: grid too large");
   AttnBlockParams p;  // the per-token kernels take its AttnParams
@@ -201,6 +219,7 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
   p.part = need ? (float*)((char*)workspace + kCounterBytes) : nullptr;
   p.sb = sb;
   p.defer = defer;
+  p.n_part = wgs;
   diag_timeline(&p.tl, &p.tl_cap);
   void* args[] = {&p};
   hipError_t e = hipLaunchKernel(fn, dim3((unsigned)wgs), dim3(kAttnThreads), args, 0, (hipStream_t)stream);

@@ -55,6 +55,9 @@ namespace specq {
 struct AttnBlockParams : AttnParams {
   int sb;     // tokens per scale block
   int defer;  // splits are merged by attn_merge_kernel behind this launch
+  // Partials, (program, split) of the active count: part holds [n_part][rows][D] of O, then [n_part][rows][2] of
+  // (m, l).
+  int64_t n_part;
 };
 
 constexpr int kBlkSub = 16;                                  // tokens of a sub-tile
@@ -643,9 +646,9 @@ __device__ __forceinline__ void attn_block_body(const AttnBlockParams& p, AttnBl
   }
 
   // ---- Splits: publish this split's valid rows, 16 bytes per lane.
-  const int64_t prog_base = (int64_t)prog * p.n_splits;
-  const int64_t n_o = (int64_t)p.B_grid * p.H_KV * p.n_qc * p.n_splits * ROWS * D;  // floats of the O region
-  const rsrc_t ors = make_rsrc(p.part + prog_base * ROWS * D, (uint32_t)(p.n_splits * ROWS * D * 4));
+  const int64_t prog_base = (int64_t)prog * ns_act;
+  const int64_t n_o = p.n_part * ROWS * D;  // floats of the O region
+  const rsrc_t ors = make_rsrc(p.part + prog_base * ROWS * D, (uint32_t)(ns_act * ROWS * D * 4));
   float* mlpart = p.part + n_o;
 #pragma unroll
   for (int it = 0; it < ITEMS; ++it)
@@ -770,8 +773,9 @@ __global__ __launch_bounds__(256) void attn_merge_kernel(AttnBlockParams p) {
   const int kv_end = L - q_len + min(qc * p.QPP + p.QPP, q_len);
   const int n = kv_end > split_tokens ? (kv_end + split_tokens - 1) / split_tokens : 1;
   if (n == 1) return;  // the row's only split has stored it
-  const int64_t base = (int64_t)prog * p.n_splits * rows + row;  // the row in split 0, in rows
-  const float* ml = p.part + (int64_t)p.B_grid * p.H_KV * p.n_qc * p.n_splits * rows * D;
+  const int ns_act = (cap + split_tokens - 1) / split_tokens;
+  const int64_t base = (int64_t)prog * ns_act * rows + row;  // the row in split 0, in rows
+  const float* ml = p.part + p.n_part * rows * D;
   const int t = threadIdx.x;
   __shared__ float wt[kBlkMergeMax], red[2][4];
   __shared__ v4f sum[NG][LN];

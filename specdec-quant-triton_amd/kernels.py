@@ -1222,10 +1222,10 @@ def paged_kv_append_block_scaled(k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_le
 
 
 @functools.lru_cache(maxsize=4096)
-def _block_attn_workspace(Bg, H, H_KV, Qg, QPP, max_pages, PAGE, dev, options) -> int:
+def _block_attn_workspace(Bg, H, H_KV, Qg, QPP, D, max_pages, PAGE, plan, dev, options) -> int:
     """Bytes a call needs: a function of its sizes, the GPU's CU count and the library options."""
     with torch.cuda.device(dev):
-        return _lib.lib().specq_paged_attn_block_workspace_size(Bg, H, H_KV, Qg, QPP, max_pages, PAGE)
+        return _lib.lib().specq_paged_attn_block_workspace_size(Bg, H, H_KV, Qg, QPP, D, max_pages, PAGE, plan)
 
 
 @functools.lru_cache(maxsize=None)
@@ -1275,7 +1275,7 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
     ck = _block_attn_info(D, f8, QPP * G, dev)
     if Bg == 0 or Qg == 0:
         return out, ck
-    need = _block_attn_workspace(Bg, H, H_KV, Qg, QPP, max_pages, PAGE, dev, _lib.options_key())
+    need = _block_attn_workspace(Bg, H, H_KV, Qg, QPP, D, max_pages, PAGE, plan is not None, dev, _lib.options_key())
     wptr, wbytes = (workspace or _ws.shared_cuda(dev)).ensure(need)
     _call_on(dev, "specq_paged_attn_block", q.data_ptr(), qs[0], qs[1], qs[2],
              kc.data_ptr(), vc.data_ptr(), f8, cs[0], cs[1], cs[2],

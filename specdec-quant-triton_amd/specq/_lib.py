@@ -90,7 +90,7 @@ SIGNATURES = {
     "specq_quantize_act_int8": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp]),
     "specq_silu_mul_quant_int8": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp,
                                            _c_int, _c_int, _c_int, _c_vp, _c_vp]),
-    "specq_paged_attn_block_workspace_size": (_c_size, [_c_int] * 7),
+    "specq_paged_attn_block_workspace_size": (_c_size, [_c_int] * 9),
     "specq_paged_attn_block": (_c_int, [_c_vp, _c_i64, _c_i64, _c_i64,
                                         _c_vp, _c_vp, _c_int, _c_i64, _c_i64, _c_i64,
                                         _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_int,

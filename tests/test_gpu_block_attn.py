@@ -301,6 +301,20 @@ def test_more_programs_than_counters():
     check(out[some], ref, 1, len(some), D, "many programs")
 
 
+def test_workspace_is_what_the_splits_in_flight_need():
+    from specq import _lib
+    size = lambda B, ql, plan, cols=256: _lib.lib().specq_paged_attn_block_workspace_size(  # noqa: E731
+        B, 32, 8, ql, max(1, min(ql, 16)), 128, cols, 16, plan)
+    assert size(64, 2048, 0) == 0  # prompt chunks that fill the GPU are not split
+    for B, ql, cols in ((1, 1, 64), (8, 9, 256), (32, 256, 8192), (64, 2048, 1024)):
+        graph = size(B, ql, 1, cols)
+        assert graph <= 256 * 1024 + 256 + 2 * 16 * max(256, B * 8) * max(1, ql // 16) * 64 * 130 * 4
+        for b in {1, B // 2 or 1, B}:
+            for q in {1, ql // 2 or 1, ql}:
+                if min(q, 16) == min(ql, 16):
+                    assert size(b, q, 0, cols) <= graph, (B, ql, cols, b, q)
+
+
 def test_streams_with_their_own_workspaces():
     from specq.workspace import Workspace
     rng = np.random.default_rng(14)
