@@ -66,8 +66,9 @@ constexpr int kBlkUnit = kBlkChunk * kAttnWaves;             // 256 tokens: one 
 constexpr int kBlkMaxUnits = 64 / 2;                         // longest split: the 64 sub-tiles a wave's lanes hold
 constexpr int kBlkOneSplit = 2;                              // tables of up to 512 tokens are one split
 constexpr int kBlkRegion = 16384;                            // LDS ring bytes of a wave
-// Up to kBlkMergeIn splits are merged by the program's last workgroup, more by a launch of their own, a
-// workgroup to each row (at most kBlkMergeMax, one per thread there).  In a graph, 5 tokens, 32 / 8 heads,
+// Up to kBlkMergeIn splits are merged by the program's last workgroup, more (and those of more programs than
+// the workspace has counters) by a launch of their own, a workgroup to each row (at most kBlkMergeMax, one
+// per thread there).  In a graph, 5 tokens, 32 / 8 heads,
 // D = 128, e4m3: 8 splits in place and by a launch 23.8 and 26.1 us (B = 4, context 8192), 14.5 and 16.2
 // (context 2048); 16 splits 25.1 and 25.5 (B = 2, context 16384), 17.2 and 15.8 (context 4096).
 constexpr int kBlkMergeIn = 8;
