@@ -1059,7 +1059,8 @@ def rotary_inv_freq(dim: int, base: float = 10000.0, scaling=None, factor: float
     scaling: None; "linear" (f / factor); "ntk" (base * factor^(dim / (dim - 2))); "wavelength" (waves longer
     than original_len / low_freq_factor divided by factor, those shorter than original_len / high_freq_factor
     kept, a blend between); "yarn" (f / factor for pairs that turn less than beta_slow times in original_len
-    tokens, f for those above beta_fast, a ramp over the pair's index between; mscale 0.1 ln(factor) + 1).
+    tokens, f for those above beta_fast, a ramp over the pair's index between, which may end past the last pair;
+    mscale 0.1 ln(factor) + 1).
     """
     dim = int(dim)
     if dim < 2 or dim % 2:
@@ -1082,7 +1083,8 @@ def rotary_inv_freq(dim: int, base: float = 10000.0, scaling=None, factor: float
         f = f * keep + f / factor * (1 - keep)
     elif scaling == "yarn":
         index = lambda turns: dim * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
-        lo, hi = max(math.floor(index(beta_fast)), 0), min(math.ceil(index(beta_slow)), dim // 2 - 1)
+        # Cut at dim - 1, not at the last pair: where that pair still turns more than beta_slow times, the ramp ends past it.
+        lo, hi = max(math.floor(index(beta_fast)), 0), min(math.ceil(index(beta_slow)), dim - 1)
         ramp = ((torch.arange(dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
         f = f / factor * ramp + f * (1 - ramp)
         mscale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0

@@ -140,6 +140,30 @@ def test_rotary_frequencies(dim):
         assert math.isclose(float(n[-1]), float(f[-1]) / 4, rel_tol=1e-12) and float(n[0]) == 1.0
 
 
+@pytest.mark.parametrize("dim,base,length,factor", [
+    (128, 10000.0, 4096, 8.0), (128, 500000.0, 131072, 4.0), (64, 1000000.0, 32768, 4.0), (20, 10000.0, 8192, 8.0),
+    # The ramp ends past the last pair: that pair still turns more than beta_slow times.
+    (8, 10000.0, 8192, 8.0), (6, 10000.0, 8192, 8.0), (4, 10000.0, 8192, 8.0), (64, 10000.0, 65536, 8.0),
+    (128, 10000.0, 131072, 8.0), (128, 10000.0, 1 << 20, 40.0),
+    (2, 10000.0, 100000, 8.0),  # ... and would end past dim - 1, where it is cut
+])
+def test_yarn_frequencies_are_the_closed_form(dim, base, length, factor):
+    """Every pair: the ramp runs from the pair that turns 32 times in `length` tokens, rounded down, to the one that
+    turns once, rounded up, within [0, dim - 1]; it may end past the last pair, dim / 2 - 1.  fp64 on both sides, some ten
+    operations of half an ulp each: 1e-13 covers them."""
+    import kernels as K
+    pair = lambda turns: dim * math.log(length / (2 * math.pi * turns)) / (2 * math.log(base))  # noqa: E731
+    lo, hi = max(math.floor(pair(32.0)), 0), min(math.ceil(pair(1.0)), dim - 1)
+    y, m = K.rotary_inv_freq(dim, base=base, scaling="yarn", factor=factor, original_len=length, device="cpu")
+    assert m == 0.1 * math.log(factor) + 1.0 and len(y) == dim // 2
+    for j in range(dim // 2):
+        f = base ** (-2.0 * j / dim)
+        ramp = min(1.0, max(0.0, (j - lo) / (hi - lo if hi > lo else 1e-3)))
+        assert math.isclose(float(y[j]), f * (1 - ramp) + f / factor * ramp, rel_tol=1e-13), j
+        if length * f / (2 * math.pi) > 1 and dim > 2:  # turns more than beta_slow times: not divided in full
+            assert float(y[j]) > f / factor * (1 + 1e-9), j
+
+
 def test_rotary_frequency_refusals():
     import kernels as K
     for kw in (dict(dim=0), dict(dim=3), dict(dim=64, scaling="cubic"), dict(dim=64, base=1.0), dict(dim=64, factor=0.0),
