@@ -1293,9 +1293,10 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
 # ----------------------------------------------------------------------------------------
 # Page tables of the paged caches
 # ----------------------------------------------------------------------------------------
-def _page_state(who: str, block_tbl, ref, *vecs):
-    """Checks the table, the counts and per-row vectors (name, tensor); returns (GPU, B, C, P)."""
-    dev = _gpu_of(who, block_tbl, ref, *(t for _, t in vecs))
+def _page_state(who: str, block_tbl, ref, *vecs, out=None):
+    """Checks the table, the counts and per-row vectors (name, tensor), and that `out`, where given, is on their GPU;
+    returns (GPU, B, C, P)."""
+    dev = _gpu_of(who, block_tbl, ref, *(t for _, t in vecs), out)
     if block_tbl.dtype != torch.int32 or block_tbl.dim() != 2 or block_tbl.shape[0] < 1 or block_tbl.shape[1] < 1 or \
             (block_tbl.stride(1) != 1 and block_tbl.shape[1] > 1):
         raise RuntimeError(f"{who}: block_tbl must be int32 [B, max_pages] with unit inner stride")
@@ -1345,7 +1346,7 @@ def paged_kv_reserve(block_tbl, ref, lens, PAGE, shortage=None, workspace=None):
     free pages run out, entries get -1.  Returns shortage, int32 [1]: how many pages are missing.
     """
     who = "paged_kv_reserve"
-    dev, B, C, P = _page_state(who, block_tbl, ref, ("lens", lens))
+    dev, B, C, P = _page_state(who, block_tbl, ref, ("lens", lens), out=shortage)
     shortage = torch.empty(1, dtype=torch.int32, device=ref.device) if shortage is None else shortage
     _int32_vec(who, "shortage", shortage, 1)
     wptr, wbytes = _pages_workspace(workspace, dev, B, C, P)
@@ -1378,7 +1379,7 @@ def paged_kv_fork(block_tbl, ref, lens, parent, caches, PAGE, shortage=None, wor
     past its tokens are let go of.  Returns shortage, int32 [1]: how many pages are missing.
     """
     who = "paged_kv_fork"
-    dev, B, C, P = _page_state(who, block_tbl, ref, ("lens", lens), ("parent", parent))
+    dev, B, C, P = _page_state(who, block_tbl, ref, ("lens", lens), ("parent", parent), out=shortage)
     n, words = _page_tensors(who, caches, P, dev)
     shortage = torch.empty(1, dtype=torch.int32, device=ref.device) if shortage is None else shortage
     _int32_vec(who, "shortage", shortage, 1)
@@ -1397,7 +1398,7 @@ def paged_kv_compact(block_tbl, ref, caches, page_map=None, workspace=None):
     [pages] holds every page's id afterwards, for other holders of ids.
     """
     who = "paged_kv_compact"
-    dev, B, C, P = _page_state(who, block_tbl, ref)
+    dev, B, C, P = _page_state(who, block_tbl, ref, out=page_map)
     n, words = _page_tensors(who, caches, P, dev)
     page_map = torch.empty(P, dtype=torch.int32, device=ref.device) if page_map is None else page_map
     _int32_vec(who, "page_map", page_map, P)

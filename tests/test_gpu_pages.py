@@ -276,3 +276,14 @@ def test_refusals():
         K.paged_kv_compact(tbl, ref, [cache], page_map=i32(9))
     K.paged_kv_copy(v[:0], v[:0], [cache])
     assert cache.view(torch.uint8).view(F8).shape == cache.shape
+
+
+def test_outputs_on_another_device_are_refused():
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=DEV)  # noqa: E731
+    tbl, ref, v = i32(3, 4), i32(10), i32(3)
+    note("pages outputs elsewhere")
+    for call in (lambda: K.paged_kv_reserve(tbl, ref, v, 16, shortage=i32(1).cpu()),
+                 lambda: K.paged_kv_fork(tbl, ref, v, v.clone(), [], 16, shortage=i32(1).cpu()),
+                 lambda: K.paged_kv_compact(tbl, ref, [], page_map=i32(10).cpu())):
+        with pytest.raises(RuntimeError, match="cpu"):
+            call()

@@ -120,6 +120,25 @@ def test_python_entry_points_want_gpu_tensors():
         K.paged_kv_copy(i, i, [])
 
 
+def test_every_tensor_is_held_to_one_gpu(monkeypatch):
+    """Nothing is launched: whatever a call would hand to a kernel has been through the check of its device."""
+    import kernels as K
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    tbl, ref, lens, parent, short, where = i32(3, 4), i32(10), i32(3), i32(3), i32(1), i32(10)
+    held, calls = [], []
+    monkeypatch.setattr(K, "_gpu_of", lambda who, *ts: held.extend(t.data_ptr() for t in ts if t is not None) or 0)
+    monkeypatch.setattr(K, "_call_on", lambda dev, name, *args: calls.append(name))
+    monkeypatch.setattr(K, "_pages_workspace", lambda *a: (0, 0))
+    for call, given in [(lambda: K.paged_kv_reserve(tbl, ref, lens, 16, shortage=short), (tbl, ref, lens, short)),
+                        (lambda: K.paged_kv_free(tbl, ref, lens, 16), (tbl, ref, lens)),
+                        (lambda: K.paged_kv_fork(tbl, ref, lens, parent, [], 16, shortage=short), (tbl, ref, lens, parent, short)),
+                        (lambda: K.paged_kv_compact(tbl, ref, [], page_map=where), (tbl, ref, where))]:
+        held.clear()
+        call()
+        assert {t.data_ptr() for t in given} <= set(held), calls[-1]
+    assert len(calls) == 4
+
+
 @pytest.mark.parametrize("dim", [2, 20, 64, 128])
 def test_rotary_frequencies(dim):
     import kernels as K
