@@ -383,7 +383,7 @@ def w8a8_matmul(a_q, sa, w_q, sw, out=None, BLOCK_M=16, BLOCK_N=None, BLOCK_K=12
         if not bm:
             cfg = KernelInfo(0, (1 if packed else 0) | 32, m_grid, N, K, 0, bn, nw, split_k).config
             bm, bn, split_k = cfg["block_m"], cfg["block_n"], cfg["split_k"]
-    ws = workspace or _ws.shared(a_q.device)
+    ws = workspace.on(a_q.get_device()) if workspace is not None else _ws.shared(a_q.device)
     if packed:
         need = _lib.lib().specq_w8a8_packed_workspace_size(m_grid, N, K, bm, bn, nw, split_k)
         wptr, wbytes = ws.ensure(need)
@@ -473,7 +473,7 @@ def w8a8_matmul_grouped(a_q, sa, weights, outs=None, BLOCK_M=16, BLOCK_N=None, n
     sw_arr = arr(ctypes.c_void_p, [sw.data_ptr() for sw in sws])
     c_arr = arr(ctypes.c_void_p, [o.data_ptr() for o in outs])
     ldc_arr = arr(ctypes.c_int64, [o.stride(0) for o in outs])
-    ws = workspace or _ws.shared(a_q.device)
+    ws = workspace.on(a_q.get_device()) if workspace is not None else _ws.shared(a_q.device)
     need = _lib.lib().specq_w8a8_grouped_workspace_size(layout, m_grid, n, n_arr, K, bm, bn, nw, split_k)
     wptr, wbytes = ws.ensure(need)
     _lib.call("specq_w8a8_grouped", layout, a_q.data_ptr(), a_q.stride(0), sa.data_ptr(), n, w_arr, ldw_arr, sw_arr,
@@ -610,7 +610,7 @@ def w4a16_matmul(a, wp, sc, group=128, out=None, BLOCK_M=16, BLOCK_N=None, BLOCK
     m_grid = int(grid_m_max) if grid_m_max is not None else M
     bm = int(BLOCK_M) if BLOCK_M else 0
     bn = 0 if not BLOCK_N else (64 if BLOCK_N <= 64 else 128)
-    ws = workspace or _ws.shared(a.device)
+    ws = workspace.on(a.get_device()) if workspace is not None else _ws.shared(a.device)
     need = _lib.lib().specq_w4a16_workspace_size(m_grid, N, K, bm, bn, 4, split_k)
     wptr, wbytes = ws.ensure(need)
     _lib.call("specq_w4a16", a.data_ptr(), a.stride(0), w_ptr, w_ld, layout,
@@ -683,7 +683,7 @@ def w4a16_matmul_grouped(a, weights, group=128, outs=None, BLOCK_M=None, BLOCK_N
     bn = 0 if not BLOCK_N else int(BLOCK_N)
     arr = lambda ct, vals: (ct * n)(*vals)  # noqa: E731
     n_arr = arr(ctypes.c_int, Ns)
-    ws = workspace or _ws.shared(a.device)
+    ws = workspace.on(a.get_device()) if workspace is not None else _ws.shared(a.device)
     need = _lib.lib().specq_w4a16_grouped_workspace_size(m_grid, n, n_arr, K, bm, bn, 4, split_k)
     wptr, wbytes = ws.ensure(need)
     _lib.call("specq_w4a16_grouped", a.data_ptr(), a.stride(0), n, arr(ctypes.c_void_p, w_ptrs),
@@ -756,7 +756,7 @@ def paged_attention(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len, QPP=None, BLOC
         raise RuntimeError("paged_attention: block_tbl and ctx_len must cover every sequence of the grid")
     G = H // H_KV
     max_pages = block_tbl.shape[1]
-    ws = workspace or _ws.shared(q.device)
+    ws = workspace.on(q.get_device()) if workspace is not None else _ws.shared(q.device)
     need = _lib.lib().specq_paged_attn_workspace_size(B_grid, H, H_KV, QLMAX, int(QPP), max_pages, PAGE)
     wptr, wbytes = ws.ensure(need)
     _lib.call("specq_paged_attn",
@@ -994,7 +994,7 @@ def w4a8_matmul(a_q, sa, wq, sw, out=None, BLOCK_M=16, BLOCK_N=None, BLOCK_K=128
     bm = int(BLOCK_M) if BLOCK_M else 0  # 0: the library picks the tile (cost model over M, N, K)
     bn = _w8a8_block_n(BLOCK_N)
     nw = int(num_warps) if num_warps else 4
-    ws = workspace or _ws.shared(a_q.device)
+    ws = workspace.on(a_q.get_device()) if workspace is not None else _ws.shared(a_q.device)
     need = _lib.lib().specq_w4a8_packed_workspace_size(m_grid, N, K, bm, bn, nw, split_k)
     wptr, wbytes = ws.ensure(need)
     _lib.call("specq_w4a8_packed", a_q.data_ptr(), a_q.stride(0), wq.data.data_ptr(),
@@ -1027,6 +1027,10 @@ def _call_on(dev: int, name: str, *args) -> None:
     else:
         with torch.cuda.device(dev):
             _lib.packed(name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+
+
+def _workspace(workspace, dev: int):
+    return _ws.shared_cuda(dev) if workspace is None else workspace.on(dev)
 
 
 def _plan_of(plan, need: int, who: str) -> int:
@@ -1278,7 +1282,7 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
     if Bg == 0 or Qg == 0:
         return out, ck
     need = _block_attn_workspace(Bg, H, H_KV, Qg, QPP, D, max_pages, PAGE, plan is not None, dev, _lib.options_key())
-    wptr, wbytes = (workspace or _ws.shared_cuda(dev)).ensure(need)
+    wptr, wbytes = _workspace(workspace, dev).ensure(need)
     _call_on(dev, "specq_paged_attn_block", q.data_ptr(), qs[0], qs[1], qs[2],
              kc.data_ptr(), vc.data_ptr(), f8, cs[0], cs[1], cs[2],
              ks.data_ptr(), vs.data_ptr(), ss[0], ss[1], ss[2], sb,
@@ -1334,7 +1338,7 @@ def _page_tensor_args(n: int, words) -> tuple:
 
 def _pages_workspace(workspace, dev: int, B: int, C: int, P: int):
     need = _lib.lib().specq_kv_pages_workspace_size(B, C, P)
-    return (workspace or _ws.shared_cuda(dev)).ensure(need)
+    return _workspace(workspace, dev).ensure(need)
 
 
 def paged_kv_reserve(block_tbl, ref, lens, PAGE, shortage=None, workspace=None):

@@ -30,6 +30,15 @@ class Workspace:
     def nbytes(self) -> int:
         return 0 if self._buf is None else self._buf.numel()
 
+    def on(self, index: int) -> "Workspace":
+        """This workspace for a call on GPU `index`, which must be its own: the kernels store through its address.  One
+        made for "cuda", without an index, belongs to the GPU of its buffer or of its first call."""
+        if self.device.index is None and self.device.type == "cuda":
+            self.device = torch.device("cuda", index) if self._buf is None else self._buf.device
+        if self.device.type != "cuda" or self.device.index != index:
+            raise RuntimeError(f"specq workspace on {self.device} given to a call on GPU {index}")
+        return self
+
     def ensure(self, nbytes: int) -> "tuple[int, int]":
         """Return (pointer, size) of a zeroed buffer of at least nbytes bytes."""
         if nbytes <= 0:

@@ -139,6 +139,31 @@ def test_every_tensor_is_held_to_one_gpu(monkeypatch):
     assert len(calls) == 4
 
 
+def test_a_workspace_on_another_device_is_refused(monkeypatch):
+    """On the host memory's, or another GPU's: nothing is launched with its address."""
+    import kernels as K
+    from specq.workspace import Workspace
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    tbl, ref, lens = i32(3, 200), i32(10), i32(3)
+    q = torch.zeros((3, 1, 8, 64), dtype=torch.float16)
+    kc, ks = torch.zeros((10, 16, 8, 64), dtype=torch.int8), torch.zeros((10, 1, 8))
+    calls = []
+    monkeypatch.setattr(K, "_gpu_of", lambda who, *ts: 0)
+    monkeypatch.setattr(K, "_call_on", lambda dev, name, *args: calls.append(name))
+    monkeypatch.setattr(K, "_block_attn_info", lambda *a: None)
+    monkeypatch.setattr(K, "_block_attn_workspace", lambda *a: 1 << 20)
+    far = Workspace("cuda:1")
+    far._buf = torch.zeros(1 << 22, dtype=torch.uint8)  # stands for memory of that GPU
+    for ws in (Workspace("cpu"), far):
+        for call in (lambda: K.paged_kv_reserve(tbl, ref, lens, 16, workspace=ws),
+                     lambda: K.paged_kv_fork(tbl, ref, lens, lens.clone(), [], 16, workspace=ws),
+                     lambda: K.paged_kv_compact(tbl, ref, [], workspace=ws),
+                     lambda: K.paged_attention_block_scaled(q, kc, kc, ks, ks, tbl, lens, workspace=ws)):
+            with pytest.raises(RuntimeError, match="workspace"):
+                call()
+    assert not calls
+
+
 @pytest.mark.parametrize("dim", [2, 20, 64, 128])
 def test_rotary_frequencies(dim):
     import kernels as K
