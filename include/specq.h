@@ -385,7 +385,8 @@ int specq_rotary(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh,
  *   ref       int32 [n_pages]: how often the tables name each page; <= 0 is free
  * Pages are handed out lowest id first, in the table's order; what cannot be had is -1, and
  * shortage[0] counts it.
- *   reserve   entries of row b's first ceil(lens[b] / PAGE) columns that name no page get one (ref 1)
+ *   reserve   entries of row b's first ceil(lens[b] / PAGE) columns that name no page get one (ref 1); at most 2^31 - 1
+ *             entries in the table
  *   free      entries past row b's first ceil(keep[b] / PAGE) columns become -1, their pages' ref falls
  *   fork      row b becomes a copy of row parent[b] (outside [0, B): empty), lens[b] that row's length.
  *             Full pages are shared; of the rows with one parent the lowest keeps its partly filled

@@ -519,6 +519,9 @@ extern "C" int specq_kv_pages_reserve(int32_t* block_tbl, int64_t s_bt, int B, i
   PagesParams p;
   if (int rc = pages_setup(p, "kv_pages_reserve", block_tbl, s_bt, B, max_pages, ref, n_pages, PAGE)) return rc;
   SPECQ_REQUIRE(lens && shortage, SPECQ_EINVAL, "kv_pages_reserve: null tensor pointer");
+  // Every entry may want a page, and a want's place among them is an int.
+  SPECQ_REQUIRE((int64_t)B * max_pages <= INT32_MAX, SPECQ_ENOTSUP, "kv_pages_reserve: block table of %lld entries is too large",
+                (long long)B * max_pages);
   if (int rc = pages_scratch(p, "kv_pages_reserve", workspace, workspace_bytes)) return rc;
   p.lens = const_cast<int32_t*>(lens);
   p.shortage = shortage;

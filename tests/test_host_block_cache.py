@@ -107,6 +107,15 @@ def test_sizes_past_their_types(built_lib):
         _lib.check(_lib.lib().specq_call_packed(b"specq_version", b"\0" * 8, 1), "specq_version")
 
 
+def test_reserve_refuses_more_entries_than_it_counts(built_lib):
+    """Wants are counted in 32 bits: a table of 2^32 entries that all want a page would count them past it, and take
+    places before the list of free pages."""
+    base = dict(bt=16, s_bt=1 << 20, B=4096, C=1 << 20, ref=16, P=100, lens=16, PAGE=1, short=16, ws=16, wsb=1 << 20, stream=0)
+    for B, C in ((4096, 1 << 20), (2048, 1 << 20), (1 << 30, 2), ((1 << 31) - 1, 1 << 5)):
+        _fail("specq_kv_pages_reserve", base, -95, B=B, C=C)
+    _fail("specq_kv_pages_reserve", base, -28, B=2047)  # 2^31 - 2^20 entries are counted
+
+
 def test_python_entry_points_want_gpu_tensors():
     import kernels as K
     z = torch.zeros((1, 1, 2, 64), dtype=torch.float16)
