@@ -347,8 +347,8 @@ int specq_paged_attn_block(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_
  * into the pages that specq_paged_attn_block reads.  Tokens, tables and plan as specq_kv_append_int8.
  * A block that new tokens reach gets s' = max(amax, 1e-8) / Q over them (Q = 127 for int8, 448 for
  * e4m3), or its present scale where that is larger and the block holds earlier tokens of the sequence;
- * codes are rne(x / s'), earlier codes rne(c s / s') where s' > s.  fp32, IEEE division.  Infinities
- * count as +-65504, NaN as 0.  Slots that hold no token of the sequence are not written.  A page that is
+ * codes are rne(x / s'), earlier codes rne(c s / s') where s' > s (NaN stays NaN).  fp32, IEEE division.
+ * New infinities count as +-65504, new NaN as 0.  Present scales are finite and not negative.  Slots that hold no token of the sequence are not written.  A page that is
  * written must be named by one entry of the table only.
  *   D must be 64, 128 or 256; cache rows 8-byte, new rows 16-byte aligned.
  * ------------------------------------------------------------------------------------- */

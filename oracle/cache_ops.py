@@ -27,7 +27,7 @@ def decode(codes, fmt):
 
 
 def encode(x, fmt):
-    """float64 values to the nearest codes, ties to even, clamped to the largest."""
+    """float64 values to the nearest codes, ties to even, clamped to the largest; e4m3 has a code for NaN."""
     m = float(QMAX[fmt])
     if fmt == "int8":
         return np.clip(np.rint(x), -m, m).astype(np.int8)
@@ -37,6 +37,7 @@ def encode(x, fmt):
     lo = np.maximum(hi - 1, 0)
     dl, dh = a - mag[lo], mag[hi] - a
     code = np.where((dl < dh) | ((dl == dh) & (lo % 2 == 0)), lo, hi)
+    code = np.where(np.isnan(x), 127, code)
     return (code | (np.signbit(x).astype(np.int64) << 7)).astype(np.uint8)
 
 

@@ -7,7 +7,7 @@
 //   s' = max(amax |x|, 1e-8) / Q;  where the block holds earlier tokens of the sequence (its positions
 //        below the first new one), s' = max(s', s) with s its scale so far;
 //   new codes      rne(x / s');
-//   earlier codes  rne(c * s / s'), clamped to +-Q, where s' > s, untouched otherwise.
+//   earlier codes  rne(c * s / s'), clamped to +-Q, where s' > s, untouched otherwise; e4m3 NaN stays NaN.
 // fp32, the quotients rounded as IEEE division rounds them.  Infinities count as +-65504 and NaN as 0, so
 // that one bad value does not take the block's other tokens with it.  Slots past the last new token are
 // not touched.
@@ -58,14 +58,17 @@ __device__ __forceinline__ uint32_t clean16(v8h& x) {
   return top16(x);
 }
 
-// Codes of eight values over the scale s.
+// Codes of eight values over the scale s, clamped to the largest; NaN stays NaN where there is a code for it.
 template <bool F8>
 __device__ __forceinline__ v2i encode8(const float (&x)[8], float s) {
   int w[2] = {0, 0};
   if constexpr (F8) {
     float q[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = fminf(fmaxf(x[j] / s, -448.f), 448.f);
+    for (int j = 0; j < 8; ++j) {
+      const float f = x[j] / s;
+      q[j] = f != f ? f : fminf(fmaxf(f, -448.f), 448.f);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * h], q[4 * h + 1], w[h], false);

@@ -183,6 +183,26 @@ def test_every_small_and_negative_zero(fmt):
             assert np.array_equal(raw(got), w), top
 
 
+def test_nan_codes_of_earlier_tokens_stay_nan():
+    """A NaN among a block's earlier e4m3 codes is NaN over the grown scale too, whatever its sign; its neighbours are
+    requantised as ever, and where the scale stays the codes do."""
+    rng = np.random.default_rng(22)
+    for size, D, SB in ((40.0, 128, 16), (1e-3, 128, 16), (40.0, 256, 512)):  # grows, stays; a block read twice
+        ctx, ql = [SB - 3, 2 * SB - 1], 4
+        kc, vc, ks, vs, bt, cl = make_cache(rng, ctx, 2, D, SB, SB, "fp8")
+        kc[:, ::5, 0, 3], kc[:, 1::7, 1, 60], vc[:, ::3, :, 9] = 0x7F, 0xFF, 0x7F
+        k, v = new_kv(rng, 2, ql, 2, D, size=size)
+        ref = C.append_block(k, v, kc, vc, ks, vs, bt, cl, ql, "fp8")
+        note(f"block append NaN codes size={size} SB={SB}")
+        t = gpu(k, v, kc, vc, ks, vs, bt, cl)
+        K.paged_kv_append_block_scaled(*t, ql)
+        torch.cuda.synchronize()
+        for got, want in zip(t[2:4], ref[:2]):
+            assert np.array_equal(C.decode(raw(got), "fp8"), C.decode(want, "fp8"), equal_nan=True)
+        assert all(np.array_equal(raw(a), b) for a, b in zip(t[4:6], ref[2:]))
+        assert (np.isnan(C.decode(ref[0], "fp8")) == np.isnan(C.decode(kc, "fp8")))[bt[0, 0], :SB - 3 - ql].all()
+
+
 def test_negative_lengths_write_nothing():
     rng = np.random.default_rng(21)
     kc, vc, ks, vs, bt, _ = make_cache(rng, [64, 64, 64], 2, 64, 16, 16, "int8")

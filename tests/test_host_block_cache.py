@@ -233,6 +233,10 @@ def test_e4m3_codes_are_torchs():
     assert np.array_equal(torch.from_numpy(x).to(torch.float8_e4m3fn).view(torch.uint8).numpy(), C.encode(x.astype(np.float64), "fp8"))
 
 
+def test_plain_codes_of_nan():
+    assert np.isnan(C.decode(C.encode(np.asarray([np.nan, -np.nan, 1.0]), "fp8"), "fp8")).tolist() == [True, True, False]
+
+
 def test_plain_append_holds_half_a_step():
     rng = np.random.default_rng(1)
     kc, ks = np.zeros((3, 32, 1, 8), np.int8), np.zeros((3, 2, 1), np.float32)
