@@ -323,7 +323,7 @@ int specq_kv_append_int8(const void* k_new, const void* v_new, int64_t s_nb, int
  *   kc, vc   codes [pages, PAGE, H_KV, D], as specq_paged_attn
  *   ks, vs   fp32 [pages, PAGE / block, H_KV], strides s_sp (page), s_sb (block), s_sh, shared
  *   block    a multiple of 16 that divides PAGE
- *   s_ko     at least D: the rows of a page must not overlap
+ *   s_ko     at least D: the rows of a page must not overlap; nor may those of the output
  *   Probabilities are rounded to fp16 once, after their V scale, against a running max of what the tokens
  *   contribute.  Scales, and e4m3 NaN codes, of tokens that a row does not see do not reach it.  A context
  *   longer than the table counts as the table's length, a negative one as 0.  Everything else as
@@ -350,7 +350,7 @@ int specq_paged_attn_block(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_
  * codes are rne(x / s'), earlier codes rne(c s / s') where s' > s (NaN stays NaN).  fp32, IEEE division.
  * New infinities count as +-65504, new NaN as 0.  Present scales are finite and not negative.  Slots that hold no token of the sequence are not written.  A page that is
  * written must be named by one entry of the table only.
- *   D must be 64, 128 or 256; cache rows 8-byte, new rows 16-byte aligned.
+ *   D must be 64, 128 or 256; cache rows 8-byte, new rows 16-byte aligned; cache rows and scales must not overlap.
  * ------------------------------------------------------------------------------------- */
 int specq_kv_append_block(const void* k_new, const void* v_new, int64_t s_nb, int64_t s_nt, int64_t s_nh,
                           void* kc, void* vc, int code_fp8, int64_t s_kp, int64_t s_ko, int64_t s_kh,
@@ -363,7 +363,8 @@ int specq_kv_append_block(const void* k_new, const void* v_new, int64_t s_nb, in
  * Rotary positions (no reference counterpart): pair j of the first R of D dimensions -- (j, j + R/2),
  * or (2j, 2j + 1) with interleaved -- is turned by pos * inv_freq[j] and scaled by mscale; the other
  * dimensions are copied.  Angles are formed in fp64, everything else in fp32 with one rounding.
- *   q, q_out  fp16 [B_grid, ql_grid, H, D], strides of their own (d contiguous); outputs may be the inputs
+ *   q, q_out  fp16 [B_grid, ql_grid, H, D], strides of their own (d contiguous); outputs may be the inputs,
+ *             their own rows must not overlap
  *   k, k_out  fp16 [B_grid, ql_grid, H_KV, D], or NULL with H_KV = 0
  *   inv_freq  fp32 or (freq_fp64) fp64 [R / 2];  R even, R <= D <= 512
  *   ctx_len   int32 [B_grid]: token i of sequence b is at ctx_len[b] - q_len + i; or, where not NULL,

@@ -177,6 +177,9 @@ static int attn_call(int kind, const void* q, int64_t s_qb, int64_t s_qt, int64_
                 SPECQ_ENOTSUP, "paged_attn: K/V cache rows must be 16-byte aligned");
   SPECQ_REQUIRE(!blk || s_ko >= D, SPECQ_ENOTSUP, "paged_attn: rows of the K/V cache overlap (token stride %lld)",
                 (long long)s_ko);
+  SPECQ_REQUIRE(!blk || (lie_apart(plan ? B_grid : n_seqs, s_ob, D) && lie_apart(plan ? ql_grid : q_len, s_ot, D) &&
+                         lie_apart(H, s_oh, D)),
+                SPECQ_ENOTSUP, "paged_attn: rows of the output overlap");
   SPECQ_REQUIRE(s_ko > 0 && 16 * s_ko + D < ((int64_t)1 << 31), SPECQ_ENOTSUP,
                 "paged_attn: token stride %lld of the K/V cache outside (0, 2^27)", (long long)s_ko);
   if (B_grid == 0) return SPECQ_OK;

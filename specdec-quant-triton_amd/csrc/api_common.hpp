@@ -56,6 +56,10 @@ inline int common_vec(std::initializer_list<uint64_t> vals) {
   return v;
 }
 
+// Whether the n entries of a written tensor's dimension, `stride` apart and `len` long, lie apart: an expanded dimension
+// (stride 0) or a closer one has several workgroups write one place.
+inline bool lie_apart(int64_t n, int64_t stride, int64_t len) { return n <= 1 || stride >= len || stride <= -len; }
+
 int launch(const void* fn, int grid, int threads, size_t lds, hipStream_t stream, void* params);
 
 // Kernels using more than 64 KiB of dynamic LDS opt in once per kernel.

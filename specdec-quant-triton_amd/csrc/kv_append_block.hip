@@ -297,6 +297,10 @@ extern "C" int specq_kv_append_block(const void* k_new, const void* v_new, int64
                 SPECQ_ENOTSUP, "kv_append_block: cache rows must be 8-byte aligned");
   SPECQ_REQUIRE((uintptr_t)ks % 4 == 0 && (uintptr_t)vs % 4 == 0, SPECQ_ENOTSUP,
                 "kv_append_block: scales must be 4-byte aligned");
+  SPECQ_REQUIRE(lie_apart(n_pages, s_kp, D) && lie_apart(PAGE, s_ko, D) && lie_apart(H_KV, s_kh, D), SPECQ_ENOTSUP,
+                "kv_append_block: cache rows overlap");
+  SPECQ_REQUIRE(lie_apart(n_pages, s_sp, 1) && lie_apart(PAGE / block, s_sb, 1) && lie_apart(H_KV, s_sh, 1), SPECQ_ENOTSUP,
+                "kv_append_block: scales overlap");
   const int tokens = plan ? ql_grid : q_len, seqs = plan ? B_grid : n_seqs;
   if (seqs == 0 || tokens == 0) return SPECQ_OK;
   KvAppendBlockParams p = {};

@@ -163,6 +163,9 @@ extern "C" int specq_rotary(const void* q, int64_t s_qb, int64_t s_qt, int64_t s
   SPECQ_REQUIRE(H > 0 && H_KV >= 0 && D > 0 && R > 0 && R <= D && R % 2 == 0, SPECQ_EINVAL,
                 "rotary: need an even number R=%d of rotated dimensions, at most head_dim %d", R, D);
   SPECQ_REQUIRE(D <= 512, SPECQ_ENOTSUP, "rotary: head_dim %d (at most 512 supported)", D);
+  SPECQ_REQUIRE(lie_apart(B_grid, s_qob, D) && lie_apart(ql_grid, s_qot, D) && lie_apart(H, s_qoh, D) &&
+                    (H_KV == 0 || (lie_apart(B_grid, s_kob, D) && lie_apart(ql_grid, s_kot, D) && lie_apart(H_KV, s_koh, D))),
+                SPECQ_ENOTSUP, "rotary: rows of an output overlap");
   const int64_t tokens = (int64_t)B_grid * ql_grid;
   SPECQ_REQUIRE(tokens <= INT32_MAX - 4, SPECQ_EINVAL, "rotary: grid too large");
   if (tokens == 0) return SPECQ_OK;

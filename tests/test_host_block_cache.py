@@ -37,6 +37,32 @@ def test_attention_refusals(built_lib):
     f(0, B=0, n_seqs=0)
 
 
+APPEND = dict(k=16, v=16, s_nb=9 * 1024, s_nt=1024, s_nh=128, kc=16, vc=16, f8=0, s_kp=16 * 1024, s_ko=1024, s_kh=128, ks=16,
+              vs=16, s_sp=16, s_sb=8, s_sh=1, block=16, bt=16, s_bt=64, max_pages=64, n_pages=100, ctx=16, B=2, n_seqs=2,
+              q_len=9, ql=9, HK=8, D=128, PAGE=32, plan=0, stream=0)
+ROTARY = dict(q=16, a=1024, b=512, c=64, k=16, d=256, e=128, f=64, qo=16, g=1024, h=512, i=64, ko=16, j=256, l=128, m=64,
+              freq=16, f64=1, ms=1.0, ctx=16, pos=0, s_pb=0, B=2, n_seqs=2, q_len=2, ql=2, H=8, HK=2, D=64, R=64, il=0,
+              plan=0, stream=0)
+
+
+def test_outputs_that_name_a_place_twice_are_refused(built_lib):
+    """Expanded tensors (a stride of 0) and rows closer than they are long: workgroups would write over one another.  A
+    dimension of one entry may have any stride."""
+    none = dict(n_seqs=0)  # what is not refused has nothing to do
+    for k in ("g", "h", "i", "j", "l", "m"):
+        _fail("specq_rotary", ROTARY, -95, **{k: 0}), _fail("specq_rotary", ROTARY, -95, **{k: 56})
+    for k in ("s_ob", "s_ot", "s_oh"):
+        _fail("specq_paged_attn_block", ATTN, -95, **{k: 0}), _fail("specq_paged_attn_block", ATTN, -95, **{k: 64})
+    _fail("specq_paged_attn_block", ATTN, 0, q_len=1, ql=1, QPP=1, s_ot=0, **none)
+    for k in ("s_kp", "s_ko", "s_kh", "s_sp", "s_sb", "s_sh"):
+        _fail("specq_kv_append_block", APPEND, -95, **{k: 0})
+        if k[2] == "k":
+            _fail("specq_kv_append_block", APPEND, -95, **{k: 64})
+    _fail("specq_kv_append_block", APPEND, 0, s_sb=0, block=32, **none)
+    _fail("specq_kv_append_block", APPEND, 0, s_sp=0, s_kp=0, n_pages=1, **none)
+    _fail("specq_kv_append_block", APPEND, 0, s_sh=0, s_kh=0, HK=1, **none)
+
+
 def test_append_refusals(built_lib):
     base = dict(k=16, v=16, s_nb=9 * 1024, s_nt=1024, s_nh=128, kc=16, vc=16, f8=0, s_kp=16 * 1024, s_ko=1024, s_kh=128, ks=16,
                 vs=16, s_sp=8, s_sb=8, s_sh=1, block=16, bt=16, s_bt=64, max_pages=64, n_pages=100, ctx=16, B=2, n_seqs=2,
