@@ -1086,6 +1086,8 @@ def rotary_inv_freq(dim: int, base: float = 10000.0, scaling=None, factor: float
         keep = ((turns - low_freq_factor) / (high_freq_factor - low_freq_factor)).clamp(0, 1)
         f = f * keep + f / factor * (1 - keep)
     elif scaling == "yarn":
+        if not beta_fast >= beta_slow > 0:
+            raise RuntimeError("rotary_inv_freq: need beta_fast >= beta_slow > 0")
         index = lambda turns: dim * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
         # Cut at dim - 1, not at the last pair: where that pair still turns more than beta_slow times, the ramp ends past it.
         lo, hi = max(math.floor(index(beta_fast)), 0), min(math.ceil(index(beta_slow)), dim - 1)
@@ -1260,7 +1262,7 @@ def paged_attention_block_scaled(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=No
     if q.dim() != 4 or q.dtype != torch.float16 or q.stride(3) != 1:
         raise RuntimeError(f"{who} expects fp16 q [B, QLMAX, H, D] with contiguous head_dim")
     B, QL, H, D = q.shape
-    if kc.dim() != 4 or kc.shape[2] < 1 or H % kc.shape[2]:
+    if H < 1 or kc.dim() != 4 or kc.shape[2] < 1 or H % kc.shape[2]:
         raise RuntimeError(f"{who}: cache {tuple(kc.shape)} does not fit q {tuple(q.shape)}")
     H_KV = kc.shape[2]
     G = H // H_KV

@@ -251,6 +251,19 @@ def test_rotary_frequency_refusals():
             K.rotary_inv_freq(device="cpu", **kw)
 
 
+def test_refusals_are_runtime_errors(monkeypatch):
+    """No query heads; yarn's numbers of turns that have no logarithm or no order."""
+    import kernels as K
+    monkeypatch.setattr(K, "_gpu_of", lambda who, *ts: 0)
+    monkeypatch.setattr(K, "_call_on", lambda dev, name, *args: None)
+    q, kc, ks = torch.zeros((1, 1, 0, 64), dtype=torch.float16), torch.zeros((2, 16, 2, 64), dtype=torch.int8), torch.zeros((2, 1, 2))
+    with pytest.raises(RuntimeError, match="does not fit"):
+        K.paged_attention_block_scaled(q, kc, kc, ks, ks, torch.zeros((1, 4), dtype=torch.int32), torch.ones(1, dtype=torch.int32))
+    for kw in (dict(beta_slow=0.0), dict(beta_slow=-1.0), dict(beta_fast=0.0), dict(beta_fast=1.0, beta_slow=2.0)):
+        with pytest.raises(RuntimeError, match="beta"):
+            K.rotary_inv_freq(64, scaling="yarn", factor=4.0, device="cpu", **kw)
+
+
 def test_e4m3_codes_are_torchs():
     t = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).float().numpy()
     assert np.array_equal(t, C.E4M3.astype(np.float32), equal_nan=True)
