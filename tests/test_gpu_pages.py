@@ -287,3 +287,57 @@ def test_outputs_on_another_device_are_refused():
                  lambda: K.paged_kv_compact(tbl, ref, [], page_map=i32(10).cpu())):
         with pytest.raises(RuntimeError, match="cpu"):
             call()
+
+
+WIDTHS = {  # bytes of a page: chunks of 16384 in full and in part, next to pages of a scale or two
+    "16 bytes": (40 * 1024 + 16, 16384, 16),
+    "one scale": (32 * 1024, 4 * 16384 + 48, 4),
+    "two scales": (20 * 1024, 8),
+    "odd": (16384 + 36, 37, 1),
+}
+
+
+@pytest.mark.parametrize("what", list(WIDTHS))
+def test_page_copies_at_every_access_width(what):
+    """Fork, compact and copy of pages that take several workgroups each, at 16, 4 and 1 bytes an access."""
+    rng = np.random.default_rng(len(what))
+    B, cols, page, P = 8, 6, 16, 60
+    make = lambda: [rng.integers(-128, 128, (P, n), dtype=np.int64).astype(np.int8) for n in WIDTHS[what]]  # noqa: E731
+
+    def held(caches, tensors, moves, step):
+        for i, (c, t) in enumerate(zip(caches, tensors)):
+            want = c.copy()
+            for a, b in moves:
+                want[b] = c[a]
+            equal(f"{step} {i}", t, want)
+
+    tbl, ref, lens = state(rng, B, cols, P - 12, page, fill=1.0)
+    ref = np.concatenate([ref, np.zeros(12, np.int32)])
+    lens[0] += lens[0] % page == 0  # a last page to copy
+    tbl[0, (lens[0] - 1) // page] = P - 1
+    ref = np.bincount(tbl[tbl >= 0], minlength=P).astype(np.int32)
+    parent = np.zeros(B, np.int32)
+    caches = make()
+    note(f"pages widths {what}")
+    tt, tr, tl, tp, *tc = gpu(tbl, ref, lens, parent, *caches)
+    K.paged_kv_fork(tt, tr, tl, tp, tc, page)
+    torch.cuda.synchronize()
+    *_, copies = C.fork(tbl, ref, lens, parent, page)
+    assert len(copies) == B - 1
+    held(caches, tc, copies, "fork")
+
+    tbl, ref, _ = state(rng, B, cols, P, page, fill=0.5)
+    caches = make()
+    tt, tr, *tc = gpu(tbl, ref, *caches)
+    K.paged_kv_compact(tt, tr, tc)
+    torch.cuda.synchronize()
+    *_, moves = C.compact(tbl, ref)
+    assert len(moves) > 4
+    held(caches, tc, moves, "compact")
+
+    caches = make()
+    src, dst = np.split(rng.permutation(P).astype(np.int32), 2)
+    tc = gpu(*caches)
+    K.paged_kv_copy(*gpu(src, dst), tc)
+    torch.cuda.synchronize()
+    held(caches, tc, list(zip(src, dst)), "copy")

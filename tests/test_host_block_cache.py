@@ -2,6 +2,8 @@
 frequencies, and the plain implementations' own properties."""
 import ctypes
 import math
+import os
+import re
 
 import numpy as np
 import pytest
@@ -131,6 +133,25 @@ def test_sizes_past_their_types(built_lib):
         _lib.check(_lib.lib().specq_call_packed(b"specq_rotary", b"\0" * 64, 8), "specq_rotary")
     with pytest.raises(RuntimeError, match="no entry point"):
         _lib.check(_lib.lib().specq_call_packed(b"specq_version", b"\0" * 8, 1), "specq_version")
+
+
+def test_kernels_keep_to_their_registers(built_lib):
+    """The compiler's report beside the library: bytes of scratch a lane, for all kernels of these operators.  The e4m3
+    programs of 64 rows at head dim 128 spill."""
+    report = os.path.join(os.path.dirname(built_lib), "libspecq.resources.txt")
+    if not os.path.exists(report):
+        pytest.skip("library without its report")
+    ours = re.compile(r"attn_block_(plan_)?kernel|attn_merge_kernel|rotary_(vec|any)_kernel|kv_append_block_kernel|pages_\w+_kernel")
+    scratch, name = {}, ""
+    for line in open(report):
+        if m := re.search(r"Function Name: (\S+)", line):
+            name = m.group(1)
+        elif (m := re.search(r"ScratchSize \[bytes/lane\]: (\d+)", line)) and ours.search(name):
+            scratch[name] = int(m.group(1))
+    assert len(scratch) >= 28 + 2 + 4 + 10 + 6
+    most = {"attn_block_kernelILi128ELi4ELb1E": 96, "attn_block_plan_kernelILi128ELi4ELb1E": 108}
+    for name, n in scratch.items():
+        assert n <= max([v for k, v in most.items() if k in name], default=0), (name, n)
 
 
 def test_reserve_refuses_more_entries_than_it_counts(built_lib):
