@@ -17,8 +17,9 @@
 // block's earlier codes and its scale are fetched together with the new values' amax pass, so that
 // the requantisation adds no round trip.  Bound by the latency of its three dependent loads (context
 // length, page id, codes) for a verification step (B = 8, 9 tokens, 8 heads of 128, int8, blocks of 16:
-// 4.0 us) and for a prompt by that and the instructions of the conversion (2 x 2048 tokens, e4m3, blocks
-// of 32, 25 MB: 10.2 us = 2.5 TB/s, and 12.9 with a division and a clamp for each value).
+// 4.1 us) and for a prompt by that and the instructions of the conversion (2 x 2048 tokens, e4m3, blocks
+// of 32, 25 MB: 10.2 us = 2.5 TB/s on one set of inputs, 11.2 over distinct ones (int8 10.9), and 12.9 with a division
+// and a clamp for each value).
 #include "api_common.hpp"
 #include "common.hpp"
 

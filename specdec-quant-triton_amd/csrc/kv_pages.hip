@@ -18,8 +18,8 @@
 // microsecond each, so the first step's counts are loaded ahead of everything else and what one part
 // hands the next stays in LDS where it fits (the table's bits up to kPagesBits words, ids up to kPagesList;
 // the workspace otherwise).  The page copies behind fork and compact are bound by HBM.  Kernel times:
-// reserve 6.8 us (32 rows of 258 columns, one page each), free 2.6, fork 3.7 + 3.8 and 4.1 for the copies of 24
-// pages of 128 KB, compact 6.2 (4104 pages) and 13.2 for the copies of a thousand pages of 32 KB (4.9 TB/s).
+// reserve 6.8 us (32 rows of 258 columns, one page each), free 2.5, fork 3.6 + 3.8 and 4.3 for the copies of 24
+// pages of 128 KB, compact 6.0 (4104 pages) and 13.1 for the copies of a thousand pages of 32 KB (4.9 TB/s).
 #include "api_common.hpp"
 #include "common.hpp"
 
@@ -389,6 +389,9 @@ __device__ __forceinline__ void copy_chunk(const uint8_t* src, uint8_t* dst, int
 // Pages src[i] -> dst[i] of every tensor; a pair with an id outside the pool is left out.  A unit is a chunk of
 // kPagesChunk bytes of a large tensor's page, four 16-byte loads a thread in flight; pages of at most a
 // quarter of that (scales) would leave most of a unit idle, and are copied with their pair's first one.
+// One access width for all tensors of a launch: next to scale pages of 4 or 8 bytes K and V go 4 bytes an access, which
+// costs nothing measurable (2048 pairs, heads of 128, in a graph, against scale pages padded to 16 bytes: one head, pages
+// of 16 tokens 7.8 and 7.7 us, of 64 tokens 12.9 and 12.8; two heads, 64 tokens 20.2 and 20.4).
 __global__ __launch_bounds__(256) void pages_copy_kernel(PagesCopyParams p) {
   if ((int)blockIdx.x < p.remap) {
     const int64_t n = (int64_t)p.B * p.C;

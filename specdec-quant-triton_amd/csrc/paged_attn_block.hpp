@@ -36,11 +36,12 @@
 //  * The waves merge through the ring, every wave writing its rows once and all threads summing eight,
 //    two row blocks at a time.  Up to kBlkMergeIn splits are merged by the program's last workgroup to
 //    arrive, more by attn_merge_kernel behind the launch.
-// Measured in a graph, 32 / 8 heads, D = 128, codes read per second: 32 sequences of one token, contexts up to
-// 8192, int8 85.5 us = 3.8 TB/s; 8 and 32 sequences of 9 tokens, context 4096, e4m3 25.9 us = 2.6 TB/s and
-// 62.9 us = 4.3 TB/s (of the 25.9, 14 are the loop, the rest start, first loads and merges); 2 x 256
-// tokens, contexts up to 4096, int8 48.3 us, e4m3 45.3, bound by instructions; one sequence of 5 tokens,
-// context 131072, 16 / 2 heads, D = 64, e4m3 21.8 us, 4.4 of them the merge launch.
+// Measured in a graph over distinct inputs, 32 / 8 heads, D = 128, codes read per second: 32 sequences of one token,
+// contexts up to 8192, int8 85.8 us = 3.8 TB/s; 8 and 32 sequences of 9 tokens, context 4096, e4m3 26.1 us = 2.6
+// TB/s and 63.2 us = 4.3 TB/s (of the 26.1, 14 are the loop, the rest start, first loads and merges); 2 x 256
+// tokens, contexts up to 4096, int8 48.3 us, e4m3 45.4, one prompt of 4096 int8 245 us, e4m3 233, bound by
+// instructions; one sequence of 5 tokens, context 131072, 16 / 2 heads, D = 64, e4m3 22.2 us, 4.9 of them the merge
+// launch.  64-row programs at D = 128 have no register left; the e4m3 ones spill 23 (plan mode 26).
 // A row's result does not depend on the rows packed with it: split boundaries, chunks and merge orders are
 // fixed, so QPP = 1, fused, eager and plan calls agree bit for bit.
 //

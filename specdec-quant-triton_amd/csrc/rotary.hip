@@ -115,7 +115,8 @@ __global__ __launch_bounds__(256) void rotary_vec_kernel(RotaryParams p) {
   }
 }
 
-// Any R, D and alignment: a thread owns pairs and copied values one by one.
+// Any R, D and alignment: a thread owns pairs and copied values one by one, 2 bytes an access.  2 x 4096 tokens, 32 / 8
+// heads, D = 80, in a graph: R = 20 here 80.6 us = 1.3 TB/s, R = 80 in the vector kernel 30.8.
 template <bool IL>
 __global__ __launch_bounds__(256) void rotary_any_kernel(RotaryParams p) {
   int b, i, pos;

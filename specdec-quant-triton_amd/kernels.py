@@ -1205,7 +1205,8 @@ def paged_kv_append_block_scaled(k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_le
     rne(x / s'), and where the scale grows the earlier codes become rne(c * s / s') (NaN stays NaN).  New
     infinities count as +-65504, new NaN as 0.  Present scales are finite and not negative.  Tokens at positions below zero, past the table or on a page outside the pool
     are skipped, every other slot keeps what it holds.  A page that the call writes must be named by one
-    entry of the table only (paged_kv_fork sees to that).  With `plan`, (n_seqs, q_len) = plan[0:2] on the device
+    entry of the table only (paged_kv_fork sees to that, unless a row is cut back into a page it shares).
+    D = 256 is for other readers: paged_attention_block_scaled takes 64 and 128.  With `plan`, (n_seqs, q_len) = plan[0:2] on the device
     and the grid covers (B, QLMAX).
     """
     who = "paged_kv_append_block_scaled"
@@ -1349,7 +1350,9 @@ def paged_kv_reserve(block_tbl, ref, lens, PAGE, shortage=None, workspace=None):
     block_tbl int32 [B, max_pages]; ref int32 [pages], how often the tables name each page (<= 0: free);
     lens int32 [B].  Entries of a row's first ceil(lens / PAGE) columns that name no page (an id outside
     [0, pages)) get the lowest free page, in the table's order; ref of a page given becomes 1.  Where the
-    free pages run out, entries get -1.  Returns shortage, int32 [1]: how many pages are missing.
+    free pages run out, entries get -1.  Returns shortage, int32 [1]: how many pages are missing (a row has no
+    more than its max_pages columns, whatever lens says).  Calls that may run beside other calls on another
+    stream need a workspace of their own, here as in paged_kv_fork and paged_kv_compact.
     """
     who = "paged_kv_reserve"
     dev, B, C, P = _page_state(who, block_tbl, ref, ("lens", lens), out=shortage)
@@ -1365,7 +1368,8 @@ def paged_kv_free(block_tbl, ref, keep, PAGE):
     """Let go of the pages past each row's first keep[b] tokens (0: the whole row), in place.
 
     Entries past a row's first ceil(keep / PAGE) columns become -1, and ref of each page they named
-    falls by one; a page that no table names any more (ref 0) is free.
+    falls by one; a page that no table names any more (ref 0) is free.  A row that keep cuts back into a page it
+    shares with another (paged_kv_fork) must not be appended to before it has a page of its own there.
     """
     who = "paged_kv_free"
     dev, B, C, P = _page_state(who, block_tbl, ref, ("keep", keep))
