@@ -369,6 +369,25 @@ def test_even_programs_of_many_tokens(D, fmt):
             assert torch.equal(out, K.paged_attention_block_scaled(*t, q_len, QPP=QPP)[0]), (q_len, QPP)
 
 
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("q_len,ctx,H,H_KV,D,PAGE,SB", [
+    (1030, [1030], 8, 2, 128, 16, 16),           # a whole prompt: no token before it, programs of 64 rows
+    (515, [1500, 515, 600], 6, 2, 128, 48, 16),  # ... of 63 rows, behind cached tokens and without
+    (700, [4000, 20], 4, 4, 64, 64, 32),         # one sequence shorter than its new tokens: its first rows are empty
+])
+def test_whole_prompts(q_len, ctx, H, H_KV, D, PAGE, SB, fmt):
+    rng = np.random.default_rng(q_len + D)
+    cache = make_cache(rng, ctx, H_KV, D, PAGE, SB, fmt)
+    q = queries(rng, len(ctx), q_len, H, D)
+    note(f"block attn whole prompts {fmt} q_len={q_len} ctx={ctx}")
+    t = gpu(q, *cache)
+    out = K.paged_attention_block_scaled(*t, q_len)[0]
+    torch.cuda.synchronize()
+    check(out, C.attention_block(q, *cache, q_len, fmt), q_len, len(ctx), D, q_len)
+    plan = torch.tensor([len(ctx), q_len], dtype=torch.int32, device=DEV)
+    assert torch.equal(out, K.paged_attention_block_scaled(*t, plan=plan)[0])
+
+
 def test_refusals():
     rng = np.random.default_rng(1)
     q, kc, vc, ks, vs, bt, cl = gpu(queries(rng, 2, 4, 8, 128), *make_cache(rng, [40, 20], 2, 128, 32, 16, "int8"))
