@@ -348,8 +348,8 @@ int specq_paged_attn_block(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_
  * A block that new tokens reach gets s' = max(amax, 1e-8) / Q over them (Q = 127 for int8, 448 for
  * e4m3), or its present scale where that is larger and the block holds earlier tokens of the sequence;
  * codes are rne(x / s'), earlier codes rne(c s / s') where s' > s (NaN stays NaN).  fp32, IEEE division.
- * New infinities count as +-65504, new NaN as 0.  Present scales are finite and not negative.  Slots that hold no token of the sequence are not written.  A page that is
- * written must be named by one entry of the table only.
+ * New infinities count as +-65504, new NaN as 0.  Present scales are finite and not negative.  Slots that hold
+ * no token of the sequence are not written.  A page that is written must be named by one entry of the table only.
  *   D must be 64, 128 or 256; cache rows 8-byte, new rows 16-byte aligned; cache rows and scales must not overlap.
  * ------------------------------------------------------------------------------------- */
 int specq_kv_append_block(const void* k_new, const void* v_new, int64_t s_nb, int64_t s_nt, int64_t s_nh,

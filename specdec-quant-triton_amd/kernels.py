@@ -1203,10 +1203,11 @@ def paged_kv_append_block_scaled(k_new, v_new, kc, vc, ks, vs, block_tbl, ctx_le
     that new tokens reach gets s' = max(amax, 1e-8) / Q (Q = 127 or 448) over them, or its present
     scale where that is larger and the block holds earlier tokens of the sequence; the new codes are
     rne(x / s'), and where the scale grows the earlier codes become rne(c * s / s') (NaN stays NaN).  New
-    infinities count as +-65504, new NaN as 0.  Present scales are finite and not negative.  Tokens at positions below zero, past the table or on a page outside the pool
-    are skipped, every other slot keeps what it holds.  A page that the call writes must be named by one
-    entry of the table only (paged_kv_fork sees to that, unless a row is cut back into a page it shares).
-    D = 256 is for other readers: paged_attention_block_scaled takes 64 and 128.  With `plan`, (n_seqs, q_len) = plan[0:2] on the device
+    infinities count as +-65504, new NaN as 0.  Present scales are finite and not negative.  Tokens at
+    positions below zero, past the table or on a page outside the pool are skipped, every other slot keeps
+    what it holds.  A page that the call writes must be named by one entry of the table only (paged_kv_fork
+    sees to that, unless a row is cut back into a page it shares).  D = 256 is for other readers:
+    paged_attention_block_scaled takes 64 and 128.  With `plan`, (n_seqs, q_len) = plan[0:2] on the device
     and the grid covers (B, QLMAX).
     """
     who = "paged_kv_append_block_scaled"
