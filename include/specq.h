@@ -414,8 +414,90 @@ int specq_kv_pages_compact(int32_t* block_tbl, int64_t s_bt, int B, int max_page
 int specq_kv_pages_copy(const int32_t* src, const int32_t* dst, int n, int n_pages, int n_tensors, void* const* base,
                         const int64_t* page_stride, const int64_t* page_bytes, void* stream);
 
-/* Calls specq_<name> (specq_rotary, specq_kv_append_block, specq_paged_attn_block or a specq_kv_pages_
- * function that returns int) with its n arguments as 64-bit words in their order: pointers and integers as they
+/* ---------------------------------------------------------------------------------------
+ * Norms of q and k for each head, with their rotary positions in the same pass (no reference counterpart):
+ *   y = x rsqrt(mean(x^2) + eps) w,  the first R of D dimensions then turned as specq_rotary turns them.
+ * fp32 with one rounding to fp16.
+ *   q_weight, k_weight  fp16 or (weight_fp32) fp32 [D], or [H, D] / [H_KV, D] with s_wq / s_wk elements from head to head
+ *             (0: one row for all heads); NULL: no weights
+ *   eps       finite, not negative.  Everything else as specq_rotary.
+ * ------------------------------------------------------------------------------------- */
+int specq_qk_norm_rotary(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh,
+                         const void* k, int64_t s_kb, int64_t s_kt, int64_t s_kh,
+                         void* q_out, int64_t s_qob, int64_t s_qot, int64_t s_qoh,
+                         void* k_out, int64_t s_kob, int64_t s_kot, int64_t s_koh,
+                         const void* q_weight, int64_t s_wq, const void* k_weight, int64_t s_wk, int weight_fp32,
+                         float eps, const void* inv_freq, int freq_fp64, float mscale,
+                         const int32_t* ctx_len, const int32_t* positions, int64_t s_pb,
+                         int B_grid, int n_seqs, int q_len, int ql_grid, int H, int H_KV, int D, int R,
+                         int interleaved, const int32_t* plan, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Attention weights gathered by the tokens of a paged int8 cache (no reference counterpart): over the rows (new token i,
+ * query head of the group) of each sequence b and KV head h, with p the softmax of specq_paged_attn's scores,
+ *   weights[b, h, t] = (t >= L - q_len ? 0 : weights[b, h, t]) + sum over rows of p_t,   t < L
+ * so new tokens start from nothing and earlier ones add up; positions from L on are not written.
+ *   q, kc, ks, block_tbl, ctx_len, sequences, plan  as specq_paged_attn (K only)
+ *   q_lens    NULL, or int32 [B_grid]: sequence b's new tokens are q's first q_lens[b] (at most q_len), which ctx_len[b]
+ *             counts: the drafts that were accepted.  0 leaves the sequence's weights as they are
+ *   weights   fp32 [B_grid, H_KV, >= max_pages * PAGE], strides s_wb, s_wh; rows must not overlap
+ *   A context longer than the table counts as the table's length, a negative one as 0.  Tokens on no page of the pool get
+ *   nothing.  Eager and plan-mode calls agree bit for bit.  At most 65536 (sequence, KV head) pairs.
+ *   Workspace: specq_paged_attn_weights_workspace_size() bytes, as the workspaces above.
+ * ------------------------------------------------------------------------------------- */
+size_t specq_paged_attn_weights_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int max_pages, int PAGE);
+int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh,
+                             const int8_t* kc, int64_t s_kp, int64_t s_ko, int64_t s_kh,
+                             const void* ks, int64_t s_sp, int64_t s_so, int64_t s_sh, int scale_fp32,
+                             const int32_t* block_tbl, int64_t s_bt, int max_pages, int n_pages,
+                             const int32_t* ctx_len, const int32_t* q_lens, float* weights, int64_t s_wb, int64_t s_wh,
+                             int B_grid, int n_seqs, int q_len, int ql_grid, int H, int H_KV, int D, int PAGE,
+                             float sm_scale, const int32_t* plan, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Eviction from a paged cache by gathered weight (no reference counterpart), in place: a sequence of ctx_len[b] > limit
+ * tokens is cut back to `budget` for each KV head: its first `sinks`, its last `recent`, and of the others those of
+ * greatest weights[b, h, t], ties to the lower position (NaN counts as -infinity).  They move together in order: token j
+ * comes from position kept[b, h, j], in every cache tensor and in the weights, and ctx_len[b] becomes budget.  A sequence
+ * stays as it is (kept[j] = j, -1 past its tokens) where it is not longer than limit, where its table names a page outside
+ * the pool, and, with ref not NULL, where it names a page with ref > 1.  A page must be named by one entry of the table
+ * only.  Pages behind the budget are let go of by specq_kv_pages_free.
+ *   weights   fp32 [B, H_KV, >= max_pages * PAGE] (specq_paged_attn_weights)
+ *   Cache tensors: at most 16, [n_pages, PAGE, H_KV] rows of row_bytes (1 to 4096) bytes; base pointers and strides in
+ *   bytes (host arrays, read during the call)
+ *   kept      int32 [B, H_KV, budget];  0 <= recent + sinks <= budget <= limit
+ *   Workspace: specq_kv_evict_workspace_size() bytes, as the workspaces above.
+ * ------------------------------------------------------------------------------------- */
+size_t specq_kv_evict_workspace_size(int B, int H_KV);
+int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int max_pages, const int32_t* ref, int n_pages,
+                   int32_t* ctx_len, float* weights, int64_t s_wb, int64_t s_wh, int H_KV, int PAGE,
+                   int n_tensors, void* const* base, const int64_t* page_stride, const int64_t* token_stride,
+                   const int64_t* head_stride, const int64_t* row_bytes, int budget, int recent, int sinks, int limit,
+                   int32_t* kept, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Beam search (no reference counterpart).
+ * select: of the candidates scores[b, w] + logits[b, w, v] - log(sum_u exp(logits[b, w, u])) of each sequence the best n,
+ *   in order, ties to the lower beam, then the lower token.  A beam with finished[b, w] != 0 has one candidate, token eos
+ *   with the score it has.  Candidates whose score is NaN or -infinity are none; what is missing is (-inf, -1, -1).
+ *   Scores are compared in fp64.
+ *   logits    fp16 or (logits_fp32) fp32 [B, W, V], strides s_lb, s_lw;  scores fp32 [B, W], row stride s_sb
+ *   finished  NULL, or bytes [B, W], row stride s_fb
+ *   out_scores fp32, out_tokens, out_parents int32 [B, n]; a parent is the row b W + w.  W, n at most 64.
+ *   Workspace: specq_beam_select_workspace_size() bytes, as the workspaces above.
+ * reorder: row r of every state becomes row parents[r], in place, within groups of `group` rows (at most 32); a parent
+ *   outside the row's group leaves the row as it is.  States: base pointers, strides from row to row and sizes of a row in
+ *   bytes (host arrays, read during the call). */
+size_t specq_beam_select_workspace_size(int B, int W, int V, int logits_fp32);
+int specq_beam_select(const void* logits, int logits_fp32, int64_t s_lb, int64_t s_lw, const float* scores, int64_t s_sb,
+                      const uint8_t* finished, int64_t s_fb, int eos, float* out_scores, int32_t* out_tokens,
+                      int32_t* out_parents, int B, int W, int V, int n, void* workspace, size_t workspace_bytes,
+                      void* stream);
+int specq_beam_reorder(const int32_t* parents, int rows, int group, int n_tensors, void* const* base,
+                       const int64_t* row_stride, const int64_t* row_bytes, void* stream);
+
+/* Calls specq_<name> (specq_rotary, specq_qk_norm_rotary, specq_kv_append_block, specq_paged_attn_block,
+ * specq_paged_attn_weights, specq_kv_evict, specq_beam_select, specq_beam_reorder or a specq_kv_pages_ function that returns int) with its n arguments as 64-bit words in their order: pointers and integers as they
  * are, floats as the bits of a double.  An integer that does not fit its argument's type is -22.  For bindings
  * that pay for every argument they convert. */
 int specq_call_packed(const char* name, const int64_t* words, int n);

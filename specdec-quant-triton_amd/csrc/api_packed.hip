@@ -52,6 +52,11 @@ extern "C" int specq_call_packed(const char* name, const int64_t* words, int n) 
   SPECQ_PACKED(specq_paged_attn_block);
   SPECQ_PACKED(specq_kv_append_block);
   SPECQ_PACKED(specq_rotary);
+  SPECQ_PACKED(specq_qk_norm_rotary);
+  SPECQ_PACKED(specq_paged_attn_weights);
+  SPECQ_PACKED(specq_kv_evict);
+  SPECQ_PACKED(specq_beam_select);
+  SPECQ_PACKED(specq_beam_reorder);
   SPECQ_PACKED(specq_kv_pages_reserve);
   SPECQ_PACKED(specq_kv_pages_free);
   SPECQ_PACKED(specq_kv_pages_fork);

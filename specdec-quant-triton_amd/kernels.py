@@ -19,8 +19,10 @@ silu_mul_quant_int8 / quantize_act_int8_gpu (kernels.py:58-62 on the device), an
 w4a8_matmul (INT4 weights on the INT8 MFMA path, the reference's REPORT.md:156
 recommendation; no reference kernel).  Without a reference counterpart: rotary_embed (positions
 of q and k), paged_kv_append_block_scaled and paged_attention_block_scaled (an int8 or e4m3
-cache with one scale for each block of tokens and head), and the cache's page tables,
-paged_kv_reserve / _free / _fork / _compact / _copy.
+cache with one scale for each block of tokens and head), the cache's page tables,
+paged_kv_reserve / _free / _fork / _compact / _copy, qk_norm_rotary (norms of q and k for each head with
+their positions), paged_attention_weights and paged_kv_evict (the attention weight that cached tokens
+gather, and eviction by it), and beam search, beam_select and beam_reorder.
 
 Every launcher takes `plan` (an int32 device tensor read by the kernel at run time) and a
 fixed grid size, so a single captured graph replays every (B, k) (reference kernels.py:14-17).
@@ -78,6 +80,7 @@ __all__ = [
     "w8a8_matmul_grouped", "w4a16_matmul_grouped", "set_weight_pack_cache", "clear_weight_pack_cache",
     "rotary_embed", "rotary_inv_freq", "paged_kv_append_block_scaled", "paged_attention_block_scaled",
     "paged_kv_reserve", "paged_kv_free", "paged_kv_fork", "paged_kv_compact", "paged_kv_copy",
+    "qk_norm_rotary", "paged_attention_weights", "paged_kv_evict", "beam_select", "beam_reorder",
 ]
 
 
@@ -1113,21 +1116,9 @@ def _rotary_out(who: str, x, shape, strides, D: int, out):
     return out, so
 
 
-def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, interleaved=False, mscale=1.0, plan=None,
-                 n_seqs=None, q_out=None, k_out=None):
-    """Rotary positions of the new tokens' q and k; returns (q_out, k_out).
-
-    q fp16 [B, QL, H, D], k fp16 [B, QL, H_KV, D] or None; inv_freq fp32 or fp64 [R / 2], R <= D <= 512
-    (rotary_inv_freq).  Pair j of the first R dimensions -- (j, j + R/2), or (2j, 2j + 1) with
-    interleaved -- is turned by pos * inv_freq[j] and scaled by mscale; the other dimensions are copied.
-    Token i of sequence b is at ctx_len[b] - q_len + i (ctx_len counts the new tokens, as the K/V append
-    and the attention have it), or at positions[b, i] (int32 [B, QL]).  Angles are formed in fp64.
-    Outputs may be the inputs (in place); they must not overlap them otherwise.  With `plan`,
-    (n_seqs, q_len) = plan[0:2] on the device and the grid covers (B, QL).  Tokens that are not active
-    are not written (an omitted output holds anything there).
-    """
-    who = "rotary_embed"
-    dev = _gpu_of(who, q, k, inv_freq, ctx_len, positions, plan, q_out, k_out)
+def _rotary_call(who: str, q, k, inv_freq, ctx_len, q_len, positions, plan, n_seqs, q_out, k_out):
+    """Checks the arguments that the rotary entry points share; returns the outputs and the C call's words: those of the
+    tensors, the frequencies', the positions', the grid and the sizes (None where there is nothing to do)."""
     shape, qs = q.shape, q.stride()
     if len(shape) != 4:
         raise RuntimeError(f"{who}: q [B, QL, H, D] expected")
@@ -1146,7 +1137,6 @@ def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, inter
     if inv_freq.dtype not in (torch.float32, torch.float64) or inv_freq.dim() != 1 or \
             (inv_freq.stride(0) != 1 and inv_freq.shape[0] > 1):
         raise RuntimeError(f"{who}: inv_freq must be a contiguous fp32 or fp64 vector")
-    R = 2 * inv_freq.shape[0]
     Bg, Qg, n_seqs, q_len = _token_grid(who, B, QL, q_len, n_seqs, plan)
     s_pb = 0
     if positions is not None:
@@ -1159,12 +1149,69 @@ def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, inter
     else:
         raise RuntimeError(f"{who}: ctx_len or positions must be given")
     if Bg == 0 or Qg == 0:
-        return q_out, k_out
-    _call_on(dev, "specq_rotary", q.data_ptr(), qs[0], qs[1], qs[2], _ptr(k), ks[0], ks[1], ks[2],
-             q_out.data_ptr(), qo[0], qo[1], qo[2], _ptr(k_out), ko[0], ko[1], ko[2],
-             inv_freq.data_ptr(), inv_freq.dtype == torch.float64, mscale,
-             _ptr(ctx_len), _ptr(positions), s_pb, Bg, n_seqs, q_len, Qg, H, H_KV, D, R,
-             bool(interleaved), _plan_of(plan, 2, who))
+        return q_out, k_out, None
+    return q_out, k_out, (
+        (q.data_ptr(), qs[0], qs[1], qs[2], _ptr(k), ks[0], ks[1], ks[2],
+         q_out.data_ptr(), qo[0], qo[1], qo[2], _ptr(k_out), ko[0], ko[1], ko[2]),
+        (inv_freq.data_ptr(), inv_freq.dtype == torch.float64),
+        (_ptr(ctx_len), _ptr(positions), s_pb, Bg, n_seqs, q_len, Qg, H, H_KV, D, 2 * inv_freq.shape[0]))
+
+
+def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, interleaved=False, mscale=1.0, plan=None,
+                 n_seqs=None, q_out=None, k_out=None):
+    """Rotary positions of the new tokens' q and k; returns (q_out, k_out).
+
+    q fp16 [B, QL, H, D], k fp16 [B, QL, H_KV, D] or None; inv_freq fp32 or fp64 [R / 2], R <= D <= 512
+    (rotary_inv_freq).  Pair j of the first R dimensions -- (j, j + R/2), or (2j, 2j + 1) with
+    interleaved -- is turned by pos * inv_freq[j] and scaled by mscale; the other dimensions are copied.
+    Token i of sequence b is at ctx_len[b] - q_len + i (ctx_len counts the new tokens, as the K/V append
+    and the attention have it), or at positions[b, i] (int32 [B, QL]).  Angles are formed in fp64.
+    Outputs may be the inputs (in place); they must not overlap them otherwise.  With `plan`,
+    (n_seqs, q_len) = plan[0:2] on the device and the grid covers (B, QL).  Tokens that are not active
+    are not written (an omitted output holds anything there).
+    """
+    who = "rotary_embed"
+    dev = _gpu_of(who, q, k, inv_freq, ctx_len, positions, plan, q_out, k_out)
+    q_out, k_out, words = _rotary_call(who, q, k, inv_freq, ctx_len, q_len, positions, plan, n_seqs, q_out, k_out)
+    if words is not None:
+        tensors, freq, rest = words
+        _call_on(dev, "specq_rotary", *tensors, *freq, mscale, *rest, bool(interleaved), _plan_of(plan, 2, who))
+    return q_out, k_out
+
+
+def _norm_weights(who: str, name: str, w, heads: int, D: int) -> int:
+    """Checks norm weights [D] or [heads, D]; returns the elements from head to head."""
+    if w is None:
+        return 0
+    if w.dtype not in (torch.float16, torch.float32) or w.dim() not in (1, 2) or w.shape[-1] != D or \
+            (w.stride(-1) != 1 and D > 1) or (w.dim() == 2 and w.shape[0] != heads):
+        raise RuntimeError(f"{who}: {name} must be fp16 or fp32 [{D}] or [{heads}, {D}] with unit inner stride")
+    return w.stride(0) if w.dim() == 2 else 0
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, inv_freq, ctx_len=None, q_len=None, positions=None, interleaved=False,
+                   mscale=1.0, eps=1e-6, plan=None, n_seqs=None, q_out=None, k_out=None):
+    """Norms of the new tokens' q and k for each head, and their rotary positions, in one pass; returns (q_out, k_out).
+
+    A head's row x becomes y = x / sqrt(mean(x^2) + eps) * weight, whose first dimensions are then turned as
+    rotary_embed turns them: fp32, rounded once.  q_weight, k_weight fp16 or fp32, both of one type, [D], or a row for
+    each head ([H, D], [H_KV, D]), or None (no weights; k_weight is None where k is).  Everything else as rotary_embed.
+    """
+    who = "qk_norm_rotary"
+    dev = _gpu_of(who, q, k, q_weight, k_weight, inv_freq, ctx_len, positions, plan, q_out, k_out)
+    q_out, k_out, words = _rotary_call(who, q, k, inv_freq, ctx_len, q_len, positions, plan, n_seqs, q_out, k_out)
+    if k is None and k_weight is not None:
+        raise RuntimeError(f"{who}: k_weight without k")
+    s_wq = _norm_weights(who, "q_weight", q_weight, q.shape[2], q.shape[3])
+    s_wk = _norm_weights(who, "k_weight", k_weight, k.shape[2], q.shape[3]) if k is not None else 0
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise RuntimeError(f"{who}: q_weight and k_weight must be of one type")
+    if words is not None:
+        tensors, freq, rest = words
+        w = q_weight if q_weight is not None else k_weight
+        _call_on(dev, "specq_qk_norm_rotary", *tensors, _ptr(q_weight), s_wq, _ptr(k_weight), s_wk,
+                 w is not None and w.dtype == torch.float32, eps, *freq, mscale, *rest, bool(interleaved),
+                 _plan_of(plan, 2, who))
     return q_out, k_out
 
 
@@ -1437,3 +1484,208 @@ def paged_kv_copy(src, dst, caches):
     m, words = _page_tensors(who, caches, P, dev)
     _call_on(dev, "specq_kv_pages_copy", src.data_ptr(), dst.data_ptr(), n, min(P, 2**31 - 1),
              *_page_tensor_args(m, words))
+
+
+# ----------------------------------------------------------------------------------------
+# Eviction by gathered attention weight
+# ----------------------------------------------------------------------------------------
+def _gathered(who: str, weights, B: int, H_KV: int, tokens: int):
+    """Checks gathered weights of at least B sequences; returns their strides."""
+    if weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[0] < B or weights.shape[1] != H_KV or \
+            weights.shape[2] < tokens or (weights.stride(2) != 1 and weights.shape[2] > 1):
+        raise RuntimeError(f"{who}: weights must be fp32 [{B}, {H_KV}, >= {tokens}] with unit inner stride")
+    return weights.stride(0), weights.stride(1)
+
+
+def paged_attention_weights(q, kc, ks, block_tbl, ctx_len, weights, q_len=None, q_lens=None, plan=None, n_seqs=None,
+                            sm_scale=None, workspace=None):
+    """Add to `weights` the attention weight that the new tokens' queries give each cached token, in place; returns it.
+
+    q fp16 [B, QLMAX, H, D], D 64 or 128; kc int8 [pages, PAGE, H_KV, D], ks fp16 or fp32 [pages, PAGE, H_KV],
+    block_tbl int32 [B, max_pages], ctx_len int32 [B] as paged_attention takes them (ctx_len counts the q_len new
+    tokens); weights fp32 [B, H_KV, T], T at least max_pages * PAGE.  For a token t of sequence b the softmax
+    probabilities p_t of paged_attention's scores are summed over the new tokens and the query heads of KV head h:
+    weights[b, h, t] grows by that sum, or becomes it where t is one of the new tokens; positions past the sequence stay.
+    q_lens int32 [B]: how many of the q_len tokens sequence b really has (accepted drafts), counted by ctx_len; 0
+    leaves its weights as they are.  Block-table ids outside [0, pages) mask their page's tokens, a context longer
+    than the table counts as the table's length.  sm_scale defaults to D^-1/2.  A NaN or infinite score makes NaN of its
+    row's share.  With `plan`, (n_seqs, q_len) = plan[0:2] on the device and the grid covers (B, QLMAX).  Calls that may
+    run at the same time on several streams need a workspace each.
+    """
+    who = "paged_attention_weights"
+    dev = _gpu_of(who, q, kc, ks, block_tbl, ctx_len, weights, q_lens, plan)
+    if q.dim() != 4 or q.dtype != torch.float16 or q.stride(3) != 1:
+        raise RuntimeError(f"{who} expects fp16 q [B, QLMAX, H, D] with contiguous head_dim")
+    B, QL, H, D = q.shape
+    shape, cs = kc.shape, kc.stride()
+    if kc.dtype != torch.int8 or len(shape) != 4 or cs[3] != 1:
+        raise RuntimeError(f"{who} expects an int8 K cache [pages, PAGE, H_KV, D] with contiguous head_dim")
+    P, PAGE, H_KV = shape[0], shape[1], shape[2]
+    if shape[3] != D or H_KV < 1 or H % H_KV:
+        raise RuntimeError(f"{who}: cache {tuple(shape)} does not fit q {tuple(q.shape)}")
+    if ks.dtype not in (torch.float16, torch.float32) or ks.shape != shape[:3]:
+        raise RuntimeError(f"{who}: scales must be fp16 or fp32 [{P}, {PAGE}, {H_KV}]")
+    Bg, Qg, n_seqs, q_len = _token_grid(who, B, QL, q_len, n_seqs, plan)
+    if block_tbl.dtype != torch.int32 or block_tbl.dim() != 2 or block_tbl.shape[0] < Bg or \
+            (block_tbl.stride(1) != 1 and block_tbl.shape[1] > 1):
+        raise RuntimeError(f"{who}: block_tbl must be int32 [B, max_pages] with unit inner stride for {Bg} sequences")
+    _int32_vec(who, "ctx_len", ctx_len, Bg)
+    if q_lens is not None:
+        _int32_vec(who, "q_lens", q_lens, Bg)
+    max_pages = block_tbl.shape[1]
+    s_wb, s_wh = _gathered(who, weights, Bg, H_KV, max_pages * PAGE)
+    if Bg == 0 or Qg == 0:
+        return weights
+    need = _lib.lib().specq_paged_attn_weights_workspace_size(Bg, H, H_KV, Qg, max_pages, PAGE)
+    wptr, wbytes = _workspace(workspace, dev).ensure(need)
+    qs, ss = q.stride(), ks.stride()
+    _call_on(dev, "specq_paged_attn_weights", q.data_ptr(), qs[0], qs[1], qs[2], kc.data_ptr(), cs[0], cs[1], cs[2],
+             ks.data_ptr(), ss[0], ss[1], ss[2], ks.dtype == torch.float32,
+             block_tbl.data_ptr(), block_tbl.stride(0) if block_tbl.shape[0] > 1 else max_pages, max_pages,
+             min(P, 2**31 - 1), ctx_len.data_ptr(), _ptr(q_lens), weights.data_ptr(), s_wb, s_wh,
+             Bg, n_seqs, q_len, Qg, H, H_KV, D, PAGE, D ** -0.5 if sm_scale is None else sm_scale,
+             _plan_of(plan, 2, who), wptr, wbytes)
+    return weights
+
+
+def paged_kv_evict(block_tbl, ctx_len, weights, caches, PAGE, budget, recent=0, sinks=0, limit=None, ref=None, kept=None,
+                   workspace=None):
+    """Cut sequences of more than `limit` tokens (default: budget) back to `budget`, in place; returns kept.
+
+    block_tbl int32 [B, max_pages]; ctx_len int32 [B]; weights fp32 [B, H_KV, >= max_pages * PAGE]
+    (paged_attention_weights); caches at most 16 tensors [pages, PAGE, H_KV, ...] of any type, the rest of each
+    contiguous (K, V and their scales with a scale for each token; a cache with block scales cannot give single tokens
+    up).  For each K/V head stay the first `sinks` tokens, the last `recent` and, of the others, those of greatest weight,
+    ties to the lower position; NaN counts as -infinity.  They move together in the order they have: token j comes from
+    position kept[b, h, j], in every tensor and in weights, and ctx_len[b] becomes budget.  What lies behind it is left
+    as it was; paged_kv_free(block_tbl, ref, ctx_len, PAGE) lets go of its pages.  A sequence stays as it is (kept[j] = j,
+    -1 past its tokens) where it is not longer than limit, where one of its table entries names no page and, with the
+    page counts `ref` given, where another row names one of its pages too.  Without `ref` the caller answers for
+    that: a page must be named by one entry of the table only.  Keys keep the positions they were turned by, so the
+    new tokens' positions go on from the uncut length (rotary_embed's `positions`).  kept int32 [B, H_KV, budget].
+    """
+    who = "paged_kv_evict"
+    dev = _gpu_of(who, block_tbl, ctx_len, weights, ref, kept, *caches)
+    if block_tbl.dtype != torch.int32 or block_tbl.dim() != 2 or block_tbl.shape[0] < 1 or block_tbl.shape[1] < 1 or \
+            (block_tbl.stride(1) != 1 and block_tbl.shape[1] > 1):
+        raise RuntimeError(f"{who}: block_tbl must be int32 [B, max_pages] with unit inner stride")
+    B, C = block_tbl.shape
+    _int32_vec(who, "ctx_len", ctx_len, B)
+    PAGE, budget = int(PAGE), int(budget)
+    limit = budget if limit is None else int(limit)
+    if PAGE < 1 or budget < 1:
+        raise RuntimeError(f"{who}: PAGE={PAGE} and budget={budget} must be at least 1")
+    if weights.dim() != 3 or weights.shape[1] < 1:
+        raise RuntimeError(f"{who}: weights must be fp32 [B, H_KV, T]")
+    H_KV = weights.shape[1]
+    s_wb, s_wh = _gathered(who, weights, B, H_KV, C * PAGE)
+    if len(caches) == 0:
+        raise RuntimeError(f"{who}: no caches of [pages, PAGE, H_KV, ...]")
+    P = caches[0].shape[0] if caches[0].dim() else 0
+    cols = ([], [], [], [], [])  # base, strides from page to page, token to token and head to head, bytes of a row
+    for t in caches:
+        if t.dim() < 3 or t.shape[0] != P or t.shape[1] != PAGE or t.shape[2] != H_KV or t.numel() == 0:
+            raise RuntimeError(f"{who}: a cache {tuple(t.shape)} must be [{P}, {PAGE}, {H_KV}, ...]")
+        if t.dim() > 3 and not t[0, 0, 0].is_contiguous():
+            raise RuntimeError(f"{who}: the rows of a cache must be contiguous")
+        size, st = t.element_size(), t.stride()
+        for col, v in zip(cols, (t.data_ptr(), st[0] * size, st[1] * size, st[2] * size, t[0, 0, 0].numel() * size)):
+            col.append(v)
+    if ref is not None:
+        _int32_vec(who, "ref", ref, P)
+    if kept is None:
+        kept = torch.empty((B, H_KV, budget), dtype=torch.int32, device=ctx_len.device)
+    elif kept.dtype != torch.int32 or kept.shape != (B, H_KV, budget) or not kept.is_contiguous():
+        raise RuntimeError(f"{who}: kept must be contiguous int32 [{B}, {H_KV}, {budget}]")
+    words = array.array("q", sum(cols, []))
+    at, n = words.buffer_info()[0], len(caches)
+    wptr, wbytes = _workspace(workspace, dev).ensure(_lib.lib().specq_kv_evict_workspace_size(B, H_KV))
+    _call_on(dev, "specq_kv_evict", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C, _ptr(ref),
+             min(P, 2**31 - 1), ctx_len.data_ptr(), weights.data_ptr(), s_wb, s_wh, H_KV, PAGE,
+             n, at, at + 8 * n, at + 16 * n, at + 24 * n, at + 32 * n, budget, int(recent), int(sinks), limit,
+             kept.data_ptr(), wptr, wbytes)
+    return kept
+
+
+# ----------------------------------------------------------------------------------------
+# Beam search
+# ----------------------------------------------------------------------------------------
+@functools.lru_cache(maxsize=4096)
+def _beam_workspace(B, W, V, fp32, dev) -> int:
+    """Bytes a call needs: a function of its sizes and the GPU's CU count."""
+    with torch.cuda.device(dev):
+        return _lib.lib().specq_beam_select_workspace_size(B, W, V, fp32)
+
+
+def beam_select(logits, scores, n=None, finished=None, eos=None, out=None, workspace=None):
+    """The best n continuations of each sequence's beams; returns (scores fp32, tokens int32, parents int32), [B, n] each.
+
+    logits fp16 or fp32 [B, W, V]; scores fp32 [B, W], the beams' log-probabilities so far (-inf: no beam).  A
+    continuation by token v has scores[b, w] + logits[b, w, v] - log(sum(exp(logits[b, w]))); a beam with
+    finished[b, w] (bool) has one, token `eos`, with the score it has.  Best first, compared in fp64, ties to the lower
+    beam, then the lower token; n defaults to W, and both are at most 64.  parents holds rows b * W + w, as
+    paged_kv_fork and beam_reorder take them.  Continuations of score -inf or NaN (logits of -inf; every one of a row that
+    holds NaN or +inf) are none; where there are fewer than n the rest has score -inf, token and parent -1.
+    Calls that may run at the same time on several streams need a workspace each.
+    """
+    who = "beam_select"
+    dev = _gpu_of(who, logits, scores, finished, *(out if out is not None else ()))
+    if logits.dtype not in (torch.float16, torch.float32) or logits.dim() != 3 or \
+            (logits.stride(2) != 1 and logits.shape[2] > 1):
+        raise RuntimeError(f"{who}: logits must be fp16 or fp32 [B, W, V] with unit inner stride")
+    B, W, V = logits.shape
+    if scores.dtype != torch.float32 or scores.shape != (B, W) or (scores.stride(1) != 1 and W > 1):
+        raise RuntimeError(f"{who}: scores must be fp32 [{B}, {W}] with unit inner stride")
+    if finished is not None and eos is None:
+        raise RuntimeError(f"{who}: finished beams go on with eos, which is not given")
+    if finished is not None and (finished.dtype != torch.bool or finished.shape != (B, W) or
+                                 (finished.stride(1) != 1 and W > 1)):
+        raise RuntimeError(f"{who}: finished must be bool [{B}, {W}] with unit inner stride")
+    n = W if n is None else int(n)
+    if n < 1 or W < 1 or V < 1:
+        raise RuntimeError(f"{who}: {n} of {W} beams over {V} tokens")
+    if out is None:
+        out = (torch.empty((B, n), dtype=torch.float32, device=logits.device),
+               *(torch.empty((B, n), dtype=torch.int32, device=logits.device) for _ in "tp"))
+    elif len(out) != 3 or any(t.shape != (B, n) or not t.is_contiguous() for t in out) or \
+            [t.dtype for t in out] != [torch.float32, torch.int32, torch.int32]:
+        raise RuntimeError(f"{who}: out must be contiguous (fp32, int32, int32) of [{B}, {n}]")
+    if B == 0:
+        return tuple(out)
+    fp32 = logits.dtype == torch.float32
+    wptr, wbytes = _workspace(workspace, dev).ensure(_beam_workspace(B, W, V, fp32, dev))
+    _call_on(dev, "specq_beam_select", logits.data_ptr(), fp32, logits.stride(0), logits.stride(1),
+             scores.data_ptr(), scores.stride(0), _ptr(finished), finished.stride(0) if finished is not None else 0,
+             int(eos) if finished is not None else 0, *(t.data_ptr() for t in out), B, W, V, n, wptr, wbytes)
+    return tuple(out)
+
+
+def beam_reorder(states, parents, group):
+    """Make row r of every state its row parents[r], in place, within groups of `group` rows (a sequence's beams).
+
+    states: tensors [rows, ...] of any type, each row contiguous (token histories, gathered weights, hidden states, a
+    dense cache), no two of them over the same memory; parents int32 [rows] (beam_select's, flattened), group at most 32.  A parent
+    outside the row's group (-1) leaves the row as it is.  A paged cache follows by paged_kv_fork.
+    """
+    who = "beam_reorder"
+    dev = _gpu_of(who, parents, *states)
+    rows, group = parents.shape[0] if parents.dim() == 1 else -1, int(group)
+    _int32_vec(who, "parents", parents, 0)
+    if group < 1 or rows % group:
+        raise RuntimeError(f"{who}: {rows} rows are no groups of {group}")
+    base, stride, nbytes = [], [], []
+    for t in states:
+        if t.dim() < 1 or t.shape[0] != rows:
+            raise RuntimeError(f"{who}: a state {tuple(t.shape)} must have {rows} rows")
+        if t.numel() == 0:
+            continue
+        if not t.is_contiguous() and not t[0].is_contiguous():
+            raise RuntimeError(f"{who}: the rows of a state must be contiguous")
+        size = t.element_size()
+        base.append(t.data_ptr())
+        stride.append(t.stride(0) * size)
+        nbytes.append(t.numel() // rows * size)
+    if not base:
+        return
+    words = array.array("q", base + stride + nbytes)
+    _call_on(dev, "specq_beam_reorder", parents.data_ptr(), rows, group, *_page_tensor_args(len(base), words))

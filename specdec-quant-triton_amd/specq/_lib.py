@@ -107,6 +107,26 @@ SIGNATURES = {
                               _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64,
                               _c_vp, _c_int, _c_float, _c_vp, _c_vp, _c_i64,
                               _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_vp]),
+    "specq_qk_norm_rotary": (_c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64,
+                                      _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64,
+                                      _c_vp, _c_i64, _c_vp, _c_i64, _c_int, _c_float,
+                                      _c_vp, _c_int, _c_float, _c_vp, _c_vp, _c_i64,
+                                      _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                      _c_vp, _c_vp]),
+    "specq_paged_attn_weights_workspace_size": (_c_size, [_c_int] * 6),
+    "specq_paged_attn_weights": (_c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64,
+                                          _c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_vp, _c_i64, _c_int, _c_int,
+                                          _c_vp, _c_vp, _c_vp, _c_i64, _c_i64,
+                                          _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                          _c_float, _c_vp, _c_vp, _c_size, _c_vp]),
+    "specq_kv_evict_workspace_size": (_c_size, [_c_int, _c_int]),
+    "specq_kv_evict": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_vp, _c_i64, _c_i64, _c_int,
+                                _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int,
+                                _c_vp, _c_vp, _c_size, _c_vp]),
+    "specq_beam_select_workspace_size": (_c_size, [_c_int] * 4),
+    "specq_beam_select": (_c_int, [_c_vp, _c_int, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_int,
+                                   _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_size, _c_vp]),
+    "specq_beam_reorder": (_c_int, [_c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp]),
     "specq_kv_pages_workspace_size": (_c_size, [_c_int, _c_int, _c_int]),
     "specq_kv_pages_reserve": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_int, _c_vp,
                                         _c_vp, _c_size, _c_vp]),
