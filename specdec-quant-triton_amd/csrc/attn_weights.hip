@@ -11,10 +11,11 @@
 //      joins them to log2 of each row's sum over all tiles
 //   2  p = exp2(s - that), summed over the rows, and the update of w
 // The scores of up to 16 rows (kAwStoreRows: plain decoding) go from 1 to 2 through the workspace; more rows compute them again.  Both ways
-// add a token's rows in one order (16 lanes, rows 16 apart in each lane, then pairs of lanes), so they give the same
-// bits, and a plan-mode call those of an eager one.
+// add a token's rows in one order (16 lanes; in each the blocks of 16 rows of either parity, then both; then pairs of
+// lanes) and join the rows' statistics in one (64 tokens, 256, all), so they give the same bits, and a plan-mode call those of an
+// eager one.
 //
-// K stays: a wave owns 64 tokens, converts their codes to fp16 matrix operands once and walks the rows 16 at a time
+// K stays: a wave holds 64 tokens, converts their codes to fp16 matrix operands once and walks the rows 16 at a time
 // (K . Q^T on v_mfma_f32_16x16x32_f16: a lane's results are four tokens of one row).  Everything behind the products is
 // fp32; log2(e) is folded into the scale.
 #include "api_common.hpp"
@@ -24,6 +25,8 @@ namespace specq {
 
 constexpr int kAwTile = 256;       // tokens of a workgroup: 4 waves of 4 sub-tiles of 16
 constexpr int kAwStoreRows = 16;   // rows whose scores go through the workspace
+constexpr int kAwFewRows = 64;     // rows whose queries a workgroup keeps in LDS
+constexpr int kAwSpan = 8;         // most tiles such a workgroup walks (its waves' lanes hold their pages, and one tile's more)
 constexpr int kAwSeg = 32;         // row blocks of 16 whose statistics are joined at a time
 constexpr int kAwSumTile = 1024;   // tokens of a workgroup that adds up stored scores
 constexpr int kAwMaxGrid = 1 << 16;
@@ -39,13 +42,27 @@ struct AwParams {
   int n_seqs, q_len, B_grid, ql_grid, G, H_KV, PAGE;
   int cap;      // tokens a row of the table holds
   int tiles;    // of cap
+  int span;     // tiles of a workgroup of few rows
   int rows;     // of a program at most: ql_grid * G
+  uint32_t g_magic;  // ceil(2^32 / G): row / G is its product's high word (rows below 2^20, G below 2^12); 0 for G = 1
   float scale_log2;
   // Workspace: scores [prog][rows][tiles * 256]; (max, sum) [prog][tiles][rows]; log2 of the rows' sums [prog][rows].
   float* scores; uint64_t* stats; float* lse;
   int32_t* counters;  // [prog]
 };
 
+// Program number `i` of the launch order.  The heads of a sequence read the same lines of scales: in blocks of eight
+// sequences they come eight workgroups apart, which puts them on one XCD, whose L2 serves them.
+__device__ __forceinline__ int aw_order(const AwParams& p, int i) {
+  const int full = p.B_grid / 8 * 8 * p.H_KV;
+  if (i >= full) return i;
+  const int blk = i / (8 * p.H_KV), rem = i - blk * (8 * p.H_KV);
+  return (blk * 8 + rem % 8) * p.H_KV + rem / 8;
+}
+// The new token of a row.
+__device__ __forceinline__ int aw_token(const AwParams& p, int row) {
+  return p.g_magic != 0 ? (int)__umulhi((uint32_t)row, p.g_magic) : row;
+}
 // A program (sequence b, KV head h): its rows, tokens and active tiles.
 struct AwProg {
   int b, h, ql, rows, L, tiles;
@@ -120,139 +137,446 @@ __device__ __forceinline__ void aw_update(const AwParams& p, const AwProg& x, in
   }
 }
 
-enum { kAwScores, kAwStats, kAwSums };  // pass 1 with and without storing the scores, pass 2 from K
+enum { kAwStats, kAwSums };  // pass 1, and pass 2 from K
 
+// Where a wave's sub-tiles lie: lane l holds those of sub-tile l (four to a tile).  A sub-tile lies in one page.  One past the
+// context or on no page of the pool is not `ok`: its codes read as nothing, its scales are the pool's first.
+struct AwPages {
+  int64_t kv, sc;  // of its first token: bytes to the codes, scales ahead
+  uint64_t ok;     // bit l: sub-tile l
+};
+__device__ __forceinline__ AwPages aw_pages(const AwParams& p, const AwProg& x, int t, int page, bool in) {
+  const bool ok = in && t < x.L && (uint32_t)page < (uint32_t)p.n_pages;
+  const int pg = ok ? page : 0, slot = ok ? t % p.PAGE : 0;
+  return {pg * p.s_kp + slot * p.s_ko + x.h * p.s_kh, pg * p.s_sp + slot * p.s_so + x.h * p.s_sh, __builtin_amdgcn_ballot_w64(ok)};
+}
+__device__ __forceinline__ int64_t aw_lane64(int64_t v, int l) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, l), hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)v >> 32), l);
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+// Codes and scales of sub-tiles l0..l0 + 3.  Always the same loads, so that the waits on them are counted, not drained.  An
+// access takes whole rows (D / 16 lanes a row): lanes that take matrix operands directly touch half of each 128-byte line
+// twice, 3.7 TB/s instead of 4.1 over a long cache; NT, the lines not kept in L2: 5.2 (loads alone).
+template <int D, bool NT, typename ST>
+__device__ __forceinline__ void aw_load(const AwParams& p, const AwPages& at, int l0, v4i (&raw)[4][D / 64], ST& scale) {
+  constexpr int GR = D / 16, NI = D / 64;
+  const int lane = lane_id(), r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const rsrc_t rs = make_rsrc(p.kc + aw_lane64(at.kv, l0 + s), kOOB);
+    const uint32_t off = oob_unless((at.ok >> (l0 + s)) & 1, (uint32_t)(lane / GR * (int)p.s_ko + 16 * (lane % GR)));
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      raw[s][i] = __builtin_amdgcn_raw_buffer_load_b128(rs, off, i * (64 / GR) * (int)p.s_ko, NT ? 2 : 0);
+  }
+  const int64_t sc = (int64_t)(((uint64_t)(uint32_t)__shfl((int)(uint32_t)((uint64_t)at.sc >> 32), l0 + g) << 32) |
+                               (uint32_t)__shfl((int)(uint32_t)at.sc, l0 + g));
+  scale = static_cast<const ST*>(p.ks)[sc + r * p.s_so];
+}
+
+// A wave's codes change hands through LDS: granule q of token T lies in slot q ^ key(T) of its row, so that neither side's
+// accesses meet in a bank.
+template <int D>
+struct AwStage {
+  v4i x[4][16][D / 16];
+  static __device__ __forceinline__ int key(int t) { return D == 128 ? t & 7 : (t >> 1) & 3; }
+  __device__ __forceinline__ void put(const v4i (&raw)[4][D / 64]) {
+    constexpr int GR = D / 16;
+    const int lane = lane_id();
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        const int t = i * (64 / GR) + lane / GR;
+        x[s][t][(lane % GR) ^ key(t)] = raw[s][i];
+      }
+  }
+  // fp16 operands of sub-tile s.  Values of matrix step u = 2 i + half: d = 64 i + 16 g + 8 half + j, for K and Q alike.
+  __device__ __forceinline__ void get(int s, v8h (&kh)[D / 32]) const {
+    const int r = lane_id() & 15, g = lane_id() >> 4;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const v4i v = x[s][r][(4 * i + g) ^ key(r)];
+      kh[2 * i] = i8x8_to_h8((uint32_t)v[0], (uint32_t)v[1]);
+      kh[2 * i + 1] = i8x8_to_h8((uint32_t)v[2], (uint32_t)v[3]);
+    }
+  }
+};
+
+// The products' scales, and -inf where the lane's row does not see the token (`all`: every row sees all).
+__device__ __forceinline__ void aw_mask(const v4f (&ksc)[4], int t0, int last, bool all, uint32_t seen, v4f (&acc)[4]) {
+  const int g = lane_id() >> 4;
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[s][i] *= ksc[s][i];
+  if (all) return;
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!(((seen >> s) & 1) && t0 + 16 * s + 4 * g + i <= last)) acc[s][i] = -INFINITY;
+}
+// Scores (in log2) of the wave's tokens with the row of lane % 16.
+template <int D>
+__device__ __forceinline__ void aw_scores(const v8h (&kh)[4][D / 32], const v8h (&qf)[D / 32], const v4f (&ksc)[4], int t0, int last,
+                                          bool all, uint32_t seen, v4f (&acc)[4]) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    acc[s] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < D / 32; ++u) acc[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[s][u], qf[u], acc[s], 0, 0, 0);
+  }
+  aw_mask(ksc, t0, last, all, seen, acc);
+}
+// (max, sum) of a row over the wave's tokens, in all lanes of the row.
+__device__ __forceinline__ uint64_t aw_stat(const v4f (&acc)[4]) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, acc[s][i]);
+  m = aw_max4(m);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l += fast_exp2(acc[s][i] - ref);
+  return aw_pack(m, aw_sum4(l));
+}
+// The rows' sums over the lanes, and the update: lanes 0..3 of each 16 have four tokens each.
+__device__ __forceinline__ void aw_finish(const AwParams& p, const AwProg& x, int t0, const v4f (&sums)[4]) {
+  const int r = lane_id() & 15, g = lane_id() >> 4;
+  v4f got = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float v = aw_sum16(sums[s][i]);
+      got[i] = r == s ? v : got[i];
+    }
+  if (r < 4 && t0 + 16 * r + 4 * g < x.L) aw_update(p, x, t0 + 16 * r + 4 * g, got);
+}
+// The last workgroup of a program joins its rows' tiles: many rows a thread each, few a group of lanes each (as many as
+// there are tiles, at most a wave).
+__device__ __forceinline__ void aw_lse(const AwParams& p, const AwProg& x, int prog) {
+  const int threads = blockDim.x;
+  const uint64_t* st = p.stats + (int64_t)prog * p.tiles * p.rows;
+  float* out = p.lse + (int64_t)prog * p.rows;
+  auto done = [&](int row, float m, float l) { out[row] = m == -INFINITY ? INFINITY : m + __builtin_amdgcn_logf(l); };
+  // Tiles k0, k0 + step, ...: eight loads in flight.
+  auto walk = [&](int row, int k0, int step, float& m, float& l) {
+    constexpr int U = 8;
+    for (int k = k0; k < x.tiles; k += U * step) {
+      uint64_t v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = k + u * step < x.tiles ? collect(st + (int64_t)(k + u * step) * p.rows + row) : aw_pack(-INFINITY, 0.f);
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) top = fmaxf(top, aw_m(v[u]));
+      const float ref = top == -INFINITY ? 0.f : top;
+      l *= fast_exp2(m - ref);
+#pragma unroll
+      for (int u = 0; u < U; ++u) l += aw_l(v[u]) * fast_exp2(aw_m(v[u]) - ref);
+      m = top;
+    }
+  };
+  if (x.rows > kAwFewRows) {
+    for (int row = threadIdx.x; row < x.rows; row += threads) {
+      float m = -INFINITY, l = 0.f;
+      walk(row, 0, 1, m, l);
+      done(row, m, l);
+    }
+    return;
+  }
+  int lanes = 1;
+  while (lanes < x.tiles && lanes < kWave) lanes *= 2;
+  for (int i = threadIdx.x; i / kWave * kWave < x.rows * lanes; i += threads) {  // whole waves
+    const int row = min(i / lanes, x.rows - 1);
+    float m = -INFINITY, l = 0.f;
+    walk(row, i % lanes, lanes, m, l);
+    float top = m;
+    for (int o = 1; o < lanes; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+    l *= fast_exp2(m - (top == -INFINITY ? 0.f : top));
+    for (int o = 1; o < lanes; o *= 2) l += __shfl_xor(l, o);
+    if (i % lanes == 0 && i / lanes < x.rows) done(row, top, l);
+  }
+}
+
+// The statistics of a workgroup's tiles, each of its four waves' joined.
+template <int ROWS, int N>
+__device__ __forceinline__ void aw_publish(const AwParams& p, const AwProg& x, int prog, int tile0, int tile1,
+                                           const uint64_t (&st)[N][4][ROWS]) {
+  const int n = (tile1 - tile0) * x.rows;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int tile = i / x.rows, row = i - tile * x.rows;
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) aw_join(m, l, aw_m(st[tile][v][row]), aw_l(st[tile][v][row]));
+    publish(p.stats + ((int64_t)prog * p.tiles + tile0 + tile) * p.rows + row, aw_pack(m, l));
+  }
+}
+
+// Up to 64 rows.  A workgroup walks `span` tiles of a program, a wave 64 tokens of each, with the next tile's codes on
+// their way while one is multiplied; all rows' queries wait in LDS.
 template <int D, typename ST, int MODE>
-__global__ __launch_bounds__(256) void aw_tile_kernel(AwParams p) {
-  constexpr int NU = D / 32;  // matrix steps over the head dimension
-  constexpr int NI = D / 64;  // 16-byte loads of a lane's token
-  constexpr int NB = 4;       // sub-tiles of 16 tokens of a wave
+__global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
+  constexpr int NU = D / 32, RB = kAwFewRows / 16;
+  __shared__ v8h s_q[RB][NU][64];
+  __shared__ AwStage<D> s_k[4];
   __shared__ float s_scale[4][64];
-  __shared__ uint64_t s_stat[MODE == kAwSums ? 1 : 4][MODE == kAwSums ? 1 : kAwSeg * 16];
+  __shared__ uint64_t s_stat[MODE == kAwSums ? 1 : kAwSpan][4][MODE == kAwSums ? 1 : kAwFewRows];
   __shared__ int s_last;
   const int lane = lane_id(), w = uniform(wave_id()), r = lane & 15, g = lane >> 4;
+  const int progs = p.B_grid * p.H_KV, spans = (p.tiles + p.span - 1) / p.span;
+  for (int64_t item = blockIdx.x; item < (int64_t)progs * spans; item += gridDim.x) {
+    const int tile0 = (int)(item / progs) * p.span, prog = aw_order(p, (int)(item % progs));
+    // The wave's sub-tile `lane` and its page, whose load does not wait for the context's length.
+    const int sub_t = (tile0 + lane / 4) * kAwTile + 64 * w + 16 * (lane & 3);
+    int page = -1;
+    if (lane < 4 * p.span && sub_t < p.cap) page = p.bt[(int64_t)(prog / p.H_KV) * p.s_bt + sub_t / p.PAGE];
+    AwProg x;
+    if (!aw_prog(p, prog, x) || tile0 >= x.tiles) continue;
+    const int blocks = (x.rows + 15) / 16, tile1 = min(tile0 + p.span, x.tiles);
+    __syncthreads();  // the last item's queries have been read
+    for (int f = threadIdx.x; f < blocks * NU * 64; f += 256) {
+      const int l = f % 64, u = (f / 64) % NU, row = min(f / (64 * NU) * 16 + (l & 15), x.rows - 1);
+      const int qi = aw_token(p, row), head = x.h * p.G + row - qi * p.G;
+      s_q[0][0][f] = *reinterpret_cast<const v8h*>(p.q + x.b * p.s_qb + qi * p.s_qt + head * p.s_qh + 64 * (u / 2) + 16 * (l >> 4) +
+                                                   8 * (u & 1));
+    }
+    const int fresh = x.L - x.ql;  // a row of new token i sees t <= fresh + i
+    const AwPages at = aw_pages(p, x, sub_t, page, lane < 4 * p.span);
+    v4i raw[4][D / 64];
+    ST scale;
+    aw_load<D, false, ST>(p, at, 0, raw, scale);
+    float lse[MODE == kAwSums ? RB : 1];
+    if constexpr (MODE == kAwSums) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        lse[rb] = INFINITY;
+        if (rb * 16 + r < x.rows) lse[rb] = p.lse[(int64_t)prog * p.rows + rb * 16 + r];
+      }
+    }
+    __syncthreads();
+    for (int tile = tile0; tile < tile1; ++tile) {
+      const int t0 = tile * kAwTile + 64 * w;
+      const uint32_t seen = (uint32_t)(at.ok >> (4 * (tile - tile0))) & 0xf;
+      // Lane (r, g) holds the scale of token t0 + 16 g + r; it needs those of tokens 16 s + 4 g + i.
+      s_k[w].put(raw);
+      s_scale[w][lane] = (float)scale * p.scale_log2;
+      aw_load<D, false, ST>(p, at, 4 * (tile + 1 - tile0), raw, scale);
+      wait_lgkm0();
+      v8h kh[4][NU];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) s_k[w].get(s, kh[s]);
+      v4f ksc[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) ksc[s] = *reinterpret_cast<const v4f*>(&s_scale[w][16 * s + 4 * g]);
+      v4f even[4], odd[4];  // sums over the blocks of either parity
+#pragma unroll
+      for (int s = 0; s < 4; ++s) even[s] = odd[s] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        if (rb >= blocks) break;
+        const int row = rb * 16 + r;
+        v8h qf[NU];
+#pragma unroll
+        for (int u = 0; u < NU; ++u) qf[u] = s_q[rb][u][lane];
+        v4f acc[4];
+        aw_scores<D>(kh, qf, ksc, t0, row < x.rows ? fresh + aw_token(p, row) : -1,
+                     t0 + 63 <= fresh && seen == 0xf && rb * 16 + 16 <= x.rows, seen, acc);
+        if constexpr (MODE == kAwSums) {
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) (rb & 1 ? odd : even)[s][i] += fast_exp2(acc[s][i] - lse[rb]);
+        } else {
+          const uint64_t st = aw_stat(acc);
+          if (g == 0) s_stat[tile - tile0][w][row] = st;
+        }
+      }
+      if constexpr (MODE == kAwSums) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) even[s] += odd[s];
+        aw_finish(p, x, t0, even);
+      }
+    }
+    if constexpr (MODE != kAwSums) {
+      __syncthreads();
+      aw_publish(p, x, prog, tile0, tile1, s_stat);
+      if (arrive_last(p.counters + prog, (x.tiles + p.span - 1) / p.span, &s_last)) aw_lse(p, x, prog);
+    }
+  }
+}
+
+// Up to 16 rows, whose scores are stored: one block of rows, so a sub-tile's operands are made where they are used and two
+// tiles' codes fit the registers.
+template <int D, typename ST>
+__global__ __launch_bounds__(256) void aw_store_kernel(AwParams p) {
+  constexpr int NU = D / 32;
+  constexpr bool kOnce = D == 128;  // nothing reads the lines again; at D = 64 the next head does
+  __shared__ AwStage<D> s_k[4];
+  __shared__ float s_scale[4][64];
+  __shared__ uint64_t s_stat[kAwSpan][4][16];
+  __shared__ int s_last;
+  const int lane = lane_id(), w = uniform(wave_id()), r = lane & 15, g = lane >> 4;
+  const int progs = p.B_grid * p.H_KV, spans = (p.tiles + p.span - 1) / p.span;
+  for (int64_t item = blockIdx.x; item < (int64_t)progs * spans; item += gridDim.x) {
+    const int tile0 = (int)(item / progs) * p.span, prog = aw_order(p, (int)(item % progs));
+    const int sub_t = (tile0 + lane / 4) * kAwTile + 64 * w + 16 * (lane & 3);
+    int page = -1;
+    if (lane < 4 * p.span && sub_t < p.cap) page = p.bt[(int64_t)(prog / p.H_KV) * p.s_bt + sub_t / p.PAGE];
+    AwProg x;
+    if (!aw_prog(p, prog, x) || tile0 >= x.tiles) continue;
+    const int tile1 = min(tile0 + p.span, x.tiles), fresh = x.L - x.ql;
+    v8h qf[NU];
+    {
+      const int row = min(r, x.rows - 1), qi = aw_token(p, row), head = x.h * p.G + row - qi * p.G;
+      const _Float16* src = p.q + x.b * p.s_qb + qi * p.s_qt + head * p.s_qh + 16 * g;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) qf[u] = *reinterpret_cast<const v8h*>(src + 64 * (u / 2) + 8 * (u & 1));
+    }
+    const int last = r < x.rows ? fresh + aw_token(p, r) : -1;  // the last token the lane's row sees
+    const AwPages at = aw_pages(p, x, sub_t, page, lane < 4 * p.span);
+    const rsrc_t out = make_rsrc(p.scores + (int64_t)prog * p.rows * p.tiles * kAwTile, kOOB);
+    const uint32_t out_row = oob_unless(r < x.rows, (uint32_t)(r * p.tiles * kAwTile + 4 * g) * 4);
+    auto work = [&](int tile, const v4i (&raw)[4][D / 64], ST scale) {
+      const int t0 = tile * kAwTile + 64 * w;
+      const uint32_t seen = (uint32_t)(at.ok >> (4 * (tile - tile0))) & 0xf;
+      s_k[w].put(raw);
+      s_scale[w][lane] = (float)scale * p.scale_log2;
+      wait_lgkm0();
+      v4f acc[4], ksc[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        v8h kh[NU];
+        s_k[w].get(s, kh);
+        acc[s] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < NU; ++u) acc[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[u], qf[u], acc[s], 0, 0, 0);
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s) ksc[s] = *reinterpret_cast<const v4f*>(&s_scale[w][16 * s + 4 * g]);
+      aw_mask(ksc, t0, last, t0 + 63 <= fresh && seen == 0xf && x.rows == 16, seen, acc);
+      // Always the same stores, too; those of tokens behind the context lie in the row's last tile.
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, acc[s]), out, out_row + 4u * (uint32_t)(t0 + 16 * s), 0, 0);
+      const uint64_t st = aw_stat(acc);
+      if (g == 0) s_stat[tile - tile0][w][r] = st;
+    };
+    v4i raw0[4][D / 64], raw1[4][D / 64];
+    ST scale0, scale1;
+    aw_load<D, kOnce, ST>(p, at, 0, raw0, scale0);
+    for (int tile = tile0; tile < tile1; tile += 2) {
+      aw_load<D, kOnce, ST>(p, at, 4 * (tile + 1 - tile0), raw1, scale1);
+      work(tile, raw0, scale0);
+      if (tile + 1 >= tile1) break;
+      aw_load<D, kOnce, ST>(p, at, 4 * (tile + 2 - tile0), raw0, scale0);
+      work(tile + 1, raw1, scale1);
+    }
+    __syncthreads();
+    aw_publish(p, x, prog, tile0, tile1, s_stat);
+    if (arrive_last(p.counters + prog, (x.tiles + p.span - 1) / p.span, &s_last)) aw_lse(p, x, prog);
+  }
+}
+
+// More rows: a workgroup owns a tile, its waves 64 tokens and the row blocks of one parity each.
+template <int D, typename ST, int MODE>
+__global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
+  constexpr int NU = D / 32;
+  __shared__ AwStage<D> s_k[8];
+  __shared__ float s_scale[8][64];
+  __shared__ uint64_t s_stat[MODE == kAwSums ? 1 : 4][MODE == kAwSums ? 1 : kAwSeg * 16];
+  __shared__ v4f s_sums[MODE == kAwSums ? 4 : 1][4][64];
+  __shared__ int s_last;
+  const int lane = lane_id(), w = uniform(wave_id()) & 3, odd = uniform(wave_id()) >> 2, r = lane & 15, g = lane >> 4;
   const int progs = p.B_grid * p.H_KV;
   for (int64_t item = blockIdx.x; item < (int64_t)progs * p.tiles; item += gridDim.x) {
-    const int tile = (int)(item / progs), prog = (int)(item - (int64_t)tile * progs);
+    const int tile = (int)(item / progs), prog = aw_order(p, (int)(item % progs)), t0 = tile * kAwTile + 64 * w;
     AwProg x;
     if (!aw_prog(p, prog, x) || tile >= x.tiles) continue;
-    const int t0 = tile * kAwTile + 64 * w;  // the wave's first token
-    // Codes and scales.  A sub-tile lies in one page; one past the context or on no page reads nothing and is not seen.
-    v4i raw[NB][NI];
-    uint32_t seen_sub = 0;
-    float scale = 0.f;
-#pragma unroll
-    for (int s = 0; s < NB; ++s) {
-      const int t = t0 + 16 * s;
-#pragma unroll
-      for (int i = 0; i < NI; ++i) raw[s][i] = v4i{0, 0, 0, 0};
-      if (t >= x.L) continue;
-      const int page = uniform(p.bt[x.b * p.s_bt + t / p.PAGE]), slot = t % p.PAGE;
-      if ((uint32_t)page >= (uint32_t)p.n_pages) continue;
-      seen_sub |= 1u << s;
-      const int8_t* src = p.kc + page * p.s_kp + (int64_t)(slot + r) * p.s_ko + x.h * p.s_kh + 16 * g;
-#pragma unroll
-      for (int i = 0; i < NI; ++i) raw[s][i] = *reinterpret_cast<const v4i*>(src + 64 * i);
-      if (g == s)
-        scale = (float)static_cast<const ST*>(p.ks)[page * p.s_sp + (int64_t)(slot + r) * p.s_so + x.h * p.s_sh];
-    }
-    // Lane (r, g) holds the scale of token t0 + 16 g + r; it needs those of tokens 16 s + 4 g + i.
-    s_scale[w][lane] = scale * p.scale_log2;
+    const int sub_t = t0 + 16 * (lane & 3);
+    const AwPages at = aw_pages(p, x, sub_t, sub_t < x.L ? p.bt[x.b * p.s_bt + sub_t / p.PAGE] : -1, lane < 4);
+    const uint32_t seen = (uint32_t)at.ok;
+    v4i raw[4][D / 64];
+    ST scale;
+    aw_load<D, false, ST>(p, at, 0, raw, scale);
+    s_k[4 * odd + w].put(raw);
+    s_scale[4 * odd + w][lane] = (float)scale * p.scale_log2;
     wait_lgkm0();
-    v4f ksc[NB];
+    v8h kh[4][NU];
 #pragma unroll
-    for (int s = 0; s < NB; ++s) ksc[s] = *reinterpret_cast<const v4f*>(&s_scale[w][16 * s + 4 * g]);
-    // Operand bytes of matrix step u = 2 i + half: d = 64 i + 16 g + 8 half + j, for K and Q alike.
-    v8h kh[NB][NU];
+    for (int s = 0; s < 4; ++s) s_k[4 * odd + w].get(s, kh[s]);
+    v4f ksc[4];
 #pragma unroll
-    for (int s = 0; s < NB; ++s)
+    for (int s = 0; s < 4; ++s) ksc[s] = *reinterpret_cast<const v4f*>(&s_scale[4 * odd + w][16 * s + 4 * g]);
+    const int fresh = x.L - x.ql, blocks = (x.rows + 15) / 16;
+    v4f sums[4];
 #pragma unroll
-      for (int u = 0; u < NU; ++u)
-        kh[s][u] = i8x8_to_h8((uint32_t)raw[s][u / 2][2 * (u & 1)], (uint32_t)raw[s][u / 2][2 * (u & 1) + 1]);
-
-    const int fresh = x.L - x.ql;  // a row of new token i sees t <= fresh + i
-    const int blocks = (x.rows + 15) / 16;
-    v4f sums[NB];
-#pragma unroll
-    for (int s = 0; s < NB; ++s) sums[s] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < 4; ++s) sums[s] = v4f{0.f, 0.f, 0.f, 0.f};
     auto load_q = [&](int rb, v8h (&qf)[NU]) {
-      const int row = min(rb * 16 + r, x.rows - 1), qi = row / p.G, head = x.h * p.G + row - qi * p.G;
+      const int row = min(rb * 16 + r, x.rows - 1), qi = aw_token(p, row), head = x.h * p.G + row - qi * p.G;
       const _Float16* src = p.q + x.b * p.s_qb + qi * p.s_qt + head * p.s_qh + 16 * g;
 #pragma unroll
       for (int u = 0; u < NU; ++u) qf[u] = *reinterpret_cast<const v8h*>(src + 64 * (u / 2) + 8 * (u & 1));
     };
-    // The first block with a row that sees the wave's first token.
-    const int first = t0 > fresh ? min((t0 - fresh) * p.G / 16, blocks) : 0;
+    // The first block with a row that sees the wave's first token, none where the wave sees nothing.
+    const int first = seen == 0 ? blocks : t0 > fresh ? min((t0 - fresh) * p.G / 16, blocks) : 0;
     for (int seg = 0; seg < blocks; seg += kAwSeg) {
       const int seg_end = min(seg + kAwSeg, blocks);
-      for (int rb = seg; rb < seg_end; ++rb) {
-        const int row = rb * 16 + r;
-        if (seen_sub == 0 || rb < first) {
-          if constexpr (MODE != kAwSums)
-            if (g == 0) s_stat[w][row - seg * 16] = aw_pack(-INFINITY, 0.f);
-          if constexpr (MODE == kAwScores) {
+      if constexpr (MODE != kAwSums)
+        for (int rb = seg + odd; rb < min(first, seg_end); rb += 2)
+          if (g == 0) s_stat[w][(rb - seg) * 16 + r] = aw_pack(-INFINITY, 0.f);
+      int rb = max(seg, first);
+      rb += (rb ^ odd) & 1;
+      // Two blocks at a time, and the next two's queries on their way.
+      v8h next[2][NU];
+      float next_lse[2];
+      auto fetch = [&](int rb) {
 #pragma unroll
-            for (int s = 0; s < NB; ++s)
-              if (row < x.rows && t0 + 16 * s < x.L)
-                *reinterpret_cast<v4f*>(p.scores + ((int64_t)prog * p.rows + row) * p.tiles * kAwTile + t0 + 16 * s + 4 * g) =
-                    v4f{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          }
-          continue;
+        for (int k = 0; k < 2; ++k) {
+          load_q(rb + 2 * k, next[k]);
+          if constexpr (MODE == kAwSums) next_lse[k] = p.lse[(int64_t)prog * p.rows + min((rb + 2 * k) * 16 + r, x.rows - 1)];
         }
-        v8h qf[NU];
-        load_q(rb, qf);
-        float lse = INFINITY;
-        if constexpr (MODE == kAwSums)
-          if (row < x.rows) lse = p.lse[(int64_t)prog * p.rows + row];
-        v4f acc[NB];
+      };
+      if (rb < seg_end) fetch(rb);
+      for (; rb < seg_end; rb += 4) {
+        v8h qf[2][NU];
+        float lse[2] = {INFINITY, INFINITY};
 #pragma unroll
-        for (int s = 0; s < NB; ++s) {
-          acc[s] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < 2; ++k) {
 #pragma unroll
-          for (int u = 0; u < NU; ++u) acc[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[s][u], qf[u], acc[s], 0, 0, 0);
+          for (int u = 0; u < NU; ++u) qf[k][u] = next[k][u];
+          if constexpr (MODE == kAwSums) lse[k] = next_lse[k];
         }
-        const int last = row < x.rows ? fresh + row / p.G : -1;  // the last token the lane's row sees
-        const bool all = t0 + 63 <= fresh && seen_sub == 0xf && rb * 16 + 16 <= x.rows;
+        fetch(rb + 4);
+        v4f acc[2][4];
 #pragma unroll
-        for (int s = 0; s < NB; ++s)
+        for (int k = 0; k < 2; ++k) {
+          const int row = (rb + 2 * k) * 16 + r;  // rows past the last see nothing
+          aw_scores<D>(kh, qf[k], ksc, t0, row < x.rows ? fresh + aw_token(p, row) : -1,
+                       t0 + 63 <= fresh && seen == 0xf && (rb + 2 * k) * 16 + 16 <= x.rows, seen, acc[k]);
+        }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            acc[s][i] *= ksc[s][i];
-            if (!all && !(((seen_sub >> s) & 1) && t0 + 16 * s + 4 * g + i <= last)) acc[s][i] = -INFINITY;
+        for (int k = 0; k < 2; ++k) {
+          if constexpr (MODE == kAwSums) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sums[s][i] += fast_exp2(acc[k][s][i] - lse[k]);
+          } else {
+            const uint64_t st = aw_stat(acc[k]);
+            if (g == 0 && rb + 2 * k < seg_end) s_stat[w][(rb + 2 * k - seg) * 16 + r] = st;
           }
-        if constexpr (MODE == kAwSums) {
-#pragma unroll
-          for (int s = 0; s < NB; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sums[s][i] += fast_exp2(acc[s][i] - lse);
-        } else {
-          if constexpr (MODE == kAwScores) {
-#pragma unroll
-            for (int s = 0; s < NB; ++s)
-              if (row < x.rows && t0 + 16 * s < x.L)
-                *reinterpret_cast<v4f*>(p.scores + ((int64_t)prog * p.rows + row) * p.tiles * kAwTile + t0 + 16 * s + 4 * g) =
-                    acc[s];
-          }
-          float m = -INFINITY;
-#pragma unroll
-          for (int s = 0; s < NB; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) m = fmaxf(m, acc[s][i]);
-          m = aw_max4(m);
-          const float ref = m == -INFINITY ? 0.f : m;
-          float l = 0.f;
-#pragma unroll
-          for (int s = 0; s < NB; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) l += fast_exp2(acc[s][i] - ref);
-          l = aw_sum4(l);
-          if (g == 0) s_stat[w][row - seg * 16] = aw_pack(m, l);
         }
       }
       if constexpr (MODE != kAwSums) {
         __syncthreads();
         const int n = min((seg_end - seg) * 16, x.rows - seg * 16);
-        for (int i = threadIdx.x; i < n; i += 256) {
+        for (int i = threadIdx.x; i < n; i += 512) {
           float m = -INFINITY, l = 0.f;
 #pragma unroll
           for (int v = 0; v < 4; ++v) aw_join(m, l, aw_m(s_stat[v][i]), aw_l(s_stat[v][i]));
@@ -262,44 +586,19 @@ __global__ __launch_bounds__(256) void aw_tile_kernel(AwParams p) {
       }
     }
     if constexpr (MODE == kAwSums) {
-      // Lanes 0..3 of each 16 update four tokens each.
-      v4f got = {0.f, 0.f, 0.f, 0.f};
+      if (odd) {
 #pragma unroll
-      for (int s = 0; s < NB; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float v = aw_sum16(sums[s][i]);
-          got[i] = r == s ? v : got[i];
-        }
-      if (r < NB && t0 + 16 * r + 4 * g < x.L) aw_update(p, x, t0 + 16 * r + 4 * g, got);
-    } else if (arrive_last(p.counters + prog, x.tiles, &s_last)) {
-      // The rows' tiles joined: many rows a thread each, few a wave each.
-      const uint64_t* st = p.stats + (int64_t)prog * p.tiles * p.rows;
-      float* out = p.lse + (int64_t)prog * p.rows;
-      auto done = [&](int row, float m, float l) { out[row] = m == -INFINITY ? INFINITY : m + __builtin_amdgcn_logf(l); };
-      if (x.rows >= 64) {
-        for (int row = threadIdx.x; row < x.rows; row += 256) {
-          float m = -INFINITY, l = 0.f;
-#pragma unroll 4
-          for (int k = 0; k < x.tiles; ++k) {
-            const uint64_t v = collect(st + (int64_t)k * p.rows + row);
-            aw_join(m, l, aw_m(v), aw_l(v));
-          }
-          done(row, m, l);
-        }
-      } else {
-        for (int row = w; row < x.rows; row += 4) {
-          float m = -INFINITY, l = 0.f;
-#pragma unroll 4
-          for (int k = lane; k < x.tiles; k += kWave) {
-            const uint64_t v = collect(st + (int64_t)k * p.rows + row);
-            aw_join(m, l, aw_m(v), aw_l(v));
-          }
-#pragma unroll
-          for (int o = 1; o < kWave; o *= 2) aw_join(m, l, __shfl_xor(m, o), __shfl_xor(l, o));
-          if (lane == 0) done(row, m, l);
-        }
+        for (int s = 0; s < 4; ++s) s_sums[w][s][lane] = sums[s];
       }
+      __syncthreads();
+      if (!odd) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) sums[s] += s_sums[w][s][lane];
+        aw_finish(p, x, t0, sums);
+      }
+      __syncthreads();
+    } else if (arrive_last(p.counters + prog, x.tiles, &s_last)) {
+      aw_lse(p, x, prog);
     }
   }
 }
@@ -337,15 +636,31 @@ __global__ __launch_bounds__(256) void aw_sum_kernel(AwParams p) {
   }
 }
 
-template <int D, int MODE>
-static const void* aw_tile_fn(bool f32) {
-  return f32 ? reinterpret_cast<const void*>(&aw_tile_kernel<D, float, MODE>)
-             : reinterpret_cast<const void*>(&aw_tile_kernel<D, _Float16, MODE>);
+template <int MODE>
+static const void* aw_fn(int D, bool f32, bool few) {
+  if (D == 64) {
+    if (f32) return few ? reinterpret_cast<const void*>(&aw_few_kernel<64, float, MODE>)
+                        : reinterpret_cast<const void*>(&aw_many_kernel<64, float, MODE>);
+    return few ? reinterpret_cast<const void*>(&aw_few_kernel<64, _Float16, MODE>)
+               : reinterpret_cast<const void*>(&aw_many_kernel<64, _Float16, MODE>);
+  }
+  if (f32) return few ? reinterpret_cast<const void*>(&aw_few_kernel<128, float, MODE>)
+                      : reinterpret_cast<const void*>(&aw_many_kernel<128, float, MODE>);
+  return few ? reinterpret_cast<const void*>(&aw_few_kernel<128, _Float16, MODE>)
+             : reinterpret_cast<const void*>(&aw_many_kernel<128, _Float16, MODE>);
+}
+static const void* aw_store_fn(int D, bool f32) {
+  if (D == 64) return f32 ? reinterpret_cast<const void*>(&aw_store_kernel<64, float>)
+                          : reinterpret_cast<const void*>(&aw_store_kernel<64, _Float16>);
+  return f32 ? reinterpret_cast<const void*>(&aw_store_kernel<128, float>)
+             : reinterpret_cast<const void*>(&aw_store_kernel<128, _Float16>);
 }
 
+// Stored scores lie within a buffer's offsets.
+static bool aw_stores(int64_t rows, int64_t tiles) { return rows <= kAwStoreRows && tiles <= (1 << 16); }
 struct AwSpace { size_t scores, stats, lse; };  // bytes
 static AwSpace aw_space(int64_t progs, int64_t rows, int64_t tiles) {
-  return {rows <= kAwStoreRows ? align_up((size_t)(progs * rows * tiles * kAwTile * 4), 256) : 0,
+  return {aw_stores(rows, tiles) ? align_up((size_t)(progs * rows * tiles * kAwTile * 4), 256) : 0,
           align_up((size_t)(progs * tiles * rows * 8), 256), align_up((size_t)(progs * rows * 4), 256)};
 }
 
@@ -379,6 +694,7 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   SPECQ_REQUIRE(PAGE % 16 == 0, SPECQ_ENOTSUP, "paged_attn_weights: PAGE %d must be a multiple of 16", PAGE);
   const int64_t cap = (int64_t)max_pages * PAGE, progs = (int64_t)B_grid * H_KV, rows = (int64_t)ql_grid * (H / H_KV);
   SPECQ_REQUIRE(cap <= (1 << 30), SPECQ_ENOTSUP, "paged_attn_weights: a table of %lld tokens is too long", (long long)cap);
+  SPECQ_REQUIRE(H / H_KV < 4096, SPECQ_ENOTSUP, "paged_attn_weights: %d query heads to a KV head", H / H_KV);
   SPECQ_REQUIRE(rows <= (1 << 20) && ql_grid <= (1 << 20), SPECQ_ENOTSUP, "paged_attn_weights: too many query rows");
   SPECQ_REQUIRE(progs <= kMaxCounters, SPECQ_ENOTSUP, "paged_attn_weights: more than %lld sequences x KV heads",
                 (long long)kMaxCounters);
@@ -386,6 +702,7 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
                 "paged_attn_weights: q rows must be 16-byte aligned");
   SPECQ_REQUIRE((uintptr_t)kc % 16 == 0 && s_kp % 16 == 0 && s_ko % 16 == 0 && s_kh % 16 == 0, SPECQ_ENOTSUP,
                 "paged_attn_weights: cache rows must be 16-byte aligned");
+  SPECQ_REQUIRE(s_ko < (1ll << 27) && s_ko >= 0, SPECQ_ENOTSUP, "paged_attn_weights: tokens %lld bytes apart", (long long)s_ko);
   SPECQ_REQUIRE((uintptr_t)ks % (scale_fp32 ? 4 : 2) == 0 && (uintptr_t)weights % 4 == 0, SPECQ_EINVAL,
                 "paged_attn_weights: scales and weights must be aligned to their type");
   SPECQ_REQUIRE(lie_apart(B_grid, s_wb, cap) && lie_apart(H_KV, s_wh, cap), SPECQ_ENOTSUP,
@@ -400,7 +717,8 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   p.w = weights; p.s_wb = s_wb; p.s_wh = s_wh;
   p.w_vec = (uintptr_t)weights % 16 == 0 && s_wb % 4 == 0 && s_wh % 4 == 0;
   p.plan = plan; p.n_seqs = n_seqs; p.q_len = q_len; p.B_grid = B_grid; p.ql_grid = ql_grid;
-  p.G = H / H_KV; p.H_KV = H_KV; p.PAGE = PAGE;
+  p.G = H / H_KV; p.g_magic = p.G > 1 ? (uint32_t)(((1ull << 32) + p.G - 1) / p.G) : 0;
+  p.H_KV = H_KV; p.PAGE = PAGE;
   p.cap = (int)cap; p.tiles = (int)ceil_div64(cap, kAwTile); p.rows = (int)rows;
   p.scale_log2 = sm_scale * 1.44269504088896340736f;
   const AwSpace space = aw_space(progs, rows, p.tiles);
@@ -412,14 +730,16 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   p.scores = reinterpret_cast<float*>(at + kCounterBytes);
   p.stats = reinterpret_cast<uint64_t*>(at + kCounterBytes + space.scores);
   p.lse = reinterpret_cast<float*>(at + kCounterBytes + space.scores + space.stats);
-  const bool store = rows <= kAwStoreRows, f32 = scale_fp32 != 0;
-  const int64_t items = progs * p.tiles, sums = progs * ceil_div64(cap, kAwSumTile);
-  const int grid = (int)(items < kAwMaxGrid ? items : kAwMaxGrid);
-  const void* one = D == 64 ? (store ? aw_tile_fn<64, kAwScores>(f32) : aw_tile_fn<64, kAwStats>(f32))
-                            : (store ? aw_tile_fn<128, kAwScores>(f32) : aw_tile_fn<128, kAwStats>(f32));
-  if (int rc = launch(one, grid, 256, 0, (hipStream_t)stream, &p)) return rc;
+  const bool store = aw_stores(rows, p.tiles), few = rows <= kAwFewRows, f32 = scale_fp32 != 0;
+  // Tiles of a workgroup of few rows: as many as leave two workgroups to a CU.
+  const int64_t tiles = progs * p.tiles, span = tiles / (2 * device_cus());
+  p.span = few ? (int)(span < 1 ? 1 : span > kAwSpan ? kAwSpan : span) : 1;
+  const int64_t items = progs * ceil_div(p.tiles, p.span), sums = progs * ceil_div64(cap, kAwSumTile);
+  const int grid = (int)(items < kAwMaxGrid ? items : kAwMaxGrid), threads = few ? 256 : 512;
+  if (int rc = launch(store ? aw_store_fn(D, f32) : aw_fn<kAwStats>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p))
+    return rc;
   if (store)
     return launch(reinterpret_cast<const void*>(&aw_sum_kernel), (int)(sums < kAwMaxGrid ? sums : kAwMaxGrid), 256, 0,
                   (hipStream_t)stream, &p);
-  return launch(D == 64 ? aw_tile_fn<64, kAwSums>(f32) : aw_tile_fn<128, kAwSums>(f32), grid, 256, 0, (hipStream_t)stream, &p);
+  return launch(aw_fn<kAwSums>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p);
 }
