@@ -5,14 +5,14 @@
 // and the best n of the W V candidates, ties to the lower beam, then the lower token.  A candidate whose score is NaN or
 // -infinity is none; where there are fewer than n the rest is (-inf, -1, -1).
 //
-// One pass over the logits, which is what bounds it.  A wave owns a segment of a row and keeps it in registers: its
-// maximum and sum of exponentials, and its candidates.  The n-th largest of the 64 lanes' maxima is a value that at least n
-// of the segment's reach, so what reaches it holds the segment's best n and few more; these go to the workspace, up to 64.
-// Where more reach it (rows of equal values) the best n are taken one by one.
-// The last workgroup of a sequence joins the segments: each row's sum, in fp64, then the candidates' scores, in fp64 too,
-// since beams whose scores lie closer than an fp32 step apart are to be told apart as the formula does; the same
-// two steps -- a value that n reach, then the few that do, ranked against one another -- give the selection.  Neither the
-// order of arrival nor that of the list has a part in the result.
+// One pass over the logits, which is what bounds it, and a second launch over what it leaves.
+//   1  A workgroup owns a part of a row and keeps it in registers: its maximum and sum of exponentials, and its
+//      candidates.  If k of the 64 lanes' maxima reach a value in each of the four waves, 4 k values of the part do; with k the
+//      fourth part of n, what reaches the least such value of a wave holds the part's best n and few more.  These are left
+//      for 2, at most kBeamSlots of them; where more reach it (equal values) the best n are taken one by one.
+//   2  A workgroup to a sequence joins each row's sums, in fp64, and forms the candidates' scores, in fp64 too, since
+//      beams whose scores lie closer than an fp32 step apart are to be told apart as the formula does.  Again a value that n
+//      reach, then the few that do, ranked against one another.  The order in which lists are filled has no part in the result.
 //
 // Reordering: row r of every state becomes row parents[r] of the same group of rows.  In place: a thread owns one column of
 // up to 16 bytes of a group's rows, reads what changes and then writes it.  Bound by HBM.
@@ -22,9 +22,12 @@
 namespace specq {
 
 constexpr int kBeamThreads = 256, kBeamWaves = kBeamThreads / kWave;
-constexpr int kBeamMax = 64;    // beams of a sequence, and candidates selected
-constexpr int kBeamSlots = 64;  // candidates of a segment
-constexpr int kBeamList = 768;  // candidates ranked against one another
+constexpr int kBeamJoin = 1024, kBeamJoinWaves = kBeamJoin / kWave;  // threads of the second launch
+constexpr int kBeamMax = 64;     // beams of a sequence, and candidates selected
+constexpr int kBeamSlots = 128;  // candidates of a part
+constexpr int kBeamList = 1024;  // candidates ranked against one another
+constexpr int kBeamGroup = 32;   // threads of the second launch that share a part
+constexpr int kBeamNear = 4;     // parts of a thread read ahead
 
 struct BeamParams {
   const void* x; int64_t s_xb, s_xw;
@@ -32,11 +35,9 @@ struct BeamParams {
   const uint8_t* done; int64_t s_db; int eos;
   float* out_score; int32_t* out_token; int32_t* out_parent;
   int W, V, n;
-  int segs;  // of a row
-  int wgs;   // of a sequence: ceil(W segs / 4)
-  // Workspace, of each segment: (max, sum), the number of candidates, and they: (value, token).
+  int parts;  // of a row
+  // Workspace, of each part: (max, sum), the number of candidates, and they: (value, token).
   uint64_t* stats; int32_t* counts; uint64_t* cands;
-  int32_t* counters;  // [B]
 };
 
 __device__ __forceinline__ uint64_t beam_pack(float a, uint32_t b) {
@@ -45,39 +46,51 @@ __device__ __forceinline__ uint64_t beam_pack(float a, uint32_t b) {
 __device__ __forceinline__ float beam_lo(uint64_t x) { return __builtin_bit_cast(float, (uint32_t)x); }
 __device__ __forceinline__ float beam_hi(uint64_t x) { return __builtin_bit_cast(float, (uint32_t)(x >> 32)); }
 
-// The n-th largest (1 <= n <= 64) of the lanes' values, no NaN among them: its key bit by bit.
-__device__ __forceinline__ float beam_nth(float v, int n) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, v), key = (u >> 31) ? ~u : u | 0x80000000u;
-  uint32_t at = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t up = at | (1u << bit);
-    if (__popcll(__builtin_amdgcn_ballot_w64(key >= up)) >= n) at = up;
+// Values that at least i and j (1..64) of the lanes' values reach, no NaN among them: the i-th and the j-th largest with the
+// lower half of their keys cut off (found bit by bit; all 32 would take twice the time and spare few candidates).
+struct BeamNth { float i, j; };
+__device__ __forceinline__ BeamNth beam_nth(float v, int i, int j) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v), key = ((u >> 31) ? ~u : u | 0x80000000u) >> 16;
+  uint32_t a = 0, b = 0;
+#pragma unroll 4
+  for (int bit = 15; bit >= 0; --bit) {
+    const uint32_t up_a = a | (1u << bit), up_b = b | (1u << bit);
+    if (__popcll(__builtin_amdgcn_ballot_w64(key >= up_a)) >= i) a = up_a;
+    if (__popcll(__builtin_amdgcn_ballot_w64(key >= up_b)) >= j) b = up_b;
   }
-  return __builtin_bit_cast(float, (at >> 31) ? at & 0x7FFFFFFFu : ~at);
+  // The least value of the key's upper half; that of -infinity's holds NaN as well, and is -infinity.
+  auto value = [](uint32_t k) {
+    return (k >> 15) ? __builtin_bit_cast(float, (k << 16) & 0x7FFFFFFFu) : k <= 0x007Fu ? -INFINITY : __builtin_bit_cast(float, ~(k << 16));
+  };
+  return {value(a), value(b)};
 }
 
 // Whether (a, i) comes before (b, j).
 template <typename T, typename I>
 __device__ __forceinline__ bool beam_before(T a, I i, T b, I j) { return a > b || (a == b && i < j); }
 
-// NV 16-byte vectors of a lane: the wave's segment is 64 NV of them.  They count from the row's start, wherever that lies (a
-// load need only be aligned to its elements): equal rows have equal sums, to the bit, and their candidates tie.
+// NV 16-byte vectors of a lane.  They count from the row's start, wherever that lies (a load need only be aligned to its
+// elements): equal rows have equal sums, to the bit, and their candidates tie.
 template <typename T, int NV>
-__device__ __forceinline__ void beam_segment(const BeamParams& p, int b, int f, uint64_t (&slots)[kBeamSlots]) {
+__global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamParams p) {
   constexpr int VE = 16 / sizeof(T), E = NV * VE;
-  const int w = f / p.segs, seg = f - w * p.segs, lane = lane_id();
-  const int64_t at = (int64_t)b * p.W * p.segs + f;
+  __shared__ uint64_t slots[kBeamSlots];
+  __shared__ float s_max[kBeamWaves], s_sum[kBeamWaves], s_some[kBeamWaves], s_all[kBeamWaves];
+  __shared__ int s_token[kBeamWaves], s_count;
+  const int64_t at = blockIdx.x;
+  const int part = (int)(at % p.parts), row_id = (int)(at / p.parts), b = row_id / p.W, w = row_id - b * p.W;
+  const int wave = uniform(wave_id()), lane = lane_id();
   if (p.done != nullptr && p.done[b * p.s_db + w] != 0) {
     // One candidate of value 0 in a row whose sum is exp(0).
-    if (lane == 0) {
-      publish(p.stats + at, seg == 0 ? beam_pack(0.f, __builtin_bit_cast(uint32_t, 1.f)) : beam_pack(-INFINITY, 0));
-      publish(p.counts + at, seg == 0 ? 1 : 0);
-      if (seg == 0) publish(p.cands + at * kBeamSlots, beam_pack(0.f, (uint32_t)p.eos));
+    if (threadIdx.x == 0) {
+      p.stats[at] = part == 0 ? beam_pack(0.f, __builtin_bit_cast(uint32_t, 1.f)) : beam_pack(-INFINITY, 0);
+      p.counts[at] = part == 0 ? 1 : 0;
+      if (part == 0) p.cands[at * kBeamSlots] = beam_pack(0.f, (uint32_t)p.eos);
     }
     return;
   }
   const T* row = static_cast<const T*>(p.x) + b * p.s_xb + w * p.s_xw;
-  const int first = (seg * NV * kWave + lane) * VE;  // the lane's first token; vector k is 64 vectors on
+  const int first = ((part * kBeamWaves + wave) * NV * kWave + lane) * VE;  // the lane's first token; vector k is 64 vectors on
   float x[E];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
@@ -92,6 +105,7 @@ __device__ __forceinline__ void beam_segment(const BeamParams& p, int b, int f, 
       for (int e = 0; e < VE; ++e) x[k * VE + e] = t + e < p.V ? (float)row[t + e] : -INFINITY;
     }
   }
+  if (threadIdx.x == 0) s_count = 0;
   float mine = -INFINITY;
 #pragma unroll
   for (int k = 0; k < E; ++k) mine = fmaxf(mine, x[k]);
@@ -104,24 +118,36 @@ __device__ __forceinline__ void beam_segment(const BeamParams& p, int b, int f, 
   for (int k = 0; k < E; ++k) sum += fast_exp2((x[k] - ref) * 1.44269504088896340736f);
 #pragma unroll
   for (int o = 1; o < kWave; o *= 2) sum += __shfl_xor(sum, o);
-  const float least = fmaxf(beam_nth(mine, p.n), -3.402823466e38f);
-  auto token = [&](int k) { return first + (k / VE) * kWave * VE + k % VE; };
-  int count = 0;
+  const BeamNth nth = beam_nth(mine, (p.n + kBeamWaves - 1) / kBeamWaves, p.n);
+  if (lane == 0) s_max[wave] = m, s_sum[wave] = sum, s_some[wave] = nth.i, s_all[wave] = nth.j;
+  __syncthreads();
+  float least = -3.402823466e38f, low = INFINITY, top = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < E; ++k) {
-    const bool in = x[k] >= least;
-    const uint64_t who = __builtin_amdgcn_ballot_w64(in);
-    if (who == 0) continue;
-    const int slot = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-    if (in && slot < kBeamSlots) slots[slot] = beam_pack(x[k], (uint32_t)token(k));
-    count += __popcll(who);
+  for (int v = 0; v < kBeamWaves; ++v) {
+    least = fmaxf(least, s_all[v]);
+    low = fminf(low, s_some[v]);
+    top = fmaxf(top, s_max[v]);
   }
+  least = fmaxf(least, low);
+  auto token = [&](int k) { return first + (k / VE) * kWave * VE + k % VE; };
+  if (m >= least) {
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const bool in = x[k] >= least;
+      if (__builtin_amdgcn_ballot_w64(in) == 0) continue;
+      if (in) {
+        const int slot = atomicAdd(&s_count, 1);
+        if (slot < kBeamSlots) slots[slot] = beam_pack(x[k], (uint32_t)token(k));
+      }
+    }
+  }
+  __syncthreads();
+  int count = s_count;
   if (count > kBeamSlots) {
     // One by one: the best behind the last taken.
     float last = INFINITY;
     int last_t = -1;
-    count = 0;
-    for (int i = 0; i < p.n; ++i) {
+    for (count = 0; count < p.n; ++count) {
       float best = -INFINITY;
       int best_t = INT32_MAX;
 #pragma unroll
@@ -133,18 +159,27 @@ __device__ __forceinline__ void beam_segment(const BeamParams& p, int b, int f, 
         const int t = __shfl_xor(best_t, o);
         if (beam_before(v, t, best, best_t)) best = v, best_t = t;
       }
+      if (lane == 0) s_some[wave] = best, s_token[wave] = best_t;
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < kBeamWaves; ++v)
+        if (beam_before(s_some[v], s_token[v], best, best_t)) best = s_some[v], best_t = s_token[v];
+      __syncthreads();
       if (best == -INFINITY) break;
-      if (lane == 0) slots[i] = beam_pack(best, (uint32_t)best_t);
+      if (threadIdx.x == 0) slots[count] = beam_pack(best, (uint32_t)best_t);
       last = best, last_t = best_t;
-      ++count;
     }
+    __syncthreads();
   }
-  wait_lgkm0();
-  if (lane == 0) {
-    publish(p.stats + at, beam_pack(m, __builtin_bit_cast(uint32_t, sum)));
-    publish(p.counts + at, count);
+  for (int i = threadIdx.x; i < count; i += kBeamThreads) p.cands[at * kBeamSlots + i] = slots[i];
+  if (threadIdx.x == 0) {
+    float all = 0.f;
+#pragma unroll
+    for (int v = 0; v < kBeamWaves; ++v)  // a NaN sum stays one, whatever its wave's maximum
+      all += s_sum[v] == 0.f ? 0.f : s_sum[v] * fast_exp2((s_max[v] - top) * 1.44269504088896340736f);
+    p.stats[at] = beam_pack(top, __builtin_bit_cast(uint32_t, all));
+    p.counts[at] = count;
   }
-  if (lane < count) publish(p.cands + at * kBeamSlots + lane, slots[lane]);
 }
 
 __device__ __forceinline__ double beam_shfl(double v, int o) {
@@ -153,120 +188,136 @@ __device__ __forceinline__ double beam_shfl(double v, int o) {
   return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
 }
 
-template <typename T, int NV>
-__global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamParams p) {
-  __shared__ uint64_t slots[kBeamWaves][kBeamSlots];
-  __shared__ double s_lse[kBeamMax], s_score[kBeamMax], s_key[kBeamList], s_best[kBeamWaves];
-  __shared__ uint64_t s_at[kBeamList], s_best_at[kBeamWaves];
-  __shared__ float s_least[kBeamWaves];
-  __shared__ int s_last, s_count;
-  const int b = (int)blockIdx.x / p.wgs, wave = uniform(wave_id()), lane = lane_id();
-  const int f = ((int)blockIdx.x - b * p.wgs) * kBeamWaves + wave, all = p.W * p.segs;
-  if (f < all) beam_segment<T, NV>(p, b, f, slots[wave]);
-  if (!arrive_last(p.counters + b, p.wgs, &s_last)) return;
-
-  // The rows' sums.
+// One workgroup runs it once, so the time its instructions take to arrive counts: every step stands in the code once, the
+// passes over the candidates among them.
+__global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamParams p) {
+  __shared__ double s_lse[kBeamMax], s_score[kBeamMax], s_key[kBeamList], s_best[kBeamJoinWaves];
+  __shared__ uint64_t s_at[kBeamList], s_best_at[kBeamJoinWaves];
+  __shared__ float s_some[kBeamJoinWaves], s_whole[kBeamJoinWaves];
+  __shared__ int s_count;
+  const int b = blockIdx.x, wave = uniform(wave_id()), lane = lane_id(), all = p.W * p.parts;
   const int64_t base = (int64_t)b * all;
-  for (int w = wave; w < p.W; w += kBeamWaves) {
-    float m = -INFINITY;
-    for (int k = lane; k < p.segs; k += kWave) m = fmaxf(m, beam_lo(collect(p.stats + base + w * p.segs + k)));
+  // A thread has candidate slots `slot` of the parts 32 apart; those of the first kBeamNear of them are read at once, before the
+  // parts' counts are known (what lies behind a count is not looked at), others where they are used.
+  const int slot = threadIdx.x % kBeamGroup, part0 = (int)threadIdx.x / kBeamGroup;
+  constexpr int kStep = kBeamJoin / kBeamGroup;
+  uint64_t near[kBeamNear];
+  int counts[kBeamNear];
 #pragma unroll
+  for (int k = 0; k < kBeamNear; ++k) {
+    const int part = part0 + k * kStep;
+    counts[k] = part < all ? p.counts[base + part] : 0;
+    near[k] = p.cands[(base + min(part, all - 1)) * kBeamSlots + slot];
+  }
+  // The rows' sums.
+  for (int w = wave; w < p.W; w += kBeamJoinWaves) {
+    const uint64_t* st = p.stats + base + w * p.parts;
+    const uint64_t v0 = lane < p.parts ? st[lane] : beam_pack(-INFINITY, 0);
+    const float score = p.scores[b * p.s_sb + w];
+    float m = beam_lo(v0);
+    for (int k = lane + kWave; k < p.parts; k += kWave) m = fmaxf(m, beam_lo(st[k]));
     for (int o = 1; o < kWave; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
     double sum = 0;
-    for (int k = lane; k < p.segs; k += kWave) {
-      const uint64_t v = collect(p.stats + base + w * p.segs + k);
+    for (int k = lane; k < p.parts; k += kWave) {
+      const uint64_t v = k == lane ? v0 : st[k];
       if (beam_lo(v) > -INFINITY || !(beam_hi(v) == 0.f)) sum += (double)beam_hi(v) * exp((double)beam_lo(v) - (double)m);
     }
-#pragma unroll
     for (int o = 1; o < kWave; o *= 2) sum += beam_shfl(sum, o);
     if (lane == 0) {
       s_lse[w] = (double)m + log(sum);
-      s_score[w] = (double)p.scores[b * p.s_sb + w];
+      s_score[w] = (double)score;
     }
   }
   if (threadIdx.x == 0) s_count = 0;
   __syncthreads();
-  // f(score, (beam, token)) of the candidates a lane has; a segment's go to other lanes than the next one's.
-  auto each = [&](auto&& g) {
-    for (int f0 = kWave * wave; f0 < all; f0 += kWave * kBeamWaves) {
-      const int mine = f0 + lane < all ? collect(p.counts + base + f0 + lane) : 0;
-      const int fs = min(kWave, all - f0);
-#pragma unroll 4
-      for (int k = 0; k < fs; ++k) {
-        const int n = __builtin_amdgcn_readlane(mine, k), i = (lane + 11 * k) & (kWave - 1);
-        if (i >= n) continue;
-        const int w = (f0 + k) / p.segs;
-        const uint64_t c = collect(p.cands + (base + f0 + k) * kBeamSlots + i);
-        const double key = ((double)beam_lo(c) - s_lse[w]) + s_score[w];
-        if (key > -(double)INFINITY) g(key, ((uint64_t)w << 32) | (c >> 32));
-      }
-    }
-  };
-  // A score that n candidates reach, as a float (rounding keeps the order).
-  float best = -INFINITY;
-  each([&](double key, uint64_t) { best = fmaxf(best, (float)key); });
-  const float reach = beam_nth(best, p.n);
-  if (lane == 0) s_least[wave] = reach;
-  __syncthreads();
-  float least = s_least[0];
-#pragma unroll
-  for (int v = 1; v < kBeamWaves; ++v) least = fmaxf(least, s_least[v]);
-  each([&](double key, uint64_t at) {
-    if ((float)key < least) return;
-    const int i = atomicAdd(&s_count, 1);
-    if (i < kBeamList) s_key[i] = key, s_at[i] = at;
-  });
-  __syncthreads();
-  const int count = s_count;
-  auto put = [&](int i, double key, uint64_t at) {
-    const int64_t o = (int64_t)b * p.n + i;
-    p.out_score[o] = (float)key;
-    p.out_token[o] = (int32_t)(uint32_t)at;
-    p.out_parent[o] = b * p.W + (int)(at >> 32);
-  };
-  auto none = [&](int i) {
-    const int64_t o = (int64_t)b * p.n + i;
-    p.out_score[o] = -INFINITY;
-    p.out_token[o] = p.out_parent[o] = -1;
-  };
-  if (count <= kBeamList) {
-    for (int i = threadIdx.x; i < count; i += kBeamThreads) {
-      const double key = s_key[i];
-      const uint64_t at = s_at[i];
-      int rank = 0;
-      for (int j = 0; j < count; ++j) rank += beam_before(s_key[j], s_at[j], key, at);
-      if (rank < p.n) put(rank, key, at);
-    }
-    for (int i = count + (int)threadIdx.x; i < p.n; i += kBeamThreads) none(i);
-    return;
-  }
-  // More than the list holds reach it (equal rows): one by one.
+  // Pass 0 finds a score that n candidates reach, as a float (rounding keeps the order), as in the first launch; pass 1
+  // lists those that do; where they are more than the list holds (equal rows), pass 2 + i finds the i-th best.
+  float best = -INFINITY, least = -INFINITY;
   double last = INFINITY;
   uint64_t last_at = 0;
-  for (int i = 0; i < p.n; ++i) {
+  for (int pass = 0;; ++pass) {
     double top = -INFINITY;
     uint64_t top_at = ~0ull;
-    each([&](double key, uint64_t at) {
-      const bool behind = i == 0 || beam_before(last, last_at, key, at);
-      if (behind && beam_before(key, at, top, top_at)) top = key, top_at = at;
-    });
+    for (int part = part0, k = 0; part < all; part += kStep, ++k) {
+      int n;
+      uint64_t c;
+      if (k < kBeamNear) {
+        n = counts[0], c = near[0];
 #pragma unroll
-    for (int o = 1; o < kWave; o *= 2) {
-      const double v = beam_shfl(top, o);
-      const uint64_t a = __builtin_bit_cast(uint64_t, beam_shfl(__builtin_bit_cast(double, top_at), o));
-      if (beam_before(v, a, top, top_at)) top = v, top_at = a;
+        for (int j = 1; j < kBeamNear; ++j)
+          if (k == j) n = counts[j], c = near[j];
+      } else {
+        n = p.counts[base + part], c = 0;
+        if (slot < n) c = p.cands[(base + part) * kBeamSlots + slot];
+      }
+      const int w = part / p.parts;
+      for (int i = slot; i < n;) {
+        const double key = ((double)beam_lo(c) - s_lse[w]) + s_score[w];
+        const uint64_t at = ((uint64_t)w << 32) | (c >> 32);
+        if (key > -(double)INFINITY) {
+          if (pass == 0) {
+            best = fmaxf(best, (float)key);
+          } else if (pass == 1) {
+            if ((float)key >= least) {
+              const int to = atomicAdd(&s_count, 1);
+              if (to < kBeamList) s_key[to] = key, s_at[to] = at;
+            }
+          } else if ((pass == 2 || beam_before(last, last_at, key, at)) && beam_before(key, at, top, top_at)) {
+            top = key, top_at = at;
+          }
+        }
+        i += kBeamGroup;
+        if (i < n) c = p.cands[(base + part) * kBeamSlots + i];
+      }
     }
-    if (lane == 0) s_best[wave] = top, s_best_at[wave] = top_at;
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < kBeamWaves; ++v)
-      if (beam_before(s_best[v], s_best_at[v], top, top_at)) top = s_best[v], top_at = s_best_at[v];
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      if (top > -(double)INFINITY) put(i, top, top_at);
-      else none(i);
+    auto put = [&](int i, double key, uint64_t at) {
+      const int64_t o = (int64_t)b * p.n + i;
+      const bool some = key > -(double)INFINITY;
+      p.out_score[o] = (float)key;
+      p.out_token[o] = some ? (int32_t)(uint32_t)at : -1;
+      p.out_parent[o] = some ? b * p.W + (int)(at >> 32) : -1;
+    };
+    if (pass == 0) {
+      const BeamNth nth = beam_nth(best, (p.n + kBeamJoinWaves - 1) / kBeamJoinWaves, p.n);
+      if (lane == 0) s_some[wave] = nth.i, s_whole[wave] = nth.j;
+      __syncthreads();
+      float low = INFINITY;
+      for (int v = 0; v < kBeamJoinWaves; ++v) {
+        least = fmaxf(least, s_whole[v]);
+        low = fminf(low, s_some[v]);
+      }
+      least = fmaxf(least, low);
+    } else if (pass == 1) {
+      __syncthreads();
+      const int count = s_count;
+      if (count > kBeamList) continue;
+      // Eight lanes rank a candidate.  Places behind the candidates are empty.
+      for (int i = threadIdx.x / 8; i < max(count, p.n); i += kBeamJoin / 8) {
+        const double key = i < count ? s_key[i] : -INFINITY;
+        const uint64_t at = i < count ? s_at[i] : 0;
+        int rank = 0;
+        if (i < count)
+          for (int j = threadIdx.x % 8; j < count; j += 8) rank += beam_before(s_key[j], s_at[j], key, at);
+        for (int o = 1; o < 8; o *= 2) rank += __shfl_xor(rank, o);
+        if (i >= count) rank = i;
+        if (threadIdx.x % 8 == 0 && rank < p.n) put(rank, key, at);
+      }
+      return;
+    } else {
+      for (int o = 1; o < kWave; o *= 2) {
+        const double v = beam_shfl(top, o);
+        const uint64_t a = __builtin_bit_cast(uint64_t, beam_shfl(__builtin_bit_cast(double, top_at), o));
+        if (beam_before(v, a, top, top_at)) top = v, top_at = a;
+      }
+      if (lane == 0) s_best[wave] = top, s_best_at[wave] = top_at;
+      __syncthreads();
+      for (int v = 0; v < kBeamJoinWaves; ++v)
+        if (beam_before(s_best[v], s_best_at[v], top, top_at)) top = s_best[v], top_at = s_best_at[v];
+      __syncthreads();
+      if (threadIdx.x == 0) put(pass - 2, top, top_at);
+      last = top, last_at = top_at;
+      if (pass == p.n + 1) return;
     }
-    last = top, last_at = top_at;
   }
 }
 
@@ -315,13 +366,11 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderParams p) {
   else reorder_column<uint8_t, WB>(at, p.stride[i], parents, p.W, row0);
 }
 
-// Vectors of a lane: 8, and 2 where 8 would give fewer than four waves to a CU.
+// Vectors of a lane: 8, and 2 where 8 would give less than a workgroup to a CU.
 static int beam_vectors(int64_t rows, int V, int size, int cus) {
-  return rows * ceil_div64((int64_t)V * size, 16 * kWave * 8) < 4 * cus ? 2 : 8;
+  return rows * ceil_div64((int64_t)V * size, 16 * kBeamThreads * 8) < cus ? 2 : 8;
 }
-static int64_t beam_segs(int V, int size, int nv) {
-  return ceil_div64((int64_t)V * size, 16 * kWave * nv);
-}
+static int64_t beam_parts(int V, int size, int nv) { return ceil_div64((int64_t)V * size, 16 * kBeamThreads * nv); }
 
 }  // namespace specq
 
@@ -330,8 +379,8 @@ using namespace specq;
 extern "C" size_t specq_beam_select_workspace_size(int B, int W, int V, int logits_fp32) {
   if (B <= 0 || W <= 0 || V <= 0) return 0;
   const int size = logits_fp32 ? 4 : 2;
-  const size_t segs = (size_t)B * W * beam_segs(V, size, beam_vectors((int64_t)B * W, V, size, device_cus()));
-  return kCounterBytes + align_up(segs * 4, 256) + segs * (8 + 8 * kBeamSlots);
+  const size_t parts = (size_t)B * W * beam_parts(V, size, beam_vectors((int64_t)B * W, V, size, device_cus()));
+  return kCounterBytes + align_up(parts * 4, 256) + parts * (8 + 8 * kBeamSlots);
 }
 
 extern "C" int specq_beam_select(const void* logits, int logits_fp32, int64_t s_lb, int64_t s_lw, const float* scores,
@@ -343,15 +392,15 @@ extern "C" int specq_beam_select(const void* logits, int logits_fp32, int64_t s_
   SPECQ_REQUIRE(B >= 0 && W > 0 && V > 0 && n > 0, SPECQ_EINVAL, "beam_select: bad sizes B=%d W=%d V=%d n=%d", B, W, V, n);
   SPECQ_REQUIRE(W <= kBeamMax && n <= kBeamMax, SPECQ_ENOTSUP, "beam_select: %d beams, %d candidates (at most %d supported)", W,
                 n, kBeamMax);
-  SPECQ_REQUIRE(V <= (1 << 28) && B <= kMaxCounters && (int64_t)B * W <= INT32_MAX, SPECQ_ENOTSUP,
+  SPECQ_REQUIRE(V <= (1 << 28) && (int64_t)B * W <= INT32_MAX, SPECQ_ENOTSUP,
                 "beam_select: vocabulary or batch too large");
   SPECQ_REQUIRE(!finished || (eos >= 0 && eos < V), SPECQ_EINVAL, "beam_select: eos %d is no token of %d", eos, V);
   SPECQ_REQUIRE((uintptr_t)logits % (logits_fp32 ? 4 : 2) == 0 && (uintptr_t)scores % 4 == 0, SPECQ_EINVAL,
                 "beam_select: logits and scores must be aligned to their type");
   if (B == 0) return SPECQ_OK;
   const int size = logits_fp32 ? 4 : 2, nv = beam_vectors((int64_t)B * W, V, size, device_cus());
-  const int64_t segs = beam_segs(V, size, nv), wgs = ceil_div64(W * segs, kBeamWaves);
-  SPECQ_REQUIRE(B * wgs <= INT32_MAX, SPECQ_ENOTSUP, "beam_select: grid too large");
+  const int64_t parts = beam_parts(V, size, nv), count = (int64_t)B * W * parts;
+  SPECQ_REQUIRE(count <= INT32_MAX, SPECQ_ENOTSUP, "beam_select: grid too large");
   const size_t need = specq_beam_select_workspace_size(B, W, V, logits_fp32);
   SPECQ_REQUIRE(workspace && workspace_bytes >= need, SPECQ_ENOSPC, "beam_select: workspace of %zu bytes required, %zu given",
                 need, workspace ? workspace_bytes : (size_t)0);
@@ -359,18 +408,17 @@ extern "C" int specq_beam_select(const void* logits, int logits_fp32, int64_t s_
   p.x = logits; p.s_xb = s_lb; p.s_xw = s_lw; p.scores = scores; p.s_sb = s_sb;
   p.done = finished; p.s_db = s_fb; p.eos = eos;
   p.out_score = out_scores; p.out_token = out_tokens; p.out_parent = out_parents;
-  p.W = W; p.V = V; p.n = n; p.segs = (int)segs; p.wgs = (int)wgs;
-  const size_t count = (size_t)B * W * segs;
-  char* at = static_cast<char*>(workspace);
-  p.counters = reinterpret_cast<int32_t*>(at);
-  p.counts = reinterpret_cast<int32_t*>(at + kCounterBytes);
-  p.stats = reinterpret_cast<uint64_t*>(at + kCounterBytes + align_up(count * 4, 256));
+  p.W = W; p.V = V; p.n = n; p.parts = (int)parts;
+  char* at = static_cast<char*>(workspace) + kCounterBytes;
+  p.counts = reinterpret_cast<int32_t*>(at);
+  p.stats = reinterpret_cast<uint64_t*>(at + align_up((size_t)count * 4, 256));
   p.cands = p.stats + count;
-  const void* fn = logits_fp32 ? (nv == 8 ? reinterpret_cast<const void*>(&beam_select_kernel<float, 8>)
-                                          : reinterpret_cast<const void*>(&beam_select_kernel<float, 2>))
-                               : (nv == 8 ? reinterpret_cast<const void*>(&beam_select_kernel<_Float16, 8>)
-                                          : reinterpret_cast<const void*>(&beam_select_kernel<_Float16, 2>));
-  return launch(fn, (int)(B * wgs), kBeamThreads, 0, (hipStream_t)stream, &p);
+  const void* fn = logits_fp32 ? (nv == 8 ? reinterpret_cast<const void*>(&beam_part_kernel<float, 8>)
+                                          : reinterpret_cast<const void*>(&beam_part_kernel<float, 2>))
+                               : (nv == 8 ? reinterpret_cast<const void*>(&beam_part_kernel<_Float16, 8>)
+                                          : reinterpret_cast<const void*>(&beam_part_kernel<_Float16, 2>));
+  if (int rc = launch(fn, (int)count, kBeamThreads, 0, (hipStream_t)stream, &p)) return rc;
+  return launch(reinterpret_cast<const void*>(&beam_join_kernel), B, kBeamJoin, 0, (hipStream_t)stream, &p);
 }
 
 extern "C" int specq_beam_reorder(const int32_t* parents, int rows, int group, int n_tensors, void* const* base,

@@ -94,7 +94,7 @@ def test_beam_refusals(built_lib):
     f = lambda code, **kw: _fail("specq_beam_select", base, code, **kw)  # noqa: E731
     for name in ("x", "scores", "os", "ot", "op"):
         f(-22, **{name: 0})
-    f(-22, W=0), f(-22, V=0), f(-22, n=0), f(-95, W=65), f(-95, n=65), f(-95, V=(1 << 28) + 1), f(-95, B=1 << 17)
+    f(-22, W=0), f(-22, V=0), f(-22, n=0), f(-95, W=65), f(-95, n=65), f(-95, V=(1 << 28) + 1), f(-95, B=1 << 30)
     f(-22, done=16, eos=-1), f(-22, done=16, eos=1000), f(-22, x=17), f(-22, f32=1, x=18), f(-22, scores=18)
     f(-28), f(-28, ws=4096, wsb=200000)
     f(0, B=0)
@@ -123,14 +123,14 @@ def test_kernels_keep_to_their_registers(built_lib):
     report = os.path.join(os.path.dirname(built_lib), "libspecq.resources.txt")
     if not os.path.exists(report):
         pytest.skip("library without its report")
-    ours = re.compile(r"qk_norm_(vec|any)_kernel|aw_\w+_kernel|evict_\w+_kernel|beam_(select|reorder)_kernel")
+    ours = re.compile(r"qk_norm_(vec|any)_kernel|aw_\w+_kernel|evict_\w+_kernel|beam_(part|join|reorder)_kernel")
     scratch, name = {}, ""
     for line in open(report):
         if m := re.search(r"Function Name: (\S+)", line):
             name = m.group(1)
         elif (m := re.search(r"ScratchSize \[bytes/lane\]: (\d+)", line)) and ours.search(name):
             scratch[name] = int(m.group(1))
-    assert len(scratch) >= 12 + 9 + 2 + 8
+    assert len(scratch) >= 12 + 21 + 2 + 9
     assert not any(scratch.values()), scratch
 
 
