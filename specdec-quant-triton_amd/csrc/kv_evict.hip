@@ -7,9 +7,11 @@
 // counts given, a page that other rows name too, stays as it is.
 //
 // Selection, one workgroup a (sequence, head): the weights as unsigned keys of the same order (tokens that stay in any
-// case have the largest key), the budget-th largest found by three passes of counting digits of 11, 11 and 10 bits from
-// the top, then one pass in the order of the positions that ranks what is above it and the first of what equals it.  Keys
-// of the first kEvKeys * 1024 tokens stay in registers, further ones are read again from L2.
+// case have the largest key); the budget-th largest by counting digits of 11, 11 and 10 bits from the top, the lower
+// ones over a list of the keys that share the upper one (over all keys where they are too many for it); then one pass in
+// the order of the positions that ranks what is above it and the first of what equals it.  Three passes over the weights,
+// 16384 at a time, the first 16384 in registers.  One workgroup for a row, so it is bound by latency: the code stands
+// in few places (unrolled, it took longer to arrive than to run: 4096 tokens 8 -> 15 us).
 //
 // Moving is in place.  Token j goes to a place at or below its own, and everything behind it starts above, so it is
 // enough that a tile of tokens has been read by all its threads before any of them writes it.  One workgroup walks one
@@ -20,12 +22,16 @@
 
 namespace specq {
 
+constexpr int kEvMove = 512;  // threads that move
 constexpr int kEvThreads = 1024, kEvWaves = kEvThreads / kWave;
 constexpr int kEvBins = 2048;
-constexpr int kEvKeys = 8;      // keys of a thread in registers: positions 4 (tid + 1024 c) + 0..3, c < 2
+constexpr int kEvStep = 4 * kEvThreads;  // positions of a chunk, four consecutive ones a thread
+constexpr int kEvGroup = 4;              // chunks that are loaded, and ranked, together
+constexpr int kEvCopies = 4;             // histograms that lanes take in turn, since many weights share a digit
+constexpr int kEvList = 8192;            // keys of one upper digit
 constexpr int kEvTensors = 16;  // cache tensors of a call
 constexpr int kEvUnits = 256;   // byte ranges of a call
-constexpr int kEvPages = 8192;  // table entries kept in LDS
+constexpr int kEvPages = 4096;  // table entries whose pages' places are kept in LDS
 constexpr int kEvBatch = 4;     // accesses of a thread in flight
 
 struct EvictParams {
@@ -44,46 +50,87 @@ struct EvictMoveParams {
   int64_t s_p[kEvTensors], s_o[kEvTensors], s_h[kEvTensors];  // bytes from page to page, token to token, head to head
   // Range u: its tensor (kEvTensors: the weights), first byte, bytes and bytes of one access.
   uint8_t tensor[kEvUnits], vec[kEvUnits]; int16_t bytes[kEvUnits]; int32_t first[kEvUnits];
-  int units;
+  int units, progs;
+  uint32_t page_magic; int page_shift;  // t / PAGE = (t * magic >> 32) >> shift for t below 2^30; magic 0: PAGE = 1
 };
 
-// Exclusive prefix of x over the workgroup; `total` is the sum.
-__device__ __forceinline__ int ev_prefix(int x, int& total, int (&part)[kEvWaves]) {
-  int v = x;
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
-  __syncthreads();  // the last call's readers of part are done
-  if (lane_id() == kWave - 1) part[wave_id()] = v;
-  __syncthreads();
-  int before = 0, all = 0;
+// Exclusive prefixes of N values over the workgroup, and their sums.
+template <int N>
+__device__ __forceinline__ void ev_prefix(int (&x)[N], int (&total)[N], int (&part)[kEvGroup][kEvWaves]) {
+  int v[N];
 #pragma unroll
-  for (int w = 0; w < kEvWaves; ++w) {
-    const int y = part[w];
-    before += w < wave_id() ? y : 0;
-    all += y;
+  for (int n = 0; n < N; ++n) {
+    v[n] = x[n];
+    v[n] += __builtin_amdgcn_update_dpp(0, v[n], 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+    v[n] += __builtin_amdgcn_update_dpp(0, v[n], 0x112, 0xf, 0xf, false);
+    v[n] += __builtin_amdgcn_update_dpp(0, v[n], 0x114, 0xf, 0xf, false);
+    v[n] += __builtin_amdgcn_update_dpp(0, v[n], 0x118, 0xf, 0xf, false);
+    v[n] += __builtin_amdgcn_update_dpp(0, v[n], 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+    v[n] += __builtin_amdgcn_update_dpp(0, v[n], 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
   }
-  total = all;
-  return before + v - x;
+  __syncthreads();  // the last call's readers of part are done
+  if (lane_id() == kWave - 1) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) part[n][wave_id()] = v[n];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    int w = part[n][lane_id() % kEvWaves];  // the waves' sums, then theirs up to each
+    w += __builtin_amdgcn_update_dpp(0, w, 0x111, 0xf, 0xf, false);
+    w += __builtin_amdgcn_update_dpp(0, w, 0x112, 0xf, 0xf, false);
+    w += __builtin_amdgcn_update_dpp(0, w, 0x114, 0xf, 0xf, false);
+    w += __builtin_amdgcn_update_dpp(0, w, 0x118, 0xf, 0xf, false);
+    const int wave = uniform(wave_id());
+    total[n] = __builtin_amdgcn_readlane(w, kEvWaves - 1);
+    x[n] = (wave > 0 ? __builtin_amdgcn_readlane(w, max(wave - 1, 0)) : 0) + v[n] - x[n];
+  }
 }
 
 // A key of the order of the weights; NaN counts as -infinity, -0 as 0.
 __device__ __forceinline__ uint32_t ev_key(float w) {
   if (!(w == w)) w = -INFINITY;
-  const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.f);
-  return (u >> 31) ? ~u : u | 0x80000000u;
+  const int u = __builtin_bit_cast(int, w + 0.f);
+  return (uint32_t)u ^ ((uint32_t)(u >> 31) | 0x80000000u);
 }
 
 __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictParams p) {
-  __shared__ int hist[kEvBins], part[kEvWaves], s_bin, s_above;
+  __shared__ int hist[kEvCopies][kEvBins], part[kEvGroup][kEvWaves], s_bin, s_above, s_in, s_list_n;
+  __shared__ uint32_t s_list[kEvList];
   const int prog = blockIdx.x, b = prog / p.H, h = prog - b * p.H, tid = threadIdx.x;
   const int L = min(max(p.ctx_len[b], 0), p.cap);
   int32_t* kept = p.kept + (int64_t)prog * p.budget;
+  const float* wr = p.w + b * p.s_wb + h * p.s_wh;
+  constexpr int kSpan = kEvGroup * kEvStep;
+  // Whether all of a chunk's tokens compete.
+  auto inner = [&](int at) { return at >= p.sinks && at + kEvStep <= L - p.recent; };
+  // Keys of the thread's positions of the group from g0 on; behind the context 0, which no weight has and none is found to be.
+  auto load = [&](int g0, uint32_t (&k)[kEvGroup][4]) {
+#pragma unroll
+    for (int c = 0; c < kEvGroup; ++c) {
+      const int t = g0 + c * kEvStep + 4 * tid;
+      v4f x = {0.f, 0.f, 0.f, 0.f};
+      if (p.w_vec && t + 4 <= L) {
+        x = *reinterpret_cast<const v4f*>(wr + t);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (t + i < L) x[i] = wr[t + i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[c][i] = ev_key(x[i]);
+      if (!inner(g0 + c * kEvStep)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          k[c][i] = t + i >= L ? 0u : t + i < p.sinks || t + i >= L - p.recent ? 0xFFFFFFFFu : k[c][i];
+      }
+    }
+  };
+  for (int i = tid; i < kEvCopies * kEvBins; i += kEvThreads) hist[0][i] = 0;
   int ok = L > p.limit;
+  uint32_t near[kEvGroup][4];
   if (ok) {
+    load(0, near);
     const int32_t* row = p.bt + b * p.s_bt;
     for (int c = tid; c < (L + p.PAGE - 1) / p.PAGE; c += kEvThreads) {
       const int id = row[c];
@@ -96,94 +143,126 @@ __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictParams p)
     for (int j = tid; j < p.budget; j += kEvThreads) kept[j] = j < L ? j : -1;
     return;
   }
-  const float* wr = p.w + b * p.s_wb + h * p.s_wh;
-  auto load = [&](int t, uint32_t (&k)[4]) {  // keys of positions t..t+3, 0 past the context
-    v4f x = {0.f, 0.f, 0.f, 0.f};
-    if (p.w_vec && t + 4 <= L) {
-      x = *reinterpret_cast<const v4f*>(wr + t);
-    } else {
+  // f(chunk of the group, the thread's four keys) of each chunk with tokens; `group` behind each four.
+  auto each = [&](auto&& f, auto&& group) {
+#pragma unroll 1
+    for (int g0 = 0; g0 < L; g0 += kSpan) {
+      uint32_t k[kEvGroup][4];
+      if (g0 == 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (t + i < L) x[i] = wr[t + i];
-    }
+        for (int c = 0; c < kEvGroup; ++c)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = t + i;
-      k[i] = at >= L ? 0u : (at < p.sinks || at >= L - p.recent) ? 0xFFFFFFFFu : ev_key(x[i]);
-    }
-  };
-  constexpr int kStep = 4 * kEvThreads;
-  uint32_t near[kEvKeys / 4][4];
+          for (int i = 0; i < 4; ++i) k[c][i] = near[c][i];
+      } else {
+        load(g0, k);
+      }
 #pragma unroll
-  for (int c = 0; c < kEvKeys / 4; ++c) load(c * kStep + 4 * tid, near[c]);
-  const int chunks = (L + kStep - 1) / kStep;
-  auto each = [&](auto&& f) {  // f(first position, keys), a chunk of 4096 positions at a time
-#pragma unroll
-    for (int c = 0; c < kEvKeys / 4; ++c)
-      if (c < chunks) f(c * kStep + 4 * tid, near[c]);
-    for (int c = kEvKeys / 4; c < chunks; ++c) {
-      uint32_t k[4];
-      load(c * kStep + 4 * tid, k);
-      f(c * kStep + 4 * tid, k);
+      for (int c = 0; c < kEvGroup; ++c) {
+        const int at = g0 + c * kEvStep;
+        if (at < L) f(c, k[c]);
+      }
+      group(g0, k);
     }
   };
+  auto nothing = [](int, const uint32_t (&)[kEvGroup][4]) {};
   // The budget-th largest key, from its top digit down: `want` of those under the digits found so far.
-  uint32_t found = 0;
+  uint32_t found = 0, known = 0;  // its digits, and a mask of them
   int want = p.budget;
-#pragma unroll
+  bool listed = false;
+#pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
-    const int low = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass < 2 ? 11 : 10, bins = 1 << bits;
-    hist[2 * tid] = hist[2 * tid + 1] = 0;
-    __syncthreads();
-    each([&](int t, const uint32_t (&k)[4]) {
+    const int low = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass < 2 ? 2048 : 1024;
+    int* mine = hist[tid % kEvCopies];
+    if (pass == 0) {
+      each([&](int, const uint32_t (&k)[4]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (t + i < L && (pass == 0 || (k[i] >> (low + bits)) == (found >> (low + bits))))
-          atomicAdd(&hist[(k[i] >> low) & (bins - 1)], 1);
-    });
+        for (int i = 0; i < 4; ++i) atomicAdd(&mine[k[i] >> 21], 1);
+      }, nothing);
+    } else if (listed) {
+      for (int i = tid; i < s_list_n; i += kEvThreads)
+        if (((s_list[i] ^ found) & known) == 0) atomicAdd(&mine[(s_list[i] >> low) & (bins - 1)], 1);
+    } else {
+      each([&](int, const uint32_t (&k)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (((k[i] ^ found) & known) == 0) atomicAdd(&mine[(k[i] >> low) & (bins - 1)], 1);
+      }, nothing);
+    }
     __syncthreads();
-    // Thread i has bins 2047 - 2 i and 2046 - 2 i: the prefix runs from the largest digit down.
-    const int hi = kEvBins - 1 - 2 * tid, n1 = hist[hi], n0 = hist[hi - 1];
-    int total;
-    const int above = ev_prefix(n1 + n0, total, part);
+    // Thread i has bins 2047 - 2 i and 2046 - 2 i, and clears them: the prefix runs from the largest digit down.
+    const int hi = kEvBins - 1 - 2 * tid;
+    int n1 = 0, n0 = 0;
+#pragma unroll
+    for (int c = 0; c < kEvCopies; ++c) {
+      v2i* at = reinterpret_cast<v2i*>(&hist[c][hi - 1]);
+      const v2i n = *at;
+      *at = v2i{0, 0};
+      n0 += n[0], n1 += n[1];
+    }
+    int sum[1] = {n1 + n0}, total[1];
+    ev_prefix(sum, total, part);
+    const int above = sum[0];
     if (above < want && above + n1 + n0 >= want) {
       const bool first = above + n1 >= want;
       s_bin = first ? hi : hi - 1;
       s_above = first ? above : above + n1;
+      s_in = first ? n1 : n0;
     }
+    if (tid == 0 && pass == 0) s_list_n = 0;
     __syncthreads();
     found |= (uint32_t)s_bin << low;
+    known |= (uint32_t)(bins - 1) << low;
     want -= s_above;
+    if (pass == 0 && s_in <= kEvList) {
+      listed = true;
+      each([&](int, const uint32_t (&k)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (((k[i] ^ found) & known) == 0) s_list[atomicAdd(&s_list_n, 1)] = k[i];
+      }, nothing);
+    }
     __syncthreads();
   }
-  // `want` keys equal to `found` stay, the lowest positions; everything larger stays.
-  int above = 0, equal = 0;
-  each([&](int t, const uint32_t (&k)[4]) {
-    int gt[4], eq[4], n = 0;  // counts of a chunk fit 16 bits
+  // `want` keys equal to `found` stay, the lowest positions; everything larger stays.  Counts of a chunk: larger keys, and equal
+  // ones above bit 16; where all equal ones stay, they count as larger.
+  const uint32_t larger = s_in == want ? found : found + 1;  // (the largest key's tokens all stay)
+  const bool ties = s_in != want;
+  int above = 0, equal = 0, count[kEvGroup] = {0, 0, 0, 0};
+  each([&](int c, const uint32_t (&k)[4]) {
+    int x = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      gt[i] = t + i < L && k[i] > found;
-      eq[i] = t + i < L && k[i] == found;
-      n += gt[i] + (eq[i] << 16);
-    }
-    int total;
-    const int before = ev_prefix(n, total, part);
-    int a = above + (before & 0xFFFF), e = equal + (before >> 16);
+    for (int i = 0; i < 4; ++i) x += k[i] >= larger;
+    if (ties) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (gt[i] || (eq[i] && e < want)) kept[a + min(e, want)] = t + i;
-      a += gt[i];
-      e += eq[i];
+      for (int i = 0; i < 4; ++i) x += (k[i] == found) << 16;
     }
-    above += total & 0xFFFF;
-    equal += total >> 16;
+    count[c] = x;
+  }, [&](int g0, const uint32_t (&k)[kEvGroup][4]) {
+    int total[kEvGroup];
+    ev_prefix(count, total, part);
+#pragma unroll
+    for (int c = 0; c < kEvGroup; ++c) {
+      if (g0 + c * kEvStep >= L) break;
+      const int t = g0 + c * kEvStep + 4 * tid;
+      int a = above + (count[c] & 0xFFFF), e = equal + (count[c] >> 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool gt = k[c][i] >= larger, eq = ties && k[c][i] == found;
+        if (gt || (eq && e < want)) kept[a + min(e, want)] = t + i;
+        a += gt;
+        e += eq;
+      }
+      above += total[c] & 0xFFFF;
+      equal += total[c] >> 16;
+      count[c] = 0;
+    }
   });
 }
 
 // One byte range of one (sequence, head): accesses of sizeof(T) bytes, `lanes` of them a token.
 template <typename T, typename F>
 __device__ __forceinline__ void evict_walk(const int32_t* kept, int budget, int lanes, F&& place) {
-  const int per = kEvThreads / lanes, sub = (int)threadIdx.x % lanes, mine = (int)threadIdx.x / lanes;
+  const int per = kEvMove / lanes, sub = (int)threadIdx.x % lanes, mine = (int)threadIdx.x / lanes;
   const bool on = mine < per;
   auto source = [&](int j) { return on && j < budget ? kept[j] : -1; };
   auto take = [&](int j0, T (&x)[kEvBatch], int (&src)[kEvBatch]) {
@@ -224,30 +303,34 @@ __device__ __forceinline__ void evict_walk(const int32_t* kept, int budget, int 
   }
 }
 
-__global__ __launch_bounds__(kEvThreads) void evict_move_kernel(EvictMoveParams p) {
-  __shared__ int32_t pages[kEvPages];
+__global__ __launch_bounds__(kEvMove) void evict_move_kernel(EvictMoveParams p) {
+  __shared__ int64_t pages[kEvPages];
   const EvictParams& e = p.e;
-  const int u = (int)blockIdx.x % p.units, prog = (int)blockIdx.x / p.units, b = prog / e.H, h = prog - b * e.H;
-  if (!uniform(e.flag[prog])) return;
+  // The ranges of one (sequence, head) run eight workgroups apart, on one XCD, whose L2 holds the lines they share.
+  const int u = (int)(blockIdx.x / 8) % p.units, prog = (int)(blockIdx.x / 8) / p.units * 8 + (int)blockIdx.x % 8;
+  if (prog >= p.progs) return;
+  const int b = prog / e.H, h = prog - b * e.H;
+  const int flag = e.flag[prog];
   const int32_t* kept = e.kept + (int64_t)prog * e.budget;
   const int tensor = p.tensor[u], vec = p.vec[u], lanes = p.bytes[u] / vec;
   if (tensor == kEvTensors) {
+    if (!uniform(flag)) return;
     if (h == 0 && threadIdx.x == 0) e.ctx_len[b] = e.budget;  // the selection is over, and this launch does not read it
     float* w = e.w + b * e.s_wb + h * e.s_wh;
     evict_walk<float>(kept, e.budget, 1, [&](int t) { return reinterpret_cast<uint8_t*>(w + t); });
     return;
   }
   const int32_t* row = e.bt + b * e.s_bt;
-  const int last = uniform(kept[e.budget - 1]) / e.PAGE;  // the highest page that is read or written
-  const bool near = last < kEvPages;
-  if (near)
-    for (int c = threadIdx.x; c <= last; c += kEvThreads) pages[c] = row[c];
-  __syncthreads();
-  uint8_t* base = p.base[tensor] + h * p.s_h[tensor] + p.first[u];
   const int64_t s_p = p.s_p[tensor], s_o = p.s_o[tensor];
+  const bool near = e.C <= kEvPages;
+  if (near)
+    for (int c = threadIdx.x; c < e.C; c += kEvMove) pages[c] = row[c] * s_p;
+  __syncthreads();
+  if (!uniform(flag)) return;
+  uint8_t* base = p.base[tensor] + h * p.s_h[tensor] + p.first[u];
   auto place = [&](int t) {
-    const int c = t / e.PAGE;
-    return base + (near ? pages[c] : row[c]) * s_p + (t - c * e.PAGE) * s_o;
+    const int c = p.page_magic != 0 ? (int)(__umulhi((uint32_t)t, p.page_magic) >> p.page_shift) : t;
+    return base + (near ? pages[c] : row[c] * s_p) + (t - c * e.PAGE) * s_o;
   };
   if (vec == 16) evict_walk<v4i>(kept, e.budget, lanes, place);
   else if (vec == 4) evict_walk<int32_t>(kept, e.budget, lanes, place);
@@ -307,7 +390,7 @@ extern "C" int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int
   p.kept = kept;
   p.flag = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + kCounterBytes);
   p.H = H_KV; p.PAGE = PAGE; p.cap = (int)cap; p.budget = budget; p.recent = recent; p.sinks = sinks; p.limit = limit;
-  // Byte ranges: rows whole, or in pieces of at least 16 bytes until there is a workgroup or two for every CU.
+  // Byte ranges: pieces of 128 bytes, or of less, down to 16, until there are three workgroups for two CUs.
   const int64_t cus = device_cus();
   int64_t piece = 128;
   auto ranges = [&](int64_t size) {
@@ -315,7 +398,7 @@ extern "C" int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int
     for (int i = 0; i < n_tensors; ++i) n += ceil_div64(row_bytes[i], size);
     return n;
   };
-  while (piece > 16 && progs * ranges(piece) < 2 * cus) piece /= 2;
+  while (piece > 16 && 2 * progs * ranges(piece) < 3 * cus) piece /= 2;
   while (ranges(piece) > kEvUnits) piece *= 2;
   for (int i = 0; i < n_tensors; ++i) {
     const uint64_t bits = (uintptr_t)base[i] | (uint64_t)page_stride[i] | (uint64_t)token_stride[i] | (uint64_t)head_stride[i] |
@@ -331,7 +414,16 @@ extern "C" int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int
   }
   m.tensor[m.units] = kEvTensors; m.vec[m.units] = 4; m.bytes[m.units] = 4;
   ++m.units;
+  m.progs = (int)progs;
+  if (PAGE > 1) {
+    int bits = 0;  // ceil(log2(PAGE))
+    while ((1ll << bits) < PAGE) ++bits;
+    // ceil(2^k / PAGE), k = 30 + bits, is off by less than PAGE <= 2^bits in 2^k, so its products with t < 2^30 by less than one.
+    const uint64_t magic = ((1ull << (30 + bits)) + PAGE - 1) / PAGE;
+    m.page_magic = (uint32_t)(bits < 2 ? magic << (2 - bits) : magic);
+    m.page_shift = bits < 2 ? 0 : bits - 2;
+  }
   hipStream_t st = (hipStream_t)stream;
   if (int rc = launch(reinterpret_cast<const void*>(&evict_select_kernel), (int)progs, kEvThreads, 0, st, &p)) return rc;
-  return launch(reinterpret_cast<const void*>(&evict_move_kernel), (int)(progs * m.units), kEvThreads, 0, st, &m);
+  return launch(reinterpret_cast<const void*>(&evict_move_kernel), (int)(align_up(progs, 8) * m.units), kEvMove, 0, st, &m);
 }
