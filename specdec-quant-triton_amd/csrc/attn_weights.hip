@@ -385,8 +385,8 @@ __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) qf[u] = s_q[rb][u][lane];
         v4f acc[4];
-        aw_scores<D>(kh, qf, ksc, t0, row < x.rows ? fresh + aw_token(p, row) : -1,
-                     t0 + 63 <= fresh && seen == 0xf && rb * 16 + 16 <= x.rows, seen, acc);
+        // Rows past the last add nothing: their statistics go nowhere, their lse is infinite.
+        aw_scores<D>(kh, qf, ksc, t0, fresh + aw_token(p, row), t0 + 63 <= fresh && seen == 0xf, seen, acc);
         if constexpr (MODE == kAwSums) {
 #pragma unroll
           for (int s = 0; s < 4; ++s)
@@ -411,8 +411,7 @@ __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
   }
 }
 
-// Up to 16 rows, whose scores are stored: one block of rows, so a sub-tile's operands are made where they are used and two
-// tiles' codes fit the registers.
+// Up to 16 rows, whose scores are stored: one block of rows, so a sub-tile's operands are made where they are used.
 template <int D, typename ST>
 __global__ __launch_bounds__(256) void aw_store_kernel(AwParams p) {
   constexpr int NU = D / 32;
@@ -438,15 +437,19 @@ __global__ __launch_bounds__(256) void aw_store_kernel(AwParams p) {
 #pragma unroll
       for (int u = 0; u < NU; ++u) qf[u] = *reinterpret_cast<const v8h*>(src + 64 * (u / 2) + 8 * (u & 1));
     }
-    const int last = r < x.rows ? fresh + aw_token(p, r) : -1;  // the last token the lane's row sees
+    const int last = fresh + aw_token(p, r);  // the last token the lane's row sees
     const AwPages at = aw_pages(p, x, sub_t, page, lane < 4 * p.span);
     const rsrc_t out = make_rsrc(p.scores + (int64_t)prog * p.rows * p.tiles * kAwTile, kOOB);
     const uint32_t out_row = oob_unless(r < x.rows, (uint32_t)(r * p.tiles * kAwTile + 4 * g) * 4);
-    auto work = [&](int tile, const v4i (&raw)[4][D / 64], ST scale) {
+    v4i raw[4][D / 64];
+    ST scale;
+    aw_load<D, kOnce, ST>(p, at, 0, raw, scale);
+    for (int tile = tile0; tile < tile1; ++tile) {
       const int t0 = tile * kAwTile + 64 * w;
       const uint32_t seen = (uint32_t)(at.ok >> (4 * (tile - tile0))) & 0xf;
       s_k[w].put(raw);
       s_scale[w][lane] = (float)scale * p.scale_log2;
+      aw_load<D, kOnce, ST>(p, at, 4 * (tile + 1 - tile0), raw, scale);
       wait_lgkm0();
       v4f acc[4], ksc[4];
 #pragma unroll
@@ -459,23 +462,13 @@ __global__ __launch_bounds__(256) void aw_store_kernel(AwParams p) {
       }
 #pragma unroll
       for (int s = 0; s < 4; ++s) ksc[s] = *reinterpret_cast<const v4f*>(&s_scale[w][16 * s + 4 * g]);
-      aw_mask(ksc, t0, last, t0 + 63 <= fresh && seen == 0xf && x.rows == 16, seen, acc);
+      aw_mask(ksc, t0, last, t0 + 63 <= fresh && seen == 0xf, seen, acc);  // rows past the last go nowhere
       // Always the same stores, too; those of tokens behind the context lie in the row's last tile.
 #pragma unroll
       for (int s = 0; s < 4; ++s)
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, acc[s]), out, out_row + 4u * (uint32_t)(t0 + 16 * s), 0, 0);
       const uint64_t st = aw_stat(acc);
       if (g == 0) s_stat[tile - tile0][w][r] = st;
-    };
-    v4i raw0[4][D / 64], raw1[4][D / 64];
-    ST scale0, scale1;
-    aw_load<D, kOnce, ST>(p, at, 0, raw0, scale0);
-    for (int tile = tile0; tile < tile1; tile += 2) {
-      aw_load<D, kOnce, ST>(p, at, 4 * (tile + 1 - tile0), raw1, scale1);
-      work(tile, raw0, scale0);
-      if (tile + 1 >= tile1) break;
-      aw_load<D, kOnce, ST>(p, at, 4 * (tile + 2 - tile0), raw0, scale0);
-      work(tile + 1, raw1, scale1);
     }
     __syncthreads();
     aw_publish(p, x, prog, tile0, tile1, s_stat);
