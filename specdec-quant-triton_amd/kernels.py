@@ -1548,6 +1548,19 @@ def paged_attention_weights(q, kc, ks, block_tbl, ctx_len, weights, q_len=None, 
     return weights
 
 
+def _cache_rows(who: str, t, pages: int, PAGE: int, H_KV: int):
+    """(base, strides from page to page, token to token and head to head, bytes of a row) of a cache [pages, PAGE, H_KV, ...]."""
+    shape, st, size = t.shape, t.stride(), t.element_size()
+    if len(shape) < 3 or shape[0] != pages or shape[1] != PAGE or shape[2] != H_KV or 0 in shape:
+        raise RuntimeError(f"{who}: a cache {tuple(shape)} must be [{pages}, {PAGE}, {H_KV}, ...]")
+    n = 1
+    for d in range(len(shape) - 1, 2, -1):
+        if st[d] != n and shape[d] != 1:
+            raise RuntimeError(f"{who}: the rows of a cache must be contiguous")
+        n *= shape[d]
+    return t.data_ptr(), st[0] * size, st[1] * size, st[2] * size, n * size
+
+
 def paged_kv_evict(block_tbl, ctx_len, weights, caches, PAGE, budget, recent=0, sinks=0, limit=None, ref=None, kept=None,
                    workspace=None):
     """Cut sequences of more than `limit` tokens (default: budget) back to `budget`, in place; returns kept.
@@ -1582,22 +1595,14 @@ def paged_kv_evict(block_tbl, ctx_len, weights, caches, PAGE, budget, recent=0, 
     if len(caches) == 0:
         raise RuntimeError(f"{who}: no caches of [pages, PAGE, H_KV, ...]")
     P = caches[0].shape[0] if caches[0].dim() else 0
-    cols = ([], [], [], [], [])  # base, strides from page to page, token to token and head to head, bytes of a row
-    for t in caches:
-        if t.dim() < 3 or t.shape[0] != P or t.shape[1] != PAGE or t.shape[2] != H_KV or t.numel() == 0:
-            raise RuntimeError(f"{who}: a cache {tuple(t.shape)} must be [{P}, {PAGE}, {H_KV}, ...]")
-        if t.dim() > 3 and not t[0, 0, 0].is_contiguous():
-            raise RuntimeError(f"{who}: the rows of a cache must be contiguous")
-        size, st = t.element_size(), t.stride()
-        for col, v in zip(cols, (t.data_ptr(), st[0] * size, st[1] * size, st[2] * size, t[0, 0, 0].numel() * size)):
-            col.append(v)
+    rows = [_cache_rows(who, t, P, PAGE, H_KV) for t in caches]
     if ref is not None:
         _int32_vec(who, "ref", ref, P)
     if kept is None:
         kept = torch.empty((B, H_KV, budget), dtype=torch.int32, device=ctx_len.device)
     elif kept.dtype != torch.int32 or kept.shape != (B, H_KV, budget) or not kept.is_contiguous():
         raise RuntimeError(f"{who}: kept must be contiguous int32 [{B}, {H_KV}, {budget}]")
-    words = array.array("q", sum(cols, []))
+    words = array.array("q", [v for col in zip(*rows) for v in col])
     at, n = words.buffer_info()[0], len(caches)
     wptr, wbytes = _workspace(workspace, dev).ensure(_lib.lib().specq_kv_evict_workspace_size(B, H_KV))
     _call_on(dev, "specq_kv_evict", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C, _ptr(ref),
