@@ -93,67 +93,73 @@ __global__ __launch_bounds__(256) void qk_norm_vec_kernel(QkNormParams p) {
 #pragma unroll
     for (int e = 0; e < NP; ++e) rotary_angle(rotary_freq(rp, NP * u + e), pos, rp.mscale, c[e], s[e]);
   }
-  constexpr int U = 4;  // heads whose loads go out together
-  for (int h0 = hl; h0 < heads; h0 += U * lanes) {
-    v8h x[U], y[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      x[k] = v8h{}, y[k] = v8h{};
-      const int h = h0 + k * lanes;
-      if (h >= heads || !some) continue;
-      const RotaryHead r = rotary_head(rp, b, i, h);
-      x[k] = *reinterpret_cast<const v8h*>(r.src + at);
-      if (!IL && turned) y[k] = *reinterpret_cast<const v8h*>(r.src + at + rp.R / 2);
-    }
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int h = h0 + k * lanes;
-      if (h >= heads) break;
-      float sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        sum = fmaf((float)x[k][e], (float)x[k][e], sum);
-        if (!IL) sum = fmaf((float)y[k][e], (float)y[k][e], sum);
-      }
-      const float scale = rsqrtf(fmaf(group_sum<UP>(sum), p.inv_d, p.eps));
-      if (!some) continue;
-      const RotaryHead r = rotary_head(rp, b, i, h);
+  // Weights and turns in one: with (x, y) a pair, its new values are scale (x cx - y sy) and scale (y cy + x sx); a value that
+  // is not turned becomes scale x cx.  Made anew where q's heads end, and for each head where each has its weights.
+  constexpr int NC = IL ? 4 : 8;
+  float cx[8], sx[NC], cy[NC], sy[NC];
+  int have = -1;
+  // A head at a time: with the loads of four or five ahead the registers leave fewer waves (2 x 4096 tokens, 32 / 8 heads of
+  // 128: 42 us against 38).
+  for (int h = hl; h < heads; h += lanes) {
+    const RotaryHead r = rotary_head(rp, b, i, h);
+    v8h x = {}, y = {};
+    if (some) x = *reinterpret_cast<const v8h*>(r.src + at);
+    if (!IL && turned) y = *reinterpret_cast<const v8h*>(r.src + at + rp.R / 2);
+    const int kind = h >= rp.H;
+    if (some && (kind != have || (kind ? p.s_wk : p.s_wq) != 0)) {
+      have = kind;
       const NormWeights w = norm_weights(p, h);
-      float wx[8];
+      float wx[8], wy[8];
       w.at8(at, wx);
-      v8h ox;
       if (!turned) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ox[e] = (_Float16)((float)x[k][e] * scale * wx[e]);
-      } else if constexpr (IL) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float a0 = (float)x[k][2 * e] * scale * wx[2 * e], a1 = (float)x[k][2 * e + 1] * scale * wx[2 * e + 1];
-          ox[2 * e] = (_Float16)(a0 * c[e] - a1 * s[e]);
-          ox[2 * e + 1] = (_Float16)(a1 * c[e] + a0 * s[e]);
-        }
+        for (int e = 0; e < 8; ++e) cx[e] = wx[e];
       } else {
-        float wy[8];
-        w.at8(at + rp.R / 2, wy);
-        v8h oy;
+        if constexpr (!IL) w.at8(at + rp.R / 2, wy);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float a0 = (float)x[k][e] * scale * wx[e], a1 = (float)y[k][e] * scale * wy[e];
-          ox[e] = (_Float16)(a0 * c[e] - a1 * s[e]);
-          oy[e] = (_Float16)(a1 * c[e] + a0 * s[e]);
+        for (int e = 0; e < NP; ++e) {
+          const float a = IL ? wx[(2 * e) & 7] : wx[e & 7], o = IL ? wx[(2 * e + 1) & 7] : wy[e & 7];
+          cx[e] = a * c[e], sx[e] = a * s[e], cy[e] = o * c[e], sy[e] = o * s[e];
         }
-        *reinterpret_cast<v8h*>(r.dst + at + rp.R / 2) = oy;
       }
-      *reinterpret_cast<v8h*>(r.dst + at) = ox;
     }
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      sum = fmaf((float)x[e], (float)x[e], sum);
+      if (!IL) sum = fmaf((float)y[e], (float)y[e], sum);
+    }
+    const float scale = rsqrtf(fmaf(group_sum<UP>(sum), p.inv_d, p.eps));
+    if (!some) continue;
+    if (!turned) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (_Float16)((float)x[e] * scale * cx[e]);
+    } else if constexpr (IL) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = (float)x[2 * e] * scale, o = (float)x[2 * e + 1] * scale;
+        x[2 * e] = (_Float16)(a * cx[e] - o * sy[e]);
+        x[2 * e + 1] = (_Float16)(o * cy[e] + a * sx[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = (float)x[e] * scale, o = (float)y[e] * scale;
+        x[e] = (_Float16)(a * cx[e] - o * sy[e]);
+        y[e] = (_Float16)(o * cy[e] + a * sx[e]);
+      }
+      *reinterpret_cast<v8h*>(r.dst + at + rp.R / 2) = y;
+    }
+    *reinterpret_cast<v8h*>(r.dst + at) = x;
   }
 }
 
 // Any R, D and alignment, 2 bytes an access: a wave owns a row, a lane every 64th of its pairs and single values, and
-// walks every fourth head.
+// walks the heads with the workgroup's other waves: 16 of them where there are few tokens, so that few rows follow one
+// another (51 tokens, 12 / 3 heads of 80: 8.3 us with four).
 constexpr int kNormItems = 8;  // pairs and values a lane has at most: D <= 512
 template <bool IL>
-__global__ __launch_bounds__(256) void qk_norm_any_kernel(QkNormParams p) {
+__global__ __launch_bounds__(1024) void qk_norm_any_kernel(QkNormParams p) {
   const RotaryParams& rp = p.r;
   int b, i, pos;
   if (!rotary_token(rp, blockIdx.x, b, i, pos)) return;
@@ -172,7 +178,7 @@ __global__ __launch_bounds__(256) void qk_norm_any_kernel(QkNormParams p) {
       i0[e] = rp.R + u - np;
     }
   }
-  for (int h = wave_id(); h < heads; h += 4) {
+  for (int h = wave_id(); h < heads; h += (int)blockDim.x / kWave) {
     const RotaryHead r = rotary_head(rp, b, i, h);
     const NormWeights w = norm_weights(p, h);
     float x[kNormItems], y[kNormItems], sum = 0.f;
@@ -255,7 +261,7 @@ extern "C" int specq_qk_norm_rotary(const void* q, int64_t s_qb, int64_t s_qt, i
   if (bits % 16 != 0 || D % 8 != 0 || R % per != 0) {
     const void* fn = interleaved ? reinterpret_cast<const void*>(&qk_norm_any_kernel<true>)
                                  : reinterpret_cast<const void*>(&qk_norm_any_kernel<false>);
-    return launch(fn, (int)tokens, 256, 0, (hipStream_t)stream, &p);
+    return launch(fn, (int)tokens, tokens <= 1024 ? 1024 : 256, 0, (hipStream_t)stream, &p);
   }
   // As the rotary kernel: few tokens have a workgroup each, many a wave each.
   r.tpt = tokens <= 1024 ? 256 : 64;
