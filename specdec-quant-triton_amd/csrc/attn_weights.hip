@@ -518,8 +518,9 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
     };
     // The first block with a row that sees the wave's first token, none where the wave sees nothing.
     const int first = seen == 0 ? blocks : t0 > fresh ? min((t0 - fresh) * p.G / 16, blocks) : 0;
-    for (int seg = 0; seg < blocks; seg += kAwSeg) {
-      const int seg_end = min(seg + kAwSeg, blocks);
+    constexpr int kSeg = MODE == kAwSums ? 1 << 30 : kAwSeg;  // sums need no segments
+    for (int seg = 0; seg < blocks; seg += kSeg) {
+      const int seg_end = min(seg + kSeg, blocks);
       if constexpr (MODE != kAwSums)
         for (int rb = seg + odd; rb < min(first, seg_end); rb += 2)
           if (g == 0) s_stat[w][(rb - seg) * 16 + r] = aw_pack(-INFINITY, 0.f);
