@@ -468,7 +468,7 @@ int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_qt, int64_t 
  *   kept      int32 [B, H_KV, budget];  0 <= recent + sinks <= budget <= limit
  *   Workspace: specq_kv_evict_workspace_size() bytes, as the workspaces above.
  * ------------------------------------------------------------------------------------- */
-size_t specq_kv_evict_workspace_size(int B, int H_KV);
+size_t specq_kv_evict_workspace_size(int B, int H_KV, int max_pages, int PAGE);
 int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int max_pages, const int32_t* ref, int n_pages,
                    int32_t* ctx_len, float* weights, int64_t s_wb, int64_t s_wh, int H_KV, int PAGE,
                    int n_tensors, void* const* base, const int64_t* page_stride, const int64_t* token_stride,

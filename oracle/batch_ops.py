@@ -78,10 +78,9 @@ def evict(bt, ctx, w, caches, budget, recent, sinks, limit, ref=None):
             src = sorted(held | set(others[:budget - len(held)]))
             kept[b, h] = src
             w[b, h, :budget] = w[b, h, src].copy()
+            t, j = np.array(src), np.arange(budget)
             for c in caches:
-                rows = [c[bt[b, t // PAGE], t % PAGE, h].copy() for t in src]
-                for j, row in enumerate(rows):
-                    c[bt[b, j // PAGE], j % PAGE, h] = row
+                c[bt[b, j // PAGE], j % PAGE, h] = c[bt[b, t // PAGE], t % PAGE, h].copy()
         ctx[b] = budget
     return kept, ctx, w, caches
 

@@ -29,6 +29,7 @@ constexpr int kEvStep = 4 * kEvThreads;  // positions of a chunk, four consecuti
 constexpr int kEvGroup = 4;              // chunks that are loaded, and ranked, together
 constexpr int kEvCopies = 4;             // histograms that lanes take in turn, since many weights share a digit
 constexpr int kEvList = 8192;            // keys of one upper digit
+constexpr int kEvSlices = 64;            // most slices of a row
 constexpr int kEvTensors = 16;  // cache tensors of a call
 constexpr int kEvUnits = 256;   // byte ranges of a call
 constexpr int kEvPages = 4096;  // table entries whose pages' places are kept in LDS
@@ -42,6 +43,10 @@ struct EvictParams {
   int32_t* kept;           // [B, H][budget]
   int32_t* flag;           // workspace, [B, H]: whether the sequence is cut back
   int H, PAGE, cap, budget, recent, sinks, limit;
+  // Long rows: slices of slice_len positions (1 to 4 chunks).  Workspace, for each slice: a histogram, whether its pages may be
+  // written, its keys above the upper digit and its keys of that digit; for each row that digit and what lies above it.
+  int slices, slice_len;
+  int32_t* hist; int32_t* slice_ok; int32_t* slice_above; int32_t* slice_n; uint32_t* list; int32_t* digit;
 };
 
 struct EvictMoveParams {
@@ -94,169 +99,356 @@ __device__ __forceinline__ uint32_t ev_key(float w) {
   return (uint32_t)u ^ ((uint32_t)(u >> 31) | 0x80000000u);
 }
 
-__global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictParams p) {
-  __shared__ int hist[kEvCopies][kEvBins], part[kEvGroup][kEvWaves], s_bin, s_above, s_in, s_list_n;
-  __shared__ uint32_t s_list[kEvList];
-  const int prog = blockIdx.x, b = prog / p.H, h = prog - b * p.H, tid = threadIdx.x;
-  const int L = min(max(p.ctx_len[b], 0), p.cap);
-  int32_t* kept = p.kept + (int64_t)prog * p.budget;
-  const float* wr = p.w + b * p.s_wb + h * p.s_wh;
-  constexpr int kSpan = kEvGroup * kEvStep;
+constexpr int kEvSpan = kEvGroup * kEvStep;  // positions of a group
+typedef uint32_t EvKeys[kEvGroup][4];
+
+// A (sequence, head)'s row of weights.
+struct EvRow {
+  const float* w;
+  int L, sinks, recent, vec;
   // Whether all of a chunk's tokens compete.
-  auto inner = [&](int at) { return at >= p.sinks && at + kEvStep <= L - p.recent; };
+  __device__ __forceinline__ bool inner(int at) const { return at >= sinks && at + kEvStep <= L - recent; }
   // Keys of the thread's positions of the group from g0 on; behind the context 0, which no weight has and none is found to be.
-  auto load = [&](int g0, uint32_t (&k)[kEvGroup][4]) {
+  __device__ __forceinline__ void load(int g0, EvKeys& k) const {
 #pragma unroll
     for (int c = 0; c < kEvGroup; ++c) {
-      const int t = g0 + c * kEvStep + 4 * tid;
+      const int t = g0 + c * kEvStep + 4 * (int)threadIdx.x;
       v4f x = {0.f, 0.f, 0.f, 0.f};
-      if (p.w_vec && t + 4 <= L) {
-        x = *reinterpret_cast<const v4f*>(wr + t);
+      if (vec && t + 4 <= L) {
+        x = *reinterpret_cast<const v4f*>(w + t);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (t + i < L) x[i] = wr[t + i];
+          if (t + i < L) x[i] = w[t + i];
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) k[c][i] = ev_key(x[i]);
       if (!inner(g0 + c * kEvStep)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          k[c][i] = t + i >= L ? 0u : t + i < p.sinks || t + i >= L - p.recent ? 0xFFFFFFFFu : k[c][i];
+          k[c][i] = t + i >= L ? 0u : t + i < sinks || t + i >= L - recent ? 0xFFFFFFFFu : k[c][i];
       }
     }
-  };
+  }
+};
+__device__ __forceinline__ EvRow ev_row(const EvictParams& p, int b, int h, int L) {
+  return {p.w + b * p.s_wb + h * p.s_wh, L, p.sinks, p.recent, p.w_vec};
+}
+// Whether the table's columns c0..c1 - 1 of row b name pages of the pool that no other row names (as far as counts are given).
+__device__ __forceinline__ int ev_pages_ok(const EvictParams& p, int b, int c0, int c1) {
+  int ok = 1;
+  for (int c = c0 + (int)threadIdx.x; c < c1; c += kEvThreads) {
+    const int id = p.bt[b * p.s_bt + c];
+    if ((uint32_t)id >= (uint32_t)p.P || (p.ref != nullptr && p.ref[id] > 1)) ok = 0;
+  }
+  return ok;
+}
+
+// One digit of the key that is looked for.
+struct EvDigit {
+  int bin, above, in;  // it, the keys with larger ones, and with it
+};
+typedef int EvHist[kEvCopies][kEvBins];
+// The digit of the want-th largest key, from its histogram (which is cleared).
+__device__ __forceinline__ EvDigit ev_digit(EvHist& hist, int want, int (&part)[kEvGroup][kEvWaves], EvDigit& shared) {
+  // Thread i has bins 2047 - 2 i and 2046 - 2 i: the prefix runs from the largest digit down.
+  const int hi = kEvBins - 1 - 2 * (int)threadIdx.x;
+  int n1 = 0, n0 = 0;
+#pragma unroll
+  for (int c = 0; c < kEvCopies; ++c) {
+    v2i* at = reinterpret_cast<v2i*>(&hist[c][hi - 1]);
+    const v2i n = *at;
+    *at = v2i{0, 0};
+    n0 += n[0], n1 += n[1];
+  }
+  int sum[1] = {n1 + n0}, total[1];
+  ev_prefix(sum, total, part);
+  const int above = sum[0];
+  if (above < want && above + n1 + n0 >= want) {
+    const bool first = above + n1 >= want;
+    shared = {first ? hi : hi - 1, first ? above : above + n1, first ? n1 : n0};
+  }
+  __syncthreads();
+  return shared;
+}
+
+// What is known of the budget-th largest key: the keys from `larger` on stay, and of those that equal `found` the first `want`.
+struct EvCut {
+  uint32_t found, larger;
+  int want;
+  bool ties;  // some equal ones do not stay (else they count as larger; the largest key's tokens all stay)
+};
+__device__ __forceinline__ EvCut ev_cut(uint32_t found, int want, int in) {
+  return {found, in == want ? found : found + 1, want, in != want};
+}
+// Ranks a group's tokens that stay, `above` larger and `equal` equal ones before them.
+__device__ __forceinline__ void ev_rank(const EvCut& cut, const EvKeys& k, int g0, int L, int& above, int& equal, int32_t* kept,
+                                        int (&part)[kEvGroup][kEvWaves]) {
+  int count[kEvGroup], total[kEvGroup];  // larger keys of a chunk, and equal ones above bit 16
+#pragma unroll
+  for (int c = 0; c < kEvGroup; ++c) {
+    count[c] = 0;
+    if (g0 + c * kEvStep >= L) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) count[c] += k[c][i] >= cut.larger;
+    if (cut.ties) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) count[c] += (k[c][i] == cut.found) << 16;
+    }
+  }
+  ev_prefix(count, total, part);
+#pragma unroll
+  for (int c = 0; c < kEvGroup; ++c) {
+    if (g0 + c * kEvStep >= L) break;
+    const int t = g0 + c * kEvStep + 4 * (int)threadIdx.x;
+    int a = above + (count[c] & 0xFFFF), e = equal + (count[c] >> 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool gt = k[c][i] >= cut.larger, eq = cut.ties && k[c][i] == cut.found;
+      if (gt || (eq && e < cut.want)) kept[a + min(e, cut.want)] = t + i;
+      a += gt;
+      e += eq;
+    }
+    above += total[c] & 0xFFFF;
+    equal += total[c] >> 16;
+  }
+}
+// A sequence that stays as it is.
+__device__ __forceinline__ void ev_stays(const EvictParams& p, int L, int32_t* kept) {
+  for (int j = threadIdx.x; j < p.budget; j += kEvThreads) kept[j] = j < L ? j : -1;
+}
+
+__global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictParams p) {
+  __shared__ EvHist hist;
+  __shared__ int part[kEvGroup][kEvWaves], s_list_n;
+  __shared__ EvDigit s_digit;
+  __shared__ uint32_t s_list[kEvList];
+  const int prog = blockIdx.x, b = prog / p.H, h = prog - b * p.H, tid = threadIdx.x;
+  const int L = min(max(p.ctx_len[b], 0), p.cap);
+  int32_t* kept = p.kept + (int64_t)prog * p.budget;
+  const EvRow row = ev_row(p, b, h, L);
   for (int i = tid; i < kEvCopies * kEvBins; i += kEvThreads) hist[0][i] = 0;
   int ok = L > p.limit;
-  uint32_t near[kEvGroup][4];
+  EvKeys near;
   if (ok) {
-    load(0, near);
-    const int32_t* row = p.bt + b * p.s_bt;
-    for (int c = tid; c < (L + p.PAGE - 1) / p.PAGE; c += kEvThreads) {
-      const int id = row[c];
-      if ((uint32_t)id >= (uint32_t)p.P || (p.ref != nullptr && p.ref[id] > 1)) ok = 0;
-    }
-    ok = __syncthreads_and(ok);
+    row.load(0, near);
+    ok = __syncthreads_and(ev_pages_ok(p, b, 0, (L + p.PAGE - 1) / p.PAGE));
   }
   if (tid == 0) p.flag[prog] = ok;
-  if (!ok) {
-    for (int j = tid; j < p.budget; j += kEvThreads) kept[j] = j < L ? j : -1;
-    return;
-  }
-  // f(chunk of the group, the thread's four keys) of each chunk with tokens; `group` behind each four.
-  auto each = [&](auto&& f, auto&& group) {
+  if (!ok) return ev_stays(p, L, kept);
+  auto each = [&](auto&& f) {  // f(first position, keys) of each group
 #pragma unroll 1
-    for (int g0 = 0; g0 < L; g0 += kSpan) {
-      uint32_t k[kEvGroup][4];
+    for (int g0 = 0; g0 < L; g0 += kEvSpan) {
+      EvKeys k;
       if (g0 == 0) {
 #pragma unroll
         for (int c = 0; c < kEvGroup; ++c)
 #pragma unroll
           for (int i = 0; i < 4; ++i) k[c][i] = near[c][i];
       } else {
-        load(g0, k);
+        row.load(g0, k);
       }
-#pragma unroll
-      for (int c = 0; c < kEvGroup; ++c) {
-        const int at = g0 + c * kEvStep;
-        if (at < L) f(c, k[c]);
-      }
-      group(g0, k);
+      f(g0, k);
     }
   };
-  auto nothing = [](int, const uint32_t (&)[kEvGroup][4]) {};
+  auto keys = [&](auto&& f) {  // f(key) of each key, and of some 0
+    each([&](int g0, const EvKeys& k) {
+#pragma unroll
+      for (int c = 0; c < kEvGroup; ++c) {
+        if (g0 + c * kEvStep >= L) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f(k[c][i]);
+      }
+    });
+  };
   // The budget-th largest key, from its top digit down: `want` of those under the digits found so far.
   uint32_t found = 0, known = 0;  // its digits, and a mask of them
-  int want = p.budget;
+  int want = p.budget, in = 0;
   bool listed = false;
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int low = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass < 2 ? 2048 : 1024;
     int* mine = hist[tid % kEvCopies];
-    if (pass == 0) {
-      each([&](int, const uint32_t (&k)[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) atomicAdd(&mine[k[i] >> 21], 1);
-      }, nothing);
-    } else if (listed) {
-      for (int i = tid; i < s_list_n; i += kEvThreads)
-        if (((s_list[i] ^ found) & known) == 0) atomicAdd(&mine[(s_list[i] >> low) & (bins - 1)], 1);
-    } else {
-      each([&](int, const uint32_t (&k)[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (((k[i] ^ found) & known) == 0) atomicAdd(&mine[(k[i] >> low) & (bins - 1)], 1);
-      }, nothing);
-    }
-    __syncthreads();
-    // Thread i has bins 2047 - 2 i and 2046 - 2 i, and clears them: the prefix runs from the largest digit down.
-    const int hi = kEvBins - 1 - 2 * tid;
-    int n1 = 0, n0 = 0;
-#pragma unroll
-    for (int c = 0; c < kEvCopies; ++c) {
-      v2i* at = reinterpret_cast<v2i*>(&hist[c][hi - 1]);
-      const v2i n = *at;
-      *at = v2i{0, 0};
-      n0 += n[0], n1 += n[1];
-    }
-    int sum[1] = {n1 + n0}, total[1];
-    ev_prefix(sum, total, part);
-    const int above = sum[0];
-    if (above < want && above + n1 + n0 >= want) {
-      const bool first = above + n1 >= want;
-      s_bin = first ? hi : hi - 1;
-      s_above = first ? above : above + n1;
-      s_in = first ? n1 : n0;
-    }
+    auto count = [&](uint32_t k) {
+      if (((k ^ found) & known) == 0) atomicAdd(&mine[(k >> low) & (bins - 1)], 1);
+    };
+    if (pass == 0) keys([&](uint32_t k) { atomicAdd(&mine[k >> 21], 1); });
+    else if (listed) for (int i = tid; i < s_list_n; i += kEvThreads) count(s_list[i]);
+    else keys(count);
     if (tid == 0 && pass == 0) s_list_n = 0;
     __syncthreads();
-    found |= (uint32_t)s_bin << low;
+    const EvDigit d = ev_digit(hist, want, part, s_digit);
+    found |= (uint32_t)d.bin << low;
     known |= (uint32_t)(bins - 1) << low;
-    want -= s_above;
-    if (pass == 0 && s_in <= kEvList) {
+    want -= d.above;
+    in = d.in;
+    if (pass == 0 && in <= kEvList) {
       listed = true;
-      each([&](int, const uint32_t (&k)[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (((k[i] ^ found) & known) == 0) s_list[atomicAdd(&s_list_n, 1)] = k[i];
-      }, nothing);
+      keys([&](uint32_t k) {
+        if (((k ^ found) & known) == 0) s_list[atomicAdd(&s_list_n, 1)] = k;
+      });
     }
     __syncthreads();
   }
-  // `want` keys equal to `found` stay, the lowest positions; everything larger stays.  Counts of a chunk: larger keys, and equal
-  // ones above bit 16; where all equal ones stay, they count as larger.
-  const uint32_t larger = s_in == want ? found : found + 1;  // (the largest key's tokens all stay)
-  const bool ties = s_in != want;
-  int above = 0, equal = 0, count[kEvGroup] = {0, 0, 0, 0};
-  each([&](int c, const uint32_t (&k)[4]) {
-    int x = 0;
+  const EvCut cut = ev_cut(found, want, in);
+  int above = 0, equal = 0;
+  each([&](int g0, const EvKeys& k) { ev_rank(cut, k, g0, L, above, equal, kept, part); });
+}
+
+// ---- The same over slices of long rows, a workgroup each, in three launches: the upper digit's histograms; the digit, from
+// all slices' (each workgroup for itself), and the slice's keys that have it, listed; the other digits, from the lists,
+// and the ranks, behind those of the slices before.  Plain stores and loads between them.
+struct EvSlice {
+  int prog, slice, b, h, L, live, g0;  // live: slices with tokens; g0: the slice's first position
+  int64_t at;                          // the slice's place among all
+};
+__device__ __forceinline__ bool ev_slice(const EvictParams& p, EvSlice& s) {
+  s.prog = (int)blockIdx.x / p.slices;
+  s.slice = (int)blockIdx.x - s.prog * p.slices;
+  s.b = s.prog / p.H;
+  s.h = s.prog - s.b * p.H;
+  s.L = min(max(p.ctx_len[s.b], 0), p.cap);
+  s.live = (s.L + p.slice_len - 1) / p.slice_len;
+  s.g0 = s.slice * p.slice_len;
+  s.at = (int64_t)s.prog * p.slices + s.slice;
+  return s.L > p.limit && s.slice < s.live;
+}
+// Keys of the slice alone: those of later ones in the group are 0.
+__device__ __forceinline__ void ev_slice_keys(const EvictParams& p, const EvSlice& s, EvKeys& k) {
+  ev_row(p, s.b, s.h, s.L).load(s.g0, k);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x += k[i] >= larger;
-    if (ties) {
+  for (int c = 0; c < kEvGroup; ++c)
+    if (c * kEvStep >= p.slice_len) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x += (k[i] == found) << 16;
+      for (int i = 0; i < 4; ++i) k[c][i] = 0;
     }
-    count[c] = x;
-  }, [&](int g0, const uint32_t (&k)[kEvGroup][4]) {
-    int total[kEvGroup];
-    ev_prefix(count, total, part);
+}
+
+__global__ __launch_bounds__(kEvThreads) void evict_slice_count_kernel(EvictParams p) {
+  __shared__ EvHist hist;
+  EvSlice s;
+  if (!ev_slice(p, s)) return;
+  EvKeys k;
+  ev_slice_keys(p, s, k);
+  for (int i = threadIdx.x; i < kEvCopies * kEvBins; i += kEvThreads) hist[0][i] = 0;
+  const int end = min(s.g0 + p.slice_len, s.L);
+  const int ok = __syncthreads_and(ev_pages_ok(p, s.b, s.g0 / p.PAGE, (end + p.PAGE - 1) / p.PAGE));
+  int* mine = hist[threadIdx.x % kEvCopies];
 #pragma unroll
-    for (int c = 0; c < kEvGroup; ++c) {
-      if (g0 + c * kEvStep >= L) break;
-      const int t = g0 + c * kEvStep + 4 * tid;
-      int a = above + (count[c] & 0xFFFF), e = equal + (count[c] >> 16);
+  for (int c = 0; c < kEvGroup; ++c) {
+    if (c * kEvStep >= p.slice_len || s.g0 + c * kEvStep >= s.L) break;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool gt = k[c][i] >= larger, eq = ties && k[c][i] == found;
-        if (gt || (eq && e < want)) kept[a + min(e, want)] = t + i;
-        a += gt;
-        e += eq;
-      }
-      above += total[c] & 0xFFFF;
-      equal += total[c] >> 16;
-      count[c] = 0;
+    for (int i = 0; i < 4; ++i) atomicAdd(&mine[k[c][i] >> 21], 1);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kEvBins; i += kEvThreads) {
+    int n = 0;
+#pragma unroll
+    for (int c = 0; c < kEvCopies; ++c) n += hist[c][i];
+    p.hist[s.at * kEvBins + i] = n;
+  }
+  if (threadIdx.x == 0) p.slice_ok[s.at] = ok;
+}
+
+__global__ __launch_bounds__(kEvThreads) void evict_slice_list_kernel(EvictParams p) {
+  __shared__ EvHist hist;
+  __shared__ int part[kEvGroup][kEvWaves], s_n;
+  __shared__ EvDigit s_digit;
+  EvSlice s;
+  if (!ev_slice(p, s)) return;
+  EvKeys k;
+  ev_slice_keys(p, s, k);
+  const int tid = threadIdx.x;
+  v2i sum = {0, 0};
+  const int32_t* counts = p.hist + (int64_t)s.prog * p.slices * kEvBins + 2 * tid;
+#pragma unroll 8
+  for (int i = 0; i < s.live; ++i) sum += *reinterpret_cast<const v2i*>(counts + (int64_t)i * kEvBins);
+#pragma unroll
+  for (int c = 0; c < kEvCopies; ++c) *reinterpret_cast<v2i*>(&hist[c][2 * tid]) = c == 0 ? sum : v2i{0, 0};
+  if (tid == 0) s_n = 0;
+  __syncthreads();
+  const EvDigit d = ev_digit(hist, p.budget, part, s_digit);
+  int above[1] = {0}, total[1];
+  uint32_t* list = p.list + s.at * p.slice_len;
+#pragma unroll
+  for (int c = 0; c < kEvGroup; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int digit = (int)(k[c][i] >> 21);  // 0 is no key's, and not the one found
+      above[0] += digit > d.bin;
+      if (digit == d.bin) list[atomicAdd(&s_n, 1)] = k[c][i];
     }
+  ev_prefix(above, total, part);
+  if (tid == 0) {
+    p.slice_n[s.at] = s_n;
+    p.slice_above[s.at] = total[0];
+    if (s.slice == 0) p.digit[2 * s.prog] = d.bin, p.digit[2 * s.prog + 1] = d.above;
+  }
+}
+
+__global__ __launch_bounds__(kEvThreads) void evict_slice_rank_kernel(EvictParams p) {
+  __shared__ EvHist hist;
+  __shared__ int part[kEvGroup][kEvWaves];
+  __shared__ EvDigit s_digit;
+  __shared__ int s_n[kEvSlices], s_before[2];
+  EvSlice s;
+  const bool some = ev_slice(p, s);
+  int32_t* kept = p.kept + (int64_t)s.prog * p.budget;
+  const int64_t first = (int64_t)s.prog * p.slices;
+  const int tid = threadIdx.x, wave = uniform(wave_id()), lane = lane_id();
+  int ok = s.L > p.limit;
+  if (ok) {
+    ok = __syncthreads_and(tid < s.live ? p.slice_ok[first + tid] : 1);
+  }
+  if (s.slice == 0) {
+    if (tid == 0) p.flag[s.prog] = ok;
+    if (!ok) ev_stays(p, s.L, kept);
+  }
+  if (!ok || !some) return;
+  EvKeys k;
+  ev_slice_keys(p, s, k);
+  for (int i = tid; i < kEvCopies * kEvBins; i += kEvThreads) hist[0][i] = 0;
+  if (tid < s.live) s_n[tid] = p.slice_n[first + tid];
+  if (tid < 2) s_before[tid] = 0;
+  __syncthreads();
+  uint32_t found = (uint32_t)p.digit[2 * s.prog] << 21, known = 0x7FFu << 21;
+  int want = p.budget - p.digit[2 * s.prog + 1], in = 0;
+  auto lists = [&](auto&& f) {  // f(slice, key); a wave takes every 16th slice's
+    for (int i = wave; i < s.live; i += kEvWaves) {
+      const uint32_t* list = p.list + (first + i) * p.slice_len;
+      const int n = s_n[i];
+#pragma unroll 4
+      for (int j = lane; j < n; j += kWave) f(i, list[j]);
+    }
+  };
+#pragma unroll 1
+  for (int pass = 1; pass < 3; ++pass) {
+    const int low = pass == 1 ? 10 : 0, bins = pass == 1 ? 2048 : 1024;
+    int* mine = hist[tid % kEvCopies];
+    lists([&](int, uint32_t k) {
+      if (((k ^ found) & known) == 0) atomicAdd(&mine[(k >> low) & (bins - 1)], 1);
+    });
+    __syncthreads();
+    const EvDigit d = ev_digit(hist, want, part, s_digit);
+    found |= (uint32_t)d.bin << low;
+    known |= (uint32_t)(bins - 1) << low;
+    want -= d.above;
+    in = d.in;
+    __syncthreads();
+  }
+  const EvCut cut = ev_cut(found, want, in);
+  // What stays of the slices before: their keys of larger digits, and of their lists.
+  int above = tid < s.slice ? p.slice_above[first + tid] : 0, equal = 0;
+  lists([&](int i, uint32_t k) {
+    if (i >= s.slice) return;
+    above += k >= cut.larger;
+    equal += cut.ties && k == cut.found;
   });
+  if (above != 0) atomicAdd(&s_before[0], above);
+  if (equal != 0) atomicAdd(&s_before[1], equal);
+  __syncthreads();
+  above = s_before[0], equal = s_before[1];
+  ev_rank(cut, k, s.g0, s.L, above, equal, kept, part);
 }
 
 // One byte range of one (sequence, head): accesses of sizeof(T) bytes, `lanes` of them a token.
@@ -342,9 +534,27 @@ __global__ __launch_bounds__(kEvMove) void evict_move_kernel(EvictMoveParams p) 
 
 using namespace specq;
 
-extern "C" size_t specq_kv_evict_workspace_size(int B, int H_KV) {
-  if (B <= 0 || H_KV <= 0) return 0;
-  return kCounterBytes + align_up((size_t)B * H_KV * 4, 256);
+namespace specq {
+namespace {
+
+// Slices of a row of `cap` positions, where it is cut: long rows, few enough to leave half of the CUs idle.  One workgroup takes
+// some 9 us and 2 more for each 4096 positions (65536 of two heads: 37 us), the three launches 25.
+struct EvSpace { int slices, slice_len; size_t words; };  // words of the workspace behind the flags
+EvSpace ev_space(int64_t progs, int64_t cap, int64_t cus) {
+  const int64_t chunks = ceil_div64(cap, kEvStep), per = ceil_div64(chunks, kEvSlices);
+  if (chunks <= 8 || per > kEvGroup || 2 * progs > cus) return {0, 0, 0};
+  const int slices = (int)ceil_div64(chunks, per), len = (int)per * kEvStep;
+  return {slices, len, (size_t)progs * (2 + (size_t)slices * (kEvBins + 3 + len))};
+}
+size_t ev_workspace(int64_t progs, const EvSpace& s) { return kCounterBytes + align_up((size_t)progs * 4, 256) + s.words * 4; }
+
+}  // namespace
+}  // namespace specq
+
+extern "C" size_t specq_kv_evict_workspace_size(int B, int H_KV, int max_pages, int PAGE) {
+  if (B <= 0 || H_KV <= 0 || max_pages <= 0 || PAGE <= 0) return 0;
+  const int64_t progs = (int64_t)B * H_KV;
+  return ev_workspace(progs, ev_space(progs, (int64_t)max_pages * PAGE, device_cus()));
 }
 
 extern "C" int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int max_pages, const int32_t* ref, int n_pages,
@@ -381,7 +591,8 @@ extern "C" int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int
     m.base[i] = static_cast<uint8_t*>(base[i]);
     m.s_p[i] = page_stride[i]; m.s_o[i] = token_stride[i]; m.s_h[i] = head_stride[i];
   }
-  const size_t need = specq_kv_evict_workspace_size(B, H_KV);
+  const EvSpace space = ev_space(progs, cap, device_cus());
+  const size_t need = ev_workspace(progs, space);
   SPECQ_REQUIRE(workspace && workspace_bytes >= need, SPECQ_ENOSPC, "kv_evict: workspace of %zu bytes required, %zu given", need,
                 workspace ? workspace_bytes : (size_t)0);
   p.bt = block_tbl; p.s_bt = s_bt; p.C = max_pages; p.P = n_pages; p.ref = ref; p.ctx_len = ctx_len;
@@ -424,6 +635,22 @@ extern "C" int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int
     m.page_shift = bits < 2 ? 0 : bits - 2;
   }
   hipStream_t st = (hipStream_t)stream;
-  if (int rc = launch(reinterpret_cast<const void*>(&evict_select_kernel), (int)progs, kEvThreads, 0, st, &p)) return rc;
+  if (space.slices == 0) {
+    if (int rc = launch(reinterpret_cast<const void*>(&evict_select_kernel), (int)progs, kEvThreads, 0, st, &p)) return rc;
+  } else {
+    const int64_t n = progs * space.slices;
+    p.slices = space.slices;
+    p.slice_len = space.slice_len;
+    p.hist = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + kCounterBytes + align_up((size_t)progs * 4, 256));
+    p.list = reinterpret_cast<uint32_t*>(p.hist + n * kEvBins);
+    p.slice_ok = p.hist + n * (kEvBins + space.slice_len);
+    p.slice_above = p.slice_ok + n;
+    p.slice_n = p.slice_above + n;
+    p.digit = p.slice_n + n;
+    for (const void* fn : {reinterpret_cast<const void*>(&evict_slice_count_kernel),
+                           reinterpret_cast<const void*>(&evict_slice_list_kernel),
+                           reinterpret_cast<const void*>(&evict_slice_rank_kernel)})
+      if (int rc = launch(fn, (int)n, kEvThreads, 0, st, &p)) return rc;
+  }
   return launch(reinterpret_cast<const void*>(&evict_move_kernel), (int)(align_up(progs, 8) * m.units), kEvMove, 0, st, &m);
 }

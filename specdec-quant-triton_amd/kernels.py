@@ -1548,6 +1548,13 @@ def paged_attention_weights(q, kc, ks, block_tbl, ctx_len, weights, q_len=None, 
     return weights
 
 
+@functools.lru_cache(maxsize=4096)
+def _evict_workspace(B, H_KV, max_pages, PAGE, dev) -> int:
+    """Bytes a call needs: a function of its sizes and the GPU's CU count."""
+    with torch.cuda.device(dev):
+        return _lib.lib().specq_kv_evict_workspace_size(B, H_KV, max_pages, PAGE)
+
+
 def _cache_rows(who: str, t, pages: int, PAGE: int, H_KV: int):
     """(base, strides from page to page, token to token and head to head, bytes of a row) of a cache [pages, PAGE, H_KV, ...]."""
     shape, st, size = t.shape, t.stride(), t.element_size()
@@ -1604,7 +1611,7 @@ def paged_kv_evict(block_tbl, ctx_len, weights, caches, PAGE, budget, recent=0, 
         raise RuntimeError(f"{who}: kept must be contiguous int32 [{B}, {H_KV}, {budget}]")
     words = array.array("q", [v for col in zip(*rows) for v in col])
     at, n = words.buffer_info()[0], len(caches)
-    wptr, wbytes = _workspace(workspace, dev).ensure(_lib.lib().specq_kv_evict_workspace_size(B, H_KV))
+    wptr, wbytes = _workspace(workspace, dev).ensure(_evict_workspace(B, H_KV, C, PAGE, dev))
     _call_on(dev, "specq_kv_evict", block_tbl.data_ptr(), block_tbl.stride(0) if B > 1 else C, B, C, _ptr(ref),
              min(P, 2**31 - 1), ctx_len.data_ptr(), weights.data_ptr(), s_wb, s_wh, H_KV, PAGE,
              n, at, at + 8 * n, at + 16 * n, at + 24 * n, at + 32 * n, budget, int(recent), int(sinks), limit,

@@ -119,7 +119,7 @@ SIGNATURES = {
                                           _c_vp, _c_vp, _c_vp, _c_i64, _c_i64,
                                           _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                           _c_float, _c_vp, _c_vp, _c_size, _c_vp]),
-    "specq_kv_evict_workspace_size": (_c_size, [_c_int, _c_int]),
+    "specq_kv_evict_workspace_size": (_c_size, [_c_int] * 4),
     "specq_kv_evict": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_vp, _c_i64, _c_i64, _c_int,
                                 _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int,
                                 _c_vp, _c_vp, _c_size, _c_vp]),

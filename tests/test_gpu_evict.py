@@ -55,6 +55,9 @@ def run_check(case, budget, recent, sinks, limit=None, ref=None, what=""):
     ([5000, 4097], 2, 64, 16, 1000, 100, 0),         # a chunk of positions and a little more
     ([9000], 1, 64, 32, 4500, 7, 1),                 # more than the registers hold
     ([64, 0, 1], 3, 16, 8, 63, 5, 50),               # rows of three heads, pages of 8
+    ([40000, 9000, 100], 1, 16, 64, 8200, 300, 5),   # a table of more tokens than one workgroup selects from
+    ([33000, 32768], 2, 16, 16, 32767, 4097, 0),
+    ([300000], 1, 16, 128, 70000, 64, 4),            # slices of more than one chunk
 ])
 def test_exact(ctx, HK, D, PAGE, budget, recent, sinks, weights):
     rng = np.random.default_rng(sum(ctx) + budget)
@@ -72,6 +75,23 @@ def test_special_weights():
     for budget in (1, 99, 250, 299):
         note(f"evict special budget={budget}")
         run_check(case, budget, 0, 0, what=f"budget {budget}")
+
+
+def test_long_rows_special_weights_and_pages():
+    """The slices of a long row: ties across them, NaN, a page that is none or shared in one of them."""
+    rng = np.random.default_rng(11)
+    case = make(rng, [50000, 36000, 45000], 1, 16, 64, "few")
+    bt, ctx, w, caches = case
+    P = len(caches[0])
+    w[0, 0, ::3], w[0, 0, 1::7], w[0, 0, 2::1001] = np.nan, -np.inf, np.inf
+    ref = np.bincount(bt[bt >= 0], minlength=P).astype(np.int32)
+    ref[bt[1, 400]] = 2
+    for budget in (1, 3000, 20000, 35999):
+        note(f"evict long special budget={budget}")
+        run_check(case, budget, 0, 0, ref=ref, what=f"budget {budget}")
+    bt[2, 700] = -1
+    note("evict long bad page")
+    run_check(case, 30000, 5000, 3, limit=40000, what="bad page")
 
 
 def test_limit_shared_and_bad_pages():
