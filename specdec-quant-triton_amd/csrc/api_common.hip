@@ -1,5 +1,6 @@
 // Shared host-side pieces of the C ABI: thread-local error text, launch wrapper, device info,
 // and the kernel-attribute query that dispatches to each kernel family.
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 #include <set>
@@ -40,8 +41,24 @@ void set_error(const char* fmt, ...) {
 
 void clear_error() { g_err[0] = '\0'; }
 
+bool nest_apart(std::initializer_list<TensorDim> dims, int64_t len) {
+  std::vector<TensorDim> d;
+  for (TensorDim x : dims)
+    if (x.n > 1) d.push_back({x.n, x.stride < 0 ? -x.stride : x.stride});
+  std::sort(d.begin(), d.end(), [](const TensorDim& a, const TensorDim& b) { return a.stride < b.stride; });
+  for (const TensorDim& x : d) {
+    if (x.stride < len) return false;
+    len += (x.n - 1) * x.stride;
+  }
+  return true;
+}
+
 int launch(const void* fn, int grid, int threads, size_t lds, hipStream_t stream, void* params) {
   if (grid <= 0) return SPECQ_OK;
+  if ((int64_t)grid * threads > UINT32_MAX) {
+    set_error("%d workgroups of %d threads are more than one launch takes", grid, threads);
+    return SPECQ_ENOTSUP;
+  }
   void* args[] = {params};
   hipError_t e = hipLaunchKernel(fn, dim3(grid), dim3(threads), args, lds, stream);
   if (e != hipSuccess) {

@@ -1,6 +1,7 @@
 // Host-side helpers shared by the C-ABI translation units: error reporting, argument checks.
 #pragma once
 #include <hip/hip_runtime.h>
+#include <initializer_list>
 #include <stdarg.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -59,6 +60,11 @@ inline int common_vec(std::initializer_list<uint64_t> vals) {
 // Whether the n entries of a written tensor's dimension, `stride` apart and `len` long, lie apart: an expanded dimension
 // (stride 0) or a closer one has several workgroups write one place.
 inline bool lie_apart(int64_t n, int64_t stride, int64_t len) { return n <= 1 || stride >= len || stride <= -len; }
+
+// Whether the rows of a written tensor, `len` long, lie apart over all its dimensions (entries, stride): taken by stride, each
+// steps over all that the ones before it cover.
+struct TensorDim { int64_t n, stride; };
+bool nest_apart(std::initializer_list<TensorDim> dims, int64_t len);
 
 int launch(const void* fn, int grid, int threads, size_t lds, hipStream_t stream, void* params);
 

@@ -699,7 +699,7 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   SPECQ_REQUIRE(s_ko < (1ll << 27) && s_ko >= 0, SPECQ_ENOTSUP, "paged_attn_weights: tokens %lld bytes apart", (long long)s_ko);
   SPECQ_REQUIRE((uintptr_t)ks % (scale_fp32 ? 4 : 2) == 0 && (uintptr_t)weights % 4 == 0, SPECQ_EINVAL,
                 "paged_attn_weights: scales and weights must be aligned to their type");
-  SPECQ_REQUIRE(lie_apart(B_grid, s_wb, cap) && lie_apart(H_KV, s_wh, cap), SPECQ_ENOTSUP,
+  SPECQ_REQUIRE(nest_apart({{B_grid, s_wb}, {H_KV, s_wh}}, cap), SPECQ_ENOTSUP,
                 "paged_attn_weights: rows of the weights overlap or are shorter than the table's %lld tokens", (long long)cap);
   if (B_grid == 0 || ql_grid == 0) return SPECQ_OK;
   AwParams p = {};

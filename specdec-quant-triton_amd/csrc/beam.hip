@@ -432,6 +432,7 @@ extern "C" int specq_beam_reorder(const int32_t* parents, int rows, int group, i
   for (int i = 0; i < n_tensors; ++i) {
     SPECQ_REQUIRE(base[i] && row_bytes[i] > 0 && (rows <= 1 || row_stride[i] >= row_bytes[i]), SPECQ_EINVAL,
                   "beam_reorder: state %d is null, empty or overlaps its own rows", i);
+    SPECQ_REQUIRE(base[i] != parents, SPECQ_EINVAL, "beam_reorder: the parents are no state");
     for (int j = 0; j < i; ++j) SPECQ_REQUIRE(base[j] != base[i], SPECQ_EINVAL, "beam_reorder: states %d and %d are one", j, i);
   }
   if (rows == 0 || group == 1) return SPECQ_OK;

@@ -572,7 +572,8 @@ extern "C" int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int
   SPECQ_REQUIRE(budget > 0 && recent >= 0 && sinks >= 0 && (int64_t)recent + sinks <= budget && limit >= budget, SPECQ_EINVAL,
                 "kv_evict: need 0 <= recent + sinks <= budget <= limit and budget > 0 (recent=%d sinks=%d budget=%d limit=%d)",
                 recent, sinks, budget, limit);
-  SPECQ_REQUIRE((uintptr_t)weights % 4 == 0 && lie_apart(B, s_wb, cap) && lie_apart(H_KV, s_wh, cap), SPECQ_ENOTSUP,
+  SPECQ_REQUIRE(budget <= (1 << 30), SPECQ_ENOTSUP, "kv_evict: a budget of %d tokens", budget);
+  SPECQ_REQUIRE((uintptr_t)weights % 4 == 0 && nest_apart({{B, s_wb}, {H_KV, s_wh}}, cap), SPECQ_ENOTSUP,
                 "kv_evict: rows of the weights overlap or are shorter than the table's %lld tokens", (long long)cap);
   SPECQ_REQUIRE(n_tensors >= 0 && n_tensors <= kEvTensors, SPECQ_ENOTSUP, "kv_evict: %d cache tensors (at most %d)", n_tensors,
                 kEvTensors);
@@ -585,8 +586,7 @@ extern "C" int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int
                   "kv_evict: cache tensor %d is null, or its rows of %lld bytes are not 1 to 4096", i, (long long)row_bytes[i]);
     for (int j = 0; j < i; ++j)
       SPECQ_REQUIRE(base[j] != base[i], SPECQ_EINVAL, "kv_evict: cache tensors %d and %d are one", j, i);
-    SPECQ_REQUIRE(lie_apart(n_pages, page_stride[i], row_bytes[i]) && lie_apart(PAGE, token_stride[i], row_bytes[i]) &&
-                      lie_apart(H_KV, head_stride[i], row_bytes[i]),
+    SPECQ_REQUIRE(nest_apart({{n_pages, page_stride[i]}, {PAGE, token_stride[i]}, {H_KV, head_stride[i]}}, row_bytes[i]),
                   SPECQ_ENOTSUP, "kv_evict: rows of cache tensor %d overlap", i);
     m.base[i] = static_cast<uint8_t*>(base[i]);
     m.s_p[i] = page_stride[i]; m.s_o[i] = token_stride[i]; m.s_h[i] = head_stride[i];

@@ -234,11 +234,11 @@ extern "C" int specq_qk_norm_rotary(const void* q, int64_t s_qb, int64_t s_qt, i
                 "qk_norm_rotary: need an even number R=%d of rotated dimensions, at most head_dim %d", R, D);
   SPECQ_REQUIRE(D <= 512, SPECQ_ENOTSUP, "qk_norm_rotary: head_dim %d (at most 512 supported)", D);
   SPECQ_REQUIRE(eps >= 0.f && eps < INFINITY, SPECQ_EINVAL, "qk_norm_rotary: eps must be finite and not negative");
-  SPECQ_REQUIRE(lie_apart(B_grid, s_qob, D) && lie_apart(ql_grid, s_qot, D) && lie_apart(H, s_qoh, D) &&
-                    (H_KV == 0 || (lie_apart(B_grid, s_kob, D) && lie_apart(ql_grid, s_kot, D) && lie_apart(H_KV, s_koh, D))),
-                SPECQ_ENOTSUP, "qk_norm_rotary: rows of an output overlap");
   const int64_t tokens = (int64_t)B_grid * ql_grid;
   SPECQ_REQUIRE(tokens <= INT32_MAX - 4, SPECQ_EINVAL, "qk_norm_rotary: grid too large");
+  SPECQ_REQUIRE(nest_apart({{B_grid, s_qob}, {ql_grid, s_qot}, {H, s_qoh}}, D) &&
+                    (H_KV == 0 || nest_apart({{B_grid, s_kob}, {ql_grid, s_kot}, {H_KV, s_koh}}, D)),
+                SPECQ_ENOTSUP, "qk_norm_rotary: rows of an output overlap");
   if (tokens == 0) return SPECQ_OK;
   QkNormParams p = {};
   RotaryParams& r = p.r;

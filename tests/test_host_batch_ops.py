@@ -36,6 +36,7 @@ def test_norm_refusals(built_lib):
     f(-22, eps=-1.0), f(-22, eps=float("nan")), f(-22, eps=float("inf")), f(-22, B=1 << 16, ql=1 << 16)
     for k in ("g", "h", "i", "j", "l", "m"):
         f(-95, **{k: 0}), f(-95, **{k: 56})
+    f(-95, h=64), f(-95, h=448), f(-95, g=512), f(-95, l=64), f(-95, j=128)  # (1, 0) and (0, 1) are, or share, one row
     f(0, B=0, n_seqs=0), f(0, ql=0, q_len=0)
 
 
@@ -47,6 +48,8 @@ def test_weights_refusals(built_lib):
     f(-22, max_pages=0), f(-22, n_pages=0), f(-22, max_pages=65), f(-95, max_pages=1 << 27, s_bt=1 << 27), f(-95, q=24), f(-95, s_qh=100)
     f(-95, kc=24), f(-95, s_kp=1000), f(-22, ks=18), f(-22, w=18), f(-95, s_wh=1023), f(-95, s_wb=0), f(-95, s_wh=0)
     f(-95, B=1 << 14, n_seqs=0), f(-95, ql=1 << 21, q_len=0), f(-28)
+    f(-95, s_wb=1024, s_wh=1024), f(-95, s_wb=1024, s_wh=2047), f(-28, s_wb=1024, s_wh=2048)  # (1, 0) and (0, 1) are one row
+    f(-95, H=8 * 4096)
     f(0, B=0, n_seqs=0), f(0, ql=0, q_len=0)
 
 
@@ -80,6 +83,8 @@ def test_evict_refusals(built_lib):
         f(-22, **{name: 0})
     f(-22, B=0), f(-22, HK=0), f(-22, C=0), f(-22, P=0), f(-22, PAGE=0), f(-22, C=65), f(-95, C=1 << 27, s_bt=1 << 27)
     f(-22, budget=0), f(-22, recent=-1), f(-22, sinks=-1), f(-22, recent=97), f(-22, recent=2 ** 31 - 1, sinks=2 ** 31 - 1), f(-22, limit=99)
+    f(-95, budget=(1 << 30) + 1, limit=2 ** 31 - 1)
+    f(-95, s_wb=1024, s_wh=1024), f(-95, sp=(15 * 1024 + 128,)), f(-95, so=(512,)), f(-28, so=(128,), sh=(2048,))
     f(-95, w=18), f(-95, s_wb=0), f(-95, s_wh=1023), f(-95, n=17), f(-95, n=-1)
     f(-22, base=(0,)), f(-22, rb=(0,)), f(-22, rb=(4097,)), f(-95, sp=(0,)), f(-95, so=(127,)), f(-95, sh=(64,))
     two = dict(n=2, sp=(16384, 16384), so=(1024, 1024), sh=(128, 128), rb=(128, 128))
@@ -104,11 +109,19 @@ def test_beam_refusals(built_lib):
     g = lambda code, **kw: _fail("specq_beam_reorder", states, code, **kw)  # noqa: E731
     g(-22, parents=0), g(-22, rows=-4), g(-22, rows=7), g(-22, group=0), g(-95, rows=33, group=33), g(-22, n=-1), g(-22, base=0)
     g(0, rows=0), g(0, group=1), g(0, n=0)
-    for i, v in ((0, (4096, 0)), (0, (4096, 4096)), (1, (128, 64)), (2, (128, 0)), (1, (-128, 128))):
+    for i, v in ((0, (4096, 0)), (0, (4096, 16)), (0, (4096, 4096)), (1, (128, 64)), (2, (128, 0)), (1, (-128, 128))):
         bad = np.asarray(v, np.int64)
         g(-22, **{("base", "stride", "bytes")[i]: bad.ctypes.data})
     wide = np.full(2, 1 << 50, np.int64)
     g(-95, stride=wide.ctypes.data, bytes=wide.ctypes.data)
+
+
+def test_launches_past_their_size(built_lib):
+    """More threads than a launch takes are refused ahead of it."""
+    _fail("specq_qk_norm_rotary", NORM, -95, B=1 << 13, ql=1 << 13, n_seqs=0, q_len=0, R=20, f=0, i=64, h=512, m=64)
+    keep = [np.asarray([v], np.int64) for v in (4096, 1 << 36, 1 << 36)]
+    _fail("specq_beam_reorder", dict(parents=16, rows=1 << 7, group=2, n=1, base=keep[0].ctypes.data, stride=keep[1].ctypes.data,
+                                     bytes=keep[2].ctypes.data, stream=0), -95)
 
 
 def test_sizes_past_their_types(built_lib):
