@@ -27,6 +27,7 @@ constexpr int kAwTile = 256;       // tokens of a workgroup: 4 waves of 4 sub-ti
 constexpr int kAwStoreRows = 16;   // rows whose scores go through the workspace
 constexpr int kAwFewRows = 64;     // rows whose queries a workgroup keeps in LDS
 constexpr int kAwSpan = 8;         // most tiles such a workgroup walks (its waves' lanes hold their pages, and one tile's more)
+constexpr int kAwLaunchRows = 1024;  // rows of a program that two launches take (their statistics: 32 bytes a token at most)
 constexpr int kAwSeg = 32;         // row blocks of 16 whose statistics are joined at a time
 constexpr int kAwSumTile = 1024;   // tokens of a workgroup that adds up stored scores
 constexpr int kAwMaxGrid = 1 << 16;
@@ -43,7 +44,8 @@ struct AwParams {
   int cap;      // tokens a row of the table holds
   int tiles;    // of cap
   int span;     // tiles of a workgroup of few rows
-  int rows;     // of a program at most: ql_grid * G
+  int rows;     // of a program and launch at most
+  int row0;     // the launch's first row: more than kAwLaunchRows have several launches one after another
   uint32_t g_magic;  // ceil(2^32 / G): row / G is its product's high word (rows below 2^20, G below 2^12); 0 for G = 1
   float scale_log2;
   // Workspace: scores [prog][rows][tiles * 256]; (max, sum) [prog][tiles][rows]; log2 of the rows' sums [prog][rows].
@@ -63,7 +65,7 @@ __device__ __forceinline__ int aw_order(const AwParams& p, int i) {
 __device__ __forceinline__ int aw_token(const AwParams& p, int row) {
   return p.g_magic != 0 ? (int)__umulhi((uint32_t)row, p.g_magic) : row;
 }
-// A program (sequence b, KV head h): its rows, tokens and active tiles.
+// A program (sequence b, KV head h): the launch's rows of it, its tokens and active tiles.
 struct AwProg {
   int b, h, ql, rows, L, tiles;
 };
@@ -77,7 +79,7 @@ __device__ __forceinline__ bool aw_prog(const AwParams& p, int prog, AwProg& x) 
   x.h = prog - x.b * p.H_KV;
   if (x.b >= n_seqs) return false;
   x.ql = p.q_lens != nullptr ? min(max(p.q_lens[x.b], 0), q_len) : q_len;
-  x.rows = x.ql * p.G;
+  x.rows = min(x.ql * p.G - p.row0, p.rows);
   x.L = min(max(p.ctx_len[x.b], 0), p.cap);
   x.tiles = (x.L + kAwTile - 1) / kAwTile;
   return x.rows > 0 && x.L > 0;
@@ -124,7 +126,7 @@ __device__ __forceinline__ void aw_join(float& m, float& l, float m2, float l2) 
 // What tokens gather is added to what they have; new ones start from nothing.
 __device__ __forceinline__ void aw_update(const AwParams& p, const AwProg& x, int t, const v4f& got) {
   float* w = p.w + x.b * p.s_wb + x.h * p.s_wh + t;
-  const int fresh = x.L - x.ql;
+  const int fresh = p.row0 == 0 ? x.L - x.ql : x.L;  // later launches add to what the first set
   if (p.w_vec && t + 4 <= x.L) {
     v4f old = *reinterpret_cast<const v4f*>(w);
 #pragma unroll
@@ -511,13 +513,13 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) sums[s] = v4f{0.f, 0.f, 0.f, 0.f};
     auto load_q = [&](int rb, v8h (&qf)[NU]) {
-      const int row = min(rb * 16 + r, x.rows - 1), qi = aw_token(p, row), head = x.h * p.G + row - qi * p.G;
+      const int row = p.row0 + min(rb * 16 + r, x.rows - 1), qi = aw_token(p, row), head = x.h * p.G + row - qi * p.G;
       const _Float16* src = p.q + x.b * p.s_qb + qi * p.s_qt + head * p.s_qh + 16 * g;
 #pragma unroll
       for (int u = 0; u < NU; ++u) qf[u] = *reinterpret_cast<const v8h*>(src + 64 * (u / 2) + 8 * (u & 1));
     };
     // The first block with a row that sees the wave's first token, none where the wave sees nothing.
-    const int first = seen == 0 ? blocks : t0 > fresh ? min((t0 - fresh) * p.G / 16, blocks) : 0;
+    const int first = seen == 0 ? blocks : t0 > fresh ? min(max((t0 - fresh) * p.G - p.row0, 0) / 16, blocks) : 0;
     constexpr int kSeg = MODE == kAwSums ? 1 << 30 : kAwSeg;  // sums need no segments
     for (int seg = 0; seg < blocks; seg += kSeg) {
       const int seg_end = min(seg + kSeg, blocks);
@@ -551,7 +553,7 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int row = (rb + 2 * k) * 16 + r;  // rows past the last see nothing
-          aw_scores<D>(kh, qf[k], ksc, t0, row < x.rows ? fresh + aw_token(p, row) : -1,
+          aw_scores<D>(kh, qf[k], ksc, t0, row < x.rows ? fresh + aw_token(p, p.row0 + row) : -1,
                        t0 + 63 <= fresh && seen == 0xf && (rb + 2 * k) * 16 + 16 <= x.rows, seen, acc[k]);
         }
 #pragma unroll
@@ -652,6 +654,7 @@ static const void* aw_store_fn(int D, bool f32) {
 
 // Stored scores lie within a buffer's offsets.
 static bool aw_stores(int64_t rows, int64_t tiles) { return rows <= kAwStoreRows && tiles <= (1 << 16); }
+static int64_t aw_launch_rows(int64_t rows) { return rows < kAwLaunchRows ? rows : kAwLaunchRows; }
 struct AwSpace { size_t scores, stats, lse; };  // bytes
 static AwSpace aw_space(int64_t progs, int64_t rows, int64_t tiles) {
   return {aw_stores(rows, tiles) ? align_up((size_t)(progs * rows * tiles * kAwTile * 4), 256) : 0,
@@ -665,7 +668,7 @@ using namespace specq;
 extern "C" size_t specq_paged_attn_weights_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int max_pages,
                                                           int PAGE) {
   if (B_grid <= 0 || H <= 0 || H_KV <= 0 || H % H_KV != 0 || ql_grid <= 0 || max_pages <= 0 || PAGE <= 0) return 0;
-  const AwSpace s = aw_space((int64_t)B_grid * H_KV, (int64_t)ql_grid * (H / H_KV),
+  const AwSpace s = aw_space((int64_t)B_grid * H_KV, aw_launch_rows((int64_t)ql_grid * (H / H_KV)),
                              ceil_div64((int64_t)max_pages * PAGE, kAwTile));
   return kCounterBytes + s.scores + s.stats + s.lse;
 }
@@ -713,9 +716,9 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   p.plan = plan; p.n_seqs = n_seqs; p.q_len = q_len; p.B_grid = B_grid; p.ql_grid = ql_grid;
   p.G = H / H_KV; p.g_magic = p.G > 1 ? (uint32_t)(((1ull << 32) + p.G - 1) / p.G) : 0;
   p.H_KV = H_KV; p.PAGE = PAGE;
-  p.cap = (int)cap; p.tiles = (int)ceil_div64(cap, kAwTile); p.rows = (int)rows;
+  p.cap = (int)cap; p.tiles = (int)ceil_div64(cap, kAwTile); p.rows = (int)aw_launch_rows(rows);
   p.scale_log2 = sm_scale * 1.44269504088896340736f;
-  const AwSpace space = aw_space(progs, rows, p.tiles);
+  const AwSpace space = aw_space(progs, p.rows, p.tiles);
   const size_t need = kCounterBytes + space.scores + space.stats + space.lse;
   SPECQ_REQUIRE(workspace && workspace_bytes >= need, SPECQ_ENOSPC,
                 "paged_attn_weights: workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
@@ -730,10 +733,13 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   p.span = few ? (int)(span < 1 ? 1 : span > kAwSpan ? kAwSpan : span) : 1;
   const int64_t items = progs * ceil_div(p.tiles, p.span), sums = progs * ceil_div64(cap, kAwSumTile);
   const int grid = (int)(items < kAwMaxGrid ? items : kAwMaxGrid), threads = few ? 256 : 512;
-  if (int rc = launch(store ? aw_store_fn(D, f32) : aw_fn<kAwStats>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p))
-    return rc;
-  if (store)
-    return launch(reinterpret_cast<const void*>(&aw_sum_kernel), (int)(sums < kAwMaxGrid ? sums : kAwMaxGrid), 256, 0,
-                  (hipStream_t)stream, &p);
-  return launch(aw_fn<kAwSums>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p);
+  for (p.row0 = 0; p.row0 < rows; p.row0 += kAwLaunchRows) {
+    if (int rc = launch(store ? aw_store_fn(D, f32) : aw_fn<kAwStats>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p))
+      return rc;
+    const int rc = store ? launch(reinterpret_cast<const void*>(&aw_sum_kernel), (int)(sums < kAwMaxGrid ? sums : kAwMaxGrid),
+                                  256, 0, (hipStream_t)stream, &p)
+                         : launch(aw_fn<kAwSums>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p);
+    if (rc != SPECQ_OK) return rc;
+  }
+  return SPECQ_OK;
 }

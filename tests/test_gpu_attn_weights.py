@@ -67,6 +67,7 @@ def check(got, case, q_lens, sm, what):
     ([5000], 3, 8, 1, 128, 128),                  # 24 rows of one head, 20 tiles
     ([400, 90], 90, 8, 2, 128, 16),               # a prompt chunk of 23 row blocks; a whole prompt
     ([600], 600, 2, 1, 64, 16),                   # more row blocks than are joined at a time
+    ([900, 620], 610, 4, 1, 128, 64),             # rows of more than one launch pair, for one sequence a prompt
     ([333, 1000], 150, 8, 2, 64, 16),             # ... whose first seen ones lie anywhere among them
     ([291, 180, 777], 177, 12, 4, 128, 48),
     ([0, 3, 20], 7, 4, 4, 128, 16),               # an empty sequence, one of fewer tokens than are new
