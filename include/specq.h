@@ -442,8 +442,11 @@ int specq_qk_norm_rotary(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh
  *             counts: the drafts that were accepted.  0 leaves the sequence's weights as they are
  *   weights   fp32 [B_grid, H_KV, >= max_pages * PAGE], strides s_wb, s_wh; rows must not overlap
  *   A context longer than the table counts as the table's length, a negative one as 0.  Tokens on no page of the pool get
- *   nothing.  Eager and plan-mode calls agree bit for bit.  At most 65536 (sequence, KV head) pairs.
- *   Workspace: specq_paged_attn_weights_workspace_size() bytes, as the workspaces above.
+ *   nothing.  A NaN or infinite score makes NaN of its row's share.  Eager and plan-mode calls agree bit for bit.  At most
+ *   65536 (sequence, KV head) pairs.
+ *   Workspace: specq_paged_attn_weights_workspace_size() bytes, as the workspaces above: for each pair and 256 tokens of
+ *   the table 8 bytes a row (1024 rows at most, more are taken in turns), and where a pair has at most 16 rows, 4 bytes a
+ *   row and token of the table.
  * ------------------------------------------------------------------------------------- */
 size_t specq_paged_attn_weights_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int max_pages, int PAGE);
 int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh,
@@ -465,7 +468,7 @@ int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_qt, int64_t 
  *   weights   fp32 [B, H_KV, >= max_pages * PAGE] (specq_paged_attn_weights)
  *   Cache tensors: at most 16, [n_pages, PAGE, H_KV] rows of row_bytes (1 to 4096) bytes; base pointers and strides in
  *   bytes (host arrays, read during the call)
- *   kept      int32 [B, H_KV, budget];  0 <= recent + sinks <= budget <= limit
+ *   kept      int32 [B, H_KV, budget];  0 <= recent + sinks <= budget <= limit, budget at most 2^30
  *   Workspace: specq_kv_evict_workspace_size() bytes, as the workspaces above.
  * ------------------------------------------------------------------------------------- */
 size_t specq_kv_evict_workspace_size(int B, int H_KV, int max_pages, int PAGE);
@@ -497,9 +500,10 @@ int specq_beam_reorder(const int32_t* parents, int rows, int group, int n_tensor
                        const int64_t* row_stride, const int64_t* row_bytes, void* stream);
 
 /* Calls specq_<name> (specq_rotary, specq_qk_norm_rotary, specq_kv_append_block, specq_paged_attn_block,
- * specq_paged_attn_weights, specq_kv_evict, specq_beam_select, specq_beam_reorder or a specq_kv_pages_ function that returns int) with its n arguments as 64-bit words in their order: pointers and integers as they
- * are, floats as the bits of a double.  An integer that does not fit its argument's type is -22.  For bindings
- * that pay for every argument they convert. */
+ * specq_paged_attn_weights, specq_kv_evict, specq_beam_select, specq_beam_reorder or a specq_kv_pages_ function that
+ * returns int) with its n arguments as 64-bit words in their order: pointers and integers as they are, floats as the
+ * bits of a double.  An integer that does not fit its argument's type is -22.  For bindings that pay for every argument
+ * they convert. */
 int specq_call_packed(const char* name, const int64_t* words, int n);
 
 /* ---------------------------------------------------------------------------------------

@@ -440,20 +440,30 @@ extern "C" int specq_beam_reorder(const int32_t* parents, int rows, int group, i
                    : group <= 8 ? reinterpret_cast<const void*>(&beam_reorder_kernel<8>)
                    : group <= 16 ? reinterpret_cast<const void*>(&beam_reorder_kernel<16>)
                                  : reinterpret_cast<const void*>(&beam_reorder_kernel<32>);
+  auto access = [&](int t) {
+    const uint64_t bits = (uintptr_t)base[t] | (uint64_t)row_stride[t] | (uint64_t)row_bytes[t];
+    return bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+  };
+  // No launch of a call is too large: one that is refused has changed nothing.
+  const int64_t most = UINT32_MAX / 256 / (rows / group);
+  int64_t per = 0;
+  for (int t = 0; t < n_tensors; ++t) {
+    if (t % kReorderTensors == 0) per = 0;
+    per += ceil_div64(row_bytes[t], 256 * access(t));
+    SPECQ_REQUIRE(per <= most, SPECQ_ENOTSUP, "beam_reorder: states too large");
+  }
   for (int t0 = 0; t0 < n_tensors; t0 += kReorderTensors) {
     ReorderParams p = {};
     p.parents = parents;
     p.W = group;
-    int64_t per = 0;
+    per = 0;
     for (int t = t0; t < n_tensors && t < t0 + kReorderTensors; ++t) {
       const int i = p.tensors++;
       p.base[i] = static_cast<uint8_t*>(base[t]);
       p.stride[i] = row_stride[t];
       p.bytes[i] = row_bytes[t];
-      const uint64_t bits = (uintptr_t)base[t] | (uint64_t)row_stride[t] | (uint64_t)row_bytes[t];
-      p.vec[i] = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+      p.vec[i] = access(t);
       per += ceil_div64(row_bytes[t], 256 * p.vec[i]);
-      SPECQ_REQUIRE(per <= INT32_MAX / (rows / group), SPECQ_ENOTSUP, "beam_reorder: states too large");
       p.first[i + 1] = (int32_t)per;
     }
     if (int rc = launch(fn, (int)(per * (rows / group)), 256, 0, (hipStream_t)stream, &p)) return rc;

@@ -1582,7 +1582,9 @@ def paged_kv_evict(block_tbl, ctx_len, weights, caches, PAGE, budget, recent=0, 
     -1 past its tokens) where it is not longer than limit, where one of its table entries names no page and, with the
     page counts `ref` given, where another row names one of its pages too.  Without `ref` the caller answers for
     that: a page must be named by one entry of the table only.  Keys keep the positions they were turned by, so the
-    new tokens' positions go on from the uncut length (rotary_embed's `positions`).  kept int32 [B, H_KV, budget].
+    new tokens' positions go on from the uncut length (rotary_embed's `positions`).  Layers that share ctx_len and the table
+    but not their caches and weights have a call each, all but the last with a copy of ctx_len.  kept int32
+    [B, H_KV, budget].
     """
     who = "paged_kv_evict"
     dev = _gpu_of(who, block_tbl, ctx_len, weights, ref, kept, *caches)

@@ -125,6 +125,16 @@ def test_launches_past_their_size(built_lib):
                                      bytes=keep[2].ctypes.data, stream=0), -95)
 
 
+def test_reorder_refuses_before_its_first_launch(built_lib):
+    """Of more states than a launch takes the last is too large: refused for that, not by the first launch."""
+    n = 65
+    base, stride = np.arange(4096, 4096 + 4096 * n, 4096, dtype=np.int64), np.full(n, 1 << 50, np.int64)
+    size = np.full(n, 128, np.int64)
+    size[-1] = 1 << 45
+    _fail("specq_beam_reorder", dict(parents=16, rows=4, group=2, n=n, base=base.ctypes.data, stride=stride.ctypes.data,
+                                     bytes=size.ctypes.data, stream=0), -95)
+
+
 def test_sizes_past_their_types(built_lib):
     from specq import _lib
     for name, args, word in (("specq_qk_norm_rotary", NORM, "B"), ("specq_paged_attn_weights", WEIGHTS, "ql")):
