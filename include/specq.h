@@ -464,7 +464,8 @@ int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_qt, int64_t 
  * comes from position kept[b, h, j], in every cache tensor and in the weights, and ctx_len[b] becomes budget.  A sequence
  * stays as it is (kept[j] = j, -1 past its tokens) where it is not longer than limit, where its table names a page outside
  * the pool, and, with ref not NULL, where it names a page with ref > 1.  A page must be named by one entry of the table
- * only.  Pages behind the budget are let go of by specq_kv_pages_free.
+ * only.  Pages behind the budget are let go of by specq_kv_pages_free.  Layers of one table and ctx_len have a call each,
+ * all but the last with a copy of ctx_len.
  *   weights   fp32 [B, H_KV, >= max_pages * PAGE] (specq_paged_attn_weights)
  *   Cache tensors: at most 16, [n_pages, PAGE, H_KV] rows of row_bytes (1 to 4096) bytes; base pointers and strides in
  *   bytes (host arrays, read during the call)
