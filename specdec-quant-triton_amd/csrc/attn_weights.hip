@@ -10,8 +10,8 @@
 //   1  scores, and (max, sum of exponentials) of each row within the tile; the last workgroup of a (sequence, head)
 //      joins them to log2 of each row's sum over all tiles
 //   2  p = exp2(s - that), summed over the rows, and the update of w
-// The scores of up to 16 rows (kAwStoreRows: plain decoding) go from 1 to 2 through the workspace; more rows compute them again.  Both ways
-// add a token's rows in one order (16 lanes; in each the blocks of 16 rows of either parity, then both; then pairs of
+// The scores of up to 16 rows (kAwStoreRows: plain decoding) go from 1 to 2 through the workspace; more rows compute them
+// again.  Both ways add a token's rows in one order (16 lanes; in each the blocks of 16 rows of either parity, then both; then pairs of
 // lanes) and join the rows' statistics in one (64 tokens, 256, all), so they give the same bits, and a plan-mode call those of an
 // eager one.
 //
@@ -205,31 +205,41 @@ struct AwStage {
   }
 };
 
-// The products' scales, and -inf where the lane's row does not see the token (`all`: every row sees all).
-__device__ __forceinline__ void aw_mask(const v4f (&ksc)[4], int t0, int last, bool all, uint32_t seen, v4f (&acc)[4]) {
+// -inf where the lane's row does not see the token.
+__device__ __forceinline__ void aw_hide(int t0, int last, uint32_t seen, v4f (&acc)[4]) {
   const int g = lane_id() >> 4;
-#pragma unroll
-  for (int s = 0; s < 4; ++s)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[s][i] *= ksc[s][i];
-  if (all) return;
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (!(((seen >> s) & 1) && t0 + 16 * s + 4 * g + i <= last)) acc[s][i] = -INFINITY;
 }
-// Scores (in log2) of the wave's tokens with the row of lane % 16.
-template <int D>
+// A product's scale and, SUB, the row's log-sum off it: not one instruction, since stored scores are rounded between the two.
+template <bool SUB>
+__device__ __forceinline__ float aw_scaled(float acc, float ksc, float lse) {
+#pragma clang fp contract(off)
+  acc *= ksc;
+  return SUB ? acc - lse : acc;
+}
+template <bool SUB>
+__device__ __forceinline__ void aw_scale(const v4f (&ksc)[4], float lse, v4f (&acc)[4]) {
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[s][i] = aw_scaled<SUB>(acc[s][i], ksc[s][i], lse);
+}
+// Scores (in log2; SUB, less the row's log-sum) of the wave's tokens with the row of lane % 16.
+template <int D, bool SUB>
 __device__ __forceinline__ void aw_scores(const v8h (&kh)[4][D / 32], const v8h (&qf)[D / 32], const v4f (&ksc)[4], int t0, int last,
-                                          bool all, uint32_t seen, v4f (&acc)[4]) {
+                                          bool all, uint32_t seen, float lse, v4f (&acc)[4]) {
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     acc[s] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < D / 32; ++u) acc[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[s][u], qf[u], acc[s], 0, 0, 0);
   }
-  aw_mask(ksc, t0, last, all, seen, acc);
+  aw_scale<SUB>(ksc, lse, acc);
+  if (!all) aw_hide(t0, last, seen, acc);  // all: every row sees all
 }
 // (max, sum) of a row over the wave's tokens, in all lanes of the row.
 __device__ __forceinline__ uint64_t aw_stat(const v4f (&acc)[4]) {
@@ -266,7 +276,10 @@ __device__ __forceinline__ void aw_lse(const AwParams& p, const AwProg& x, int p
   const int threads = blockDim.x;
   const uint64_t* st = p.stats + (int64_t)prog * p.tiles * p.rows;
   float* out = p.lse + (int64_t)prog * p.rows;
-  auto done = [&](int row, float m, float l) { out[row] = m == -INFINITY ? INFINITY : m + __builtin_amdgcn_logf(l); };
+  // Of a row that sees nothing an infinite one, so that it gives 0; a maximum knows no NaN, the sum does.
+  auto done = [&](int row, float m, float l) {
+    out[row] = m == -INFINITY && l == l ? INFINITY : m + __builtin_amdgcn_logf(l);
+  };
   // Tiles k0, k0 + step, ...: eight loads in flight.
   auto walk = [&](int row, int k0, int step, float& m, float& l) {
     constexpr int U = 8;
@@ -388,12 +401,13 @@ __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
         for (int u = 0; u < NU; ++u) qf[u] = s_q[rb][u][lane];
         v4f acc[4];
         // Rows past the last add nothing: their statistics go nowhere, their lse is infinite.
-        aw_scores<D>(kh, qf, ksc, t0, fresh + aw_token(p, row), t0 + 63 <= fresh && seen == 0xf, seen, acc);
+        aw_scores<D, MODE == kAwSums>(kh, qf, ksc, t0, fresh + aw_token(p, row), t0 + 63 <= fresh && seen == 0xf, seen,
+                                      lse[MODE == kAwSums ? rb : 0], acc);
         if constexpr (MODE == kAwSums) {
 #pragma unroll
           for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) (rb & 1 ? odd : even)[s][i] += fast_exp2(acc[s][i] - lse[rb]);
+            for (int i = 0; i < 4; ++i) (rb & 1 ? odd : even)[s][i] += fast_exp2(acc[s][i]);
         } else {
           const uint64_t st = aw_stat(acc);
           if (g == 0) s_stat[tile - tile0][w][row] = st;
@@ -464,12 +478,20 @@ __global__ __launch_bounds__(256) void aw_store_kernel(AwParams p) {
       }
 #pragma unroll
       for (int s = 0; s < 4; ++s) ksc[s] = *reinterpret_cast<const v4f*>(&s_scale[w][16 * s + 4 * g]);
-      aw_mask(ksc, t0, last, t0 + 63 <= fresh && seen == 0xf, seen, acc);  // rows past the last go nowhere
+      aw_scale<false>(ksc, 0.f, acc);
+      const bool all = t0 + 63 <= fresh && seen == 0xf;
+      if (!all) aw_hide(t0, last, seen, acc);  // rows past the last go nowhere
+      const uint64_t st = aw_stat(acc);
+      // What is seen is stored as finite, what is not as -inf, which adds nothing even to a row whose log-sum is NaN.
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[s][i] = fmaxf(acc[s][i], -3.402823466e38f);
+      if (!all) aw_hide(t0, last, seen, acc);
       // Always the same stores, too; those of tokens behind the context lie in the row's last tile.
 #pragma unroll
       for (int s = 0; s < 4; ++s)
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4i, acc[s]), out, out_row + 4u * (uint32_t)(t0 + 16 * s), 0, 0);
-      const uint64_t st = aw_stat(acc);
       if (g == 0) s_stat[tile - tile0][w][r] = st;
     }
     __syncthreads();
@@ -478,16 +500,24 @@ __global__ __launch_bounds__(256) void aw_store_kernel(AwParams p) {
   }
 }
 
-// More rows: a workgroup owns a tile, its waves 64 tokens and the row blocks of one parity each.
+// More rows: a workgroup owns a tile, its waves 64 tokens and the row blocks of one parity each.  64 rows' queries at a time
+// come through LDS, whole rows a load, while the 64 before are multiplied.  Loaded by each wave as its matrix operands,
+// nearly every lane's 16 bytes were an access of their own: 2 x 256 tokens, 32 / 8 heads of 128, contexts of 4096 and less
+// took 77 us in both launches; now 43 + 31 less what they share, 69.  At two waves a SIMD (K's operands are 64 registers) the vector
+// instructions have 60 % of the cycles and the matrix ones 26 %.  Put between one another by hand, 45 % of the matrix
+// cycles had vector ones beside them, and the sums took 35 us instead of 31.
 template <int D, typename ST, int MODE>
 __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
-  constexpr int NU = D / 32;
+  constexpr int NU = D / 32, GQ = D / 8, kLoads = 64 * GQ / 512;  // 16-byte granules of a query row; loads of a thread
   __shared__ AwStage<D> s_k[8];
+  __shared__ v8h s_q[2][64][GQ];
   __shared__ float s_scale[8][64];
   __shared__ uint64_t s_stat[MODE == kAwSums ? 1 : 4][MODE == kAwSums ? 1 : kAwSeg * 16];
   __shared__ v4f s_sums[MODE == kAwSums ? 4 : 1][4][64];
   __shared__ int s_last;
   const int lane = lane_id(), w = uniform(wave_id()) & 3, odd = uniform(wave_id()) >> 2, r = lane & 15, g = lane >> 4;
+  // Granule q of row t lies in slot q ^ key(t): 16 rows' granules meet in no bank.
+  auto key = [](int t) { return D == 128 ? t & 15 : (t >> 1) & 7; };
   const int progs = p.B_grid * p.H_KV;
   for (int64_t item = blockIdx.x; item < (int64_t)progs * p.tiles; item += gridDim.x) {
     const int tile = (int)(item / progs), prog = aw_order(p, (int)(item % progs)), t0 = tile * kAwTile + 64 * w;
@@ -512,49 +542,76 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
     v4f sums[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) sums[s] = v4f{0.f, 0.f, 0.f, 0.f};
-    auto load_q = [&](int rb, v8h (&qf)[NU]) {
-      const int row = p.row0 + min(rb * 16 + r, x.rows - 1), qi = aw_token(p, row), head = x.h * p.G + row - qi * p.G;
-      const _Float16* src = p.q + x.b * p.s_qb + qi * p.s_qt + head * p.s_qh + 16 * g;
-#pragma unroll
-      for (int u = 0; u < NU; ++u) qf[u] = *reinterpret_cast<const v8h*>(src + 64 * (u / 2) + 8 * (u & 1));
+    // The first row block that sees token t.
+    auto first_of = [&](int t) { return t > fresh ? min(max((t - fresh) * p.G - p.row0, 0) / 16, blocks) : 0; };
+    int rb = first_of(tile * kAwTile) & ~3;  // four blocks at a time, from the first that sees the tile's first token
+    // A thread's rows of the blocks to be fetched.  Their places go on by 64 rows: products for each cost 1 us of 32.
+    const int step_q = 64 / p.G, step_h = 64 - step_q * p.G;
+    const _Float16* const q0 = p.q + x.b * p.s_qb + x.h * p.G * p.s_qh + 8 * (threadIdx.x % GQ);
+    auto place = [&](int row, int& head) {
+      const int qi = aw_token(p, p.row0 + row);
+      head = p.row0 + row - qi * p.G;
+      return q0 + qi * p.s_qt + head * p.s_qh;
     };
-    // The first block with a row that sees the wave's first token, none where the wave sees nothing.
-    const int first = seen == 0 ? blocks : t0 > fresh ? min(max((t0 - fresh) * p.G - p.row0, 0) / 16, blocks) : 0;
+    int head[kLoads], row[kLoads], last_head;
+    const _Float16 *from[kLoads], *const end = place(x.rows - 1, last_head);
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      row[n] = rb * 16 + ((int)threadIdx.x + 512 * n) / GQ;
+      from[n] = place(row[n], head[n]);
+    }
+    v8h next[kLoads];
+    float next_lse[2] = {0.f, 0.f};
+    auto fetch = [&](int b) {  // what four blocks need; past the last row, that row
+#pragma unroll
+      for (int n = 0; n < kLoads; ++n) {
+        next[n] = *reinterpret_cast<const v8h*>(row[n] < x.rows ? from[n] : end);
+        row[n] += 64;
+        head[n] += step_h;
+        from[n] += step_q * p.s_qt + step_h * p.s_qh;
+        if (head[n] >= p.G) {
+          head[n] -= p.G;
+          from[n] += p.s_qt - p.G * p.s_qh;
+        }
+      }
+      if constexpr (MODE == kAwSums) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) next_lse[k] = p.lse[(int64_t)prog * p.rows + min((b + odd + 2 * k) * 16 + r, x.rows - 1)];
+      }
+    };
+    int slot = 0;
+    auto stage = [&] {
+#pragma unroll
+      for (int n = 0; n < kLoads; ++n) {
+        const int i = (int)threadIdx.x + 512 * n, t = i / GQ;
+        s_q[slot][t][(i % GQ) ^ key(t)] = next[n];
+      }
+    };
     constexpr int kSeg = MODE == kAwSums ? 1 << 30 : kAwSeg;  // sums need no segments
-    for (int seg = 0; seg < blocks; seg += kSeg) {
-      const int seg_end = min(seg + kSeg, blocks);
+    int seg = 0, seg_end = 0;
+    auto keep = [&](int b, uint64_t st) {
       if constexpr (MODE != kAwSums)
-        for (int rb = seg + odd; rb < min(first, seg_end); rb += 2)
-          if (g == 0) s_stat[w][(rb - seg) * 16 + r] = aw_pack(-INFINITY, 0.f);
-      int rb = max(seg, first);
-      rb += (rb ^ odd) & 1;
-      // Two blocks at a time, and the next two's queries on their way.
-      v8h next[2][NU];
-      float next_lse[2];
-      auto fetch = [&](int rb) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          load_q(rb + 2 * k, next[k]);
-          if constexpr (MODE == kAwSums) next_lse[k] = p.lse[(int64_t)prog * p.rows + min((rb + 2 * k) * 16 + r, x.rows - 1)];
-        }
-      };
-      if (rb < seg_end) fetch(rb);
-      for (; rb < seg_end; rb += 4) {
-        v8h qf[2][NU];
-        float lse[2] = {INFINITY, INFINITY};
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-#pragma unroll
-          for (int u = 0; u < NU; ++u) qf[k][u] = next[k][u];
-          if constexpr (MODE == kAwSums) lse[k] = next_lse[k];
-        }
+        if (g == 0 && b < seg_end) s_stat[w][(b - seg) * 16 + r] = st;
+    };
+    if (rb < blocks) fetch(rb);
+    for (; seg < blocks; seg += kSeg) {
+      seg_end = min(seg + kSeg, blocks);
+      if constexpr (MODE != kAwSums)
+        for (int b = seg + odd; b < min(rb, seg_end); b += 2) keep(b, aw_pack(-INFINITY, 0.f));
+      for (; rb < seg_end; rb += 4, slot ^= 1) {
+        stage();
+        const float lse[2] = {next_lse[0], next_lse[1]};
         fetch(rb + 4);
+        wg_barrier_lds();  // the other slot has been read, and is written next
         v4f acc[2][4];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int row = (rb + 2 * k) * 16 + r;  // rows past the last see nothing
-          aw_scores<D>(kh, qf[k], ksc, t0, row < x.rows ? fresh + aw_token(p, p.row0 + row) : -1,
-                       t0 + 63 <= fresh && seen == 0xf && (rb + 2 * k) * 16 + 16 <= x.rows, seen, acc[k]);
+          const int b = rb + odd + 2 * k, at = b * 16 + r;  // rows past the last see nothing
+          v8h qf[NU];
+#pragma unroll
+          for (int u = 0; u < NU; ++u) qf[u] = s_q[slot][(odd + 2 * k) * 16 + r][(8 * (u / 2) + 2 * g + (u & 1)) ^ key(r)];
+          aw_scores<D, MODE == kAwSums>(kh, qf, ksc, t0, at < x.rows ? fresh + aw_token(p, p.row0 + at) : -1,
+                                        t0 + 63 <= fresh && seen == 0xf && b * 16 + 16 <= x.rows, seen, lse[k], acc[k]);
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -562,10 +619,9 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) sums[s][i] += fast_exp2(acc[k][s][i] - lse[k]);
+              for (int i = 0; i < 4; ++i) sums[s][i] += fast_exp2(acc[k][s][i]);
           } else {
-            const uint64_t st = aw_stat(acc[k]);
-            if (g == 0 && rb + 2 * k < seg_end) s_stat[w][(rb + 2 * k - seg) * 16 + r] = st;
+            keep(rb + odd + 2 * k, aw_stat(acc[k]));
           }
         }
       }
@@ -614,12 +670,27 @@ __global__ __launch_bounds__(256) void aw_sum_kernel(AwParams p) {
       e[k] = v4f{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (k < x.rows) e[k] = *reinterpret_cast<const v4f*>(sc + (int64_t)k * p.tiles * kAwTile);
     }
+    float lse[kAwStoreRows];
+    bool nan = false;
 #pragma unroll
     for (int k = 0; k < kAwStoreRows; ++k) {
-      const float lse = k < x.rows ? p.lse[(int64_t)prog * p.rows + k] : INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) e[k][i] = fast_exp2(e[k][i] - lse);
+      lse[k] = k < x.rows ? p.lse[(int64_t)prog * p.rows + k] : INFINITY;
+      nan |= !(lse[k] == lse[k]);
     }
+    if (uniform((int)nan)) {  // a row gives its NaN to what it sees alone
+#pragma unroll
+      for (int k = 0; k < kAwStoreRows; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(lse[k] == lse[k]) && !(e[k][i] == -INFINITY)) e[k][i] = lse[k];
+#pragma unroll
+      for (int k = 0; k < kAwStoreRows; ++k)
+        if (!(lse[k] == lse[k])) lse[k] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < kAwStoreRows; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[k][i] = fast_exp2(e[k][i] - lse[k]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -727,6 +798,9 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   p.scores = reinterpret_cast<float*>(at + kCounterBytes);
   p.stats = reinterpret_cast<uint64_t*>(at + kCounterBytes + space.scores);
   p.lse = reinterpret_cast<float*>(at + kCounterBytes + space.scores + space.stats);
+  // Stored scores against scores formed twice (us, 8 KV heads of 128): 4 rows, 8 sequences of 4096: 20.3, 24.6; 32 of 8192: 82,
+  // 121; 16 rows, 8 of 4096: 27.3, 24.8; one of 32768: 28.6, 32.8.  Queries in LDS for the whole call against 64 rows at a
+  // time: 20 rows, 8 of 4096: 28.7, 58.6; 64 rows: 37.7, 58.5; one of 32768: 54, 69.
   const bool store = aw_stores(rows, p.tiles), few = rows <= kAwFewRows, f32 = scale_fp32 != 0;
   // Tiles of a workgroup of few rows: as many as leave two workgroups to a CU.
   const int64_t tiles = progs * p.tiles, span = tiles / (2 * device_cus());

@@ -267,3 +267,17 @@ def test_empty_and_refusals():
         with pytest.raises(RuntimeError):
             K.paged_attention_weights(*args, **kw)
     assert torch.equal(w, before)
+
+
+@pytest.mark.parametrize("QL,G,ctx", [(4, 4, 700), (9, 4, 700), (300, 2, 700), (700, 2, 700)])
+def test_a_nan_row_shares_nothing_out_to_tokens_it_does_not_see(QL, G, ctx):
+    """16, 36, 600 and 1400 rows: stored scores, scores formed twice, and those of one and two pairs of launches."""
+    rng = np.random.default_rng(23)
+    q, kc, ks, bt, cl, w = make(rng, [ctx], QL, 2 * G, 2, 64, 16, True)
+    bad, i = q.copy(), QL // 2 - 1
+    bad[0, i, 1] = np.nan  # a head of the first group
+    got = [K.paged_attention_weights(*gpu(x, kc, ks, bt, cl, w)).cpu().numpy() for x in (q, bad)]
+    sees = ctx - QL + i + 1
+    assert np.isnan(got[1][0, 0, :sees]).sum() == sees
+    assert (got[1][0, 0, sees:] != got[0][0, 0, sees:]).sum() == 0
+    assert (got[1][0, 1] != got[0][0, 1]).sum() == 0
