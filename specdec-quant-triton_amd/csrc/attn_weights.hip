@@ -18,6 +18,9 @@
 // K stays: a wave holds 64 tokens, converts their codes to fp16 matrix operands once and walks the rows 16 at a time
 // (K . Q^T on v_mfma_f32_16x16x32_f16: a lane's results are four tokens of one row).  Everything behind the products is
 // fp32; log2(e) is folded into the scale.
+// 8 KV heads of 128 (us): a new token of 32 sequences of up to 8192, stored scores, 52 + 10, codes and scores at 3.4 TB/s (loads
+// alone 5.2); 9 of 8 sequences of 4096, formed twice, 19 + 14, half of it fixed phases; 256 of 2 of up to 4096, 42 + 30, bound by
+// vector instructions at two waves a SIMD.
 #include "api_common.hpp"
 #include "common.hpp"
 

@@ -14,8 +14,11 @@
 //      beams whose scores lie closer than an fp32 step apart are to be told apart as the formula does.  Again a value that n
 //      reach, then the few that do, ranked against one another.  The order in which lists are filled has no part in the result.
 //
+// 16 x 8 rows of 128257 fp32 logits: 17.2 us (66 MB, 3.8 TB/s) and 12; 4 of 32000 fp16: 5.7 and 6.5.  The second launch waits for
+// memory three times over, whatever its size.
+//
 // Reordering: row r of every state becomes row parents[r] of the same group of rows.  In place: a thread owns one column of
-// up to 16 bytes of a group's rows, reads what changes and then writes it.  Bound by HBM.
+// up to 16 bytes of a group's rows, reads what changes and then writes it.  Bound by HBM: 16 x 8 rows of 418 KB, 13.7 us.
 #include "api_common.hpp"
 #include "common.hpp"
 
