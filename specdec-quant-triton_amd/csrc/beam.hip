@@ -14,7 +14,7 @@
 //      beams whose scores lie closer than an fp32 step apart are to be told apart as the formula does.  Again a value that n
 //      reach, then the few that do, ranked against one another.  The order in which lists are filled has no part in the result.
 //
-// 16 x 8 rows of 128257 fp32 logits: 17.2 us (66 MB, 3.8 TB/s) and 12; 4 of 32000 fp16: 5.7 and 6.5.  The second launch waits for
+// 16 x 8 rows of 128257 fp32 logits: 17.2 us (66 MB, 3.8 TB/s) and 8.8; 4 of 32000 fp16: 5.6 and 5.9.  The second launch waits for
 // memory three times over, whatever its size.
 //
 // Reordering: row r of every state becomes row parents[r] of the same group of rows.  In place: a thread owns one column of
@@ -29,8 +29,10 @@ constexpr int kBeamJoin = 1024, kBeamJoinWaves = kBeamJoin / kWave;  // threads 
 constexpr int kBeamMax = 64;     // beams of a sequence, and candidates selected
 constexpr int kBeamSlots = 128;  // candidates of a part
 constexpr int kBeamList = 1024;  // candidates ranked against one another
-constexpr int kBeamGroup = 32;   // threads of the second launch that share a part
-constexpr int kBeamNear = 4;     // parts of a thread read ahead
+// Threads of the second launch that share a part.  32 (and two slots, or a slot of four parts, read ahead): 11.7 us instead of 8.8 for
+// 16 x 8 rows of 16 parts; 16: 10.3.
+constexpr int kBeamGroup = 8;
+constexpr int kBeamNear = 3;     // slots of a thread read ahead
 
 struct BeamParams {
   const void* x; int64_t s_xb, s_xw;
@@ -200,18 +202,14 @@ __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamParams p) {
   __shared__ int s_count;
   const int b = blockIdx.x, wave = uniform(wave_id()), lane = lane_id(), all = p.W * p.parts;
   const int64_t base = (int64_t)b * all;
-  // A thread has candidate slots `slot` of the parts 32 apart; those of the first kBeamNear of them are read at once, before the
-  // parts' counts are known (what lies behind a count is not looked at), others where they are used.
+  // A thread has every kBeamGroup-th candidate slot of every kStep-th part; the first kBeamNear of its first part are read at
+  // once, before the part's count is known (what lies behind it is not looked at), others where they are used.
   const int slot = threadIdx.x % kBeamGroup, part0 = (int)threadIdx.x / kBeamGroup;
   constexpr int kStep = kBeamJoin / kBeamGroup;
   uint64_t near[kBeamNear];
-  int counts[kBeamNear];
+  const int count0 = part0 < all ? p.counts[base + part0] : 0;
 #pragma unroll
-  for (int k = 0; k < kBeamNear; ++k) {
-    const int part = part0 + k * kStep;
-    counts[k] = part < all ? p.counts[base + part] : 0;
-    near[k] = p.cands[(base + min(part, all - 1)) * kBeamSlots + slot];
-  }
+  for (int k = 0; k < kBeamNear; ++k) near[k] = p.cands[(base + min(part0, all - 1)) * kBeamSlots + slot + k * kBeamGroup];
   // The rows' sums.
   for (int w = wave; w < p.W; w += kBeamJoinWaves) {
     const uint64_t* st = p.stats + base + w * p.parts;
@@ -241,20 +239,16 @@ __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamParams p) {
   for (int pass = 0;; ++pass) {
     double top = -INFINITY;
     uint64_t top_at = ~0ull;
-    for (int part = part0, k = 0; part < all; part += kStep, ++k) {
-      int n;
-      uint64_t c;
-      if (k < kBeamNear) {
-        n = counts[0], c = near[0];
+    for (int part = part0; part < all; part += kStep) {
+      const bool first = part == part0;
+      const int n = first ? count0 : p.counts[base + part];
+      const int w = part / p.parts;
+      for (int i = slot, k = 0; i < n; i += kBeamGroup, ++k) {
+        uint64_t c = near[0];
 #pragma unroll
         for (int j = 1; j < kBeamNear; ++j)
-          if (k == j) n = counts[j], c = near[j];
-      } else {
-        n = p.counts[base + part], c = 0;
-        if (slot < n) c = p.cands[(base + part) * kBeamSlots + slot];
-      }
-      const int w = part / p.parts;
-      for (int i = slot; i < n;) {
+          if (k == j) c = near[j];
+        if (!first || k >= kBeamNear) c = p.cands[(base + part) * kBeamSlots + i];
         const double key = ((double)beam_lo(c) - s_lse[w]) + s_score[w];
         const uint64_t at = ((uint64_t)w << 32) | (c >> 32);
         if (key > -(double)INFINITY) {
@@ -269,8 +263,6 @@ __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamParams p) {
             top = key, top_at = at;
           }
         }
-        i += kBeamGroup;
-        if (i < n) c = p.cands[(base + part) * kBeamSlots + i];
       }
     }
     auto put = [&](int i, double key, uint64_t at) {
