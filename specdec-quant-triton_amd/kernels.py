@@ -1639,7 +1639,8 @@ def beam_select(logits, scores, n=None, finished=None, eos=None, out=None, works
     finished[b, w] (bool) has one, token `eos`, with the score it has.  Best first, compared in fp64, ties to the lower
     beam, then the lower token; n defaults to W, and both are at most 64.  parents holds rows b * W + w, as
     paged_kv_fork and beam_reorder take them.  Continuations of score -inf or NaN (logits of -inf; every one of a row that
-    holds NaN or +inf) are none; where there are fewer than n the rest has score -inf, token and parent -1.
+    holds NaN or +inf) are none; where there are fewer than n the rest has score -inf, token and parent -1.  `out` may hold
+    `scores` itself where n is W.
     Calls that may run at the same time on several streams need a workspace each.
     """
     who = "beam_select"

@@ -74,6 +74,20 @@ def test_large_batch(f32):
     check(got, x, s, 16, what="large")
 
 
+@pytest.mark.parametrize("n", [1, 40, 64])
+def test_many_parts_and_scores_in_place(n):
+    """64 beams of more parts than threads read ahead; with n = W the new scores may replace the old ones."""
+    rng = np.random.default_rng(11)
+    x, s = make(rng, 2, 64, 40001, True)
+    note(f"beam parts n={n}")
+    tx, ts = gpu(x, s)
+    out = (ts if n == 64 else torch.empty((2, n), device=DEV), *(torch.empty((2, n), dtype=torch.int32, device=DEV) for _ in "tp"))
+    got = K.beam_select(tx, ts, n, out=out)
+    torch.cuda.synchronize()
+    assert got[0].data_ptr() == out[0].data_ptr()
+    check(got, x, s, n, what="parts")
+
+
 def test_finished_beams_and_missing_ones():
     """A finished beam goes on with eos alone; a beam of score -inf has nothing; banned tokens are none."""
     rng = np.random.default_rng(2)
