@@ -30,7 +30,8 @@ constexpr int kAwTile = 256;       // tokens of a workgroup: 4 waves of 4 sub-ti
 constexpr int kAwStoreRows = 16;   // rows whose scores go through the workspace
 constexpr int kAwFewRows = 64;     // rows whose queries a workgroup keeps in LDS
 constexpr int kAwSpan = 8;         // most tiles such a workgroup walks (its waves' lanes hold their pages, and one tile's more)
-constexpr int kAwLaunchRows = 1024;  // rows of a program that two launches take (their statistics: 32 bytes a token at most)
+constexpr int kAwSegRows = 1024;   // rows of a segment, whose sums over the rows are added to the weights in one piece
+constexpr int kAwSegs = 8;         // most segments of a launch
 constexpr int kAwSeg = 32;         // row blocks of 16 whose statistics are joined at a time
 constexpr int kAwSumTile = 1024;   // tokens of a workgroup that adds up stored scores
 constexpr int kAwMaxGrid = 1 << 16;
@@ -47,13 +48,15 @@ struct AwParams {
   int cap;      // tokens a row of the table holds
   int tiles;    // of cap
   int span;     // tiles of a workgroup of few rows
-  int rows;     // of a program and launch at most
-  int row0;     // the launch's first row: more than kAwLaunchRows have several launches one after another
+  int rows;     // of a program and segment at most
+  int row0;     // the launch's first row: more than segs * kAwSegRows have several pairs of launches one after another
+  int segs;     // of a launch
   uint32_t g_magic;  // ceil(2^32 / G): row / G is its product's high word (rows below 2^20, G below 2^12); 0 for G = 1
   float scale_log2;
-  // Workspace: scores [prog][rows][tiles * 256]; (max, sum) [prog][tiles][rows]; log2 of the rows' sums [prog][rows].
-  float* scores; uint64_t* stats; float* lse;
-  int32_t* counters;  // [prog]
+  // Workspace: scores [prog][rows][tiles * 256]; (max, sum) [prog][seg][tiles][rows]; log2 of the rows' sums [prog][seg][rows];
+  // sums of a segment's rows [prog][seg][tiles * 256], two tokens a word.
+  float* scores; uint64_t* stats; float* lse; uint64_t* sums;
+  int32_t* counters;  // [prog][seg], then [prog][tile]
 };
 
 // Program number `i` of the launch order.  The heads of a sequence read the same lines of scales: in blocks of eight
@@ -68,11 +71,11 @@ __device__ __forceinline__ int aw_order(const AwParams& p, int i) {
 __device__ __forceinline__ int aw_token(const AwParams& p, int row) {
   return p.g_magic != 0 ? (int)__umulhi((uint32_t)row, p.g_magic) : row;
 }
-// A program (sequence b, KV head h): the launch's rows of it, its tokens and active tiles.
+// A program (sequence b, KV head h): its rows from row0 on, of a segment at most, its tokens and active tiles.
 struct AwProg {
   int b, h, ql, rows, L, tiles;
 };
-__device__ __forceinline__ bool aw_prog(const AwParams& p, int prog, AwProg& x) {
+__device__ __forceinline__ bool aw_prog(const AwParams& p, int prog, AwProg& x, int row0 = 0) {
   int n_seqs = p.n_seqs, q_len = p.q_len;
   if (p.plan != nullptr) {
     n_seqs = min(max(p.plan[0], 0), p.B_grid);
@@ -82,7 +85,7 @@ __device__ __forceinline__ bool aw_prog(const AwParams& p, int prog, AwProg& x) 
   x.h = prog - x.b * p.H_KV;
   if (x.b >= n_seqs) return false;
   x.ql = p.q_lens != nullptr ? min(max(p.q_lens[x.b], 0), q_len) : q_len;
-  x.rows = min(x.ql * p.G - p.row0, p.rows);
+  x.rows = min(x.ql * p.G - row0, p.rows);
   x.L = min(max(p.ctx_len[x.b], 0), p.cap);
   x.tiles = (x.L + kAwTile - 1) / kAwTile;
   return x.rows > 0 && x.L > 0;
@@ -126,21 +129,34 @@ __device__ __forceinline__ void aw_join(float& m, float& l, float m2, float l2) 
   m = top;
 }
 
-// What tokens gather is added to what they have; new ones start from nothing.
-__device__ __forceinline__ void aw_update(const AwParams& p, const AwProg& x, int t, const v4f& got) {
+// What tokens gather, `n` pieces of it, is added to what they have; new ones start from nothing (where `start`: others have
+// been set by an earlier launch).
+template <typename F>
+__device__ __forceinline__ void aw_update(const AwParams& p, const AwProg& x, int t, bool start, int n, F&& piece) {
   float* w = p.w + x.b * p.s_wb + x.h * p.s_wh + t;
-  const int fresh = p.row0 == 0 ? x.L - x.ql : x.L;  // later launches add to what the first set
-  if (p.w_vec && t + 4 <= x.L) {
-    v4f old = *reinterpret_cast<const v4f*>(w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) old[i] = (t + i >= fresh ? 0.f : old[i]) + got[i];
-    *reinterpret_cast<v4f*>(w) = old;
+  const int fresh = start ? x.L - x.ql : x.L;
+  const bool vec = p.w_vec && t + 4 <= x.L;
+  v4f v = {0.f, 0.f, 0.f, 0.f};
+  if (vec) {
+    v = *reinterpret_cast<const v4f*>(w);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (t + i < x.L) w[i] = (t + i >= fresh ? 0.f : w[i]) + got[i];
+      if (t + i < x.L) v[i] = w[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (t + i >= fresh) v[i] = 0.f;
+  for (int k = 0; k < n; ++k) v += piece(k);
+  if (vec) {
+    *reinterpret_cast<v4f*>(w) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (t + i < x.L) w[i] = v[i];
   }
 }
+
 
 enum { kAwStats, kAwSums };  // pass 1, and pass 2 from K
 
@@ -260,9 +276,10 @@ __device__ __forceinline__ uint64_t aw_stat(const v4f (&acc)[4]) {
     for (int i = 0; i < 4; ++i) l += fast_exp2(acc[s][i] - ref);
   return aw_pack(m, aw_sum4(l));
 }
-// The rows' sums over the lanes, and the update: lanes 0..3 of each 16 have four tokens each.
-__device__ __forceinline__ void aw_finish(const AwParams& p, const AwProg& x, int t0, const v4f (&sums)[4]) {
-  const int r = lane_id() & 15, g = lane_id() >> 4;
+// The rows' sums over the lanes: lanes 0..3 of each 16 have four tokens each, from aw_first(t0) on.
+__device__ __forceinline__ int aw_first(int t0) { return t0 + 16 * (lane_id() & 15) + 4 * (lane_id() >> 4); }
+__device__ __forceinline__ v4f aw_rows(const v4f (&sums)[4]) {
+  const int r = lane_id() & 15;
   v4f got = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int s = 0; s < 4; ++s)
@@ -271,14 +288,14 @@ __device__ __forceinline__ void aw_finish(const AwParams& p, const AwProg& x, in
       const float v = aw_sum16(sums[s][i]);
       got[i] = r == s ? v : got[i];
     }
-  if (r < 4 && t0 + 16 * r + 4 * g < x.L) aw_update(p, x, t0 + 16 * r + 4 * g, got);
+  return got;
 }
 // The last workgroup of a program joins its rows' tiles: many rows a thread each, few a group of lanes each (as many as
 // there are tiles, at most a wave).
-__device__ __forceinline__ void aw_lse(const AwParams& p, const AwProg& x, int prog) {
+__device__ __forceinline__ void aw_lse(const AwParams& p, const AwProg& x, int at) {  // at: of [prog][seg]
   const int threads = blockDim.x;
-  const uint64_t* st = p.stats + (int64_t)prog * p.tiles * p.rows;
-  float* out = p.lse + (int64_t)prog * p.rows;
+  const uint64_t* st = p.stats + (int64_t)at * p.tiles * p.rows;
+  float* out = p.lse + (int64_t)at * p.rows;
   // Of a row that sees nothing an infinite one, so that it gives 0; a maximum knows no NaN, the sum does.
   auto done = [&](int row, float m, float l) {
     out[row] = m == -INFINITY && l == l ? INFINITY : m + __builtin_amdgcn_logf(l);
@@ -419,7 +436,8 @@ __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
       if constexpr (MODE == kAwSums) {
 #pragma unroll
         for (int s = 0; s < 4; ++s) even[s] += odd[s];
-        aw_finish(p, x, t0, even);
+        const v4f got = aw_rows(even);
+        if (r < 4 && aw_first(t0) < x.L) aw_update(p, x, aw_first(t0), true, 1, [&](int) { return got; });
       }
     }
     if constexpr (MODE != kAwSums) {
@@ -521,11 +539,16 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
   const int lane = lane_id(), w = uniform(wave_id()) & 3, odd = uniform(wave_id()) >> 2, r = lane & 15, g = lane >> 4;
   // Granule q of row t lies in slot q ^ key(t): 16 rows' granules meet in no bank.
   auto key = [](int t) { return D == 128 ? t & 15 : (t >> 1) & 7; };
-  const int progs = p.B_grid * p.H_KV;
-  for (int64_t item = blockIdx.x; item < (int64_t)progs * p.tiles; item += gridDim.x) {
-    const int tile = (int)(item / progs), prog = aw_order(p, (int)(item % progs)), t0 = tile * kAwTile + 64 * w;
+  const int progs = p.B_grid * p.H_KV, per = p.segs * progs;
+  for (int64_t item = blockIdx.x; item < (int64_t)per * p.tiles; item += gridDim.x) {
+    const int tile = (int)(item / per), some = (int)(item % per), seg_i = some / progs, row0 = p.row0 + seg_i * kAwSegRows;
+    const int prog = aw_order(p, some - seg_i * progs), index = prog * p.segs + seg_i, t0 = tile * kAwTile + 64 * w;
     AwProg x;
-    if (!aw_prog(p, prog, x) || tile >= x.tiles) continue;
+    if (!aw_prog(p, prog, x, row0) || tile >= x.tiles) continue;
+    // The segment's last row sees its tiles up to this one.
+    const int last_t = x.L - x.ql + aw_token(p, row0 + x.rows - 1);
+    x.tiles = last_t < 0 ? 0 : last_t / kAwTile + 1;
+    if (tile >= x.tiles) continue;
     const int sub_t = t0 + 16 * (lane & 3);
     const AwPages at = aw_pages(p, x, sub_t, sub_t < x.L ? p.bt[x.b * p.s_bt + sub_t / p.PAGE] : -1, lane < 4);
     const uint32_t seen = (uint32_t)at.ok;
@@ -546,14 +569,14 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) sums[s] = v4f{0.f, 0.f, 0.f, 0.f};
     // The first row block that sees token t.
-    auto first_of = [&](int t) { return t > fresh ? min(max((t - fresh) * p.G - p.row0, 0) / 16, blocks) : 0; };
+    auto first_of = [&](int t) { return t > fresh ? min(max((t - fresh) * p.G - row0, 0) / 16, blocks) : 0; };
     int rb = first_of(tile * kAwTile) & ~3;  // four blocks at a time, from the first that sees the tile's first token
     // A thread's rows of the blocks to be fetched.  Their places go on by 64 rows: products for each cost 1 us of 32.
     const int step_q = 64 / p.G, step_h = 64 - step_q * p.G;
     const _Float16* const q0 = p.q + x.b * p.s_qb + x.h * p.G * p.s_qh + 8 * (threadIdx.x % GQ);
     auto place = [&](int row, int& head) {
-      const int qi = aw_token(p, p.row0 + row);
-      head = p.row0 + row - qi * p.G;
+      const int qi = aw_token(p, row0 + row);
+      head = row0 + row - qi * p.G;
       return q0 + qi * p.s_qt + head * p.s_qh;
     };
     int head[kLoads], row[kLoads], last_head;
@@ -579,7 +602,7 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
       }
       if constexpr (MODE == kAwSums) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) next_lse[k] = p.lse[(int64_t)prog * p.rows + min((b + odd + 2 * k) * 16 + r, x.rows - 1)];
+        for (int k = 0; k < 2; ++k) next_lse[k] = p.lse[(int64_t)index * p.rows + min((b + odd + 2 * k) * 16 + r, x.rows - 1)];
       }
     };
     int slot = 0;
@@ -613,7 +636,7 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
           v8h qf[NU];
 #pragma unroll
           for (int u = 0; u < NU; ++u) qf[u] = s_q[slot][(odd + 2 * k) * 16 + r][(8 * (u / 2) + 2 * g + (u & 1)) ^ key(r)];
-          aw_scores<D, MODE == kAwSums>(kh, qf, ksc, t0, at < x.rows ? fresh + aw_token(p, p.row0 + at) : -1,
+          aw_scores<D, MODE == kAwSums>(kh, qf, ksc, t0, at < x.rows ? fresh + aw_token(p, row0 + at) : -1,
                                         t0 + 63 <= fresh && seen == 0xf && b * 16 + 16 <= x.rows, seen, lse[k], acc[k]);
         }
 #pragma unroll
@@ -635,7 +658,7 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
           float m = -INFINITY, l = 0.f;
 #pragma unroll
           for (int v = 0; v < 4; ++v) aw_join(m, l, aw_m(s_stat[v][i]), aw_l(s_stat[v][i]));
-          publish(p.stats + ((int64_t)prog * p.tiles + tile) * p.rows + seg * 16 + i, aw_pack(m, l));
+          publish(p.stats + ((int64_t)index * p.tiles + tile) * p.rows + seg * 16 + i, aw_pack(m, l));
         }
         __syncthreads();
       }
@@ -646,14 +669,34 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
         for (int s = 0; s < 4; ++s) s_sums[w][s][lane] = sums[s];
       }
       __syncthreads();
+      // The segments of this launch that have rows which see the tile, and whether an earlier launch had any.
+      const int base = p.row0 / kAwSegRows, from_seg = max(tile * kAwTile - fresh, 0) * p.G / kAwSegRows, seg0 = max(from_seg - base, 0);
+      const int seg1 = min(p.segs, (x.ql * p.G - p.row0 + kAwSegRows - 1) / kAwSegRows);
+      const bool start = from_seg >= base, alone = seg1 - seg0 == 1;
+      auto words = [&](int seg, int t) { return p.sums + ((int64_t)(prog * p.segs + seg) * p.tiles * kAwTile + t) / 2; };
       if (!odd) {
 #pragma unroll
         for (int s = 0; s < 4; ++s) sums[s] += s_sums[w][s][lane];
-        aw_finish(p, x, t0, sums);
+        const v4f got = aw_rows(sums);
+        const int t = aw_first(t0);
+        if (r < 4 && alone && t < x.L) aw_update(p, x, t, start, 1, [&](int) { return got; });
+        if (r < 4 && !alone) {
+          publish(words(seg_i, t), aw_pack(got[0], got[1]));
+          publish(words(seg_i, t) + 1, aw_pack(got[2], got[3]));
+        }
       }
-      __syncthreads();
-    } else if (arrive_last(p.counters + prog, x.tiles, &s_last)) {
-      aw_lse(p, x, prog);
+      if (alone) {
+        __syncthreads();
+      } else if (arrive_last(p.counters + per + (int64_t)prog * p.tiles + tile, seg1 - seg0, &s_last)) {
+        const int t = tile * kAwTile + 4 * (int)threadIdx.x;
+        if (threadIdx.x < kAwTile / 4 && t < x.L)
+          aw_update(p, x, t, start, seg1 - seg0, [&](int k) {
+            const uint64_t a = collect(words(seg0 + k, t)), b = collect(words(seg0 + k, t) + 1);
+            return v4f{aw_m(a), aw_l(a), aw_m(b), aw_l(b)};
+          });
+      }
+    } else if (arrive_last(p.counters + index, x.tiles, &s_last)) {
+      aw_lse(p, x, index);
     }
   }
 }
@@ -702,7 +745,7 @@ __global__ __launch_bounds__(256) void aw_sum_kernel(AwParams p) {
       for (int k = 0; k < 16; k += 4) e[k][i] += e[k + 2][i];
       e[0][i] = (e[0][i] + e[4][i]) + (e[8][i] + e[12][i]);
     }
-    aw_update(p, x, t, e[0]);
+    aw_update(p, x, t, true, 1, [&](int) { return e[0]; });
   }
 }
 
@@ -728,11 +771,18 @@ static const void* aw_store_fn(int D, bool f32) {
 
 // Stored scores lie within a buffer's offsets.
 static bool aw_stores(int64_t rows, int64_t tiles) { return rows <= kAwStoreRows && tiles <= (1 << 16); }
-static int64_t aw_launch_rows(int64_t rows) { return rows < kAwLaunchRows ? rows : kAwLaunchRows; }
-struct AwSpace { size_t scores, stats, lse; };  // bytes
+struct AwSpace { int64_t rows, segs; size_t scores, stats, lse, sums; };  // rows of a segment, segments of a launch; bytes
 static AwSpace aw_space(int64_t progs, int64_t rows, int64_t tiles) {
-  return {aw_stores(rows, tiles) ? align_up((size_t)(progs * rows * tiles * kAwTile * 4), 256) : 0,
-          align_up((size_t)(progs * tiles * rows * 8), 256), align_up((size_t)(progs * rows * 4), 256)};
+  AwSpace a = {};
+  a.rows = rows < kAwSegRows ? rows : kAwSegRows;
+  a.scores = aw_stores(rows, tiles) ? align_up((size_t)(progs * rows * tiles * kAwTile * 4), 256) : 0;
+  // As many segments as there are, where their counters find room and they need no more than 64 MiB.
+  for (a.segs = ceil_div64(rows, kAwSegRows) < kAwSegs ? ceil_div64(rows, kAwSegRows) : kAwSegs;; --a.segs) {
+    a.stats = align_up((size_t)(a.segs * progs * tiles * a.rows * 8), 256);
+    a.lse = align_up((size_t)(a.segs * progs * a.rows * 4), 256);
+    a.sums = a.segs > 1 ? (size_t)(a.segs * progs * tiles * kAwTile * 4) : 0;
+    if (a.segs <= 1 || (progs * (a.segs + tiles) * 4 <= (int64_t)kCounterBytes && a.stats + a.sums <= 64u << 20)) return a;
+  }
 }
 
 }  // namespace specq
@@ -742,9 +792,8 @@ using namespace specq;
 extern "C" size_t specq_paged_attn_weights_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int max_pages,
                                                           int PAGE) {
   if (B_grid <= 0 || H <= 0 || H_KV <= 0 || H % H_KV != 0 || ql_grid <= 0 || max_pages <= 0 || PAGE <= 0) return 0;
-  const AwSpace s = aw_space((int64_t)B_grid * H_KV, aw_launch_rows((int64_t)ql_grid * (H / H_KV)),
-                             ceil_div64((int64_t)max_pages * PAGE, kAwTile));
-  return kCounterBytes + s.scores + s.stats + s.lse;
+  const AwSpace s = aw_space((int64_t)B_grid * H_KV, (int64_t)ql_grid * (H / H_KV), ceil_div64((int64_t)max_pages * PAGE, kAwTile));
+  return kCounterBytes + s.scores + s.stats + s.lse + s.sums;
 }
 
 extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh, const int8_t* kc,
@@ -790,10 +839,12 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   p.plan = plan; p.n_seqs = n_seqs; p.q_len = q_len; p.B_grid = B_grid; p.ql_grid = ql_grid;
   p.G = H / H_KV; p.g_magic = p.G > 1 ? (uint32_t)(((1ull << 32) + p.G - 1) / p.G) : 0;
   p.H_KV = H_KV; p.PAGE = PAGE;
-  p.cap = (int)cap; p.tiles = (int)ceil_div64(cap, kAwTile); p.rows = (int)aw_launch_rows(rows);
+  p.cap = (int)cap; p.tiles = (int)ceil_div64(cap, kAwTile);
   p.scale_log2 = sm_scale * 1.44269504088896340736f;
-  const AwSpace space = aw_space(progs, p.rows, p.tiles);
-  const size_t need = kCounterBytes + space.scores + space.stats + space.lse;
+  const AwSpace space = aw_space(progs, rows, p.tiles);
+  p.rows = (int)space.rows;
+  p.segs = (int)space.segs;
+  const size_t need = kCounterBytes + space.scores + space.stats + space.lse + space.sums;
   SPECQ_REQUIRE(workspace && workspace_bytes >= need, SPECQ_ENOSPC,
                 "paged_attn_weights: workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
   char* at = static_cast<char*>(workspace);
@@ -801,6 +852,7 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   p.scores = reinterpret_cast<float*>(at + kCounterBytes);
   p.stats = reinterpret_cast<uint64_t*>(at + kCounterBytes + space.scores);
   p.lse = reinterpret_cast<float*>(at + kCounterBytes + space.scores + space.stats);
+  p.sums = reinterpret_cast<uint64_t*>(at + kCounterBytes + space.scores + space.stats + space.lse);
   // Stored scores against scores formed twice (us, 8 KV heads of 128): 4 rows, 8 sequences of 4096: 20.3, 24.6; 32 of 8192: 82,
   // 121; 16 rows, 8 of 4096: 27.3, 24.8; one of 32768: 28.6, 32.8.  Queries in LDS for the whole call against 64 rows at a
   // time: 20 rows, 8 of 4096: 28.7, 58.6; 64 rows: 37.7, 58.5; one of 32768: 54, 69.
@@ -808,9 +860,9 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   // Tiles of a workgroup of few rows: as many as leave two workgroups to a CU.
   const int64_t tiles = progs * p.tiles, span = tiles / (2 * device_cus());
   p.span = few ? (int)(span < 1 ? 1 : span > kAwSpan ? kAwSpan : span) : 1;
-  const int64_t items = progs * ceil_div(p.tiles, p.span), sums = progs * ceil_div64(cap, kAwSumTile);
+  const int64_t items = progs * ceil_div(p.tiles, p.span) * p.segs, sums = progs * ceil_div64(cap, kAwSumTile);
   const int grid = (int)(items < kAwMaxGrid ? items : kAwMaxGrid), threads = few ? 256 : 512;
-  for (p.row0 = 0; p.row0 < rows; p.row0 += kAwLaunchRows) {
+  for (p.row0 = 0; p.row0 < rows; p.row0 += p.segs * kAwSegRows) {
     if (int rc = launch(store ? aw_store_fn(D, f32) : aw_fn<kAwStats>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p))
       return rc;
     const int rc = store ? launch(reinterpret_cast<const void*>(&aw_sum_kernel), (int)(sums < kAwMaxGrid ? sums : kAwMaxGrid),
