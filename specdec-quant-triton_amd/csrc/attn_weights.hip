@@ -11,9 +11,10 @@
 //      joins them to log2 of each row's sum over all tiles
 //   2  p = exp2(s - that), summed over the rows, and the update of w
 // The scores of up to 16 rows (kAwStoreRows: plain decoding) go from 1 to 2 through the workspace; more rows compute them
-// again.  Both ways add a token's rows in one order (16 lanes; in each the blocks of 16 rows of either parity, then both; then pairs of
-// lanes) and join the rows' statistics in one (64 tokens, 256, all), so they give the same bits, and a plan-mode call those of an
-// eager one.
+// again.  Both ways add a token's rows in one order (16 lanes; in each the blocks of 16 rows of either parity, then both; then
+// pairs of lanes; then units of 512 rows one after another) and join the rows' statistics in one (64 tokens, 256, all), so they
+// give the same bits, and a plan-mode call those of an eager one.  Workgroups take one or two units each, and the last of a
+// tile's adds theirs up.
 //
 // K stays: a wave holds 64 tokens, converts their codes to fp16 matrix operands once and walks the rows 16 at a time
 // (K . Q^T on v_mfma_f32_16x16x32_f16: a lane's results are four tokens of one row).  Everything behind the products is
@@ -30,8 +31,10 @@ constexpr int kAwTile = 256;       // tokens of a workgroup: 4 waves of 4 sub-ti
 constexpr int kAwStoreRows = 16;   // rows whose scores go through the workspace
 constexpr int kAwFewRows = 64;     // rows whose queries a workgroup keeps in LDS
 constexpr int kAwSpan = 8;         // most tiles such a workgroup walks (its waves' lanes hold their pages, and one tile's more)
-constexpr int kAwSegRows = 1024;   // rows of a segment, whose sums over the rows are added to the weights in one piece
-constexpr int kAwSegs = 8;         // most segments of a launch
+constexpr int kAwUnitRows = 512;   // rows whose sums are added to the weights in one piece
+constexpr int kAwSegUnits = 2;     // most units of a workgroup
+constexpr int kAwSegs = 8;         // most such segments of a launch
+constexpr int kAwFill = 256;       // workgroups that fill the GPU: fewer take a unit each
 constexpr int kAwSeg = 32;         // row blocks of 16 whose statistics are joined at a time
 constexpr int kAwSumTile = 1024;   // tokens of a workgroup that adds up stored scores
 constexpr int kAwMaxGrid = 1 << 16;
@@ -49,12 +52,12 @@ struct AwParams {
   int tiles;    // of cap
   int span;     // tiles of a workgroup of few rows
   int rows;     // of a program and segment at most
-  int row0;     // the launch's first row: more than segs * kAwSegRows have several pairs of launches one after another
-  int segs;     // of a launch
+  int row0;     // the launch's first row: more than segs * seg_rows have several pairs of launches one after another
+  int seg_rows, segs;  // rows of a workgroup's segment (a unit or more), segments of a launch
   uint32_t g_magic;  // ceil(2^32 / G): row / G is its product's high word (rows below 2^20, G below 2^12); 0 for G = 1
   float scale_log2;
   // Workspace: scores [prog][rows][tiles * 256]; (max, sum) [prog][seg][tiles][rows]; log2 of the rows' sums [prog][seg][rows];
-  // sums of a segment's rows [prog][seg][tiles * 256], two tokens a word.
+  // sums of a unit's rows [prog][unit][tiles * 256], two tokens a word.
   float* scores; uint64_t* stats; float* lse; uint64_t* sums;
   int32_t* counters;  // [prog][seg], then [prog][tile]
 };
@@ -129,26 +132,26 @@ __device__ __forceinline__ void aw_join(float& m, float& l, float m2, float l2) 
   m = top;
 }
 
-// What tokens gather, `n` pieces of it, is added to what they have; new ones start from nothing (where `start`: others have
-// been set by an earlier launch).
-template <typename F>
-__device__ __forceinline__ void aw_update(const AwParams& p, const AwProg& x, int t, bool start, int n, F&& piece) {
-  float* w = p.w + x.b * p.s_wb + x.h * p.s_wh + t;
-  const int fresh = start ? x.L - x.ql : x.L;
-  const bool vec = p.w_vec && t + 4 <= x.L;
+// The weights of tokens t..t + 3; new ones start from nothing (`start`: unless an earlier launch has set them).
+__device__ __forceinline__ v4f aw_get(const AwParams& p, const AwProg& x, int t, bool start) {
+  const float* w = p.w + x.b * p.s_wb + x.h * p.s_wh + t;
   v4f v = {0.f, 0.f, 0.f, 0.f};
-  if (vec) {
+  if (p.w_vec && t + 4 <= x.L) {
     v = *reinterpret_cast<const v4f*>(w);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (t + i < x.L) v[i] = w[i];
   }
+  const int fresh = start ? x.L - x.ql : x.L;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (t + i >= fresh) v[i] = 0.f;
-  for (int k = 0; k < n; ++k) v += piece(k);
-  if (vec) {
+  return v;
+}
+__device__ __forceinline__ void aw_put(const AwParams& p, const AwProg& x, int t, const v4f& v) {
+  float* w = p.w + x.b * p.s_wb + x.h * p.s_wh + t;
+  if (p.w_vec && t + 4 <= x.L) {
     *reinterpret_cast<v4f*>(w) = v;
   } else {
 #pragma unroll
@@ -156,7 +159,6 @@ __device__ __forceinline__ void aw_update(const AwParams& p, const AwProg& x, in
       if (t + i < x.L) w[i] = v[i];
   }
 }
-
 
 enum { kAwStats, kAwSums };  // pass 1, and pass 2 from K
 
@@ -437,7 +439,7 @@ __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
 #pragma unroll
         for (int s = 0; s < 4; ++s) even[s] += odd[s];
         const v4f got = aw_rows(even);
-        if (r < 4 && aw_first(t0) < x.L) aw_update(p, x, aw_first(t0), true, 1, [&](int) { return got; });
+        if (const int t = aw_first(t0); r < 4 && t < x.L) aw_put(p, x, t, aw_get(p, x, t, true) + got);
       }
     }
     if constexpr (MODE != kAwSums) {
@@ -541,7 +543,7 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
   auto key = [](int t) { return D == 128 ? t & 15 : (t >> 1) & 7; };
   const int progs = p.B_grid * p.H_KV, per = p.segs * progs;
   for (int64_t item = blockIdx.x; item < (int64_t)per * p.tiles; item += gridDim.x) {
-    const int tile = (int)(item / per), some = (int)(item % per), seg_i = some / progs, row0 = p.row0 + seg_i * kAwSegRows;
+    const int tile = (int)(item / per), some = (int)(item % per), seg_i = some / progs, row0 = p.row0 + seg_i * p.seg_rows;
     const int prog = aw_order(p, some - seg_i * progs), index = prog * p.segs + seg_i, t0 = tile * kAwTile + 64 * w;
     AwProg x;
     if (!aw_prog(p, prog, x, row0) || tile >= x.tiles) continue;
@@ -568,6 +570,16 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
     v4f sums[4];
 #pragma unroll
     for (int s = 0; s < 4; ++s) sums[s] = v4f{0.f, 0.f, 0.f, 0.f};
+    // Segments of this launch that have rows which see the tile, from the first such row on; the weights so far of the lane's
+    // tokens, where no other workgroup adds to them.
+    const int first_row = max(tile * kAwTile - fresh, 0) * p.G, seg0 = max(first_row - p.row0, 0) / p.seg_rows;
+    const int seg1 = min(p.segs, (x.ql * p.G - p.row0 + p.seg_rows - 1) / p.seg_rows), my_t = aw_first(t0);
+    const bool alone = seg1 - seg0 == 1, start = first_row >= p.row0, mine = !odd && r < 4 && my_t < x.L;
+    auto words = [&](int unit, int t) {  // of the launch
+      return p.sums + (((int64_t)prog * (p.segs * p.seg_rows / kAwUnitRows) + unit) * p.tiles * kAwTile + t) / 2;
+    };
+    v4f weight = {0.f, 0.f, 0.f, 0.f};
+    if (MODE == kAwSums && alone && mine) weight = aw_get(p, x, my_t, start);
     // The first row block that sees token t.
     auto first_of = [&](int t) { return t > fresh ? min(max((t - fresh) * p.G - row0, 0) / 16, blocks) : 0; };
     int rb = first_of(tile * kAwTile) & ~3;  // four blocks at a time, from the first that sees the tile's first token
@@ -650,6 +662,28 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
             keep(rb + odd + 2 * k, aw_stat(acc[k]));
           }
         }
+        if constexpr (MODE == kAwSums) {
+          if (rb + 4 >= blocks || (rb + 4) % (kAwUnitRows / 16) == 0) {  // a unit ends: both parities, then the lanes
+            if (odd) {
+#pragma unroll
+              for (int s = 0; s < 4; ++s) s_sums[w][s][lane] = sums[s];
+            }
+            wg_barrier_lds();
+            if (!odd) {
+#pragma unroll
+              for (int s = 0; s < 4; ++s) sums[s] += s_sums[w][s][lane];
+              const v4f got = aw_rows(sums);
+              weight += got;
+              if (r < 4 && !alone) {
+                uint64_t* to = words((row0 - p.row0 + rb * 16) / kAwUnitRows, my_t);
+                publish(to, aw_pack(got[0], got[1]));
+                publish(to + 1, aw_pack(got[2], got[3]));
+              }
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) sums[s] = v4f{0.f, 0.f, 0.f, 0.f};
+          }
+        }
       }
       if constexpr (MODE != kAwSums) {
         __syncthreads();
@@ -664,36 +698,21 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
       }
     }
     if constexpr (MODE == kAwSums) {
-      if (odd) {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) s_sums[w][s][lane] = sums[s];
-      }
-      __syncthreads();
-      // The segments of this launch that have rows which see the tile, and whether an earlier launch had any.
-      const int base = p.row0 / kAwSegRows, from_seg = max(tile * kAwTile - fresh, 0) * p.G / kAwSegRows, seg0 = max(from_seg - base, 0);
-      const int seg1 = min(p.segs, (x.ql * p.G - p.row0 + kAwSegRows - 1) / kAwSegRows);
-      const bool start = from_seg >= base, alone = seg1 - seg0 == 1;
-      auto words = [&](int seg, int t) { return p.sums + ((int64_t)(prog * p.segs + seg) * p.tiles * kAwTile + t) / 2; };
-      if (!odd) {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) sums[s] += s_sums[w][s][lane];
-        const v4f got = aw_rows(sums);
-        const int t = aw_first(t0);
-        if (r < 4 && alone && t < x.L) aw_update(p, x, t, start, 1, [&](int) { return got; });
-        if (r < 4 && !alone) {
-          publish(words(seg_i, t), aw_pack(got[0], got[1]));
-          publish(words(seg_i, t) + 1, aw_pack(got[2], got[3]));
-        }
-      }
       if (alone) {
+        if (mine) aw_put(p, x, my_t, weight);
         __syncthreads();
       } else if (arrive_last(p.counters + per + (int64_t)prog * p.tiles + tile, seg1 - seg0, &s_last)) {
+        // The last of the tile's workgroups adds the units up in their order.
+        const int unit1 = (min(x.ql * p.G - p.row0, p.segs * p.seg_rows) + kAwUnitRows - 1) / kAwUnitRows;
         const int t = tile * kAwTile + 4 * (int)threadIdx.x;
-        if (threadIdx.x < kAwTile / 4 && t < x.L)
-          aw_update(p, x, t, start, seg1 - seg0, [&](int k) {
-            const uint64_t a = collect(words(seg0 + k, t)), b = collect(words(seg0 + k, t) + 1);
-            return v4f{aw_m(a), aw_l(a), aw_m(b), aw_l(b)};
-          });
+        if (threadIdx.x < kAwTile / 4 && t < x.L) {
+          v4f v = aw_get(p, x, t, start);
+          for (int unit = max(first_row - p.row0, 0) / kAwUnitRows; unit < unit1; ++unit) {
+            const uint64_t a = collect(words(unit, t)), b = collect(words(unit, t) + 1);
+            v += v4f{aw_m(a), aw_l(a), aw_m(b), aw_l(b)};
+          }
+          aw_put(p, x, t, v);
+        }
       }
     } else if (arrive_last(p.counters + index, x.tiles, &s_last)) {
       aw_lse(p, x, index);
@@ -745,7 +764,7 @@ __global__ __launch_bounds__(256) void aw_sum_kernel(AwParams p) {
       for (int k = 0; k < 16; k += 4) e[k][i] += e[k + 2][i];
       e[0][i] = (e[0][i] + e[4][i]) + (e[8][i] + e[12][i]);
     }
-    aw_update(p, x, t, true, 1, [&](int) { return e[0]; });
+    aw_put(p, x, t, aw_get(p, x, t, true) + e[0]);
   }
 }
 
@@ -771,16 +790,20 @@ static const void* aw_store_fn(int D, bool f32) {
 
 // Stored scores lie within a buffer's offsets.
 static bool aw_stores(int64_t rows, int64_t tiles) { return rows <= kAwStoreRows && tiles <= (1 << 16); }
-struct AwSpace { int64_t rows, segs; size_t scores, stats, lse, sums; };  // rows of a segment, segments of a launch; bytes
+struct AwSpace { int64_t seg_rows, segs, rows; size_t scores, stats, lse, sums; };  // as in AwParams; bytes
 static AwSpace aw_space(int64_t progs, int64_t rows, int64_t tiles) {
   AwSpace a = {};
-  a.rows = rows < kAwSegRows ? rows : kAwSegRows;
   a.scores = aw_stores(rows, tiles) ? align_up((size_t)(progs * rows * tiles * kAwTile * 4), 256) : 0;
+  // Two units a workgroup, or one where that fills no more than the GPU.  256 tokens at 4096, 8 heads of 4 queries, one sequence:
+  // 68 us, 45; two (twice as many workgroups as CUs): 78, 83.
+  a.seg_rows = kAwUnitRows * (progs * tiles * ceil_div64(rows, kAwUnitRows) <= kAwFill ? 1 : kAwSegUnits);
+  a.rows = rows < a.seg_rows ? rows : a.seg_rows;
   // As many segments as there are, where their counters find room and they need no more than 64 MiB.
-  for (a.segs = ceil_div64(rows, kAwSegRows) < kAwSegs ? ceil_div64(rows, kAwSegRows) : kAwSegs;; --a.segs) {
+  const int64_t segs = ceil_div64(rows, a.seg_rows);
+  for (a.segs = segs < kAwSegs ? segs : kAwSegs;; --a.segs) {
     a.stats = align_up((size_t)(a.segs * progs * tiles * a.rows * 8), 256);
     a.lse = align_up((size_t)(a.segs * progs * a.rows * 4), 256);
-    a.sums = a.segs > 1 ? (size_t)(a.segs * progs * tiles * kAwTile * 4) : 0;
+    a.sums = a.segs > 1 ? (size_t)(a.segs * (a.seg_rows / kAwUnitRows) * progs * tiles * kAwTile * 4) : 0;
     if (a.segs <= 1 || (progs * (a.segs + tiles) * 4 <= (int64_t)kCounterBytes && a.stats + a.sums <= 64u << 20)) return a;
   }
 }
@@ -843,6 +866,7 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   p.scale_log2 = sm_scale * 1.44269504088896340736f;
   const AwSpace space = aw_space(progs, rows, p.tiles);
   p.rows = (int)space.rows;
+  p.seg_rows = (int)space.seg_rows;
   p.segs = (int)space.segs;
   const size_t need = kCounterBytes + space.scores + space.stats + space.lse + space.sums;
   SPECQ_REQUIRE(workspace && workspace_bytes >= need, SPECQ_ENOSPC,
@@ -862,7 +886,7 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   p.span = few ? (int)(span < 1 ? 1 : span > kAwSpan ? kAwSpan : span) : 1;
   const int64_t items = progs * ceil_div(p.tiles, p.span) * p.segs, sums = progs * ceil_div64(cap, kAwSumTile);
   const int grid = (int)(items < kAwMaxGrid ? items : kAwMaxGrid), threads = few ? 256 : 512;
-  for (p.row0 = 0; p.row0 < rows; p.row0 += p.segs * kAwSegRows) {
+  for (p.row0 = 0; p.row0 < rows; p.row0 += p.segs * p.seg_rows) {
     if (int rc = launch(store ? aw_store_fn(D, f32) : aw_fn<kAwStats>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p))
       return rc;
     const int rc = store ? launch(reinterpret_cast<const void*>(&aw_sum_kernel), (int)(sums < kAwMaxGrid ? sums : kAwMaxGrid),

@@ -67,7 +67,8 @@ def check(got, case, q_lens, sm, what):
     ([5000], 3, 8, 1, 128, 128),                  # 24 rows of one head, 20 tiles
     ([400, 90], 90, 8, 2, 128, 16),               # a prompt chunk of 23 row blocks; a whole prompt
     ([600], 600, 2, 1, 64, 16),                   # more row blocks than are joined at a time
-    ([900, 620], 610, 4, 1, 128, 64),             # rows of more than one launch pair, for one sequence a prompt
+    ([900, 620], 610, 4, 1, 128, 64),             # rows of several segments, for one sequence nearly a prompt
+    ([1100], 1100, 8, 1, 64, 16),                 # and of several pairs of launches
     ([333, 1000], 150, 8, 2, 64, 16),             # ... whose first seen ones lie anywhere among them
     ([291, 180, 777], 177, 12, 4, 128, 48),
     ([0, 3, 20], 7, 4, 4, 128, 16),               # an empty sequence, one of fewer tokens than are new
@@ -271,7 +272,7 @@ def test_empty_and_refusals():
 
 @pytest.mark.parametrize("QL,G,ctx", [(4, 4, 700), (9, 4, 700), (300, 2, 700), (700, 2, 700)])
 def test_a_nan_row_shares_nothing_out_to_tokens_it_does_not_see(QL, G, ctx):
-    """16, 36, 600 and 1400 rows: stored scores, scores formed twice, and those of one and two pairs of launches."""
+    """16, 36, 600 and 1400 rows: stored scores, scores formed twice, in one pass of the queries and in segments."""
     rng = np.random.default_rng(23)
     q, kc, ks, bt, cl, w = make(rng, [ctx], QL, 2 * G, 2, 64, 16, True)
     bad, i = q.copy(), QL // 2 - 1
@@ -281,3 +282,24 @@ def test_a_nan_row_shares_nothing_out_to_tokens_it_does_not_see(QL, G, ctx):
     assert np.isnan(got[1][0, 0, :sees]).sum() == sees
     assert (got[1][0, 0, sees:] != got[0][0, 0, sees:]).sum() == 0
     assert (got[1][0, 1] != got[0][0, 1]).sum() == 0
+
+
+@pytest.mark.parametrize("QL,H,HK,D", [(150, 8, 1, 128), (300, 8, 1, 64), (40, 8, 2, 128), (700, 4, 2, 128),
+                                       (1100, 8, 1, 64)])
+def test_the_table_size_does_not_change_a_bit(QL, H, HK, D):
+    """A table of many more columns, and a plan-mode call of more tokens and sequences, split the rows otherwise."""
+    rng = np.random.default_rng(QL)
+    q, kc, ks, bt, cl, w = make(rng, [QL + 200, QL], QL, H, HK, D, 16, False)
+    note(f"attn_weights table size QL={QL}")
+    want = K.paged_attention_weights(*gpu(q, kc, ks, bt, cl, w))
+    wide = np.full((5, 9000), -1, np.int32)
+    wide[:2, :bt.shape[1]] = bt
+    more = np.zeros((5, HK, 9000 * 16), np.float32)
+    more[:2, :, :w.shape[2]] = w
+    got = K.paged_attention_weights(*gpu(q, kc, ks, wide[:2], cl, more[:2]))
+    assert torch.equal(got[:, :, :w.shape[2]], want) and not got[:, :, w.shape[2]:].any()
+    q5, cl5 = np.zeros((5, QL + 500, H, D), np.float16), np.zeros(5, np.int32)
+    q5[:2, :QL], cl5[:2] = q, cl
+    plan = torch.tensor([2, QL], dtype=torch.int32, device=DEV)
+    got = K.paged_attention_weights(*gpu(q5, kc, ks, wide, cl5, more), plan=plan)
+    assert torch.equal(got[:2, :, :w.shape[2]], want) and not got[2:].any()
