@@ -14,7 +14,7 @@
 //      beams whose scores lie closer than an fp32 step apart are to be told apart as the formula does.  Again a value that n
 //      reach, then the few that do, ranked against one another.  The order in which lists are filled has no part in the result.
 //
-// 16 x 8 rows of 128257 fp32 logits: 17.2 us (66 MB, 3.8 TB/s) and 8.8; 4 of 32000 fp16: 5.6 and 5.9.  The second launch waits for
+// 16 x 8 rows of 128257 fp32 logits: 17.1 us (66 MB, 3.9 TB/s) and 8.9; 4 of 32000 fp16: 5.5 and 5.9.  The second launch waits for
 // memory three times over, whatever its size.
 //
 // Reordering: row r of every state becomes row parents[r] of the same group of rows.  In place: a thread owns one column of

@@ -9,8 +9,8 @@
 // (interleaved, one vector) or 8 values that are not turned -- so the row is read once, stays in registers over the sum
 // of its squares (a few lane exchanges) and is written once.  The lanes make their angles once for the heads they walk.
 // In place works: every value of a row is an operand of the sum that each store waits for.
-// Prompts are bound by HBM (2 x 4096 tokens, 32 / 8 heads of 128: 168 MB in 33.8 us, the rate of a copy), steps by the launch
-// (one token 4.9 us; 51 tokens of 12 / 3 heads of 80, which the vector kernel does not take, 5.1).
+// Prompts are bound by HBM (2 x 4096 tokens, 32 / 8 heads of 128: 168 MB in 33.7 us, the rate of a copy), steps by the launch
+// (one token 4.6 us; 51 tokens of 12 / 3 heads of 80, which the vector kernel does not take, 5.1).
 #include "api_common.hpp"
 #include "rotary.hpp"
 
