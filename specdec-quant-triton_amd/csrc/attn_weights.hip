@@ -319,7 +319,7 @@ __device__ __forceinline__ void aw_lse(const AwParams& p, const AwProg& x, int a
       m = top;
     }
   };
-  if (x.rows > kAwFewRows) {
+  if (x.ql * p.G > kAwFewRows) {  // of the program, not of a segment: a row's order is the same in any
     for (int row = threadIdx.x; row < x.rows; row += threads) {
       float m = -INFINITY, l = 0.f;
       walk(row, 0, 1, m, l);

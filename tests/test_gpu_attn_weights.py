@@ -285,7 +285,7 @@ def test_a_nan_row_shares_nothing_out_to_tokens_it_does_not_see(QL, G, ctx):
 
 
 @pytest.mark.parametrize("QL,H,HK,D", [(150, 8, 1, 128), (300, 8, 1, 64), (40, 8, 2, 128), (700, 4, 2, 128),
-                                       (1100, 8, 1, 64)])
+                                       (1100, 8, 1, 64), (68, 8, 1, 128)])
 def test_the_table_size_does_not_change_a_bit(QL, H, HK, D):
     """A table of many more columns, and a plan-mode call of more tokens and sequences, split the rows otherwise."""
     rng = np.random.default_rng(QL)
