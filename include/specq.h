@@ -484,7 +484,7 @@ int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int max_pages,
  * select: of the candidates scores[b, w] + logits[b, w, v] - log(sum_u exp(logits[b, w, u])) of each sequence the best n,
  *   in order, ties to the lower beam, then the lower token.  A beam with finished[b, w] != 0 has one candidate, token eos
  *   with the score it has.  Candidates whose score is NaN or -infinity are none; what is missing is (-inf, -1, -1).
- *   Scores are compared in fp64.
+ *   Scores are formed and compared in fp64; a row's log-sum is within 2^-33.
  *   logits    fp16 or (logits_fp32) fp32 [B, W, V], strides s_lb, s_lw;  scores fp32 [B, W], row stride s_sb
  *   finished  NULL, or bytes [B, W], row stride s_fb
  *   out_scores fp32, out_tokens, out_parents int32 [B, n]; a parent is the row b W + w.  W, n at most 64.

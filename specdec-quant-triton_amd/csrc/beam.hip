@@ -10,12 +10,15 @@
 //      candidates.  If k of the 64 lanes' maxima reach a value in each of the four waves, 4 k values of the part do; with k the
 //      fourth part of n, what reaches the least such value of a wave holds the part's best n and few more.  These are left
 //      for 2, at most kBeamSlots of them; where more reach it (equal values) the best n are taken one by one.
-//   2  A workgroup to a sequence joins each row's sums, in fp64, and forms the candidates' scores, in fp64 too, since
-//      beams whose scores lie closer than an fp32 step apart are to be told apart as the formula does.  Again a value that n
-//      reach, then the few that do, ranked against one another.  The order in which lists are filled has no part in the result.
+//   2  A workgroup to a sequence joins each row's sums and forms the candidates' scores.  Again a value that n reach, then the
+//      few that do, ranked against one another.  The order in which lists are filled has no part in the result.
+// Exponentials (within 2^-34 of themselves), sums, logarithms and scores are fp64, so beams are told apart as the formula does
+// where their scores lie closer than fp32 steps: fp32 sums put a row's log-sum off by 2^-23, and with it all of its beam.
 //
-// 16 x 8 rows of 128257 fp32 logits: 17.1 us (66 MB, 3.9 TB/s) and 8.9; 4 of 32000 fp16: 5.5 and 5.9.  The second launch waits for
-// memory three times over, whatever its size.
+// 16 x 8 rows of 128257 fp32 logits: 20.5 us (66 MB, 3.2 TB/s; with fp32 exponentials 17.1) and 9.1; 4 of 32000 fp16: 6.1 and 5.8.
+// An exponential is 15 fp64 instructions of the rate of fp32 ones.  Fewer vectors a lane, for more waves, leave the first launch at
+// 20.5 and give the second more parts to join (4: 13.0 us); sums that start with the first loads keep more registers (22.8).  The
+// second launch waits for memory three times over, whatever its size.
 //
 // Reordering: row r of every state becomes row parents[r] of the same group of rows.  In place: a thread owns one column of
 // up to 16 bytes of a group's rows, reads what changes and then writes it.  Bound by HBM: 16 x 8 rows of 418 KB, 13.7 us.
@@ -41,15 +44,38 @@ struct BeamParams {
   float* out_score; int32_t* out_token; int32_t* out_parent;
   int W, V, n;
   int parts;  // of a row
-  // Workspace, of each part: (max, sum), the number of candidates, and they: (value, token).
-  uint64_t* stats; int32_t* counts; uint64_t* cands;
+  // Workspace, of each part: maximum, sum, the number of candidates, and they: (value, token).
+  float* tops; double* sums; int32_t* counts; uint64_t* cands;
 };
 
 __device__ __forceinline__ uint64_t beam_pack(float a, uint32_t b) {
   return (uint64_t)__builtin_bit_cast(uint32_t, a) | ((uint64_t)b << 32);
 }
 __device__ __forceinline__ float beam_lo(uint64_t x) { return __builtin_bit_cast(float, (uint32_t)x); }
-__device__ __forceinline__ float beam_hi(uint64_t x) { return __builtin_bit_cast(float, (uint32_t)(x >> 32)); }
+
+// 2^(x log2 e - ref), where that is no more than 1: 2^n of the nearest whole number n, which adding 1.5 * 2^52 leaves in the lower bits,
+// and a polynomial that meets 2^f on |f| <= 1/2 in the Chebyshev points of degree 7, off by at most 2^-34 of itself.  What is below
+// 2^-1000 counts as that; -infinity too, and NaN.
+__device__ __forceinline__ double beam_exp(float x, double ref) {
+  constexpr double kWhole = 6755399441055744.;
+  const double t = fmax(fma((double)x, 1.4426950408889634074, -ref), -1000.), w = t + kWhole, f = t - (w - kWhole);
+  double e = 1.5303699001378845e-05;
+  e = fma(e, f, 1.5469729140704658e-04);
+  e = fma(e, f, 1.3333478480888061e-03);
+  e = fma(e, f, 9.618025613598036e-03);
+  e = fma(e, f, 5.550410906317715e-02);
+  e = fma(e, f, 2.4022651213495422e-01);
+  e = fma(e, f, 6.931471805568341e-01);
+  e = fma(e, f, 9.999999999595622e-01);
+  v2i u = __builtin_bit_cast(v2i, e);
+  u[1] += __builtin_bit_cast(v2i, w)[0] << 20;
+  return __builtin_bit_cast(double, u);
+}
+__device__ __forceinline__ double beam_shfl(double v, int o) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __shfl_xor((uint32_t)u, o), hi = __shfl_xor((uint32_t)(u >> 32), o);
+  return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
+}
 
 // Values that at least i and j (1..64) of the lanes' values reach, no NaN among them: the i-th and the j-th largest with the
 // lower half of their keys cut off (found bit by bit; all 32 would take twice the time and spare few candidates).
@@ -80,7 +106,8 @@ template <typename T, int NV>
 __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamParams p) {
   constexpr int VE = 16 / sizeof(T), E = NV * VE;
   __shared__ uint64_t slots[kBeamSlots];
-  __shared__ float s_max[kBeamWaves], s_sum[kBeamWaves], s_some[kBeamWaves], s_all[kBeamWaves];
+  __shared__ double s_sum[kBeamWaves];
+  __shared__ float s_max[kBeamWaves], s_some[kBeamWaves], s_all[kBeamWaves];
   __shared__ int s_token[kBeamWaves], s_count;
   const int64_t at = blockIdx.x;
   const int part = (int)(at % p.parts), row_id = (int)(at / p.parts), b = row_id / p.W, w = row_id - b * p.W;
@@ -88,7 +115,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamParams p) {
   if (p.done != nullptr && p.done[b * p.s_db + w] != 0) {
     // One candidate of value 0 in a row whose sum is exp(0).
     if (threadIdx.x == 0) {
-      p.stats[at] = part == 0 ? beam_pack(0.f, __builtin_bit_cast(uint32_t, 1.f)) : beam_pack(-INFINITY, 0);
+      p.tops[at] = part == 0 ? 0.f : -INFINITY;
+      p.sums[at] = part == 0 ? 1. : 0.;
       p.counts[at] = part == 0 ? 1 : 0;
       if (part == 0) p.cands[at * kBeamSlots] = beam_pack(0.f, (uint32_t)p.eos);
     }
@@ -117,12 +145,20 @@ __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamParams p) {
   float m = mine;
 #pragma unroll
   for (int o = 1; o < kWave; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
-  const float ref = m == -INFINITY ? 0.f : m;
-  float sum = 0.f;
+  const double ref = (m == -INFINITY ? 0. : (double)m) * 1.4426950408889634074;
+  double sum = 0;
+  bool nan = m == INFINITY;
 #pragma unroll
-  for (int k = 0; k < E; ++k) sum += fast_exp2((x[k] - ref) * 1.44269504088896340736f);
+  for (int k = 0; k < E; k += 2) {
+    nan |= __builtin_isunordered(x[k], x[k + 1]);
+    sum += beam_exp(x[k], ref);
+    sum += beam_exp(x[k + 1], ref);
+  }
 #pragma unroll
-  for (int o = 1; o < kWave; o *= 2) sum += __shfl_xor(sum, o);
+  for (int o = 1; o < kWave; o *= 2) sum += beam_shfl(sum, o);
+  // Nothing, where there is no value; a row that holds NaN or +infinity has no sum.
+  if (m == -INFINITY) sum = 0;
+  if (__builtin_amdgcn_ballot_w64(nan) != 0) sum = __builtin_nan("");
   const BeamNth nth = beam_nth(mine, (p.n + kBeamWaves - 1) / kBeamWaves, p.n);
   if (lane == 0) s_max[wave] = m, s_sum[wave] = sum, s_some[wave] = nth.i, s_all[wave] = nth.j;
   __syncthreads();
@@ -177,20 +213,17 @@ __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamParams p) {
     __syncthreads();
   }
   for (int i = threadIdx.x; i < count; i += kBeamThreads) p.cands[at * kBeamSlots + i] = slots[i];
-  if (threadIdx.x == 0) {
-    float all = 0.f;
+  // The waves' sums, a lane each.
+  double all = threadIdx.x < kBeamWaves ? s_sum[threadIdx.x] : 0.;
+  // A NaN sum stays one, whatever its wave's maximum.
+  if (threadIdx.x < kBeamWaves && all != 0.) all *= beam_exp(s_max[threadIdx.x], (double)top * 1.4426950408889634074);
 #pragma unroll
-    for (int v = 0; v < kBeamWaves; ++v)  // a NaN sum stays one, whatever its wave's maximum
-      all += s_sum[v] == 0.f ? 0.f : s_sum[v] * fast_exp2((s_max[v] - top) * 1.44269504088896340736f);
-    p.stats[at] = beam_pack(top, __builtin_bit_cast(uint32_t, all));
+  for (int o = 1; o < kBeamWaves; o *= 2) all += beam_shfl(all, o);
+  if (threadIdx.x == 0) {
+    p.tops[at] = top;
+    p.sums[at] = all;
     p.counts[at] = count;
   }
-}
-
-__device__ __forceinline__ double beam_shfl(double v, int o) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __shfl_xor((uint32_t)u, o), hi = __shfl_xor((uint32_t)(u >> 32), o);
-  return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
 }
 
 // One workgroup runs it once, so the time its instructions take to arrive counts: every step stands in the code once, the
@@ -212,16 +245,19 @@ __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamParams p) {
   for (int k = 0; k < kBeamNear; ++k) near[k] = p.cands[(base + min(part0, all - 1)) * kBeamSlots + slot + k * kBeamGroup];
   // The rows' sums.
   for (int w = wave; w < p.W; w += kBeamJoinWaves) {
-    const uint64_t* st = p.stats + base + w * p.parts;
-    const uint64_t v0 = lane < p.parts ? st[lane] : beam_pack(-INFINITY, 0);
+    const float* tops = p.tops + base + w * p.parts;
+    const double* sums = p.sums + base + w * p.parts;
+    const float top0 = lane < p.parts ? tops[lane] : -INFINITY;
+    const double sum0 = lane < p.parts ? sums[lane] : 0.;
     const float score = p.scores[b * p.s_sb + w];
-    float m = beam_lo(v0);
-    for (int k = lane + kWave; k < p.parts; k += kWave) m = fmaxf(m, beam_lo(st[k]));
+    float m = top0;
+    for (int k = lane + kWave; k < p.parts; k += kWave) m = fmaxf(m, tops[k]);
     for (int o = 1; o < kWave; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
     double sum = 0;
     for (int k = lane; k < p.parts; k += kWave) {
-      const uint64_t v = k == lane ? v0 : st[k];
-      if (beam_lo(v) > -INFINITY || !(beam_hi(v) == 0.f)) sum += (double)beam_hi(v) * exp((double)beam_lo(v) - (double)m);
+      const float t = k == lane ? top0 : tops[k];
+      const double v = k == lane ? sum0 : sums[k];
+      if (v != 0.) sum += v * beam_exp(t, (double)m * 1.4426950408889634074);
     }
     for (int o = 1; o < kWave; o *= 2) sum += beam_shfl(sum, o);
     if (lane == 0) {
@@ -375,7 +411,7 @@ extern "C" size_t specq_beam_select_workspace_size(int B, int W, int V, int logi
   if (B <= 0 || W <= 0 || V <= 0) return 0;
   const int size = logits_fp32 ? 4 : 2;
   const size_t parts = (size_t)B * W * beam_parts(V, size, beam_vectors((int64_t)B * W, V, size, device_cus()));
-  return kCounterBytes + align_up(parts * 4, 256) + parts * (8 + 8 * kBeamSlots);
+  return kCounterBytes + align_up(parts * 4, 256) + parts * (8 + 8 * kBeamSlots + 4);
 }
 
 extern "C" int specq_beam_select(const void* logits, int logits_fp32, int64_t s_lb, int64_t s_lw, const float* scores,
@@ -406,8 +442,9 @@ extern "C" int specq_beam_select(const void* logits, int logits_fp32, int64_t s_
   p.W = W; p.V = V; p.n = n; p.parts = (int)parts;
   char* at = static_cast<char*>(workspace) + kCounterBytes;
   p.counts = reinterpret_cast<int32_t*>(at);
-  p.stats = reinterpret_cast<uint64_t*>(at + align_up((size_t)count * 4, 256));
-  p.cands = p.stats + count;
+  p.sums = reinterpret_cast<double*>(at + align_up((size_t)count * 4, 256));
+  p.cands = reinterpret_cast<uint64_t*>(p.sums + count);
+  p.tops = reinterpret_cast<float*>(p.cands + count * kBeamSlots);
   const void* fn = logits_fp32 ? (nv == 8 ? reinterpret_cast<const void*>(&beam_part_kernel<float, 8>)
                                           : reinterpret_cast<const void*>(&beam_part_kernel<float, 2>))
                                : (nv == 8 ? reinterpret_cast<const void*>(&beam_part_kernel<_Float16, 8>)

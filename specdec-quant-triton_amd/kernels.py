@@ -1636,8 +1636,8 @@ def beam_select(logits, scores, n=None, finished=None, eos=None, out=None, works
 
     logits fp16 or fp32 [B, W, V]; scores fp32 [B, W], the beams' log-probabilities so far (-inf: no beam).  A
     continuation by token v has scores[b, w] + logits[b, w, v] - log(sum(exp(logits[b, w]))); a beam with
-    finished[b, w] (bool) has one, token `eos`, with the score it has.  Best first, compared in fp64, ties to the lower
-    beam, then the lower token; n defaults to W, and both are at most 64.  parents holds rows b * W + w, as
+    finished[b, w] (bool) has one, token `eos`, with the score it has.  Best first, formed and compared in fp64 (a row's
+    log-sum is within 2^-33), ties to the lower beam, then the lower token; n defaults to W, and both are at most 64.  parents holds rows b * W + w, as
     paged_kv_fork and beam_reorder take them.  Continuations of score -inf or NaN (logits of -inf; every one of a row that
     holds NaN or +inf) are none; where there are fewer than n the rest has score -inf, token and parent -1.  `out` may hold
     `scores` itself where n is W.

@@ -269,3 +269,48 @@ def test_reorder_refusals():
             K.beam_reorder(states, parents, group)
     torch.cuda.synchronize()
     assert torch.equal(x, before)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("V", [1001, 128257])
+def test_beams_closer_than_an_fp32_step_of_their_scores(V, f32):
+    """The best candidates of two different rows, some 2^-28 apart at scores of -1 to -20, whose fp32 steps are 2^-24 and more.
+
+    Every row's log-sum is off by less than 2^-33.9 (exponentials within 2^-34 of themselves, sums in fp64), and what is behind it
+    is fp64 of values below 2^7, within 2^-44: candidates further apart than 2^-32 are ordered as the formula has them.  The
+    second beam's score is chosen so that the difference is no more than half of its fp32 step (below 2^-26) and a little."""
+    rng = np.random.default_rng(V)
+    B = 48
+    x, _ = make(rng, B, 2, V, f32, 2.0)
+    lse = lambda r: r.max() + np.log(np.exp(r - r.max()).sum())  # noqa: E731
+    best = np.array([[r.max() - lse(r) for r in b.astype(np.float64)] for b in x])
+    s = np.zeros((B, 2), np.float32)
+    s[:, 0] = rng.uniform(0.001, 0.25, B)
+    # Beam 1's score, within +-0.25 of 0, makes up what its best candidate lacks against beam 0's; rows too far apart are moved.
+    for b in range(B):
+        d = best[b, 0] + s[b, 0].astype(np.float64) - best[b, 1]
+        s[b, 1] = d
+        if abs(d) > 0.25:  # all of a row's logits but its largest shifted until the largest are alike
+            at = x[b, 1].argmax()
+            lo, hi = np.float64(-20.0), np.float64(20.0)
+            for _ in range(60):
+                mid = (lo + hi) / 2
+                r = x[b, 1].astype(np.float64) + mid
+                r[at] = x[b, 1, at]
+                lo, hi = (mid, hi) if r[at] - lse(r) > best[b, 0] else (lo, mid)
+            top = x[b, 1, at]
+            x[b, 1] = np.minimum((x[b, 1].astype(np.float64) + lo).astype(x.dtype), top)
+            x[b, 1, at] = top
+            r = x[b, 1].astype(np.float64)
+            s[b, 1] = best[b, 0] + s[b, 0].astype(np.float64) - (r.max() - lse(r))
+    want, token, parent, _ = O.beam_select(x, s, 2)
+    apart = want[:, 0] - want[:, 1]
+    note(f"beam close V={V} f32={f32}")
+    got = K.beam_select(*gpu(x, s), 2)
+    torch.cuda.synchronize()
+    sure = (apart > 2.0 ** -32) & (parent[:, 0] != parent[:, 1])
+    assert sure.sum() > B // 2 and (apart[sure] < 2.0 ** -24).sum() > B // 2  # the case is what it says
+    assert np.array_equal(got[2].cpu().numpy()[sure], parent[sure])
+    assert np.array_equal(got[1].cpu().numpy()[sure], token[sure])
+    err = np.abs(got[0].cpu().numpy().astype(np.float64) - want)
+    assert (err <= 2.0 ** -32 + 2.0 ** -24 * np.abs(want)).all()
