@@ -303,3 +303,59 @@ def test_the_table_size_does_not_change_a_bit(QL, H, HK, D):
     plan = torch.tensor([2, QL], dtype=torch.int32, device=DEV)
     got = K.paged_attention_weights(*gpu(q5, kc, ks, wide, cl5, more), plan=plan)
     assert torch.equal(got[:2, :, :w.shape[2]], want) and not got[2:].any()
+
+
+@pytest.mark.parametrize("QL,G,PAGE", [(1, 4, 64), (3, 8, 16)])
+def test_batches_whose_workgroups_walk_several_tiles(QL, G, PAGE):
+    """17 sequences of 8 heads, tables of 12 tiles: two blocks of eight sequences and one more, three tiles a workgroup; stored
+    scores and a tile's worth of rows formed twice."""
+    rng = np.random.default_rng(31)
+    ctx = [3000, 1, 255, 256, 257, 512, 513, 2999, 0, 768, 1025, 2048, 1537, 100, 2900, 1793, 2305]
+    case = make(rng, ctx, QL, 8 * G, 8, 64, PAGE, False)
+    lens = np.asarray([QL] * 7 + [0] + [QL] * 9, np.int32)
+    case[3][4, 0] = case[3][11, 2048 // PAGE - 1] = -1
+    note(f"attn_weights many tiles QL={QL} G={G}")
+    t = gpu(*case)
+    K.paged_attention_weights(*t, q_lens=gpu(lens)[0])
+    torch.cuda.synchronize()
+    check(t[5], case, lens.tolist(), 64 ** -0.5, "tiles")
+    # A sequence by itself, a tile a workgroup, has the same bits.
+    for b in (0, 4, 11, 14):
+        one = gpu(case[0][b:b + 1], case[1], case[2], case[3][b:b + 1], case[4][b:b + 1], case[5][b:b + 1])
+        K.paged_attention_weights(*one)
+        torch.cuda.synchronize()
+        assert torch.equal(one[5][0], t[5][b])
+
+
+@pytest.mark.parametrize("QL,G", [(40, 4), (180, 4), (600, 4)])
+def test_many_rows_of_some_drafts_bad_pages_and_masked_scales(QL, G):
+    """160, 720 and 2400 rows: q_lens of none, one, one segment's worth, and all; pages that are none on and off the rows'
+    diagonal; a context past its table; NaN and infinite scales behind the contexts."""
+    rng = np.random.default_rng(QL)
+    HK, D, PAGE = 2, 64, 16
+    ctx = [QL + 300, QL + 35, QL + 1, 700, QL // 2]
+    case = make(rng, ctx, QL, G * HK, HK, D, PAGE, True)
+    q, kc, ks, bt, cl, w = case
+    lens = [QL, min(QL, 1024 // G), 0, 1, QL]  # the last has more new tokens than it is long
+    for b, n in enumerate(ctx):
+        if n % PAGE:
+            ks[bt[b, n // PAGE], n % PAGE:] = np.nan
+            ks[bt[b, n // PAGE], n % PAGE + 1:] = np.inf
+    bt[0, [0, 7, 300 // PAGE + 1, (300 + QL // 2) // PAGE]] = -1, 2 ** 31 - 1, len(kc), -9
+    cl[3] = bt.shape[1] * PAGE + 50  # its table's length counts
+    bt[3, 40:] = -1
+    note(f"attn_weights many rows QL={QL}")
+    t = gpu(*case)
+    K.paged_attention_weights(*t, q_lens=gpu(np.asarray(lens, np.int32))[0], sm_scale=0.1)
+    torch.cuda.synchronize()
+    ks[~np.isfinite(ks)] = 0
+    check(t[5], case, lens, 0.1, "many rows")
+    # In plan mode, with room for more tokens and sequences, the same bits.
+    more = np.zeros((7, QL + 70, *q.shape[2:]), np.float16)
+    more[:5, :QL] = q
+    pad = lambda a, v: np.concatenate((a, np.full((2, *a.shape[1:]), v, a.dtype)))  # noqa: E731
+    plan = torch.tensor([5, QL], dtype=torch.int32, device=DEV)
+    p = gpu(more, kc, ks, pad(bt, 0), pad(cl, 90), pad(w, 1.5))
+    K.paged_attention_weights(*p, q_lens=gpu(np.asarray([*lens, 3, 3], np.int32))[0], sm_scale=0.1, plan=plan)
+    torch.cuda.synchronize()
+    assert torch.equal(p[5][:5], t[5]) and bool((p[5][5:] == 1.5).all())

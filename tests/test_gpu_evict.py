@@ -231,3 +231,42 @@ def test_refusals():
             K.paged_kv_evict(**dict(good, **kw))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip((tc, tw, *tcs), before))
+
+
+@pytest.mark.parametrize("weights", ["spread", "few", "zero", "signed"])
+@pytest.mark.parametrize("ctx,budget,recent,sinks", [
+    ([20000], 9000, 100, 4),           # more than one group of chunks
+    ([16385, 32000], 16384, 1, 0),     # the first group and a token; nearly two groups
+    ([32768], 30000, 29000, 5),
+])
+def test_tables_of_several_groups_in_one_workgroup(ctx, budget, recent, sinks, weights):
+    """Tables of 16385 to 32768 tokens: more than a workgroup keeps in registers, less than is cut into slices."""
+    rng = np.random.default_rng(budget)
+    note(f"evict groups ctx={ctx} budget={budget} weights={weights}")
+    case = make(rng, ctx, 1, 16, 64, weights)
+    bt = case[0][:, :512]  # 32768 tokens at most
+    run_check((np.ascontiguousarray(bt), case[1], np.ascontiguousarray(case[2][:, :, :bt.shape[1] * 64]), case[3]), budget, recent, sinks,
+              what="groups")
+
+
+def test_long_rows_of_many_heads():
+    """A table of more than 32768 tokens with more rows than leave half of the CUs idle: one workgroup a row."""
+    rng = np.random.default_rng(40)
+    HK, PAGE, L, budget = 129, 64, 33500, 7001
+    C = -(-L // PAGE)
+    bt = rng.permutation(C).astype(np.int32)[None]
+    w = rng.integers(0, 5000, (1, HK, C * PAGE)).astype(np.float32)
+    cache = rng.integers(0, 1 << 31, (C, PAGE, HK)).astype(np.int32)
+    tb, tc, tw, tk = gpu(bt, np.asarray([L], np.int32), w, cache)
+    note("evict many heads")
+    kept = K.paged_kv_evict(tb, tc, tw, [tk], PAGE, budget, 50, 3)
+    torch.cuda.synchronize()
+    key = w[0, :, :L].copy()
+    key[:, :3] = key[:, L - 50:] = np.inf
+    want = np.sort(np.argsort(-key, axis=1, kind="stable")[:, :budget], axis=1)
+    assert np.array_equal(kept.cpu().numpy()[0], want) and tc.item() == budget
+    rows = cache[bt[0]].reshape(C * PAGE, HK)
+    got = tk.cpu().numpy()[bt[0]].reshape(C * PAGE, HK)
+    assert np.array_equal(got[:budget], np.take_along_axis(rows, want.T, 0)) and np.array_equal(got[budget:], rows[budget:])
+    assert np.array_equal(tw.cpu().numpy()[0, :, :budget], np.take_along_axis(w[0], want, 1))
+    assert np.array_equal(tw.cpu().numpy()[0, :, budget:], w[0, :, budget:])

@@ -187,3 +187,22 @@ def test_empty_and_refusals():
     # One row of weights for all heads may be an expanded one.
     K.qk_norm_rotary(q, None, w.expand(4, 64), None, f, c)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,R,per_head", [(80, 20, False), (90, 90, True)])
+def test_prompts_of_unaligned_heads(D, R, per_head, interleaved):
+    """More than 1024 tokens of heads that the vector form does not take: four waves a token."""
+    rng = np.random.default_rng(D)
+    B, QL, H, HK = 3, 401, 5, 2
+    q, k = rand16(rng, B, QL, H, D, size=3.0), rand16(rng, B, QL, HK, D, size=0.2)
+    wq, wk = (rng.uniform(0.5, 1.5, (h, D) if per_head else D).astype(np.float16) for h in (H, HK))
+    f, _ = K.rotary_inv_freq(R, device="cpu")
+    ctx = rng.integers(QL, 100000, B).astype(np.int32)
+    pos = ctx[:, None] - QL + np.arange(QL)[None]
+    note(f"qk_norm unaligned prompt D={D} R={R} interleaved={interleaved}")
+    tq, tk, twq, twk, tc = gpu(q, k, wq, wk, ctx)
+    qo, ko = K.qk_norm_rotary(tq, tk, twq, twk, f.to(DEV), tc, interleaved=interleaved)
+    torch.cuda.synchronize()
+    check(qo, q, wq, 1e-6, f.numpy(), pos, interleaved, 1.0, "q")
+    check(ko, k, wk, 1e-6, f.numpy(), pos, interleaved, 1.0, "k")
