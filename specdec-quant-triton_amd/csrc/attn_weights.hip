@@ -8,8 +8,10 @@
 // K alone is read, V is not needed.  A softmax has to know its whole row before any of its values can be added up over
 // the rows, so the work is two launches over the same tiles of 256 tokens:
 //   1  scores, and (max, sum of exponentials) of each row within the tile; the last workgroup of a (sequence, head)
-//      joins them to log2 of each row's sum over all tiles
-//   2  p = exp2(s - that), summed over the rows, and the update of w
+//      joins them to each row's max and the reciprocal of its sum over all tiles
+//   2  p = exp2(s - max) / sum, summed over the rows, and the update of w
+// Max and sum stay apart: in one number, max + log2(sum), the sum's part would be rounded to the steps of the max, the same way in
+// all of a row's probabilities (2^-21 of them at scores of 10, 2^-10 at 16000).
 // The scores of up to 16 rows (kAwStoreRows: plain decoding) go from 1 to 2 through the workspace; more rows compute them
 // again.  Both ways add a token's rows in one order (16 lanes; in each the blocks of 16 rows of either parity, then both; then
 // pairs of lanes; then units of 512 rows one after another) and join the rows' statistics in one (64 tokens, 256, all), so they
@@ -19,7 +21,7 @@
 // K stays: a wave holds 64 tokens, converts their codes to fp16 matrix operands once and walks the rows 16 at a time
 // (K . Q^T on v_mfma_f32_16x16x32_f16: a lane's results are four tokens of one row).  Everything behind the products is
 // fp32; log2(e) is folded into the scale.
-// 8 KV heads of 128 (us): a new token of 32 sequences of up to 8192, stored scores, 52 + 10, codes and scores at 3.4 TB/s (loads
+// 8 KV heads of 128 (us): a new token of 32 sequences of up to 8192, stored scores, 53 + 8, codes and scores at 3.4 TB/s (loads
 // alone 5.2); 9 of 8 sequences of 4096, formed twice, 19 + 14, half of it fixed phases; 256 of 2 of up to 4096, 43 + 33, bound by
 // vector instructions at two waves a SIMD.
 #include "api_common.hpp"
@@ -56,9 +58,9 @@ struct AwParams {
   int seg_rows, segs;  // rows of a workgroup's segment (a unit or more), segments of a launch
   uint32_t g_magic;  // ceil(2^32 / G): row / G is its product's high word (rows below 2^20, G below 2^12); 0 for G = 1
   float scale_log2;
-  // Workspace: scores [prog][rows][tiles * 256]; (max, sum) [prog][seg][tiles][rows]; log2 of the rows' sums [prog][seg][rows];
+  // Workspace: scores [prog][rows][tiles * 256]; (max, sum) [prog][seg][tiles][rows]; the rows' (max, 1 / sum) [prog][seg][rows];
   // sums of a unit's rows [prog][unit][tiles * 256], two tokens a word.
-  float* scores; uint64_t* stats; float* lse; uint64_t* sums;
+  float* scores; uint64_t* stats; uint64_t* norms; uint64_t* sums;
   int32_t* counters;  // [prog][seg], then [prog][tile]
 };
 
@@ -235,31 +237,32 @@ __device__ __forceinline__ void aw_hide(int t0, int last, uint32_t seen, v4f (&a
     for (int i = 0; i < 4; ++i)
       if (!(((seen >> s) & 1) && t0 + 16 * s + 4 * g + i <= last)) acc[s][i] = -INFINITY;
 }
-// A product's scale and, SUB, the row's log-sum off it: not one instruction, since stored scores are rounded between the two.
+// A product's scale and, SUB, the row's max off it: not one instruction, since stored scores, and those of the row's sum, are
+// rounded between the two.
 template <bool SUB>
-__device__ __forceinline__ float aw_scaled(float acc, float ksc, float lse) {
+__device__ __forceinline__ float aw_scaled(float acc, float ksc, float top) {
 #pragma clang fp contract(off)
   acc *= ksc;
-  return SUB ? acc - lse : acc;
+  return SUB ? acc - top : acc;
 }
 template <bool SUB>
-__device__ __forceinline__ void aw_scale(const v4f (&ksc)[4], float lse, v4f (&acc)[4]) {
+__device__ __forceinline__ void aw_scale(const v4f (&ksc)[4], float top, v4f (&acc)[4]) {
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[s][i] = aw_scaled<SUB>(acc[s][i], ksc[s][i], lse);
+    for (int i = 0; i < 4; ++i) acc[s][i] = aw_scaled<SUB>(acc[s][i], ksc[s][i], top);
 }
-// Scores (in log2; SUB, less the row's log-sum) of the wave's tokens with the row of lane % 16.
+// Scores (in log2; SUB, less the row's max) of the wave's tokens with the row of lane % 16.
 template <int D, bool SUB>
 __device__ __forceinline__ void aw_scores(const v8h (&kh)[4][D / 32], const v8h (&qf)[D / 32], const v4f (&ksc)[4], int t0, int last,
-                                          bool all, uint32_t seen, float lse, v4f (&acc)[4]) {
+                                          bool all, uint32_t seen, float top, v4f (&acc)[4]) {
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     acc[s] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < D / 32; ++u) acc[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[s][u], qf[u], acc[s], 0, 0, 0);
   }
-  aw_scale<SUB>(ksc, lse, acc);
+  aw_scale<SUB>(ksc, top, acc);
   if (!all) aw_hide(t0, last, seen, acc);  // all: every row sees all
 }
 // (max, sum) of a row over the wave's tokens, in all lanes of the row.
@@ -294,13 +297,13 @@ __device__ __forceinline__ v4f aw_rows(const v4f (&sums)[4]) {
 }
 // The last workgroup of a program joins its rows' tiles: many rows a thread each, few a group of lanes each (as many as
 // there are tiles, at most a wave).
-__device__ __forceinline__ void aw_lse(const AwParams& p, const AwProg& x, int at) {  // at: of [prog][seg]
+__device__ __forceinline__ void aw_norms(const AwParams& p, const AwProg& x, int at) {  // at: of [prog][seg]
   const int threads = blockDim.x;
   const uint64_t* st = p.stats + (int64_t)at * p.tiles * p.rows;
-  float* out = p.lse + (int64_t)at * p.rows;
-  // Of a row that sees nothing an infinite one, so that it gives 0; a maximum knows no NaN, the sum does.
+  uint64_t* out = p.norms + (int64_t)at * p.rows;
+  // Of a row that sees nothing an infinite max, so that it gives 0; a maximum knows no NaN, the sum does, and makes the max one.
   auto done = [&](int row, float m, float l) {
-    out[row] = m == -INFINITY && l == l ? INFINITY : m + __builtin_amdgcn_logf(l);
+    out[row] = !(l == l) ? aw_pack(l, 1.f) : m == -INFINITY ? aw_pack(INFINITY, 0.f) : aw_pack(m, 1.f / l);
   };
   // Tiles k0, k0 + step, ...: eight loads in flight.
   auto walk = [&](int row, int k0, int step, float& m, float& l) {
@@ -388,12 +391,12 @@ __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
     v4i raw[4][D / 64];
     ST scale;
     aw_load<D, false, ST>(p, at, 0, raw, scale);
-    float lse[MODE == kAwSums ? RB : 1];
+    uint64_t norm[MODE == kAwSums ? RB : 1];
     if constexpr (MODE == kAwSums) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        lse[rb] = INFINITY;
-        if (rb * 16 + r < x.rows) lse[rb] = p.lse[(int64_t)prog * p.rows + rb * 16 + r];
+        norm[rb] = aw_pack(INFINITY, 0.f);
+        if (rb * 16 + r < x.rows) norm[rb] = p.norms[(int64_t)prog * p.rows + rb * 16 + r];
       }
     }
     __syncthreads();
@@ -422,14 +425,17 @@ __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) qf[u] = s_q[rb][u][lane];
         v4f acc[4];
-        // Rows past the last add nothing: their statistics go nowhere, their lse is infinite.
+        // Rows past the last add nothing: their statistics go nowhere, their max is infinite.
         aw_scores<D, MODE == kAwSums>(kh, qf, ksc, t0, fresh + aw_token(p, row), t0 + 63 <= fresh && seen == 0xf, seen,
-                                      lse[MODE == kAwSums ? rb : 0], acc);
+                                      MODE == kAwSums ? aw_m(norm[rb]) : 0.f, acc);
         if constexpr (MODE == kAwSums) {
 #pragma unroll
           for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) (rb & 1 ? odd : even)[s][i] += fast_exp2(acc[s][i]);
+            for (int i = 0; i < 4; ++i) {
+              v4f& sum = (rb & 1 ? odd : even)[s];
+              sum[i] = fmaf(fast_exp2(acc[s][i]), aw_l(norm[rb]), sum[i]);
+            }
         } else {
           const uint64_t st = aw_stat(acc);
           if (g == 0) s_stat[tile - tile0][w][row] = st;
@@ -445,7 +451,7 @@ __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
     if constexpr (MODE != kAwSums) {
       __syncthreads();
       aw_publish(p, x, prog, tile0, tile1, s_stat);
-      if (arrive_last(p.counters + prog, (x.tiles + p.span - 1) / p.span, &s_last)) aw_lse(p, x, prog);
+      if (arrive_last(p.counters + prog, (x.tiles + p.span - 1) / p.span, &s_last)) aw_norms(p, x, prog);
     }
   }
 }
@@ -505,7 +511,7 @@ __global__ __launch_bounds__(256) void aw_store_kernel(AwParams p) {
       const bool all = t0 + 63 <= fresh && seen == 0xf;
       if (!all) aw_hide(t0, last, seen, acc);  // rows past the last go nowhere
       const uint64_t st = aw_stat(acc);
-      // What is seen is stored as finite, what is not as -inf, which adds nothing even to a row whose log-sum is NaN.
+      // What is seen is stored as finite, what is not as -inf, which adds nothing even to a row whose max is NaN.
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -519,7 +525,7 @@ __global__ __launch_bounds__(256) void aw_store_kernel(AwParams p) {
     }
     __syncthreads();
     aw_publish(p, x, prog, tile0, tile1, s_stat);
-    if (arrive_last(p.counters + prog, (x.tiles + p.span - 1) / p.span, &s_last)) aw_lse(p, x, prog);
+    if (arrive_last(p.counters + prog, (x.tiles + p.span - 1) / p.span, &s_last)) aw_norms(p, x, prog);
   }
 }
 
@@ -599,7 +605,7 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
       from[n] = place(row[n], head[n]);
     }
     v8h next[kLoads];
-    float next_lse[2] = {0.f, 0.f};
+    uint64_t next_norm[2] = {0, 0};
     auto fetch = [&](int b) {  // what four blocks need; past the last row, that row
 #pragma unroll
       for (int n = 0; n < kLoads; ++n) {
@@ -614,7 +620,7 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
       }
       if constexpr (MODE == kAwSums) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) next_lse[k] = p.lse[(int64_t)index * p.rows + min((b + odd + 2 * k) * 16 + r, x.rows - 1)];
+        for (int k = 0; k < 2; ++k) next_norm[k] = p.norms[(int64_t)index * p.rows + min((b + odd + 2 * k) * 16 + r, x.rows - 1)];
       }
     };
     int slot = 0;
@@ -638,7 +644,7 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
         for (int b = seg + odd; b < min(rb, seg_end); b += 2) keep(b, aw_pack(-INFINITY, 0.f));
       for (; rb < seg_end; rb += 4, slot ^= 1) {
         stage();
-        const float lse[2] = {next_lse[0], next_lse[1]};
+        const uint64_t norm[2] = {next_norm[0], next_norm[1]};
         fetch(rb + 4);
         wg_barrier_lds();  // the other slot has been read, and is written next
         v4f acc[2][4];
@@ -649,7 +655,7 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
 #pragma unroll
           for (int u = 0; u < NU; ++u) qf[u] = s_q[slot][(odd + 2 * k) * 16 + r][(8 * (u / 2) + 2 * g + (u & 1)) ^ key(r)];
           aw_scores<D, MODE == kAwSums>(kh, qf, ksc, t0, at < x.rows ? fresh + aw_token(p, row0 + at) : -1,
-                                        t0 + 63 <= fresh && seen == 0xf && b * 16 + 16 <= x.rows, seen, lse[k], acc[k]);
+                                        t0 + 63 <= fresh && seen == 0xf && b * 16 + 16 <= x.rows, seen, aw_m(norm[k]), acc[k]);
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -657,7 +663,7 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
 #pragma unroll
             for (int s = 0; s < 4; ++s)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) sums[s][i] += fast_exp2(acc[k][s][i]);
+              for (int i = 0; i < 4; ++i) sums[s][i] = fmaf(fast_exp2(acc[k][s][i]), aw_l(norm[k]), sums[s][i]);
           } else {
             keep(rb + odd + 2 * k, aw_stat(acc[k]));
           }
@@ -715,13 +721,16 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
         }
       }
     } else if (arrive_last(p.counters + index, x.tiles, &s_last)) {
-      aw_lse(p, x, index);
+      aw_norms(p, x, index);
     }
   }
 }
 
-// Pass 2 from stored scores: a thread owns four tokens, and adds their rows in the order of the lanes above.
-__global__ __launch_bounds__(256) void aw_sum_kernel(AwParams p) {
+// Pass 2 from stored scores of up to R rows: a thread owns four tokens, and adds their rows in the order of the lanes above.  32
+// sequences of up to 8192, 4 rows: 7.6 us with R = 4, 12 with 16.
+template <int R>
+__global__ __launch_bounds__(256, 4) void aw_sum_kernel(AwParams p) {
+#pragma clang fp contract(off)  // a probability is rounded before it is added, as the first addition to nothing does it above
   const int progs = p.B_grid * p.H_KV, tiles = (p.cap + kAwSumTile - 1) / kAwSumTile;
   for (int64_t item = blockIdx.x; item < (int64_t)progs * tiles; item += gridDim.x) {
     const int tile = (int)(item / progs), prog = (int)(item - (int64_t)tile * progs);
@@ -729,41 +738,39 @@ __global__ __launch_bounds__(256) void aw_sum_kernel(AwParams p) {
     const int t = tile * kAwSumTile + 4 * (int)threadIdx.x;
     if (!aw_prog(p, prog, x) || t >= x.L) continue;
     const float* sc = p.scores + (int64_t)prog * p.rows * p.tiles * kAwTile + t;
-    v4f e[kAwStoreRows];
+    v4f e[R];
 #pragma unroll
-    for (int k = 0; k < kAwStoreRows; ++k) {
+    for (int k = 0; k < R; ++k) {
       e[k] = v4f{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (k < x.rows) e[k] = *reinterpret_cast<const v4f*>(sc + (int64_t)k * p.tiles * kAwTile);
     }
-    float lse[kAwStoreRows];
+    float top[R], inv[R];
     bool nan = false;
 #pragma unroll
-    for (int k = 0; k < kAwStoreRows; ++k) {
-      lse[k] = k < x.rows ? p.lse[(int64_t)prog * p.rows + k] : INFINITY;
-      nan |= !(lse[k] == lse[k]);
+    for (int k = 0; k < R; ++k) {
+      const uint64_t norm = k < x.rows ? p.norms[(int64_t)prog * p.rows + k] : aw_pack(INFINITY, 0.f);
+      top[k] = aw_m(norm), inv[k] = aw_l(norm);
+      nan |= !(top[k] == top[k]);
     }
     if (uniform((int)nan)) {  // a row gives its NaN to what it sees alone
 #pragma unroll
-      for (int k = 0; k < kAwStoreRows; ++k)
+      for (int k = 0; k < R; ++k)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (!(lse[k] == lse[k]) && !(e[k][i] == -INFINITY)) e[k][i] = lse[k];
+          if (!(top[k] == top[k]) && !(e[k][i] == -INFINITY)) e[k][i] = top[k];
 #pragma unroll
-      for (int k = 0; k < kAwStoreRows; ++k)
-        if (!(lse[k] == lse[k])) lse[k] = 0.f;
+      for (int k = 0; k < R; ++k)
+        if (!(top[k] == top[k])) top[k] = 0.f;
     }
 #pragma unroll
-    for (int k = 0; k < kAwStoreRows; ++k)
+    for (int k = 0; k < R; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) e[k][i] = fast_exp2(e[k][i] - lse[k]);
+      for (int i = 0; i < 4; ++i) e[k][i] = fast_exp2(e[k][i] - top[k]) * inv[k];
+    // Pairs, pairs of these, and the fours.
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int o = 1; o < R; o *= 2)
 #pragma unroll
-      for (int k = 0; k < 16; k += 2) e[k][i] += e[k + 1][i];
-#pragma unroll
-      for (int k = 0; k < 16; k += 4) e[k][i] += e[k + 2][i];
-      e[0][i] = (e[0][i] + e[4][i]) + (e[8][i] + e[12][i]);
-    }
+      for (int k = 0; k + o < R; k += 2 * o) e[k] += e[k + o];
     aw_put(p, x, t, aw_get(p, x, t, true) + e[0]);
   }
 }
@@ -781,6 +788,10 @@ static const void* aw_fn(int D, bool f32, bool few) {
   return few ? reinterpret_cast<const void*>(&aw_few_kernel<128, _Float16, MODE>)
              : reinterpret_cast<const void*>(&aw_many_kernel<128, _Float16, MODE>);
 }
+static const void* aw_sum_fn(int64_t rows) {
+  if (rows <= 4) return reinterpret_cast<const void*>(&aw_sum_kernel<4>);
+  return rows <= 8 ? reinterpret_cast<const void*>(&aw_sum_kernel<8>) : reinterpret_cast<const void*>(&aw_sum_kernel<16>);
+}
 static const void* aw_store_fn(int D, bool f32) {
   if (D == 64) return f32 ? reinterpret_cast<const void*>(&aw_store_kernel<64, float>)
                           : reinterpret_cast<const void*>(&aw_store_kernel<64, _Float16>);
@@ -790,7 +801,7 @@ static const void* aw_store_fn(int D, bool f32) {
 
 // Stored scores lie within a buffer's offsets.
 static bool aw_stores(int64_t rows, int64_t tiles) { return rows <= kAwStoreRows && tiles <= (1 << 16); }
-struct AwSpace { int64_t seg_rows, segs, rows; size_t scores, stats, lse, sums; };  // as in AwParams; bytes
+struct AwSpace { int64_t seg_rows, segs, rows; size_t scores, stats, norms, sums; };  // as in AwParams; bytes
 static AwSpace aw_space(int64_t progs, int64_t rows, int64_t tiles) {
   AwSpace a = {};
   a.scores = aw_stores(rows, tiles) ? align_up((size_t)(progs * rows * tiles * kAwTile * 4), 256) : 0;
@@ -802,7 +813,7 @@ static AwSpace aw_space(int64_t progs, int64_t rows, int64_t tiles) {
   const int64_t segs = ceil_div64(rows, a.seg_rows);
   for (a.segs = segs < kAwSegs ? segs : kAwSegs;; --a.segs) {
     a.stats = align_up((size_t)(a.segs * progs * tiles * a.rows * 8), 256);
-    a.lse = align_up((size_t)(a.segs * progs * a.rows * 4), 256);
+    a.norms = align_up((size_t)(a.segs * progs * a.rows * 8), 256);
     a.sums = a.segs > 1 ? (size_t)(a.segs * (a.seg_rows / kAwUnitRows) * progs * tiles * kAwTile * 4) : 0;
     if (a.segs <= 1 || (progs * (a.segs + tiles) * 4 <= (int64_t)kCounterBytes && a.stats + a.sums <= 64u << 20)) return a;
   }
@@ -816,7 +827,7 @@ extern "C" size_t specq_paged_attn_weights_workspace_size(int B_grid, int H, int
                                                           int PAGE) {
   if (B_grid <= 0 || H <= 0 || H_KV <= 0 || H % H_KV != 0 || ql_grid <= 0 || max_pages <= 0 || PAGE <= 0) return 0;
   const AwSpace s = aw_space((int64_t)B_grid * H_KV, (int64_t)ql_grid * (H / H_KV), ceil_div64((int64_t)max_pages * PAGE, kAwTile));
-  return kCounterBytes + s.scores + s.stats + s.lse + s.sums;
+  return kCounterBytes + s.scores + s.stats + s.norms + s.sums;
 }
 
 extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh, const int8_t* kc,
@@ -868,15 +879,15 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   p.rows = (int)space.rows;
   p.seg_rows = (int)space.seg_rows;
   p.segs = (int)space.segs;
-  const size_t need = kCounterBytes + space.scores + space.stats + space.lse + space.sums;
+  const size_t need = kCounterBytes + space.scores + space.stats + space.norms + space.sums;
   SPECQ_REQUIRE(workspace && workspace_bytes >= need, SPECQ_ENOSPC,
                 "paged_attn_weights: workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
   char* at = static_cast<char*>(workspace);
   p.counters = reinterpret_cast<int32_t*>(at);
   p.scores = reinterpret_cast<float*>(at + kCounterBytes);
   p.stats = reinterpret_cast<uint64_t*>(at + kCounterBytes + space.scores);
-  p.lse = reinterpret_cast<float*>(at + kCounterBytes + space.scores + space.stats);
-  p.sums = reinterpret_cast<uint64_t*>(at + kCounterBytes + space.scores + space.stats + space.lse);
+  p.norms = reinterpret_cast<uint64_t*>(at + kCounterBytes + space.scores + space.stats);
+  p.sums = reinterpret_cast<uint64_t*>(at + kCounterBytes + space.scores + space.stats + space.norms);
   // Stored scores against scores formed twice (us, 8 KV heads of 128): 4 rows, 8 sequences of 4096: 20.3, 24.6; 32 of 8192: 82,
   // 121; 16 rows, 8 of 4096: 27.3, 24.8; one of 32768: 28.6, 32.8.  Queries in LDS for the whole call against 64 rows at a
   // time: 20 rows, 8 of 4096: 28.7, 58.6; 64 rows: 37.7, 58.5; one of 32768: 54, 69.
@@ -889,7 +900,7 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   for (p.row0 = 0; p.row0 < rows; p.row0 += p.segs * p.seg_rows) {
     if (int rc = launch(store ? aw_store_fn(D, f32) : aw_fn<kAwStats>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p))
       return rc;
-    const int rc = store ? launch(reinterpret_cast<const void*>(&aw_sum_kernel), (int)(sums < kAwMaxGrid ? sums : kAwMaxGrid),
+    const int rc = store ? launch(aw_sum_fn(rows), (int)(sums < kAwMaxGrid ? sums : kAwMaxGrid),
                                   256, 0, (hipStream_t)stream, &p)
                          : launch(aw_fn<kAwSums>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p);
     if (rc != SPECQ_OK) return rc;

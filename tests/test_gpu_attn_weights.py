@@ -305,6 +305,27 @@ def test_the_table_size_does_not_change_a_bit(QL, H, HK, D):
     assert torch.equal(got[:2, :, :w.shape[2]], want) and not got[2:].any()
 
 
+@pytest.mark.parametrize("QL,G", [(1, 4), (3, 5), (9, 8), (40, 3)])
+def test_rows_add_up_to_one_whatever_their_scores(QL, G):
+    """Scores of some 16000 that differ by a few: 4 rows (stored), 15, 72 and 120.  A score is rounded, but alike in the row's sum
+    and in its probabilities, so a row adds up to 1: within the exponentials (2^-23 each) of both passes and of four joins, at
+    most 60 additions of the row's sum (2^-24 each) and 40 over the rows, and the reciprocal, in all (6 * 2 + 101) 2^-24 < 2^-17."""
+    rng = np.random.default_rng(QL)
+    HK, D, PAGE, ctx = 8, 64, 16, [3000, 700]
+    q, kc, ks, bt, cl, w = make(rng, ctx, QL, HK * G, HK, D, PAGE, True)
+    kc[..., :32], ks[:] = 127, 1.0
+    q[..., :32], q[..., 32:] = 8, 0.01 * q[..., 32:]
+    w[:] = 0
+    note(f"attn_weights sums QL={QL} G={G}")
+    got = K.paged_attention_weights(*gpu(q, kc, ks, bt, cl, w), sm_scale=0.5)
+    torch.cuda.synchronize()
+    got = got.double().cpu().numpy()
+    for b, n in enumerate(ctx):
+        total = got[b, :, :n].sum(-1) / (QL * G)
+        assert (got[b, :, :n] > 0).sum() > HK * 100  # the rows are spread out
+        assert (np.abs(total - 1) < 2.0 ** -17).all(), f"sequence {b}: off by {np.abs(total - 1).max():.2e}"
+
+
 @pytest.mark.parametrize("QL,G,PAGE", [(1, 4, 64), (3, 8, 16)])
 def test_batches_whose_workgroups_walk_several_tiles(QL, G, PAGE):
     """17 sequences of 8 heads, tables of 12 tiles: two blocks of eight sequences and one more, three tiles a workgroup; stored
