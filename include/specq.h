@@ -445,8 +445,9 @@ int specq_qk_norm_rotary(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh
  *   nothing.  A NaN or infinite score makes NaN of its row's share.  Eager and plan-mode calls agree bit for bit.  At most
  *   65536 (sequence, KV head) pairs.
  *   Workspace: specq_paged_attn_weights_workspace_size() bytes, as the workspaces above: for each pair and 256 tokens of
- *   the table 8 bytes a row (1024 rows, or up to 8192 where that stays below 64 MiB; more are taken in turns), and
- *   where a pair has at most 16 rows, 4 bytes a row and token of the table.
+ *   the table 8 bytes a row (1024 rows, or up to 8192 where that stays below 256 MiB; more are taken in turns), and
+ *   where a pair has at most 16 rows, 4 bytes a row and token of the table.  Batches that would need more than 256 MiB are
+ *   taken some sequences at a time, so that it is exceeded only where a single sequence with that table needs more.
  * ------------------------------------------------------------------------------------- */
 size_t specq_paged_attn_weights_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int max_pages, int PAGE);
 int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh,

@@ -40,6 +40,10 @@ constexpr int kAwFill = 256;       // workgroups that fill the GPU: fewer take a
 constexpr int kAwSeg = 32;         // row blocks of 16 whose statistics are joined at a time
 constexpr int kAwSumTile = 1024;   // tokens of a workgroup that adds up stored scores
 constexpr int kAwMaxGrid = 1 << 16;
+// Bytes that scores, statistics and sums of a launch take at most, unless one sequence needs more: they are as wide as the table, however
+// short the contexts, so a large batch is taken some sequences at a time.  A further pair of launches takes some 8 us, where the
+// scores alone of 256 MiB take more than 50 each way.
+constexpr int64_t kAwMost = 256 << 20;
 
 struct AwParams {
   const _Float16* q; int64_t s_qb, s_qt, s_qh;
@@ -49,6 +53,7 @@ struct AwParams {
   const int32_t* ctx_len; const int32_t* q_lens;
   float* w; int64_t s_wb, s_wh; int w_vec;  // w_vec: its rows are 16-byte aligned
   const int32_t* plan;
+  int b0;  // the launch's first sequence in a plan's count; tensors and sizes are those from it on
   int n_seqs, q_len, B_grid, ql_grid, G, H_KV, PAGE;
   int cap;      // tokens a row of the table holds
   int tiles;    // of cap
@@ -83,7 +88,7 @@ struct AwProg {
 __device__ __forceinline__ bool aw_prog(const AwParams& p, int prog, AwProg& x, int row0 = 0) {
   int n_seqs = p.n_seqs, q_len = p.q_len;
   if (p.plan != nullptr) {
-    n_seqs = min(max(p.plan[0], 0), p.B_grid);
+    n_seqs = min(max(p.plan[0] - p.b0, 0), p.B_grid);
     q_len = min(max(p.plan[1], 0), p.ql_grid);
   }
   x.b = prog / p.H_KV;
@@ -799,23 +804,28 @@ static const void* aw_store_fn(int D, bool f32) {
              : reinterpret_cast<const void*>(&aw_store_kernel<128, _Float16>);
 }
 
-// Stored scores lie within a buffer's offsets.
-static bool aw_stores(int64_t rows, int64_t tiles) { return rows <= kAwStoreRows && tiles <= (1 << 16); }
-struct AwSpace { int64_t seg_rows, segs, rows; size_t scores, stats, norms, sums; };  // as in AwParams; bytes
-static AwSpace aw_space(int64_t progs, int64_t rows, int64_t tiles) {
+// Whether scores are stored, the sequences of a launch, rows and segments as in AwParams, bytes.
+struct AwSpace { bool store; int64_t seqs, seg_rows, segs, rows; size_t scores, stats, norms, sums; };
+static AwSpace aw_space(int64_t B, int64_t H_KV, int64_t rows, int64_t tiles) {
   AwSpace a = {};
-  a.scores = aw_stores(rows, tiles) ? align_up((size_t)(progs * rows * tiles * kAwTile * 4), 256) : 0;
   // Two units a workgroup, or one where that fills no more than the GPU.  256 tokens at 4096, 8 heads of 4 queries, one sequence:
   // 68 us, 45; two (twice as many workgroups as CUs): 78, 83.
-  a.seg_rows = kAwUnitRows * (progs * tiles * ceil_div64(rows, kAwUnitRows) <= kAwFill ? 1 : kAwSegUnits);
+  a.seg_rows = kAwUnitRows * (B * H_KV * tiles * ceil_div64(rows, kAwUnitRows) <= kAwFill ? 1 : kAwSegUnits);
   a.rows = rows < a.seg_rows ? rows : a.seg_rows;
-  // As many segments as there are, where their counters find room and they need no more than 64 MiB.
+  // Scores of one sequence, where they are stored (those of a program lie within a buffer's offsets by that), and all it needs.
+  const int64_t norms = H_KV * a.rows * (tiles + 1) * 8, scores = H_KV * rows * tiles * kAwTile * 4;
+  a.store = rows <= kAwStoreRows && norms + scores <= kAwMost;
+  const int64_t one = norms + (a.store ? scores : 0), most = one < kAwMost ? kAwMost / one : 1;
+  a.seqs = ceil_div64(B, ceil_div64(B, most));  // turns of much the same size
+  const int64_t progs = a.seqs * H_KV;
+  a.scores = a.store ? align_up((size_t)(a.seqs * scores), 256) : 0;
+  // As many segments as there are, where their counters, and they, find room.
   const int64_t segs = ceil_div64(rows, a.seg_rows);
   for (a.segs = segs < kAwSegs ? segs : kAwSegs;; --a.segs) {
     a.stats = align_up((size_t)(a.segs * progs * tiles * a.rows * 8), 256);
     a.norms = align_up((size_t)(a.segs * progs * a.rows * 8), 256);
     a.sums = a.segs > 1 ? (size_t)(a.segs * (a.seg_rows / kAwUnitRows) * progs * tiles * kAwTile * 4) : 0;
-    if (a.segs <= 1 || (progs * (a.segs + tiles) * 4 <= (int64_t)kCounterBytes && a.stats + a.sums <= 64u << 20)) return a;
+    if (a.segs <= 1 || (progs * (a.segs + tiles) * 4 <= (int64_t)kCounterBytes && a.stats + a.norms + a.sums <= (size_t)kAwMost)) return a;
   }
 }
 
@@ -826,7 +836,7 @@ using namespace specq;
 extern "C" size_t specq_paged_attn_weights_workspace_size(int B_grid, int H, int H_KV, int ql_grid, int max_pages,
                                                           int PAGE) {
   if (B_grid <= 0 || H <= 0 || H_KV <= 0 || H % H_KV != 0 || ql_grid <= 0 || max_pages <= 0 || PAGE <= 0) return 0;
-  const AwSpace s = aw_space((int64_t)B_grid * H_KV, (int64_t)ql_grid * (H / H_KV), ceil_div64((int64_t)max_pages * PAGE, kAwTile));
+  const AwSpace s = aw_space(B_grid, H_KV, (int64_t)ql_grid * (H / H_KV), ceil_div64((int64_t)max_pages * PAGE, kAwTile));
   return kCounterBytes + s.scores + s.stats + s.norms + s.sums;
 }
 
@@ -870,12 +880,12 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   p.ctx_len = ctx_len; p.q_lens = q_lens;
   p.w = weights; p.s_wb = s_wb; p.s_wh = s_wh;
   p.w_vec = (uintptr_t)weights % 16 == 0 && s_wb % 4 == 0 && s_wh % 4 == 0;
-  p.plan = plan; p.n_seqs = n_seqs; p.q_len = q_len; p.B_grid = B_grid; p.ql_grid = ql_grid;
+  p.plan = plan; p.q_len = q_len; p.ql_grid = ql_grid;
   p.G = H / H_KV; p.g_magic = p.G > 1 ? (uint32_t)(((1ull << 32) + p.G - 1) / p.G) : 0;
   p.H_KV = H_KV; p.PAGE = PAGE;
   p.cap = (int)cap; p.tiles = (int)ceil_div64(cap, kAwTile);
   p.scale_log2 = sm_scale * 1.44269504088896340736f;
-  const AwSpace space = aw_space(progs, rows, p.tiles);
+  const AwSpace space = aw_space(B_grid, H_KV, rows, p.tiles);
   p.rows = (int)space.rows;
   p.seg_rows = (int)space.seg_rows;
   p.segs = (int)space.segs;
@@ -891,19 +901,28 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   // Stored scores against scores formed twice (us, 8 KV heads of 128): 4 rows, 8 sequences of 4096: 20.3, 24.6; 32 of 8192: 82,
   // 121; 16 rows, 8 of 4096: 27.3, 24.8; one of 32768: 28.6, 32.8.  Queries in LDS for the whole call against 64 rows at a
   // time: 20 rows, 8 of 4096: 28.7, 58.6; 64 rows: 37.7, 58.5; one of 32768: 54, 69.
-  const bool store = aw_stores(rows, p.tiles), few = rows <= kAwFewRows, f32 = scale_fp32 != 0;
-  // Tiles of a workgroup of few rows: as many as leave two workgroups to a CU.
-  const int64_t tiles = progs * p.tiles, span = tiles / (2 * device_cus());
-  p.span = few ? (int)(span < 1 ? 1 : span > kAwSpan ? kAwSpan : span) : 1;
-  const int64_t items = progs * ceil_div(p.tiles, p.span) * p.segs, sums = progs * ceil_div64(cap, kAwSumTile);
-  const int grid = (int)(items < kAwMaxGrid ? items : kAwMaxGrid), threads = few ? 256 : 512;
-  for (p.row0 = 0; p.row0 < rows; p.row0 += p.segs * p.seg_rows) {
-    if (int rc = launch(store ? aw_store_fn(D, f32) : aw_fn<kAwStats>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p))
-      return rc;
-    const int rc = store ? launch(aw_sum_fn(rows), (int)(sums < kAwMaxGrid ? sums : kAwMaxGrid),
-                                  256, 0, (hipStream_t)stream, &p)
-                         : launch(aw_fn<kAwSums>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p);
-    if (rc != SPECQ_OK) return rc;
+  const bool store = space.store, few = rows <= kAwFewRows, f32 = scale_fp32 != 0;
+  for (; p.b0 < B_grid; p.b0 += (int)space.seqs) {
+    p.B_grid = (int)(B_grid - p.b0 < space.seqs ? B_grid - p.b0 : space.seqs);
+    p.n_seqs = n_seqs < p.b0 ? 0 : n_seqs - p.b0 < p.B_grid ? n_seqs - p.b0 : p.B_grid;
+    const int64_t some = (int64_t)p.B_grid * H_KV;
+    // Tiles of a workgroup of few rows: as many as leave two workgroups to a CU.
+    const int64_t tiles = some * p.tiles, span = tiles / (2 * device_cus());
+    p.span = few ? (int)(span < 1 ? 1 : span > kAwSpan ? kAwSpan : span) : 1;
+    const int64_t items = some * ceil_div(p.tiles, p.span) * p.segs, sums = some * ceil_div64(cap, kAwSumTile);
+    const int grid = (int)(items < kAwMaxGrid ? items : kAwMaxGrid), threads = few ? 256 : 512;
+    for (p.row0 = 0; p.row0 < rows; p.row0 += p.segs * p.seg_rows) {
+      if (int rc = launch(store ? aw_store_fn(D, f32) : aw_fn<kAwStats>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p))
+        return rc;
+      const int rc = store ? launch(aw_sum_fn(rows), (int)(sums < kAwMaxGrid ? sums : kAwMaxGrid), 256, 0, (hipStream_t)stream, &p)
+                           : launch(aw_fn<kAwSums>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p);
+      if (rc != SPECQ_OK) return rc;
+    }
+    p.q += space.seqs * s_qb;
+    p.bt += space.seqs * s_bt;
+    p.ctx_len += space.seqs;
+    if (p.q_lens != nullptr) p.q_lens += space.seqs;
+    p.w += space.seqs * s_wb;
   }
   return SPECQ_OK;
 }

@@ -380,3 +380,35 @@ def test_many_rows_of_some_drafts_bad_pages_and_masked_scales(QL, G):
     K.paged_attention_weights(*p, q_lens=gpu(np.asarray([*lens, 3, 3], np.int32))[0], sm_scale=0.1, plan=plan)
     torch.cuda.synchronize()
     assert torch.equal(p[5][:5], t[5]) and bool((p[5][5:] == 1.5).all())
+
+
+@pytest.mark.parametrize("B,QL,G,ctx", [
+    (7, 4, 4, [900, 3, 2000, 0, 300, 1, 1200]),          # stored: 64 MiB of scores a sequence
+    (150, 8, 8, [700, 5, 300]),                          # 64 rows: 2 MiB of statistics a sequence
+    (9, 260, 4, [600, 260, 1500, 300, 0, 100, 333]),     # 1040 rows, 32 MiB a sequence and segment
+])
+def test_batches_that_are_taken_in_turns(B, QL, G, ctx):
+    """Tables of 131072 columns' tokens: not all sequences' scores, statistics and sums find room at once."""
+    rng = np.random.default_rng(B)
+    HK, D, PAGE, wide = 8, 64, 16, 8192
+    ctx = (ctx * B)[:B]
+    q, kc, ks, bt, cl, w = make(rng, ctx, QL, HK * G, HK, D, PAGE, False)
+    tq, tk, ts, tb, tc, tw = gpu(q, kc, ks, bt, cl, w)
+    lens = gpu(rng.integers(0, QL + 1, B).astype(np.int32))[0]
+    cols, T = bt.shape[1], w.shape[2]
+    wbt = torch.full((B, wide), -1, dtype=torch.int32, device=DEV)
+    wbt[:, :cols] = tb
+    note(f"attn_weights turns B={B} QL={QL}")
+    for plan in (None, (B, QL), (B - 1, QL - 1), (1, QL)):
+        ww = torch.zeros((B, HK, wide * PAGE), device=DEV)
+        ww[:, :, :T] = tw
+        want = tw.clone()
+        if plan is None:
+            K.paged_attention_weights(tq, tk, ts, wbt, tc, ww, q_lens=lens)
+            K.paged_attention_weights(tq, tk, ts, tb, tc, want, q_lens=lens)
+        else:
+            K.paged_attention_weights(tq, tk, ts, wbt, tc, ww, plan=torch.tensor(plan, dtype=torch.int32, device=DEV))
+            K.paged_attention_weights(tq, tk, ts, tb, tc, want, n_seqs=plan[0], q_len=plan[1])
+        torch.cuda.synchronize()
+        assert torch.equal(ww[:, :, :T], want), f"plan {plan}"
+        assert not ww[:, :, T:].any()

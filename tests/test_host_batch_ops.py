@@ -67,6 +67,15 @@ def test_weights_workspace_covers_what_a_call_asks_for(built_lib):
     assert size(0, 32, 8, 1, 64, 16) == size(2, 30, 8, 1, 64, 16) == size(2, 32, 8, 1, 64, 0) == 0
 
 
+@pytest.mark.parametrize("B,H,HK,ql,tokens", [
+    (32, 32, 8, 1, 131072), (32, 64, 8, 2, 131072), (256, 32, 8, 1, 131072), (256, 32, 8, 9, 131072), (64, 32, 8, 4096, 131072),
+    (8192, 64, 8, 2, 32768), (1, 64, 8, 2, 524288), (3, 8, 8, 1, 1 << 22), (2, 8, 1, 2048, 1 << 20)])
+def test_weights_workspace_has_a_bound(built_lib, B, H, HK, ql, tokens):
+    """Wide tables: some sequences at a time, whatever the batch.  What one sequence needs with 1024 rows lies within it here."""
+    from specq import _lib
+    assert _lib.lib().specq_paged_attn_weights_workspace_size(B, H, HK, ql, tokens // 16, 16) <= (256 << 20) + (256 << 10) + 4096
+
+
 def _evict(n=1, base=(4096,), sp=(16 * 1024,), so=(1024,), sh=(128,), rb=(128,), **kw):
     keep = [np.asarray(v, np.int64) for v in (base, sp, so, sh, rb)]
     a = dict(bt=16, s_bt=64, B=2, C=64, ref=0, P=100, ctx=16, w=16, s_wb=8 * 1024, s_wh=1024, HK=8, PAGE=16, n=n,
