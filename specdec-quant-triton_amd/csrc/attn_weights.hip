@@ -24,6 +24,8 @@
 // 8 KV heads of 128 (us): a new token of 32 sequences of up to 8192, stored scores, 53 + 8, codes and scores at 3.4 TB/s (loads
 // alone 5.2); 9 of 8 sequences of 4096, formed twice, 19 + 14, half of it fixed phases; 256 of 2 of up to 4096, 43 + 33, bound by
 // vector instructions at two waves a SIMD.
+#include <algorithm>
+
 #include "api_common.hpp"
 #include "common.hpp"
 
@@ -39,7 +41,8 @@ constexpr int kAwSegs = 8;         // most such segments of a launch
 constexpr int kAwFill = 256;       // workgroups that fill the GPU: fewer take a unit each
 constexpr int kAwSeg = 32;         // row blocks of 16 whose statistics are joined at a time
 constexpr int kAwSumTile = 1024;   // tokens of a workgroup that adds up stored scores
-constexpr int kAwMaxGrid = 1 << 16;
+// Most workgroups a CU of a launch of 256 threads, of 512, and of the one that sums stored scores; they come back for more.
+constexpr int kAwFewGrid = 8, kAwManyGrid = 4, kAwSumGrid = 16;
 // Bytes that scores, statistics and sums of a launch take at most, unless one sequence needs more: they are as wide as the table, however
 // short the contexts, so a large batch is taken some sequences at a time.  A further pair of launches takes some 8 us, where the
 // scores alone of 256 MiB take more than 50 each way.
@@ -57,7 +60,7 @@ struct AwParams {
   int n_seqs, q_len, B_grid, ql_grid, G, H_KV, PAGE;
   int cap;      // tokens a row of the table holds
   int tiles;    // of cap
-  int span;     // tiles of a workgroup of few rows
+  int span;     // tiles of a workgroup of few rows, at most
   int rows;     // of a program and segment at most
   int row0;     // the launch's first row: more than segs * seg_rows have several pairs of launches one after another
   int seg_rows, segs;  // rows of a workgroup's segment (a unit or more), segments of a launch
@@ -99,6 +102,20 @@ __device__ __forceinline__ bool aw_prog(const AwParams& p, int prog, AwProg& x, 
   x.L = min(max(p.ctx_len[x.b], 0), p.cap);
   x.tiles = (x.L + kAwTile - 1) / kAwTile;
   return x.rows > 0 && x.L > 0;
+}
+
+// Tables are often much wider than the contexts, and an empty workgroup takes its turn as well: a prompt of 4096 tokens in a table of
+// 131072 took 1200 us where one of 4096 takes 405, 9 tokens of 32 sequences of 1000 110 us and 33.  So a workgroup that comes back
+// for its second item looks how long the longest sequence is, and items behind that are none: `live`, with `per` items to every
+// `step` tiles (these: 370 and 42 us; calls without a second item 0 to 1 % longer).
+__device__ __forceinline__ int64_t aw_live(const AwParams& p, int64_t item, int64_t live, int64_t per, int step) {
+  if (item >= live || item != (int64_t)blockIdx.x + gridDim.x) return live;
+  const int n = p.plan != nullptr ? min(max(p.plan[0] - p.b0, 0), p.B_grid) : p.n_seqs;
+  int longest = 0;
+  for (int b = lane_id(); b < n; b += kWave) longest = max(longest, p.ctx_len[b]);
+  for (int o = 1; o < kWave; o *= 2) longest = max(longest, __shfl_xor(longest, o));
+  const int tiles = (min(uniform(longest), p.cap) + kAwTile - 1) / kAwTile;
+  return min(live, per * ((tiles + step - 1) / step));
 }
 
 __device__ __forceinline__ float aw_max4(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -349,22 +366,24 @@ __device__ __forceinline__ void aw_norms(const AwParams& p, const AwProg& x, int
   }
 }
 
-// The statistics of a workgroup's tiles, each of its four waves' joined.
+// The statistics of a workgroup's `tiles` tiles, `step` apart, each of its four waves' joined.
 template <int ROWS, int N>
-__device__ __forceinline__ void aw_publish(const AwParams& p, const AwProg& x, int prog, int tile0, int tile1,
+__device__ __forceinline__ void aw_publish(const AwParams& p, const AwProg& x, int prog, int tile0, int step, int tiles,
                                            const uint64_t (&st)[N][4][ROWS]) {
-  const int n = (tile1 - tile0) * x.rows;
-  for (int i = threadIdx.x; i < n; i += 256) {
+  for (int i = threadIdx.x; i < tiles * x.rows; i += 256) {
     const int tile = i / x.rows, row = i - tile * x.rows;
     float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int v = 0; v < 4; ++v) aw_join(m, l, aw_m(st[tile][v][row]), aw_l(st[tile][v][row]));
-    publish(p.stats + ((int64_t)prog * p.tiles + tile0 + tile) * p.rows + row, aw_pack(m, l));
+    publish(p.stats + ((int64_t)prog * p.tiles + tile0 + tile * step) * p.rows + row, aw_pack(m, l));
   }
 }
 
-// Up to 64 rows.  A workgroup walks `span` tiles of a program, a wave 64 tokens of each, with the next tile's codes on
-// their way while one is multiplied; all rows' queries wait in LDS.
+// Up to 64 rows.  A workgroup walks up to `span` tiles of a program, a wave 64 tokens of each, with the next tile's codes on
+// their way while one is multiplied; all rows' queries wait in LDS.  The tiles lie as far apart as the program has workgroups, so
+// that a context shorter than the table is shared out to all of them and their pages can be looked up before its length is known:
+// 9 tokens at 4096 in a table of 131072, 8 sequences: 42 us (side by side 50), one: 19 (45).  Stored scores are written side by
+// side: tiles apart took 55 us for 53 where the workgroups are many enough.
 template <int D, typename ST, int MODE>
 __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
   constexpr int NU = D / 32, RB = kAwFewRows / 16;
@@ -375,15 +394,16 @@ __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
   __shared__ int s_last;
   const int lane = lane_id(), w = uniform(wave_id()), r = lane & 15, g = lane >> 4;
   const int progs = p.B_grid * p.H_KV, spans = (p.tiles + p.span - 1) / p.span;
-  for (int64_t item = blockIdx.x; item < (int64_t)progs * spans; item += gridDim.x) {
-    const int tile0 = (int)(item / progs) * p.span, prog = aw_order(p, (int)(item % progs));
+  int64_t live = (int64_t)progs * spans;
+  for (int64_t item = blockIdx.x; item < live; item += gridDim.x, live = aw_live(p, item, live, progs, 1)) {
+    const int tile0 = (int)(item / progs), prog = aw_order(p, (int)(item % progs));
     // The wave's sub-tile `lane` and its page, whose load does not wait for the context's length.
-    const int sub_t = (tile0 + lane / 4) * kAwTile + 64 * w + 16 * (lane & 3);
+    const int sub_t = (tile0 + min(lane / 4, p.span - 1) * spans) * kAwTile + 64 * w + 16 * (lane & 3);
     int page = -1;
     if (lane < 4 * p.span && sub_t < p.cap) page = p.bt[(int64_t)(prog / p.H_KV) * p.s_bt + sub_t / p.PAGE];
     AwProg x;
     if (!aw_prog(p, prog, x) || tile0 >= x.tiles) continue;
-    const int blocks = (x.rows + 15) / 16, tile1 = min(tile0 + p.span, x.tiles);
+    const int blocks = (x.rows + 15) / 16;
     __syncthreads();  // the last item's queries have been read
     for (int f = threadIdx.x; f < blocks * NU * 64; f += 256) {
       const int l = f % 64, u = (f / 64) % NU, row = min(f / (64 * NU) * 16 + (l & 15), x.rows - 1);
@@ -405,13 +425,13 @@ __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
       }
     }
     __syncthreads();
-    for (int tile = tile0; tile < tile1; ++tile) {
+    for (int n = 0, tile = tile0; tile < x.tiles; ++n, tile += spans) {
       const int t0 = tile * kAwTile + 64 * w;
-      const uint32_t seen = (uint32_t)(at.ok >> (4 * (tile - tile0))) & 0xf;
+      const uint32_t seen = (uint32_t)(at.ok >> (4 * n)) & 0xf;
       // Lane (r, g) holds the scale of token t0 + 16 g + r; it needs those of tokens 16 s + 4 g + i.
       s_k[w].put(raw);
       s_scale[w][lane] = (float)scale * p.scale_log2;
-      aw_load<D, false, ST>(p, at, 4 * (tile + 1 - tile0), raw, scale);
+      aw_load<D, false, ST>(p, at, 4 * (n + 1), raw, scale);
       wait_lgkm0();
       v8h kh[4][NU];
 #pragma unroll
@@ -443,7 +463,7 @@ __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
             }
         } else {
           const uint64_t st = aw_stat(acc);
-          if (g == 0) s_stat[tile - tile0][w][row] = st;
+          if (g == 0) s_stat[n][w][row] = st;
         }
       }
       if constexpr (MODE == kAwSums) {
@@ -455,8 +475,8 @@ __global__ __launch_bounds__(256, 2) void aw_few_kernel(AwParams p) {
     }
     if constexpr (MODE != kAwSums) {
       __syncthreads();
-      aw_publish(p, x, prog, tile0, tile1, s_stat);
-      if (arrive_last(p.counters + prog, (x.tiles + p.span - 1) / p.span, &s_last)) aw_norms(p, x, prog);
+      aw_publish(p, x, prog, tile0, spans, (x.tiles - tile0 + spans - 1) / spans, s_stat);
+      if (arrive_last(p.counters + prog, min(spans, x.tiles), &s_last)) aw_norms(p, x, prog);
     }
   }
 }
@@ -472,7 +492,8 @@ __global__ __launch_bounds__(256) void aw_store_kernel(AwParams p) {
   __shared__ int s_last;
   const int lane = lane_id(), w = uniform(wave_id()), r = lane & 15, g = lane >> 4;
   const int progs = p.B_grid * p.H_KV, spans = (p.tiles + p.span - 1) / p.span;
-  for (int64_t item = blockIdx.x; item < (int64_t)progs * spans; item += gridDim.x) {
+  int64_t live = (int64_t)progs * spans;
+  for (int64_t item = blockIdx.x; item < live; item += gridDim.x, live = aw_live(p, item, live, progs, p.span)) {
     const int tile0 = (int)(item / progs) * p.span, prog = aw_order(p, (int)(item % progs));
     const int sub_t = (tile0 + lane / 4) * kAwTile + 64 * w + 16 * (lane & 3);
     int page = -1;
@@ -529,7 +550,7 @@ __global__ __launch_bounds__(256) void aw_store_kernel(AwParams p) {
       if (g == 0) s_stat[tile - tile0][w][r] = st;
     }
     __syncthreads();
-    aw_publish(p, x, prog, tile0, tile1, s_stat);
+    aw_publish(p, x, prog, tile0, 1, tile1 - tile0, s_stat);
     if (arrive_last(p.counters + prog, (x.tiles + p.span - 1) / p.span, &s_last)) aw_norms(p, x, prog);
   }
 }
@@ -553,7 +574,8 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
   // Granule q of row t lies in slot q ^ key(t): 16 rows' granules meet in no bank.
   auto key = [](int t) { return D == 128 ? t & 15 : (t >> 1) & 7; };
   const int progs = p.B_grid * p.H_KV, per = p.segs * progs;
-  for (int64_t item = blockIdx.x; item < (int64_t)per * p.tiles; item += gridDim.x) {
+  int64_t live = (int64_t)per * p.tiles;
+  for (int64_t item = blockIdx.x; item < live; item += gridDim.x, live = aw_live(p, item, live, per, 1)) {
     const int tile = (int)(item / per), some = (int)(item % per), seg_i = some / progs, row0 = p.row0 + seg_i * p.seg_rows;
     const int prog = aw_order(p, some - seg_i * progs), index = prog * p.segs + seg_i, t0 = tile * kAwTile + 64 * w;
     AwProg x;
@@ -734,49 +756,55 @@ __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
 // Pass 2 from stored scores of up to R rows: a thread owns four tokens, and adds their rows in the order of the lanes above.  32
 // sequences of up to 8192, 4 rows: 7.6 us with R = 4, 12 with 16.
 template <int R>
-__global__ __launch_bounds__(256, 4) void aw_sum_kernel(AwParams p) {
+__device__ __forceinline__ void aw_sum(const AwParams& p, const AwProg& x, int prog, int t) {
 #pragma clang fp contract(off)  // a probability is rounded before it is added, as the first addition to nothing does it above
-  const int progs = p.B_grid * p.H_KV, tiles = (p.cap + kAwSumTile - 1) / kAwSumTile;
-  for (int64_t item = blockIdx.x; item < (int64_t)progs * tiles; item += gridDim.x) {
-    const int tile = (int)(item / progs), prog = (int)(item - (int64_t)tile * progs);
-    AwProg x;
-    const int t = tile * kAwSumTile + 4 * (int)threadIdx.x;
-    if (!aw_prog(p, prog, x) || t >= x.L) continue;
-    const float* sc = p.scores + (int64_t)prog * p.rows * p.tiles * kAwTile + t;
-    v4f e[R];
+  const float* sc = p.scores + (int64_t)prog * p.rows * p.tiles * kAwTile + t;
+  v4f e[R];
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      e[k] = v4f{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (k < x.rows) e[k] = *reinterpret_cast<const v4f*>(sc + (int64_t)k * p.tiles * kAwTile);
-    }
-    float top[R], inv[R];
-    bool nan = false;
+  for (int k = 0; k < R; ++k) {
+    e[k] = v4f{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (k < x.rows) e[k] = *reinterpret_cast<const v4f*>(sc + (int64_t)k * p.tiles * kAwTile);
+  }
+  float top[R], inv[R];
+  bool nan = false;
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const uint64_t norm = k < x.rows ? p.norms[(int64_t)prog * p.rows + k] : aw_pack(INFINITY, 0.f);
-      top[k] = aw_m(norm), inv[k] = aw_l(norm);
-      nan |= !(top[k] == top[k]);
-    }
-    if (uniform((int)nan)) {  // a row gives its NaN to what it sees alone
-#pragma unroll
-      for (int k = 0; k < R; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!(top[k] == top[k]) && !(e[k][i] == -INFINITY)) e[k][i] = top[k];
-#pragma unroll
-      for (int k = 0; k < R; ++k)
-        if (!(top[k] == top[k])) top[k] = 0.f;
-    }
+  for (int k = 0; k < R; ++k) {
+    const uint64_t norm = k < x.rows ? p.norms[(int64_t)prog * p.rows + k] : aw_pack(INFINITY, 0.f);
+    top[k] = aw_m(norm), inv[k] = aw_l(norm);
+    nan |= !(top[k] == top[k]);
+  }
+  if (uniform((int)nan)) {  // a row gives its NaN to what it sees alone
 #pragma unroll
     for (int k = 0; k < R; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) e[k][i] = fast_exp2(e[k][i] - top[k]) * inv[k];
-    // Pairs, pairs of these, and the fours.
+      for (int i = 0; i < 4; ++i)
+        if (!(top[k] == top[k]) && !(e[k][i] == -INFINITY)) e[k][i] = top[k];
 #pragma unroll
-    for (int o = 1; o < R; o *= 2)
+    for (int k = 0; k < R; ++k)
+      if (!(top[k] == top[k])) top[k] = 0.f;
+  }
 #pragma unroll
-      for (int k = 0; k + o < R; k += 2 * o) e[k] += e[k + o];
-    aw_put(p, x, t, aw_get(p, x, t, true) + e[0]);
+  for (int k = 0; k < R; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[k][i] = fast_exp2(e[k][i] - top[k]) * inv[k];
+  // Pairs, pairs of these, and the fours.
+#pragma unroll
+  for (int o = 1; o < R; o *= 2)
+#pragma unroll
+    for (int k = 0; k + o < R; k += 2 * o) e[k] += e[k + o];
+  aw_put(p, x, t, aw_get(p, x, t, true) + e[0]);
+}
+
+template <int R>
+__global__ __launch_bounds__(256, 4) void aw_sum_kernel(AwParams p) {
+  const int progs = p.B_grid * p.H_KV, tiles = (p.cap + kAwSumTile - 1) / kAwSumTile;
+  int64_t live = (int64_t)progs * tiles;
+  for (int64_t item = blockIdx.x; item < live; item += gridDim.x, live = aw_live(p, item, live, progs, kAwSumTile / kAwTile)) {
+    const int tile = (int)(item / progs), prog = (int)(item - (int64_t)tile * progs);
+    AwProg x;
+    const int t = tile * kAwSumTile + 4 * (int)threadIdx.x;
+    if (!aw_prog(p, prog, x)) continue;
+    if (t < x.L) aw_sum<R>(p, x, prog, t);
   }
 }
 
@@ -910,11 +938,12 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
     const int64_t tiles = some * p.tiles, span = tiles / (2 * device_cus());
     p.span = few ? (int)(span < 1 ? 1 : span > kAwSpan ? kAwSpan : span) : 1;
     const int64_t items = some * ceil_div(p.tiles, p.span) * p.segs, sums = some * ceil_div64(cap, kAwSumTile);
-    const int grid = (int)(items < kAwMaxGrid ? items : kAwMaxGrid), threads = few ? 256 : 512;
+    const int threads = few ? 256 : 512, cus = device_cus();
+    const int grid = (int)std::min<int64_t>(items, (few ? kAwFewGrid : kAwManyGrid) * cus);
     for (p.row0 = 0; p.row0 < rows; p.row0 += p.segs * p.seg_rows) {
       if (int rc = launch(store ? aw_store_fn(D, f32) : aw_fn<kAwStats>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p))
         return rc;
-      const int rc = store ? launch(aw_sum_fn(rows), (int)(sums < kAwMaxGrid ? sums : kAwMaxGrid), 256, 0, (hipStream_t)stream, &p)
+      const int rc = store ? launch(aw_sum_fn(rows), (int)std::min<int64_t>(sums, kAwSumGrid * cus), 256, 0, (hipStream_t)stream, &p)
                            : launch(aw_fn<kAwSums>(D, f32, few), grid, threads, 0, (hipStream_t)stream, &p);
       if (rc != SPECQ_OK) return rc;
     }

@@ -412,3 +412,27 @@ def test_batches_that_are_taken_in_turns(B, QL, G, ctx):
         torch.cuda.synchronize()
         assert torch.equal(ww[:, :, :T], want), f"plan {plan}"
         assert not ww[:, :, T:].any()
+
+
+@pytest.mark.parametrize("QL,G", [(1, 2), (9, 2), (40, 2)])
+def test_more_items_than_workgroups(QL, G):
+    """300 sequences of 8 heads: workgroups come back for more, up to the longest sequence.  In parts, the same bits."""
+    rng = np.random.default_rng(77)
+    B, HK, D, PAGE = 300, 8, 64, 16
+    ctx = rng.integers(0, 300, B)
+    ctx[[3, 120, 121, 299]] = 1900, 1300, 1800, 2000
+    case = make(rng, ctx.tolist(), QL, G * HK, HK, D, PAGE, False)
+    lens = rng.integers(0, QL + 1, B).astype(np.int32)
+    lens[[3, 299]] = QL
+    note(f"attn_weights many items QL={QL}")
+    tq, tk, ts, tb, tc, tw = gpu(*case)
+    tl = gpu(lens)[0]
+    parts = tw.clone()
+    K.paged_attention_weights(tq, tk, ts, tb, tc, tw, q_lens=tl)
+    for b in range(0, B, 20):
+        at = slice(b, b + 20)
+        K.paged_attention_weights(tq[at], tk, ts, tb[at], tc[at], parts[at], q_lens=tl[at])
+    torch.cuda.synchronize()
+    assert torch.equal(tw, parts)
+    for at in (slice(0, 8), slice(118, 124), slice(295, 300)):
+        check(tw[at], (case[0][at], case[1], case[2], case[3][at], case[4][at], case[5][at]), lens[at].tolist(), D ** -0.5, f"{at}")
