@@ -471,6 +471,7 @@ int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_qt, int64_t 
  *   Cache tensors: at most 16, [n_pages, PAGE, H_KV] rows of row_bytes (1 to 4096) bytes; base pointers and strides in
  *   bytes (host arrays, read during the call)
  *   kept      int32 [B, H_KV, budget];  0 <= recent + sinks <= budget <= limit, budget at most 2^30
+ *   B H_KV below 2^22, and times the 128-byte pieces of a token in all tensors, and one more, below 2^23
  *   Workspace: specq_kv_evict_workspace_size() bytes, as the workspaces above.
  * ------------------------------------------------------------------------------------- */
 size_t specq_kv_evict_workspace_size(int B, int H_KV, int max_pages, int PAGE);

@@ -572,6 +572,8 @@ extern "C" int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int
   const int64_t cap = (int64_t)max_pages * PAGE, progs = (int64_t)B * H_KV;
   SPECQ_REQUIRE(cap <= (1 << 30) && progs <= (1 << 22), SPECQ_ENOTSUP, "kv_evict: a table of %lld tokens or %lld rows is too large",
                 (long long)cap, (long long)progs);
+  // Either launch is of fewer than 2^32 threads, or neither is made.
+  SPECQ_REQUIRE(progs * kEvThreads <= UINT32_MAX, SPECQ_ENOTSUP, "kv_evict: %lld sequences x heads to choose from", (long long)progs);
   SPECQ_REQUIRE(budget > 0 && recent >= 0 && sinks >= 0 && (int64_t)recent + sinks <= budget && limit >= budget, SPECQ_EINVAL,
                 "kv_evict: need 0 <= recent + sinks <= budget <= limit and budget > 0 (recent=%d sinks=%d budget=%d limit=%d)",
                 recent, sinks, budget, limit);
@@ -629,6 +631,9 @@ extern "C" int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int
   m.tensor[m.units] = kEvTensors; m.vec[m.units] = 4; m.bytes[m.units] = 4;
   ++m.units;
   m.progs = (int)progs;
+  const int64_t moves = (int64_t)align_up(progs, 8) * m.units;
+  SPECQ_REQUIRE(moves * kEvMove <= UINT32_MAX, SPECQ_ENOTSUP, "kv_evict: %lld sequences x heads of %d byte ranges each are too many",
+                (long long)progs, m.units);
   if (PAGE > 1) {
     int bits = 0;  // ceil(log2(PAGE))
     while ((1ll << bits) < PAGE) ++bits;
@@ -655,5 +660,5 @@ extern "C" int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int
                            reinterpret_cast<const void*>(&evict_slice_rank_kernel)})
       if (int rc = launch(fn, (int)n, kEvThreads, 0, st, &p)) return rc;
   }
-  return launch(reinterpret_cast<const void*>(&evict_move_kernel), (int)(align_up(progs, 8) * m.units), kEvMove, 0, st, &m);
+  return launch(reinterpret_cast<const void*>(&evict_move_kernel), (int)moves, kEvMove, 0, st, &m);
 }

@@ -105,6 +105,14 @@ def test_evict_refusals(built_lib):
     f(-28, base=(4096, 1 << 20), **two)
 
 
+def test_evict_refuses_what_a_launch_does_not_take_before_the_first(built_lib):
+    """A selection of 2^32 threads and more, and a move of them behind a selection that could have run."""
+    for kw in (dict(B=1 << 19), dict(B=1 << 17, sp=(16 * 8 * 4096,), so=(8 * 4096,), sh=(4096,), rb=(4096,))):
+        keep, a = _evict(**kw, ws=4096, wsb=1 << 40)
+        _fail("specq_kv_evict", a, -95)
+        del keep
+
+
 def test_beam_refusals(built_lib):
     base = dict(x=16, f32=0, s_lb=4 * 1000, s_lw=1000, scores=16, s_sb=4, done=0, s_fb=4, eos=0, os=16, ot=16, op=16, B=2, W=4,
                 V=1000, n=4, ws=0, wsb=0, stream=0)
