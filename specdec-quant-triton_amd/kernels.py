@@ -1116,9 +1116,27 @@ def _rotary_out(who: str, x, shape, strides, D: int, out):
     return out, so
 
 
-def _rotary_call(who: str, q, k, inv_freq, ctx_len, q_len, positions, plan, n_seqs, q_out, k_out):
-    """Checks the arguments that the rotary entry points share; returns the outputs and the C call's words: those of the
-    tensors, the frequencies', the positions', the grid and the sizes (None where there is nothing to do)."""
+def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, interleaved=False, mscale=1.0, plan=None,
+                 n_seqs=None, q_out=None, k_out=None, _norm=None):
+    """Rotary positions of the new tokens' q and k; returns (q_out, k_out).
+
+    q fp16 [B, QL, H, D], k fp16 [B, QL, H_KV, D] or None; inv_freq fp32 or fp64 [R / 2], R <= D <= 512
+    (rotary_inv_freq).  Pair j of the first R dimensions -- (j, j + R/2), or (2j, 2j + 1) with
+    interleaved -- is turned by pos * inv_freq[j] and scaled by mscale; the other dimensions are copied.
+    Token i of sequence b is at ctx_len[b] - q_len + i (ctx_len counts the new tokens, as the K/V append
+    and the attention have it), or at positions[b, i] (int32 [B, QL]).  Angles are formed in fp64.
+    Outputs may be the inputs (in place); they must not overlap them otherwise.  With `plan`,
+    (n_seqs, q_len) = plan[0:2] on the device and the grid covers (B, QL).  Tokens that are not active
+    are not written (an omitted output holds anything there).
+    """
+    # _norm: qk_norm_rotary's (q_weight, k_weight, eps).  One body, since a function between it and the callers costs a step 4 %.
+    if _norm is None:
+        who = "rotary_embed"
+        dev = _gpu_of(who, q, k, inv_freq, ctx_len, positions, plan, q_out, k_out)
+    else:
+        who = "qk_norm_rotary"
+        q_weight, k_weight, eps = _norm
+        dev = _gpu_of(who, q, k, q_weight, k_weight, inv_freq, ctx_len, positions, plan, q_out, k_out)
     shape, qs = q.shape, q.stride()
     if len(shape) != 4:
         raise RuntimeError(f"{who}: q [B, QL, H, D] expected")
@@ -1148,34 +1166,30 @@ def _rotary_call(who: str, q, k, inv_freq, ctx_len, q_len, positions, plan, n_se
         _int32_vec(who, "ctx_len", ctx_len, Bg)
     else:
         raise RuntimeError(f"{who}: ctx_len or positions must be given")
+    if _norm is not None:
+        if k is None and k_weight is not None:
+            raise RuntimeError(f"{who}: k_weight without k")
+        s_wq = _norm_weights(who, "q_weight", q_weight, H, D)
+        s_wk = _norm_weights(who, "k_weight", k_weight, H_KV, D)
+        w = q_weight if q_weight is not None else k_weight
+        if k_weight is not None and w.dtype != k_weight.dtype:
+            raise RuntimeError(f"{who}: q_weight and k_weight must be of one type")
     if Bg == 0 or Qg == 0:
-        return q_out, k_out, None
-    return q_out, k_out, (
-        (q.data_ptr(), qs[0], qs[1], qs[2], _ptr(k), ks[0], ks[1], ks[2],
-         q_out.data_ptr(), qo[0], qo[1], qo[2], _ptr(k_out), ko[0], ko[1], ko[2]),
-        (inv_freq.data_ptr(), inv_freq.dtype == torch.float64),
-        (_ptr(ctx_len), _ptr(positions), s_pb, Bg, n_seqs, q_len, Qg, H, H_KV, D, 2 * inv_freq.shape[0]))
-
-
-def rotary_embed(q, k, inv_freq, ctx_len=None, q_len=None, positions=None, interleaved=False, mscale=1.0, plan=None,
-                 n_seqs=None, q_out=None, k_out=None):
-    """Rotary positions of the new tokens' q and k; returns (q_out, k_out).
-
-    q fp16 [B, QL, H, D], k fp16 [B, QL, H_KV, D] or None; inv_freq fp32 or fp64 [R / 2], R <= D <= 512
-    (rotary_inv_freq).  Pair j of the first R dimensions -- (j, j + R/2), or (2j, 2j + 1) with
-    interleaved -- is turned by pos * inv_freq[j] and scaled by mscale; the other dimensions are copied.
-    Token i of sequence b is at ctx_len[b] - q_len + i (ctx_len counts the new tokens, as the K/V append
-    and the attention have it), or at positions[b, i] (int32 [B, QL]).  Angles are formed in fp64.
-    Outputs may be the inputs (in place); they must not overlap them otherwise.  With `plan`,
-    (n_seqs, q_len) = plan[0:2] on the device and the grid covers (B, QL).  Tokens that are not active
-    are not written (an omitted output holds anything there).
-    """
-    who = "rotary_embed"
-    dev = _gpu_of(who, q, k, inv_freq, ctx_len, positions, plan, q_out, k_out)
-    q_out, k_out, words = _rotary_call(who, q, k, inv_freq, ctx_len, q_len, positions, plan, n_seqs, q_out, k_out)
-    if words is not None:
-        tensors, freq, rest = words
-        _call_on(dev, "specq_rotary", *tensors, *freq, mscale, *rest, bool(interleaved), _plan_of(plan, 2, who))
+        return q_out, k_out
+    R = 2 * inv_freq.shape[0]
+    if _norm is None:
+        _call_on(dev, "specq_rotary", q.data_ptr(), qs[0], qs[1], qs[2], _ptr(k), ks[0], ks[1], ks[2],
+                 q_out.data_ptr(), qo[0], qo[1], qo[2], _ptr(k_out), ko[0], ko[1], ko[2],
+                 inv_freq.data_ptr(), inv_freq.dtype == torch.float64, mscale,
+                 _ptr(ctx_len), _ptr(positions), s_pb, Bg, n_seqs, q_len, Qg, H, H_KV, D, R,
+                 bool(interleaved), _plan_of(plan, 2, who))
+    else:
+        _call_on(dev, "specq_qk_norm_rotary", q.data_ptr(), qs[0], qs[1], qs[2], _ptr(k), ks[0], ks[1], ks[2],
+                 q_out.data_ptr(), qo[0], qo[1], qo[2], _ptr(k_out), ko[0], ko[1], ko[2],
+                 _ptr(q_weight), s_wq, _ptr(k_weight), s_wk, w is not None and w.dtype == torch.float32, eps,
+                 inv_freq.data_ptr(), inv_freq.dtype == torch.float64, mscale,
+                 _ptr(ctx_len), _ptr(positions), s_pb, Bg, n_seqs, q_len, Qg, H, H_KV, D, R,
+                 bool(interleaved), _plan_of(plan, 2, who))
     return q_out, k_out
 
 
@@ -1197,22 +1211,8 @@ def qk_norm_rotary(q, k, q_weight, k_weight, inv_freq, ctx_len=None, q_len=None,
     rotary_embed turns them: fp32, rounded once.  q_weight, k_weight fp16 or fp32, both of one type, [D], or a row for
     each head ([H, D], [H_KV, D]), or None (no weights; k_weight is None where k is).  Everything else as rotary_embed.
     """
-    who = "qk_norm_rotary"
-    dev = _gpu_of(who, q, k, q_weight, k_weight, inv_freq, ctx_len, positions, plan, q_out, k_out)
-    q_out, k_out, words = _rotary_call(who, q, k, inv_freq, ctx_len, q_len, positions, plan, n_seqs, q_out, k_out)
-    if k is None and k_weight is not None:
-        raise RuntimeError(f"{who}: k_weight without k")
-    s_wq = _norm_weights(who, "q_weight", q_weight, q.shape[2], q.shape[3])
-    s_wk = _norm_weights(who, "k_weight", k_weight, k.shape[2], q.shape[3]) if k is not None else 0
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise RuntimeError(f"{who}: q_weight and k_weight must be of one type")
-    if words is not None:
-        tensors, freq, rest = words
-        w = q_weight if q_weight is not None else k_weight
-        _call_on(dev, "specq_qk_norm_rotary", *tensors, _ptr(q_weight), s_wq, _ptr(k_weight), s_wk,
-                 w is not None and w.dtype == torch.float32, eps, *freq, mscale, *rest, bool(interleaved),
-                 _plan_of(plan, 2, who))
-    return q_out, k_out
+    return rotary_embed(q, k, inv_freq, ctx_len, q_len, positions, interleaved, mscale, plan, n_seqs, q_out, k_out,
+                        (q_weight, k_weight, eps))
 
 
 def _block_cache(who: str, kc, vc, ks, vs, block_tbl, ctx_len, seqs: int, H_KV: int, D: int):
