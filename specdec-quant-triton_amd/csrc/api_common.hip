@@ -1,6 +1,5 @@
 // Shared host-side pieces of the C ABI: thread-local error text, launch wrapper, device info,
 // and the kernel-attribute query that dispatches to each kernel family.
-#include <algorithm>
 #include <atomic>
 #include <mutex>
 #include <set>
@@ -42,13 +41,22 @@ void set_error(const char* fmt, ...) {
 void clear_error() { g_err[0] = '\0'; }
 
 bool nest_apart(std::initializer_list<TensorDim> dims, int64_t len) {
-  std::vector<TensorDim> d;
-  for (TensorDim x : dims)
-    if (x.n > 1) d.push_back({x.n, x.stride < 0 ? -x.stride : x.stride});
-  std::sort(d.begin(), d.end(), [](const TensorDim& a, const TensorDim& b) { return a.stride < b.stride; });
-  for (const TensorDim& x : d) {
-    if (x.stride < len) return false;
-    len += (x.n - 1) * x.stride;
+  // No allocation, which could throw through the C entry points; 128 bits, since strides and sizes are the caller's.
+  typedef __int128 wide;
+  struct { wide n, stride; } d[4];
+  int count = 0;
+  for (TensorDim x : dims) {
+    if (x.n <= 1) continue;
+    if (count == 4) return false;
+    const wide stride = x.stride < 0 ? -(wide)x.stride : (wide)x.stride;
+    int i = count++;
+    for (; i > 0 && d[i - 1].stride > stride; --i) d[i] = d[i - 1];
+    d[i] = {x.n, stride};
+  }
+  wide end = len;
+  for (int i = 0; i < count; ++i) {
+    if (d[i].stride < end) return false;
+    end += (d[i].n - 1) * d[i].stride;
   }
   return true;
 }

@@ -61,8 +61,8 @@ inline int common_vec(std::initializer_list<uint64_t> vals) {
 // (stride 0) or a closer one has several workgroups write one place.
 inline bool lie_apart(int64_t n, int64_t stride, int64_t len) { return n <= 1 || stride >= len || stride <= -len; }
 
-// Whether the rows of a written tensor, `len` long, lie apart over all its dimensions (entries, stride): taken by stride, each
-// steps over all that the ones before it cover.
+// Whether the rows of a written tensor, `len` long, lie apart over all its dimensions (entries, stride; at most four): taken by
+// stride, each steps over all that the ones before it cover.
 struct TensorDim { int64_t n, stride; };
 bool nest_apart(std::initializer_list<TensorDim> dims, int64_t len);
 

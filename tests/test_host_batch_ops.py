@@ -105,6 +105,14 @@ def test_evict_refusals(built_lib):
     f(-28, base=(4096, 1 << 20), **two)
 
 
+def test_rows_far_apart_and_overlapping(built_lib):
+    """Strides whose extents pass 64 bits do not hide rows that overlap."""
+    f = lambda code, **kw: _fail("specq_paged_attn_weights", WEIGHTS, code, B=9, n_seqs=9, H=36, HK=9, **kw)  # noqa: E731
+    f(-95, s_wb=1 << 62, s_wh=1 << 62)  # one stride for both: eight steps of it are 2^65
+    f(-95, s_wb=-(1 << 62), s_wh=1 << 62), f(-95, s_wb=-(1 << 63), s_wh=-(1 << 63))
+    f(-28, s_wb=9 * 1024, s_wh=-1024)   # apart; no workspace
+
+
 def test_evict_refuses_what_a_launch_does_not_take_before_the_first(built_lib):
     """A selection of 2^32 threads and more, and a move of them behind a selection that could have run."""
     for kw in (dict(B=1 << 19), dict(B=1 << 17, sp=(16 * 8 * 4096,), so=(8 * 4096,), sh=(4096,), rb=(4096,))):
