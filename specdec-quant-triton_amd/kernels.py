@@ -1497,6 +1497,12 @@ def _gathered(who: str, weights, B: int, H_KV: int, tokens: int):
     return weights.stride(0), weights.stride(1)
 
 
+@functools.lru_cache(maxsize=4096)
+def _weights_workspace(B, H, H_KV, QL, max_pages, PAGE) -> int:
+    """Bytes a call needs: a function of its sizes."""
+    return _lib.lib().specq_paged_attn_weights_workspace_size(B, H, H_KV, QL, max_pages, PAGE)
+
+
 def paged_attention_weights(q, kc, ks, block_tbl, ctx_len, weights, q_len=None, q_lens=None, plan=None, n_seqs=None,
                             sm_scale=None, workspace=None):
     """Add to `weights` the attention weight that the new tokens' queries give each cached token, in place; returns it.
@@ -1536,8 +1542,7 @@ def paged_attention_weights(q, kc, ks, block_tbl, ctx_len, weights, q_len=None, 
     s_wb, s_wh = _gathered(who, weights, Bg, H_KV, max_pages * PAGE)
     if Bg == 0 or Qg == 0:
         return weights
-    need = _lib.lib().specq_paged_attn_weights_workspace_size(Bg, H, H_KV, Qg, max_pages, PAGE)
-    wptr, wbytes = _workspace(workspace, dev).ensure(need)
+    wptr, wbytes = _workspace(workspace, dev).ensure(_weights_workspace(Bg, H, H_KV, Qg, max_pages, PAGE))
     qs, ss = q.stride(), ks.stride()
     _call_on(dev, "specq_paged_attn_weights", q.data_ptr(), qs[0], qs[1], qs[2], kc.data_ptr(), cs[0], cs[1], cs[2],
              ks.data_ptr(), ss[0], ss[1], ss[2], ks.dtype == torch.float32,
