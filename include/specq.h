@@ -442,7 +442,7 @@ int specq_qk_norm_rotary(const void* q, int64_t s_qb, int64_t s_qt, int64_t s_qh
  *             counts: the drafts that were accepted.  0 leaves the sequence's weights as they are
  *   weights   fp32 [B_grid, H_KV, >= max_pages * PAGE], strides s_wb, s_wh; rows must not overlap
  *   A context longer than the table counts as the table's length, a negative one as 0.  Tokens on no page of the pool get
- *   nothing.  A NaN or infinite score makes NaN of its row's share.  Eager and plan-mode calls agree bit for bit.  At most
+ *   nothing.  A score of -infinity gives its token nothing; one of NaN or +infinity makes NaN of its row's share.  Eager and plan-mode calls agree bit for bit.  At most
  *   65536 (sequence, KV head) pairs.
  *   Workspace: specq_paged_attn_weights_workspace_size() bytes, as the workspaces above: for each pair and 256 tokens of
  *   the table 8 bytes a row (1024 rows, or up to 8192 where that stays below 256 MiB; more are taken in turns), and
@@ -485,7 +485,7 @@ int specq_kv_evict(const int32_t* block_tbl, int64_t s_bt, int B, int max_pages,
  * Beam search (no reference counterpart).
  * select: of the candidates scores[b, w] + logits[b, w, v] - log(sum_u exp(logits[b, w, u])) of each sequence the best n,
  *   in order, ties to the lower beam, then the lower token.  A beam with finished[b, w] != 0 has one candidate, token eos
- *   with the score it has.  Candidates whose score is NaN or -infinity are none; what is missing is (-inf, -1, -1).
+ *   with the score it has.  Candidates whose score is NaN or, in fp32, -infinity are none; what is missing is (-inf, -1, -1).
  *   Scores are formed and compared in fp64; a row's log-sum is within 2^-33.
  *   logits    fp16 or (logits_fp32) fp32 [B, W, V], strides s_lb, s_lw;  scores fp32 [B, W], row stride s_sb
  *   finished  NULL, or bytes [B, W], row stride s_fb

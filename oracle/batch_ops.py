@@ -101,7 +101,8 @@ def beam_select(logits, scores, n, finished=None, eos=None):
             if not np.isfinite(m) or np.isnan(x).any():
                 continue
             flat[w] = (x - (m + np.log(np.exp(x - m).sum()))) + c
-        flat = np.where(flat > -np.inf, flat, -np.inf).ravel()
+        with np.errstate(over="ignore"):
+            flat = np.where(flat.astype(np.float32) > -np.inf, flat, -np.inf).ravel()  # as it is given out
         order = np.argsort(-flat, kind="stable")
         order = order[flat[order] > -np.inf]
         k = min(n, len(order))

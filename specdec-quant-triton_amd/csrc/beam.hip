@@ -2,8 +2,8 @@
 //
 // Selection, for each sequence b of W beams with scores c_w (log-probabilities so far) and logits x_w over V tokens:
 //   c_w,v = c_w + x_w,v - log sum_u exp(x_w,u);   a finished beam has one candidate, its eos, with the score it has
-// and the best n of the W V candidates, ties to the lower beam, then the lower token.  A candidate whose score is NaN or
-// -infinity is none; where there are fewer than n the rest is (-inf, -1, -1).
+// and the best n of the W V candidates, ties to the lower beam, then the lower token.  A candidate whose score, rounded to fp32, is
+// NaN or -infinity is none; where there are fewer than n the rest is (-inf, -1, -1).
 //
 // One pass over the logits, which is what bounds it, and a second launch over what it leaves.
 //   1  A workgroup owns a part of a row and keeps it in registers: its maximum and sum of exponentials, and its
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamParams p) {
         if (!first || k >= kBeamNear) c = p.cands[(base + part) * kBeamSlots + i];
         const double key = ((double)beam_lo(c) - s_lse[w]) + s_score[w];
         const uint64_t at = ((uint64_t)w << 32) | (c >> 32);
-        if (key > -(double)INFINITY) {
+        if ((float)key > -INFINITY) {  // as it is given out: one that fp32 has no number for is none
           if (pass == 0) {
             best = fmaxf(best, (float)key);
           } else if (pass == 1) {
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamParams p) {
     }
     auto put = [&](int i, double key, uint64_t at) {
       const int64_t o = (int64_t)b * p.n + i;
-      const bool some = key > -(double)INFINITY;
+      const bool some = (float)key > -INFINITY;
       p.out_score[o] = (float)key;
       p.out_token[o] = some ? (int32_t)(uint32_t)at : -1;
       p.out_parent[o] = some ? b * p.W + (int)(at >> 32) : -1;

@@ -1514,8 +1514,8 @@ def paged_attention_weights(q, kc, ks, block_tbl, ctx_len, weights, q_len=None, 
     weights[b, h, t] grows by that sum, or becomes it where t is one of the new tokens; positions past the sequence stay.
     q_lens int32 [B]: how many of the q_len tokens sequence b really has (accepted drafts), counted by ctx_len; 0
     leaves its weights as they are.  Block-table ids outside [0, pages) mask their page's tokens, a context longer
-    than the table counts as the table's length.  sm_scale defaults to D^-1/2.  A NaN or infinite score makes NaN of its
-    row's share.  With `plan`, (n_seqs, q_len) = plan[0:2] on the device and the grid covers (B, QLMAX).  Calls that may
+    than the table counts as the table's length.  sm_scale defaults to D^-1/2.  A score of -infinity gives its token
+    nothing, one of NaN or +infinity makes NaN of its row's share.  With `plan`, (n_seqs, q_len) = plan[0:2] on the device and the grid covers (B, QLMAX).  Calls that may
     run at the same time on several streams need a workspace each.
     """
     who = "paged_attention_weights"
@@ -1643,8 +1643,8 @@ def beam_select(logits, scores, n=None, finished=None, eos=None, out=None, works
     continuation by token v has scores[b, w] + logits[b, w, v] - log(sum(exp(logits[b, w]))); a beam with
     finished[b, w] (bool) has one, token `eos`, with the score it has.  Best first, formed and compared in fp64 (a row's
     log-sum is within 2^-33), ties to the lower beam, then the lower token; n defaults to W, and both are at most 64.  parents holds rows b * W + w, as
-    paged_kv_fork and beam_reorder take them.  Continuations of score -inf or NaN (logits of -inf; every one of a row that
-    holds NaN or +inf) are none; where there are fewer than n the rest has score -inf, token and parent -1.  `out` may hold
+    paged_kv_fork and beam_reorder take them.  Continuations of score -inf in fp32 or NaN (logits of -inf; every one of a row
+    that holds NaN or +inf) are none; where there are fewer than n the rest has score -inf, token and parent -1.  `out` may hold
     `scores` itself where n is W.
     Calls that may run at the same time on several streams need a workspace each.
     """

@@ -436,3 +436,19 @@ def test_more_items_than_workgroups(QL, G):
     assert torch.equal(tw, parts)
     for at in (slice(0, 8), slice(118, 124), slice(295, 300)):
         check(tw[at], (case[0][at], case[1], case[2], case[3][at], case[4][at], case[5][at]), lens[at].tolist(), D ** -0.5, f"{at}")
+
+
+@pytest.mark.parametrize("QL", [1, 9, 40])
+def test_scores_that_are_infinite(QL):
+    """A scale of infinity: tokens of score -inf get nothing from a row, one of +inf makes NaN of what the row sees."""
+    rng = np.random.default_rng(51)
+    q, kc, ks, bt, cl, w = make(rng, [200], QL, 4, 2, 64, 16, True)
+    q, w = np.abs(q) + np.float16(0.25), np.zeros_like(w)
+    page, slot = bt[0, 3], 5  # token 53, seen by every row
+    kc[page, slot, 0], kc[page, slot, 1], ks[page, slot] = -1, 1, np.inf
+    note(f"attn_weights infinite QL={QL}")
+    got = K.paged_attention_weights(*gpu(q, kc, ks, bt, cl, w)).cpu().numpy()[0]
+    assert got[0, 53] == 0 and np.isfinite(got[0]).all()
+    assert abs(got[0, :200].astype(np.float64).sum() - 2 * QL) < 2.0 ** -16 * 2 * QL
+    first = 200 - QL + 1  # what the first new token sees
+    assert np.isnan(got[1, :first]).all() and not got[:, 200:].any()

@@ -314,3 +314,18 @@ def test_beams_closer_than_an_fp32_step_of_their_scores(V, f32):
     assert np.array_equal(got[1].cpu().numpy()[sure], token[sure])
     err = np.abs(got[0].cpu().numpy().astype(np.float64) - want)
     assert (err <= 2.0 ** -32 + 2.0 ** -24 * np.abs(want)).all()
+
+
+def test_lowest_values_as_masks():
+    """Beams that are not there and banned tokens by fp32's lowest value, not by -inf: either alone is a candidate, the last of
+    all; both together have no fp32 score, and are none.  Next to the lowest value the logits' differences are below half a step
+    of fp64 (2^74), so that a beam of that score has its tokens tie, in their order."""
+    low = np.finfo(np.float32).min
+    x = np.full((2, 2, 300), low, np.float32)
+    x[:, :, [3, 200]] = 1.0, 2.0
+    s = np.array([[-1, low], [low, low]], np.float32)
+    note("beam lowest values")
+    score, token, parent = (t.cpu().numpy() for t in K.beam_select(*gpu(x, s), 6))
+    assert token.tolist() == [[200, 3, 0, 1, 2, 4], [3, 200, 3, 200, -1, -1]]
+    assert parent.tolist() == [[0] * 6, [2, 2, 3, 3, -1, -1]]
+    assert (score[0, 2:] == low).all() and np.isneginf(score[1, 4:]).all() and np.isfinite(score[1, :4]).all()
