@@ -926,9 +926,14 @@ extern "C" int specq_paged_attn_weights(const void* q, int64_t s_qb, int64_t s_q
   p.stats = reinterpret_cast<uint64_t*>(at + kCounterBytes + space.scores);
   p.norms = reinterpret_cast<uint64_t*>(at + kCounterBytes + space.scores + space.stats);
   p.sums = reinterpret_cast<uint64_t*>(at + kCounterBytes + space.scores + space.stats + space.norms);
-  // Stored scores against scores formed twice (us, 8 KV heads of 128): 4 rows, 8 sequences of 4096: 20.3, 24.6; 32 of 8192: 82,
-  // 121; 16 rows, 8 of 4096: 27.3, 24.8; one of 32768: 28.6, 32.8.  Queries in LDS for the whole call against 64 rows at a
-  // time: 20 rows, 8 of 4096: 28.7, 58.6; 64 rows: 37.7, 58.5; one of 32768: 54, 69.
+  // Stored scores against scores formed twice (us, 8 KV heads of 128, tables as wide as the contexts):
+  //           8 x 4096      32 x 8192     1 x 32768     32 x 1024
+  //    4 rows 17.7, 23.3    81.5, 111.5   19.7, 29.1    17.2, 21.9
+  //   12      24.1, 23.4    103, 114      25.1, 31.5    24.4, 22.8
+  //   16      27.4, 23.2    122, 114      27.9, 32.5    25.1, 22.4
+  // At 16 either gains as often as it loses, by as much; one sequence gains the most.
+  // Queries in LDS for the whole call against 64 rows at a time: 20 rows, 8 of 4096: 28.7, 58.6; 64 rows: 37.7, 58.5; one of
+  // 32768: 54, 69.
   const bool store = space.store, few = rows <= kAwFewRows, f32 = scale_fp32 != 0;
   for (; p.b0 < B_grid; p.b0 += (int)space.seqs) {
     p.B_grid = (int)(B_grid - p.b0 < space.seqs ? B_grid - p.b0 : space.seqs);
