@@ -16,7 +16,7 @@
 // where their scores lie closer than fp32 steps: fp32 sums put a row's log-sum off by 2^-23, and with it all of its beam.
 //
 // 16 x 8 rows of 128257 fp32 logits: 20.5 us (66 MB, 3.2 TB/s; with fp32 exponentials 17.1) and 9.1; 4 of 32000 fp16: 6.1 and 5.8.
-// An exponential is 15 fp64 instructions of the rate of fp32 ones.  Fewer vectors a lane, for more waves, leave the first launch at
+// An exponential is 16 fp64 instructions of the rate of fp32 ones.  Fewer vectors a lane, for more waves, leave the first launch at
 // 20.5 and give the second more parts to join (4: 13.0 us); sums that start with the first loads keep more registers (22.8).  The
 // second launch waits for memory three times over, whatever its size.
 //
@@ -53,12 +53,12 @@ __device__ __forceinline__ uint64_t beam_pack(float a, uint32_t b) {
 }
 __device__ __forceinline__ float beam_lo(uint64_t x) { return __builtin_bit_cast(float, (uint32_t)x); }
 
-// 2^(x log2 e - ref), where that is no more than 1: 2^n of the nearest whole number n, which adding 1.5 * 2^52 leaves in the lower bits,
-// and a polynomial that meets 2^f on |f| <= 1/2 in the Chebyshev points of degree 7, off by at most 2^-34 of itself.  What is below
-// 2^-1000 counts as that; -infinity too, and NaN.
+// exp(x - ref), ref >= x.  The difference comes first, exact where it counts whatever the logits' size; then 2^n of the nearest whole
+// number n, which adding 1.5 * 2^52 leaves in the lower bits, and a polynomial that meets 2^f on |f| <= 1/2 in the Chebyshev points
+// of degree 7, off by at most 2^-34 of itself.  What is below 2^-1000 counts as that; -infinity too, and NaN.
 __device__ __forceinline__ double beam_exp(float x, double ref) {
   constexpr double kWhole = 6755399441055744.;
-  const double t = fmax(fma((double)x, 1.4426950408889634074, -ref), -1000.), w = t + kWhole, f = t - (w - kWhole);
+  const double t = fmax(((double)x - ref) * 1.4426950408889634074, -1000.), w = t + kWhole, f = t - (w - kWhole);
   double e = 1.5303699001378845e-05;
   e = fma(e, f, 1.5469729140704658e-04);
   e = fma(e, f, 1.3333478480888061e-03);
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamParams p) {
   float m = mine;
 #pragma unroll
   for (int o = 1; o < kWave; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
-  const double ref = (m == -INFINITY ? 0. : (double)m) * 1.4426950408889634074;
+  const double ref = m == -INFINITY ? 0. : (double)m;
   double sum = 0;
   bool nan = m == INFINITY;
 #pragma unroll
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamParams p) {
   // The waves' sums, a lane each.
   double all = threadIdx.x < kBeamWaves ? s_sum[threadIdx.x] : 0.;
   // A NaN sum stays one, whatever its wave's maximum.
-  if (threadIdx.x < kBeamWaves && all != 0.) all *= beam_exp(s_max[threadIdx.x], (double)top * 1.4426950408889634074);
+  if (threadIdx.x < kBeamWaves && all != 0.) all *= beam_exp(s_max[threadIdx.x], top);
 #pragma unroll
   for (int o = 1; o < kBeamWaves; o *= 2) all += beam_shfl(all, o);
   if (threadIdx.x == 0) {
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamParams p) {
     for (int k = lane; k < p.parts; k += kWave) {
       const float t = k == lane ? top0 : tops[k];
       const double v = k == lane ? sum0 : sums[k];
-      if (v != 0.) sum += v * beam_exp(t, (double)m * 1.4426950408889634074);
+      if (v != 0.) sum += v * beam_exp(t, m);
     }
     for (int o = 1; o < kWave; o *= 2) sum += beam_shfl(sum, o);
     if (lane == 0) {

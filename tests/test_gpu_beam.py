@@ -329,3 +329,18 @@ def test_lowest_values_as_masks():
     assert token.tolist() == [[200, 3, 0, 1, 2, 4], [3, 200, 3, 200, -1, -1]]
     assert parent.tolist() == [[0] * 6, [2, 2, 3, 3, -1, -1]]
     assert (score[0, 2:] == low).all() and np.isneginf(score[1, 4:]).all() and np.isfinite(score[1, :4]).all()
+
+
+@pytest.mark.parametrize("size", [1e6, 1e15, 1e20, 1e38])
+def test_logits_of_any_size(size):
+    """A row's sum is relative to its largest logit, whatever that is: rows of 10^6 to 10^38, constant ones among them, and of
+    fp32's lowest value throughout."""
+    rng = np.random.default_rng(12)
+    x = (size * rng.uniform(-1, 1, (3, 4, 3000))).astype(np.float32)
+    x[0, 1], x[0, 2], x[1, 0] = size, -size, np.finfo(np.float32).min
+    x[1, 1, 5:90] = x[1, 1].max()
+    s = np.array([[-1, -2, -3, -4], [-0.5, -8, -9, -10], [-1, -1, -1, -1]], np.float32)
+    note(f"beam size {size}")
+    got = K.beam_select(*gpu(x, s), 12)
+    torch.cuda.synchronize()
+    check(got, x, s, 12, ties=True, what=f"size {size}")
