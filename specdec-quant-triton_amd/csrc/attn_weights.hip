@@ -21,9 +21,10 @@
 // K stays: a wave holds 64 tokens, converts their codes to fp16 matrix operands once and walks the rows 16 at a time
 // (K . Q^T on v_mfma_f32_16x16x32_f16: a lane's results are four tokens of one row).  Everything behind the products is
 // fp32; log2(e) is folded into the scale.
-// 8 KV heads of 128 (us): a new token of 32 sequences of up to 8192, stored scores, 53 + 8, codes and scores at 3.4 TB/s (loads
-// alone 5.2); 9 of 8 sequences of 4096, formed twice, 19 + 14, half of it fixed phases; 256 of 2 of up to 4096, 43 + 33, bound by
-// vector instructions at two waves a SIMD.
+// 8 KV heads of 128 (us): a new token of 32 sequences of up to 8192, stored scores, 51 + 7, codes and scores at 3.4 TB/s (loads
+// alone 5.2; the CUs are busy 60 % of the time, since spans of tiles are cut from the table and not from the lengths); 9 of 8
+// sequences of 4096, formed twice, 20 + 14, half of it fixed phases; 256 of 2 of up to 4096, 43 + 34, bound by vector instructions
+// at two waves a SIMD.
 #include <algorithm>
 
 #include "api_common.hpp"
@@ -558,9 +559,9 @@ __global__ __launch_bounds__(256) void aw_store_kernel(AwParams p) {
 // More rows: a workgroup owns a tile, its waves 64 tokens and the row blocks of one parity each.  64 rows' queries at a time
 // come through LDS, whole rows a load, while the 64 before are multiplied.  Loaded by each wave as its matrix operands,
 // nearly every lane's 16 bytes were an access of their own: 2 x 256 tokens, 32 / 8 heads of 128, contexts of 4096 and less
-// took 77 us in both launches instead of 69.  At two waves a SIMD (K's operands are 64 registers) the vector
-// instructions have 60 % of the cycles and the matrix ones 26 %.  Put between one another by hand, 45 % of the matrix
-// cycles had vector ones beside them, and the sums took 35 us where they had taken 31.
+// took 77 us in both launches instead of 69.  At two waves a SIMD (K's operands are 64 registers, and the shared memory has room
+// for one workgroup a CU) the vector instructions have 61 % of a busy CU's cycles and the matrix ones 25 %, 30 % of which have
+// vector ones beside them.  Put between one another by hand, 45 % had, and the sums took 35 us where they had taken 31.
 template <int D, typename ST, int MODE>
 __global__ __launch_bounds__(512) void aw_many_kernel(AwParams p) {
   constexpr int NU = D / 32, GQ = D / 8, kLoads = 64 * GQ / 512;  // 16-byte granules of a query row; loads of a thread

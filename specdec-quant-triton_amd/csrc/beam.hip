@@ -15,13 +15,15 @@
 // Exponentials (within 2^-34 of themselves), sums, logarithms and scores are fp64, so beams are told apart as the formula does
 // where their scores lie closer than fp32 steps: fp32 sums put a row's log-sum off by 2^-23, and with it all of its beam.
 //
-// 16 x 8 rows of 128257 fp32 logits: 20.5 us (66 MB, 3.2 TB/s; with fp32 exponentials 17.1) and 9.1; 4 of 32000 fp16: 6.1 and 5.8.
-// An exponential is 16 fp64 instructions of the rate of fp32 ones.  Fewer vectors a lane, for more waves, leave the first launch at
-// 20.5 and give the second more parts to join (4: 13.0 us); sums that start with the first loads keep more registers (22.8).  The
-// second launch waits for memory three times over, whatever its size.
+// 16 x 8 rows of 128257 fp32 logits, a quarter of them finished: 21.4 us (50 MB; with fp32 exponentials 17.1) and 9.0; 4 of 32000
+// fp16: 5.9 and 5.8.  An exponential is 16 fp64 instructions of the rate of fp32 ones, and vector instructions have 58 % of a busy
+// CU's cycles: they follow the loads of a wave instead of running beside them.  Fewer vectors a lane, for more waves, leave the first
+// launch as it is and give the second more parts to join (4: 13 us); sums that start with the first loads keep more registers (1 us
+// more).  The second launch waits for memory three times over, whatever its size.
 //
 // Reordering: row r of every state becomes row parents[r] of the same group of rows.  In place: a thread owns one column of
-// up to 16 bytes of a group's rows, reads what changes and then writes it.  Bound by HBM: 16 x 8 rows of 418 KB, 13.7 us.
+// up to 16 bytes of a group's rows, reads what changes and then writes it.  16 x 8 rows of 418 KB, 57 MB: 16.2 us from HBM (3.5
+// TB/s), 11.7 where the last-level cache holds them from one call to the next.
 #include "api_common.hpp"
 #include "common.hpp"
 

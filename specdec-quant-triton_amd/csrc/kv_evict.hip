@@ -16,10 +16,11 @@
 // Moving is in place.  Token j goes to a place at or below its own, and everything behind it starts above, so it is
 // enough that a tile of tokens has been read by all its threads before any of them writes it.  One workgroup walks one
 // byte range of the rows of one (sequence, head) of one tensor; ranges are independent, so narrow ranges make more
-// workgroups where there are few sequences and heads.  Bound by the lines a CU has in flight, since each workgroup walks its
-// tokens in order: 8 sequences of up to 4096 tokens to 2048, 8 heads of 128: 11 us to choose, 24.5 to move 35 MB; one of 65536 to
-// 8191, two heads of 64: 25 and 25.  By way of the workspace, with as many workgroups as there is work, the latter took 10 us less
-// and shorter rows 4 us more.
+// workgroups where there are few sequences and heads.  Bound by that walk, one tile after another with a barrier each, in few
+// workgroups: 8 sequences of up to 4096 tokens to 2048, 8 heads of 128: 11 us to choose, 24 to move (28 MB read, 26 written; the
+// CUs are busy 48 % of the time, since only sequences that are cut have work, and their waves wait in 58 % of it; eight accesses of
+// a thread in flight instead of four change nothing); one of 65536 to 8191, two heads of 64: 25 and 25, by 22 workgroups.  By way
+// of the workspace, with as many workgroups as there is work, the latter took 10 us less and shorter rows 4 us more.
 #include "api_common.hpp"
 #include "common.hpp"
 

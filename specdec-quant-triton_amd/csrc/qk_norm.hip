@@ -158,7 +158,8 @@ __global__ __launch_bounds__(256) void qk_norm_vec_kernel(QkNormParams p) {
 
 // Any R, D and alignment, 2 bytes an access: a wave owns a row, a lane every 64th of its pairs and single values, and
 // walks the heads with the workgroup's other waves: 16 of them where there are few tokens, so that few rows follow one
-// another (51 tokens, 12 / 3 heads of 80: 8.3 us with four).
+// another (51 tokens, 12 / 3 heads of 80: 8.3 us with four).  Prompts are bound by its narrow accesses: 2 x 4096 tokens of
+// such heads, 39 MB, 51 us.
 constexpr int kNormItems = 8;  // pairs and values a lane has at most: D <= 512
 template <bool IL>
 __global__ __launch_bounds__(1024) void qk_norm_any_kernel(QkNormParams p) {
